@@ -693,6 +693,100 @@ int qkv_paged_decode_attention_layers(
     int32_t out_dtype, void* workspace, int64_t ws_bytes, int32_t n_splits, void* stream);
 
 /* ------------------------------------------------------------------------
+ * 8-bit paged cache (no reference counterpart: the reference's page manager,
+ * quashkv/integrations/vllm_backend.py:82-195, keeps 3-bit codes of one length
+ * for all sequences).  Requests of any lengths share one pool; K and V are
+ * int8 or float8 e4m3 codes with an fp32 scale per block of 16 tokens and
+ * head, value = code * scale.  Pages hold n = page_tokens (64 << k, k = 0..5)
+ * tokens of all H kv heads of one request:
+ *   kpool  num_pages x H x n x d           one byte a code
+ *   vpool  num_pages x H x n / 16 x d x 16 a block's 16 tokens innermost
+ *   kscale, vscale  num_pages x H x n / 16 fp32
+ * (pools 16-byte aligned).  A slot names a token's place: page * n + t % n;
+ * slots outside [0, num_pages * n) are left out of every call.  Rows of keys,
+ * values and queries are (rows, heads, d) with row and head strides in
+ * elements, the last axis dense.
+ * ---------------------------------------------------------------------- */
+#define QKV_CODES_I8 0   /* int8, largest code 127 */
+#define QKV_CODES_E4M3 1 /* float8 e4m3 (finite), largest code 448 */
+
+/* Page tables and slot maps of B requests (<= 16000) from their lengths:
+ * request b holds lens[b] tokens and brings new_lens[b] (negative: 0), whose
+ * rows follow those of request b - 1 in the batch.  It is served wholly or not
+ * at all: not, if its rows end behind `rows`, its pages behind pages_per_seq,
+ * or if it needs pages and the pages needed up to it, in request order, exceed
+ * the free ones.
+ *   table       B x pages_per_seq: entries of newly opened pages are written
+ *   free_list   num_pages entries, the first free_count[0] of them free pages;
+ *               pages are taken from its end
+ *   q_start     B + 1: each request's first row (whether served or not)
+ *   q_lens      B: rows served (new_lens, or 0)
+ *   kv_lens     B: lens + q_lens; may be lens
+ *   slots, positions  `rows`: a row's slot (-1: not served) and token position
+ *   free_count_out    may be free_count
+ *   scratch     B int32 */
+int qkv_page_plan(const int32_t* lens, const int32_t* new_lens, int32_t B, int32_t* table,
+                  int32_t pages_per_seq, const int32_t* free_list, int32_t num_pages,
+                  const int32_t* free_count, int32_t page_tokens, int64_t rows,
+                  int32_t* q_start, int32_t* q_lens, int32_t* kv_lens, int64_t* slots,
+                  int32_t* positions, int32_t* free_count_out, int32_t* scratch,
+                  void* stream);
+
+/* The pages of every request with done[b] != 0 go back to the end of the free
+ * list (request order, page order); its length becomes 0. */
+int qkv_page_release(int32_t* lens, const uint8_t* done, int32_t B, const int32_t* table,
+                     int32_t pages_per_seq, int32_t* free_list, int32_t num_pages,
+                     int32_t* free_count, int32_t page_tokens, void* stream);
+
+/* Quantise keys and values (rows, H, d), fp32, fp16 or bf16, into their slots.
+ * Rows of one block follow each other with ascending slots, as qkv_page_plan
+ * makes them; each slot is named once.  A block's tokens before the first one
+ * that a call brings keep their values: at the block's scale, or, where the new
+ * tokens need a larger one, quantised anew; its tokens behind are dropped.
+ *   a = max |x| over the finite new values of the block and head
+ *   scale = 0 if a = 0, else max(a / Z, 2^-100), Z = 127 or 448; the larger of
+ *           it and the block's scale where that holds earlier tokens
+ *   code = nearest to x * fp32(1 / scale), ties to even, at most Z; NaN: 0 */
+int qkv_kv8_append(int32_t in_dtype, const void* keys, int64_t k_row_stride,
+                   int64_t k_head_stride, const void* values, int64_t v_row_stride,
+                   int64_t v_head_stride, const int64_t* slots, int64_t rows, int32_t H,
+                   int32_t d, int32_t fmt, void* kpool, float* kscale, void* vpool,
+                   float* vscale, int32_t num_pages, int32_t page_tokens, void* stream);
+
+/* The values at the slots: keys and values, dense (rows, H, d) of out_dtype;
+ * rows whose slot is outside the pool become 0. */
+int qkv_kv8_read(const int64_t* slots, int64_t rows, int32_t H, int32_t d, int32_t fmt,
+                 const void* kpool, const float* kscale, const void* vpool,
+                 const float* vscale, int32_t num_pages, int32_t page_tokens, void* keys,
+                 void* values, int32_t out_dtype, void* stream);
+
+/* softmax(scale q K^T) V of each request's queries over its first kv_lens[b]
+ * tokens; causal: query i of q_len sits at token kv_len - q_len + i.
+ *   q, out      (rows, Hq, d); head h reads kv head h / (Hq / Hkv); out dense.
+ *               Rows of no request are left as they are; queries that see no
+ *               token give 0.
+ *   q_start     B + 1 first rows, ascending; null: request b's rows are
+ *               [b rows / B, (b + 1) rows / B)
+ *   q_lens      rows of each request from q_start[b] on; null: up to the next
+ *               request's
+ *   kv_lens     at most pages_per_seq pages' tokens count; tokens whose table
+ *               entry names no page of the pool are left out
+ *   max_q       the longest request's rows, as far as known (<= rows): picks
+ *               the kernels, not the result
+ *   workspace   qkv_kv8_attention_workspace_bytes(...) bytes, 256-byte aligned,
+ *               of this call alone until it has run; nothing in it need be set */
+int64_t qkv_kv8_attention_workspace_bytes(int32_t B, int64_t rows, int32_t Hq, int32_t Hkv,
+                                          int32_t d, int64_t max_q);
+int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_stride,
+                      int64_t q_head_stride, int64_t rows, const void* kpool,
+                      const float* kscale, const void* vpool, const float* vscale, int32_t fmt,
+                      int32_t num_pages, int32_t page_tokens, const int32_t* table,
+                      int32_t pages_per_seq, const int32_t* q_start, const int32_t* q_lens,
+                      const int32_t* kv_lens, int32_t B, int32_t Hq, int32_t Hkv, int32_t d,
+                      int64_t max_q, float scale, int32_t causal, void* out, int32_t out_dtype,
+                      void* workspace, int64_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Measurement helper (no reference counterpart): streams `bytes` (a multiple
  * of 16, 16-byte aligned) of `buf` with 16-byte loads, `unroll` (4, 8, 16)
  * per lane in flight, nontemporal loads if `nontemporal`, over `grid`

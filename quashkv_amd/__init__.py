@@ -14,6 +14,7 @@ from .engine import QuashKVEngine
 from .packing import pack_bits, unpack_bits
 from .nn_search import QuashIndex
 from .mixed_precision import MixedPrecisionMSEQuantizer, MixedPrecisionIPQuantizer
+from .paged8 import PagedKV8Engine, PagedKV8Store
 
 __all__ = [
     "LloydMaxCodebook",
@@ -23,6 +24,8 @@ __all__ = [
     "QuashIndex",
     "MixedPrecisionMSEQuantizer",
     "MixedPrecisionIPQuantizer",
+    "PagedKV8Engine",
+    "PagedKV8Store",
     "pack_bits",
     "unpack_bits",
 ]

@@ -24,6 +24,7 @@ QKV_F32, QKV_F16, QKV_BF16 = 0, 1, 2
 QKV_MODE_MSE, QKV_MODE_IP = 0, 1
 QKV_FMT_UNPACKED, QKV_FMT_PACKED, QKV_FMT_KPLANES, QKV_FMT_VTILES = 0, 1, 2, 3
 QKV_FLAG_PACKED, QKV_FLAG_PRE_ROTATED = 1, 2
+QKV_CODES_I8, QKV_CODES_E4M3 = 0, 1
 NOALLOC_SCRATCH_BYTES = 16 << 20  # QKV_NOALLOC_SCRATCH_BYTES
 
 _DTYPE = {torch.float32: QKV_F32, torch.float16: QKV_F16, torch.bfloat16: QKV_BF16}
@@ -122,6 +123,17 @@ _SIGS = {
                                           _i32,
                                           _i32, _i32, _i32, _i32, _i32, _i32, _p, _p, _p, _p,
                                           _f32, _f32, _i32, _p, _i32, _p, _i64, _i32, _p]),
+    "qkv_page_plan": (_i32, [_p, _p, _i32, _p, _i32, _p, _i32, _p, _i32, _i64, _p, _p, _p, _p,
+                             _p, _p, _p, _p]),
+    "qkv_page_release": (_i32, [_p, _p, _i32, _p, _i32, _p, _i32, _p, _i32, _p]),
+    "qkv_kv8_append": (_i32, [_i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i32, _i32, _i32,
+                              _p, _p, _p, _p, _i32, _i32, _p]),
+    "qkv_kv8_read": (_i32, [_p, _i64, _i32, _i32, _i32, _p, _p, _p, _p, _i32, _i32, _p, _p, _i32,
+                            _p]),
+    "qkv_kv8_attention_workspace_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32, _i64]),
+    "qkv_kv8_attention": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p, _i32, _i32, _i32,
+                                 _p, _i32, _p, _p, _p, _i32, _i32, _i32, _i32, _i64, _f32, _i32,
+                                 _p, _i32, _p, _i64, _p]),
     "qkv_hbm_read_probe": (_i32, [_p, _i64, _p, _i32, _i32, _i32, _p]),
     "qkv_paged_decode_attention_layers": (_i32, [_i32, _p, _i32, _p, _p, _p, _p, _p, _i32, _i32,
                                                  _i32, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32,

@@ -11,7 +11,8 @@ uses ``block_size``.  Here a layer keeps its tokens in the paged store
 table per sequence) whenever the paged kernels cover the configuration (head_size 128
 with key_bits 2..4, or 64 with key_bits 2 or 3), and a contiguous-store QuashKVEngine
 otherwise; both
-give the same codes and attention.  ``block_size`` must divide the page
+give the same codes and attention.  key_bits = value_bits = 8 keeps the layer in the
+8-bit paged cache (quashkv_amd.paged8).  ``block_size`` must divide the page
 (vLLM blocks then map onto page slots).
 """
 
@@ -27,6 +28,7 @@ from ..engine import QuashKVEngine
 from ..kernels import CompressedBlock
 from ..quantizer import _default_device
 from ..paged import PAGE_TOKENS, PagedQuashKVEngine, compressed_blocks
+from ..paged8 import PagedKV8Engine
 
 try:
     from vllm.v1.attention.backend import AttentionBackend, AttentionImpl  # noqa: F401
@@ -40,7 +42,7 @@ except ImportError:
 @dataclass
 class QuashKVPageConfig:
     """Compressed KV page configuration (quashkv/integrations/vllm_backend.py:68-75)."""
-    key_bits: int = 3       # 2-bit MSE + 1-bit QJL
+    key_bits: int = 3       # 2-bit MSE + 1-bit QJL; 8 (both): the 8-bit cache
     value_bits: int = 3     # 3-bit MSE
     block_size: int = 16    # tokens per vLLM block; divides the 64-token page
     seed: int = 42
@@ -59,6 +61,10 @@ class QuashKVPageManager:
         self.head_size = head_size
         self.config = config
         self.device = device
+        if config.key_bits == 8 and config.value_bits == 8:
+            self.paged = True
+            self.engine = PagedKV8Engine(head_dim=head_size, device=device)
+            return
         kw = dict(head_dim=head_size, key_bits=config.key_bits, value_bits=config.value_bits,
                   seed=config.seed + layer_idx, device=device)
         self.paged = PagedQuashKVEngine.covers(head_size, config.key_bits, config.value_bits)
@@ -73,6 +79,9 @@ class QuashKVPageManager:
 
     def get_compressed_blocks(self) -> list[CompressedBlock]:
         """Unpacked per-append blocks (mse codes, QJL bits, norms, value codes)."""
+        if isinstance(self.engine, PagedKV8Engine):
+            raise ValueError("the 8-bit cache has no codebook blocks; read its values with "
+                             "engine.store.read(slots)")
         return compressed_blocks(self.engine)
 
     def attention(self, queries: torch.Tensor, scale: Optional[float] = None) -> torch.Tensor:

@@ -1,0 +1,539 @@
+"""8-bit paged KV cache for ragged batches, with its page tables on the device.
+
+The 2 to 4 bit stores hold one length for all sequences and hand out pages on
+the host.  A serving batch has requests of any lengths, and an 8-bit cache is
+nearly lossless: this module holds K and V as int8 or float8 (e4m3) codes with
+one fp32 scale per block of 16 tokens and head, and plans pages, slots and
+positions on the GPU from the requests' lengths, so that a decode step (plan,
+append, attention) runs without the host and can be captured into a graph.
+
+Store formats (n = page_tokens = 64 << k; value = code * scale):
+
+* ``kpool`` (P, H, n, d), ``vpool`` (P, H, n / 16, d, 16): codes, a V block's
+  tokens innermost; ``kscale`` / ``vscale`` (P, H, n / 16) fp32.
+* ``table`` (B, W) int32: token t of request b lies in page table[b, t // n],
+  at slot page * n + t % n.
+* ``free`` (P,) int32 with ``free_count`` (1,): the first free_count entries are
+  free pages, taken from the end.
+
+Operators: :func:`plan_pages`, :func:`release_pages`, :func:`append_kv8`,
+:func:`read_kv8`, :func:`attention_kv8`; :class:`PagedKV8Store` holds the
+tensors and calls them; :class:`PagedKV8Engine` is the engine interface
+(append / attention / clear over sequences of one length) on that store.
+All calls run on the current stream of the tensors' device and never
+synchronise.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _native as N
+from .paged import PAGE_SIZES, PAGE_TOKENS
+from .quantizer import _default_device
+
+BLOCK_TOKENS = 16
+CODE_DTYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
+_FMT = {torch.int8: N.QKV_CODES_I8, torch.float8_e4m3fn: N.QKV_CODES_E4M3}
+
+
+class _On:
+    """Makes ``dev`` the current device for a library call (launches go to the
+    current device, whatever device the tensors' stream belongs to)."""
+
+    __slots__ = ("was", "dev")
+
+    def __init__(self, dev: torch.device):
+        self.dev = dev.index if dev.index is not None else torch.cuda.current_device()
+
+    def __enter__(self):
+        self.was = torch.cuda.current_device()
+        if self.was != self.dev:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *exc):
+        if self.was != self.dev:
+            torch.cuda.set_device(self.was)
+
+
+def _want(t: torch.Tensor, what: str, dtype: torch.dtype, shape: Optional[tuple] = None) -> None:
+    if t.dtype != dtype:
+        raise ValueError(f"{what} must be {dtype}; got {t.dtype}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{what} must have shape {shape}; got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+
+
+@dataclass
+class PagePlan:
+    """What :func:`plan_pages` found out about a step's rows (device tensors)."""
+    q_start: torch.Tensor      # (B + 1,) int32: each request's first row
+    q_lens: torch.Tensor       # (B,) int32: rows served, 0 where a request was refused
+    kv_lens: torch.Tensor      # (B,) int32: cached tokens after the step
+    slots: torch.Tensor        # (rows,) int64: a row's place in the pool, -1: none
+    positions: torch.Tensor    # (rows,) int32: a row's token position, 0: none
+    free_count: torch.Tensor   # (1,) int32: free pages left
+    scratch: torch.Tensor      # (B,) int32 workspace
+    max_q_len: int             # bound of q_lens, as far as the host knows
+
+    @classmethod
+    def empty(cls, B: int, rows: int, device, kv_lens: Optional[torch.Tensor] = None,
+              free_count: Optional[torch.Tensor] = None,
+              max_q_len: Optional[int] = None) -> "PagePlan":
+        if rows < 0:
+            raise ValueError(f"rows must not be negative; got {rows}")
+        i32 = dict(dtype=torch.int32, device=device)
+        return cls(torch.empty(B + 1, **i32), torch.empty(B, **i32),
+                   torch.empty(B, **i32) if kv_lens is None else kv_lens,
+                   torch.empty(rows, dtype=torch.int64, device=device), torch.empty(rows, **i32),
+                   torch.empty(1, **i32) if free_count is None else free_count,
+                   torch.empty(B, **i32), rows if max_q_len is None else max_q_len)
+
+
+def plan_pages(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor,
+               free: torch.Tensor, free_count: torch.Tensor, rows: int, page_tokens: int,
+               out: Optional[PagePlan] = None) -> PagePlan:
+    """Pages, slots and positions of the tokens that B requests bring.
+
+    Request b holds ``lens[b]`` tokens and brings ``new_lens[b]`` (negative
+    counts as 0); the batch has ``rows`` rows, request b's behind those of
+    request b - 1, and rows behind the last are padding.  New pages come from
+    the end of ``free[:free_count]`` and are written into ``table``; every other
+    result is in the plan, or in ``out``, whose ``kv_lens`` / ``free_count`` may be
+    ``lens`` / ``free_count`` themselves.
+
+    A request is served wholly or not at all (``q_lens`` 0, slots -1, its
+    length kept): not, when its rows end behind ``rows`` or its pages behind the
+    table's width, or when it needs pages and the pages needed up to it, in
+    request order, exceed the free ones."""
+    dev = N.require_gpu(table, lens, new_lens, free, free_count, what="plan_pages")
+    if table.dim() != 2:
+        raise ValueError("page table must be a 2-D int32 tensor")
+    B, width = table.shape
+    _want(table, "page table", torch.int32)
+    _want(lens, "lens", torch.int32, (B,))
+    _want(new_lens, "new_lens", torch.int32, (B,))
+    if free.dim() != 1:
+        raise ValueError("free must be a 1-D int32 tensor")
+    _want(free, "free", torch.int32)
+    _want(free_count, "free_count", torch.int32, (1,))
+    if out is None:
+        out = PagePlan.empty(B, rows, dev)
+    else:
+        for name, dt, shape in (("q_start", torch.int32, (B + 1,)), ("q_lens", torch.int32, (B,)),
+                                ("kv_lens", torch.int32, (B,)), ("slots", torch.int64, (rows,)),
+                                ("positions", torch.int32, (rows,)),
+                                ("free_count", torch.int32, (1,)),
+                                ("scratch", torch.int32, (B,))):
+            _want(getattr(out, name), f"out.{name}", dt, shape)
+        N.require_gpu(table, out.q_start, out.q_lens, out.kv_lens, out.slots, out.positions,
+                      out.free_count, out.scratch, what="plan_pages")
+    with _On(dev):
+        N.check(N.lib().qkv_page_plan(
+            lens.data_ptr(), new_lens.data_ptr(), B, table.data_ptr(), width, free.data_ptr(),
+            free.numel(), free_count.data_ptr(), page_tokens, rows, out.q_start.data_ptr(),
+            out.q_lens.data_ptr(), out.kv_lens.data_ptr(), out.slots.data_ptr(),
+            out.positions.data_ptr(), out.free_count.data_ptr(), out.scratch.data_ptr(),
+            N.stream(dev)))
+    return out
+
+
+def release_pages(table: torch.Tensor, lens: torch.Tensor, done: torch.Tensor,
+                  free: torch.Tensor, free_count: torch.Tensor, page_tokens: int) -> None:
+    """The pages of the requests with ``done`` ((B,) bool) go back to the free
+    list and their lengths become 0, all in place."""
+    dev = N.require_gpu(table, lens, done, free, free_count, what="release_pages")
+    if table.dim() != 2:
+        raise ValueError("page table must be a 2-D int32 tensor")
+    B, width = table.shape
+    _want(table, "page table", torch.int32)
+    _want(lens, "lens", torch.int32, (B,))
+    _want(done, "done", torch.bool, (B,))
+    if free.dim() != 1:
+        raise ValueError("free must be a 1-D int32 tensor")
+    _want(free, "free", torch.int32)
+    _want(free_count, "free_count", torch.int32, (1,))
+    with _On(dev):
+        N.check(N.lib().qkv_page_release(
+            lens.data_ptr(), done.data_ptr(), B, table.data_ptr(), width, free.data_ptr(),
+            free.numel(), free_count.data_ptr(), page_tokens, N.stream(dev)))
+
+
+def _check_pools(kpool: torch.Tensor, kscale: torch.Tensor, vpool: torch.Tensor,
+                 vscale: torch.Tensor) -> tuple[int, int, int, int, int]:
+    """(pages, H, page tokens, d, code format) of the pools."""
+    if kpool.dim() != 4:
+        raise ValueError("kpool must be (pages, kv heads, page_tokens, head_dim)")
+    P, H, n, d = kpool.shape
+    fmt = _FMT.get(kpool.dtype)
+    if fmt is None:
+        raise ValueError(f"kpool must be int8 or float8_e4m3fn; got {kpool.dtype}")
+    if n not in PAGE_SIZES:
+        raise ValueError(f"page_tokens {n} must be one of {PAGE_SIZES}")
+    nb = n // BLOCK_TOKENS
+    _want(kpool, "kpool", kpool.dtype)
+    _want(vpool, "vpool", kpool.dtype, (P, H, nb, d, BLOCK_TOKENS))
+    _want(kscale, "kscale", torch.float32, (P, H, nb))
+    _want(vscale, "vscale", torch.float32, (P, H, nb))
+    return P, H, n, d, fmt
+
+
+def _dense_last(x: torch.Tensor) -> torch.Tensor:
+    """x with unit stride along the head_dim (other strides are passed on)."""
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
+def append_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kpool: torch.Tensor,
+               kscale: torch.Tensor, vpool: torch.Tensor, vscale: torch.Tensor) -> None:
+    """Quantise rows k, v (rows, H, d; fp32, fp16 or bf16, any row and head
+    strides) into the pools at ``slots`` ((rows,) int64, as plan_pages makes them:
+    the rows of a block follow each other, each slot once; -1 skips a row).
+
+    A block's scale covers its largest finite value.  Tokens that the block
+    holds already keep their codes while the scale stands and are quantised anew
+    where the new ones need a larger scale; NaN becomes 0, infinities the
+    largest code."""
+    dev = N.require_gpu(k, v, slots, kpool, kscale, vpool, vscale, what="append_kv8")
+    P, H, n, d, fmt = _check_pools(kpool, kscale, vpool, vscale)
+    rows = k.shape[0] if k.dim() == 3 else -1
+    if k.shape != v.shape or tuple(k.shape) != (rows, H, d) or k.dtype != v.dtype:
+        raise ValueError(f"expected keys and values of shape (rows, {H}, {d}) and one type; got "
+                         f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
+    _want(slots, "slots", torch.int64, (rows,))
+    k, v = _dense_last(k), _dense_last(v)
+    with _On(dev):
+        N.check(N.lib().qkv_kv8_append(
+            N.dtype_code(k.dtype), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+            v.stride(0), v.stride(1), slots.data_ptr(), rows, H, d, fmt, kpool.data_ptr(),
+            kscale.data_ptr(), vpool.data_ptr(), vscale.data_ptr(), P, n, N.stream(dev)))
+
+
+def read_kv8(slots: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
+             vpool: torch.Tensor, vscale: torch.Tensor,
+             out_dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+    """(keys, values) (rows, H, d) that the cache holds at ``slots`` ((rows,)
+    int64, any order); rows whose slot is outside the pool become 0."""
+    dev = N.require_gpu(slots, kpool, kscale, vpool, vscale, what="read_kv8")
+    P, H, n, d, fmt = _check_pools(kpool, kscale, vpool, vscale)
+    rows = slots.numel()
+    _want(slots, "slots", torch.int64, (rows,))
+    dt = N.dtype_code(out_dtype)
+    k = torch.empty(rows, H, d, dtype=out_dtype, device=dev)
+    v = torch.empty_like(k)
+    with _On(dev):
+        N.check(N.lib().qkv_kv8_read(
+            slots.data_ptr(), rows, H, d, fmt, kpool.data_ptr(), kscale.data_ptr(),
+            vpool.data_ptr(), vscale.data_ptr(), P, n, k.data_ptr(), v.data_ptr(), dt,
+            N.stream(dev)))
+    return k, v
+
+
+def attention_kv8(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
+                  vpool: torch.Tensor, vscale: torch.Tensor, table: torch.Tensor,
+                  kv_lens: torch.Tensor, q_start: Optional[torch.Tensor] = None,
+                  q_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                  causal: bool = False, out_dtype: torch.dtype = torch.float32,
+                  max_q_len: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of query rows (rows, Hq, d; fp32, fp16 or bf16, any row and head
+    strides) over each request's first ``kv_lens[b]`` cached tokens.
+
+    Request b's rows are ``q_start[b] ... + q_lens[b]`` (without q_lens up to the
+    next request's; without q_start the rows are split evenly).  ``causal``
+    places query i of q_len at token kv_len - q_len + i.  Queries that see no
+    token give 0; rows of no request keep what ``out`` holds (0 where this
+    call makes it).  Head h reads kv head h // (Hq // H).
+
+    ``max_q_len``: the longest request's rows where the caller knows it (1 in a
+    decode step); it picks the kernels, not the result.  ``workspace`` (uint8,
+    :func:`attention_kv8_workspace_bytes`) must belong to one call at a time."""
+    dev = N.require_gpu(q, kpool, kscale, vpool, vscale, table, kv_lens, q_start, q_lens, out,
+                        workspace, what="attention_kv8")
+    P, H, n, d, fmt = _check_pools(kpool, kscale, vpool, vscale)
+    if q.dim() != 3 or q.shape[2] != d or q.shape[1] == 0 or q.shape[1] % H != 0:
+        raise ValueError(f"queries {tuple(q.shape)} do not match the cache (rows, a multiple of "
+                         f"{H} heads, {d})")
+    rows, Hq, _ = q.shape
+    if table.dim() != 2:
+        raise ValueError("page table must be a 2-D int32 tensor")
+    B, width = table.shape
+    _want(table, "page table", torch.int32)
+    _want(kv_lens, "kv_lens", torch.int32, (B,))
+    if q_start is not None:
+        _want(q_start, "q_start", torch.int32, (B + 1,))
+    elif q_lens is not None:
+        raise ValueError("q_lens needs q_start")
+    elif B == 0 or rows % B != 0:
+        raise ValueError(f"without q_start the rows ({rows}) must be a multiple of the "
+                         f"requests ({B})")
+    if q_lens is not None:
+        _want(q_lens, "q_lens", torch.int32, (B,))
+    if out is None:
+        make = torch.empty if q_start is None else torch.zeros
+        out = make(rows, Hq, d, dtype=out_dtype, device=dev)
+    else:
+        _want(out, "out", out.dtype, (rows, Hq, d))
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    longest = rows // max(B, 1) if q_start is None else rows
+    if max_q_len is not None:
+        longest = max(0, min(longest, int(max_q_len)))
+    q = _dense_last(q)
+    if workspace is None:
+        workspace = torch.empty(attention_kv8_workspace_bytes(B, rows, Hq, H, d, longest),
+                                dtype=torch.uint8, device=dev)
+    else:
+        _want(workspace, "workspace", torch.uint8)
+    with _On(dev):
+        N.check(N.lib().qkv_kv8_attention(
+            q.data_ptr(), N.dtype_code(q.dtype), q.stride(0), q.stride(1), rows,
+            kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(), vscale.data_ptr(), fmt, P, n,
+            table.data_ptr(), width, N.ptr(q_start), N.ptr(q_lens), kv_lens.data_ptr(), B, Hq, H,
+            d, longest, float(scale), 1 if causal else 0, out.data_ptr(),
+            N.dtype_code(out.dtype), workspace.data_ptr(), workspace.numel(), N.stream(dev)))
+    return out
+
+
+def attention_kv8_workspace_bytes(B: int, rows: int, Hq: int, H: int, d: int,
+                                  max_q_len: int) -> int:
+    """Bytes of the workspace that attention_kv8 needs at these sizes."""
+    return N.lib().qkv_kv8_attention_workspace_bytes(B, rows, Hq, H, d, max_q_len)
+
+
+class PagedKV8Store:
+    """Pools, page table and free list of a batch of B requests, on the device.
+
+    A step::
+
+        plan = store.plan(new_lens, rows)          # who gets how many tokens
+        store.append(k, v, plan)                   # (rows, H, d)
+        out = store.attention(q, plan)             # (rows, Hq, d), causal
+        store.release(done)                        # finished requests' pages
+
+    ``code`` is "int8" or "fp8" (float8 e4m3).  Nothing here reads a length back
+    to the host, so a step can be captured; :meth:`grow` adds pages."""
+
+    def __init__(self, B: int, H: int, d: int, num_pages: int, device,
+                 page_tokens: int = PAGE_TOKENS, pages_per_seq: Optional[int] = None,
+                 code: str = "int8"):
+        if code not in CODE_DTYPES:
+            raise ValueError(f"code {code!r} must be one of {tuple(CODE_DTYPES)}")
+        if d not in (64, 96, 128):
+            raise ValueError(f"the 8-bit cache runs head_dim 64, 96 or 128; got {d}")
+        if page_tokens not in PAGE_SIZES:
+            raise ValueError(f"page_tokens {page_tokens} must be one of {PAGE_SIZES}")
+        if B < 1 or H < 1 or num_pages < 1:
+            raise ValueError(f"need at least one request, head and page; got {B}, {H}, {num_pages}")
+        self.B, self.H, self.d, self.pt, self.code = B, H, d, page_tokens, code
+        dev, nb = torch.device(device), page_tokens // BLOCK_TOKENS
+        self.kpool = torch.zeros(num_pages, H, page_tokens, d, dtype=torch.int8,
+                                 device=dev).view(CODE_DTYPES[code])
+        self.vpool = torch.zeros(num_pages, H, nb, d, BLOCK_TOKENS, dtype=torch.int8,
+                                 device=dev).view(CODE_DTYPES[code])
+        self.kscale = torch.zeros(num_pages, H, nb, dtype=torch.float32, device=dev)
+        self.vscale = torch.zeros_like(self.kscale)
+        self.table = torch.zeros(B, pages_per_seq or num_pages, dtype=torch.int32, device=dev)
+        self.lens = torch.zeros(B, dtype=torch.int32, device=dev)
+        # the lowest page is handed out first
+        self.free = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=dev)
+        self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=dev)
+        self.device = self.lens.device
+
+    @property
+    def num_pages(self) -> int:
+        return self.kpool.shape[0]
+
+    @property
+    def pages_per_seq(self) -> int:
+        return self.table.shape[1]
+
+    def pools(self) -> dict:
+        return dict(kpool=self.kpool, kscale=self.kscale, vpool=self.vpool, vscale=self.vscale)
+
+    def plan(self, new_lens: torch.Tensor, rows: int, max_q_len: Optional[int] = None,
+             out: Optional[PagePlan] = None) -> PagePlan:
+        """plan_pages for this step's ``new_lens`` ((B,) int32, device); the store's
+        lengths, table and free list move on.  ``out`` takes the plan of an earlier
+        step of the same ``rows`` (a captured step keeps one)."""
+        if out is None:
+            out = PagePlan.empty(self.B, rows, self.device, self.lens, self.free_count, max_q_len)
+        elif out.kv_lens is not self.lens or out.free_count is not self.free_count:
+            raise ValueError("out must be a plan that this store made")
+        elif max_q_len is not None:
+            out.max_q_len = max_q_len
+        return plan_pages(self.table, self.lens, new_lens, self.free, self.free_count, rows,
+                          self.pt, out=out)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, plan: PagePlan) -> None:
+        append_kv8(k, v, plan.slots, **self.pools())
+
+    def read(self, slots: torch.Tensor, out_dtype: torch.dtype = torch.float32):
+        return read_kv8(slots, **self.pools(), out_dtype=out_dtype)
+
+    def attention(self, q: torch.Tensor, plan: PagePlan, scale: Optional[float] = None,
+                  causal: bool = True, out_dtype: torch.dtype = torch.float32,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return attention_kv8(q, **self.pools(), table=self.table, kv_lens=plan.kv_lens,
+                             q_start=plan.q_start, q_lens=plan.q_lens, scale=scale, causal=causal,
+                             out_dtype=out_dtype, max_q_len=plan.max_q_len, out=out)
+
+    def release(self, done: Optional[torch.Tensor] = None) -> None:
+        """Finished requests' pages back to the pool (all requests' without ``done``)."""
+        if done is None:
+            done = torch.ones(self.B, dtype=torch.bool, device=self.device)
+        release_pages(self.table, self.lens, done, self.free, self.free_count, self.pt)
+
+    def grow(self, num_pages: int, pages_per_seq: Optional[int] = None) -> None:
+        """At least ``num_pages`` pages in the pool and ``pages_per_seq`` in the
+        table (new tensors: a captured step has to be captured again)."""
+        old, more = self.num_pages, num_pages - self.num_pages
+        if more > 0:
+            for name in ("kpool", "vpool", "kscale", "vscale"):
+                t = getattr(self, name)
+                new = torch.zeros(num_pages, *t.shape[1:], device=self.device,
+                                  dtype=torch.int8 if t.element_size() == 1 else t.dtype)
+                new = new.view(t.dtype)
+                new[:old].view(torch.uint8).copy_(t.view(torch.uint8))
+                setattr(self, name, new)
+            # the new pages go under the free ones: [new pages, old free list]
+            ids = torch.arange(num_pages - 1, old - 1, -1, dtype=torch.int32, device=self.device)
+            self.free = torch.cat([ids, self.free])
+            self.free_count += more
+        if pages_per_seq is not None and pages_per_seq > self.pages_per_seq:
+            pad = torch.zeros(self.B, pages_per_seq - self.pages_per_seq, dtype=torch.int32,
+                              device=self.device)
+            self.table = torch.cat([self.table, pad], 1)
+
+    def to(self, device) -> None:
+        self.device = torch.device(device)
+        for name in ("kpool", "vpool", "kscale", "vscale", "table", "lens", "free", "free_count"):
+            setattr(self, name, getattr(self, name).to(self.device))
+        self.device = self.lens.device
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size()
+                   for t in (self.kpool, self.kscale, self.vpool, self.vscale))
+
+
+class PagedKV8Engine:
+    """The engine interface (QuashKVEngine: append / attention / clear over B
+    sequences of one length) on the 8-bit paged store.  No rotation, codebook or
+    seed: ``key_bits`` and ``value_bits`` are 8."""
+
+    def __init__(self, head_dim: int = 128, device=None, num_pages: int = 0,
+                 page_tokens: int = PAGE_TOKENS, code: str = "int8"):
+        if head_dim not in (64, 96, 128):
+            raise ValueError(f"the 8-bit cache runs head_dim 64, 96 or 128; got {head_dim}")
+        if code not in CODE_DTYPES:
+            raise ValueError(f"code {code!r} must be one of {tuple(CODE_DTYPES)}")
+        if page_tokens not in PAGE_SIZES:
+            raise ValueError(f"page_tokens {page_tokens} must be one of {PAGE_SIZES}")
+        self.head_dim, self.key_bits, self.value_bits = head_dim, 8, 8
+        self.device = _default_device(device)
+        self.initial_pages, self.page_tokens, self.code = num_pages, page_tokens, code
+        self._store: Optional[PagedKV8Store] = None
+        self._total_tokens = 0
+        self._appends = 0
+
+    def append(self, keys: torch.Tensor, values: torch.Tensor) -> None:
+        """Quantise (B, H, S, d) keys / values into the pages behind the cached ones."""
+        dev = N.require_gpu(keys, values, what="PagedKV8Engine.append")
+        if keys.dim() != 4 or keys.shape != values.shape or keys.shape[-1] != self.head_dim:
+            raise ValueError(
+                f"Expected keys and values of shape (batch, n_heads, seq_len, {self.head_dim}); "
+                f"got {tuple(keys.shape)} and {tuple(values.shape)}")
+        B, H, S, d = keys.shape
+        n, T = self.page_tokens, self._total_tokens
+        st = self._store
+        if st is not None and ((st.B, st.H) != (B, H) or st.device != dev):
+            if T:
+                raise ValueError(f"append shape (B={B}, H={H}) on {dev} does not match the cache "
+                                 f"(B={st.B}, H={st.H}) on {st.device}")
+            st = self._store = None  # empty (cleared): any shape
+        if B == 0 or H == 0:
+            raise ValueError(f"need at least one sequence and head; got {tuple(keys.shape)}")
+        need = -(-(T + S) // n)      # pages a sequence
+        if st is None:
+            st = self._store = PagedKV8Store(B, H, d, max(self.initial_pages, B * need, 1), dev, n,
+                                             max(need, 1), self.code)
+        if B * need > st.num_pages or need > st.pages_per_seq:
+            st.grow(max(2 * st.num_pages, B * need) if B * need > st.num_pages else st.num_pages,
+                    max(2 * st.pages_per_seq, need))
+        if keys.dtype != values.dtype or keys.dtype not in (torch.float32, torch.float16,
+                                                            torch.bfloat16):
+            keys, values = keys.float(), values.float()
+        if S > 0:
+            new = torch.full((B,), S, dtype=torch.int32, device=dev)
+            plan = st.plan(new, B * S, max_q_len=S)
+            st.append(keys.transpose(1, 2).reshape(B * S, H, d),
+                      values.transpose(1, 2).reshape(B * S, H, d), plan)
+        self._total_tokens += S
+        self._appends += 1
+
+    def attention(self, queries: torch.Tensor, scale: Optional[float] = None,
+                  causal: bool = False, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """Attention of (B, Hq, Q, d) queries over every cached token, Hq a
+        multiple of the kv heads; causal: query i sits at token T - Q + i."""
+        if self._total_tokens == 0:
+            raise ValueError("No compressed KV blocks in cache. Call append() first.")
+        st = self._store
+        N.require_gpu(queries, what="PagedKV8Engine.attention")
+        if (queries.dim() != 4 or queries.shape[0] != st.B or queries.shape[3] != self.head_dim
+                or queries.shape[1] % st.H != 0):
+            raise ValueError(f"queries {tuple(queries.shape)} do not match the cache "
+                             f"(B={st.B}, kv heads={st.H}, head_dim={self.head_dim})")
+        B, Hq, Q, d = queries.shape
+        q = queries.transpose(1, 2).reshape(B * Q, Hq, d)
+        if q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            q = q.float()
+        out = attention_kv8(q, **st.pools(), table=st.table, kv_lens=st.lens, scale=scale,
+                            causal=causal, out_dtype=out_dtype)
+        return out.view(B, Q, Hq, d).transpose(1, 2).contiguous()
+
+    def clear(self) -> None:
+        if self._store is not None:
+            self._store.release()
+        self._total_tokens = self._appends = 0
+
+    @property
+    def store(self) -> Optional[PagedKV8Store]:
+        return self._store
+
+    @property
+    def total_tokens(self) -> int:
+        return self._total_tokens
+
+    @property
+    def num_blocks(self) -> int:
+        return self._appends
+
+    def compression_ratio(self, original_dtype: torch.dtype = torch.float16) -> float:
+        """Bits of a token's K and V in ``original_dtype`` over those held: 8 a
+        value and an fp32 scale for each half of a 16-token block."""
+        if self._total_tokens == 0:
+            return 1.0
+        bits = 2 * (8 * self.head_dim + 32 / BLOCK_TOKENS)
+        return 2 * self.head_dim * torch.finfo(original_dtype).bits / bits
+
+    def actual_memory_bytes(self) -> int:
+        """Bytes of the codes and scales of the cached tokens."""
+        if self._total_tokens == 0:
+            return 0
+        T, st = self._total_tokens, self._store
+        return st.B * st.H * 2 * (T * self.head_dim + 4 * (-(-T // BLOCK_TOKENS)))
+
+    def to(self, device) -> "PagedKV8Engine":
+        self.device = torch.device(device)
+        if self._store is not None:
+            self._store.to(device)
+        return self
+
+    def __repr__(self) -> str:
+        pages = 0 if self._store is None else self._store.num_pages
+        return (f"PagedKV8Engine(head_dim={self.head_dim}, code={self.code}, "
+                f"cached_tokens={self._total_tokens}, pages={pages}, device={self.device})")
