@@ -1,15 +1,47 @@
 // Attention of a ragged batch of queries over the 8-bit paged cache (qkv_kv8.h).
+//
+// Mathematics.  With block scales ks, vs (16 tokens and a head each), codes kc, vc and
+// c = scale log2(e):  y_t = c ks (q . kc_t) + log2(vs),  p'_t = 2^(y_t - m),
+//   out = (sum p'_t vc_t) / (sum p'_t / vs):
+// the value scale enters the softmax's exponent, where it costs an addend of a
+// multiply-add instead of a product per weight, and the running maximum m is taken
+// over y, so that a weight's 16 bits are spent where |p v| is large.  Codes are exact
+// in f16, and so are 16-bit queries times a power of two per row; fp32 queries, and
+// the weights of fp32 results, are f16 pairs hi + lo (22 bits).
+//
+// Layout.  Scores are S^T = K Q^T on v_mfma_f32_16x16x32_f16 (rows tokens, columns the
+// query rows that share a kv head), values O^T = V^T P^T.  Row m of score tile i is token
+// 16 (m / 4) + 4 i + m % 4 of 64, so that lane (n, g) holds the scores of query row n and of
+// all 16 tokens of block g: one pair of scales per lane, and its weights are, as they
+// stand, the B operand of the value product, whose A operand is 16 bytes of a V block.
+// Nothing of K, V or P passes through LDS.
 #include <algorithm>
 
 #include "qkv_kv8.h"
 
 namespace {
 
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+constexpr int kStep = 64;        // tokens of a wave's step
+constexpr int kRows = 16;        // query rows of a decode tile
+constexpr int kWaves = 4;
+constexpr int kThr = 64 * kWaves;
+constexpr float kHead = 8.f;     // the running maximum may lag by 2^8 before a rescale
+constexpr float kUp = 7.f;       // largest weight in f16: 2^(kUp + kHead) at most, 2^kUp at least,
+                                 // so that f16's smallest step is 2^-31 of it
+constexpr float kLog2e = 1.44269504088896340736f;
+
 struct Att {
   const void* q;
   int64_t q_ts, q_hs;
-  int32_t q_dtype;
-  int64_t rows;
+  int32_t q_dtype, q_vec;
+  int32_t rows;
   const uint8_t* kpool;
   const float* kscale;
   const uint8_t* vpool;
@@ -20,99 +52,568 @@ struct Att {
   const int32_t* q_start;
   const int32_t* q_lens;
   const int32_t* kv_lens;
-  int32_t B, Hq, H, uniform_q;
+  int32_t B, Hq, H, G, uniform_q;
   float scale;
   int32_t causal;
   void* out;
-  int32_t out_dtype;
+  int32_t out_dtype, out_vec;
+  int32_t target;   // pieces that a launch aims at, per kv head
+  int32_t nslots;   // partial results that the workspace holds
+  float* part_o;    // [slot][row][D]
+  float* part_ml;   // [slot][row][2]
 };
 
-template <bool FP8>
-__device__ __forceinline__ float value_of(uint32_t code) {
-  if constexpr (FP8)
-    return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(code & 0xffu), 0);
-  else
-    return static_cast<float>(static_cast<int8_t>(code));
+// Request b's rows in this launch and its tokens.
+struct Req {
+  int32_t q0, ql, kv;
+};
+
+__device__ __forceinline__ Req request(const Att& A, int b) {
+  Req r;
+  if (A.q_start == nullptr) {
+    r.q0 = b * A.uniform_q;
+    r.ql = A.uniform_q;
+  } else {
+    r.q0 = A.q_start[b];
+    r.ql = A.q_lens ? A.q_lens[b] : A.q_start[b + 1] - r.q0;
+    r.ql = min(max(r.ql, 0), A.rows);
+  }
+  const int64_t room = int64_t(A.width) << A.lg, kv = A.kv_lens[b];
+  r.kv = static_cast<int32_t>(kv < 0 ? 0 : kv < room ? kv : room);
+  return r;
 }
 
-// A wave per (request, query, query head).
-template <int D, bool FP8>
-__global__ __launch_bounds__(64) void attend_rows(Att A) {
-  __shared__ float qs[D], ps[64];
-  const int lane = threadIdx.x, hq = blockIdx.y, h = hq / (A.Hq / A.H);
-  const int64_t r = blockIdx.x;
-  int b;
-  int64_t i, qlen;
-  if (A.q_start == nullptr) {
-    b = static_cast<int>(r / A.uniform_q);
-    i = r - int64_t(b) * A.uniform_q;
-    qlen = A.uniform_q;
-  } else {
-    if (r < A.q_start[0] || r >= A.q_start[A.B]) return;
-    int lo = 0, hi = A.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (A.q_start[mid] <= r) lo = mid;
-      else hi = mid;
-    }
-    b = lo;
-    i = r - A.q_start[b];
-    qlen = A.q_lens ? A.q_lens[b] : A.q_start[b + 1] - A.q_start[b];
-    if (i >= qlen) return;
+// One workgroup's part of the launch: steps [s0, s1) of tile `rt` of request b.
+struct Piece {
+  Req r;
+  int32_t b, rt, s0, s1;
+  int32_t slot;   // of its partial result (of the tile's first one), -1: not cut
+  int32_t parts;  // pieces of the tile
+};
+
+struct Shared {
+  int64_t sum[kWaves];
+  int32_t scan[kWaves][3];
+  int32_t found[3];  // b, piece (tile) within the request, first slot of the request
+};
+
+// Piece number `want` of the launch, or with TILE the whole of tile `want`.  A tile's steps are cut into pieces of C, the
+// smallest C (whole rounds of the four waves) that keeps the launch near its target; so
+// long requests are shared by many workgroups and short ones are not cut.  Every workgroup
+// finds its own piece by prefix sums over the requests: no launch and no host knowledge
+// of the lengths is needed.
+template <bool TILE>
+__device__ __forceinline__ bool locate(const Att& A, int want, Shared& sh, Piece& P) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto cost = [&](const Req& r, int& tiles, int& steps) {
+    tiles = (r.ql * A.G + kRows - 1) / kRows;
+    steps = max(1, (r.kv + kStep - 1) / kStep);
+  };
+  int64_t sum = 0;
+  for (int b = tid; b < A.B; b += kThr) {
+    int tiles, steps;
+    cost(request(A, b), tiles, steps);
+    sum += int64_t(tiles) * steps;
   }
-  const int64_t n = int64_t(1) << A.lg;
-  int64_t kv = A.kv_lens[b];
-  if (kv > int64_t(A.width) * n) kv = int64_t(A.width) * n;
-  const int64_t end = A.causal ? kv - qlen + i + 1 : kv;
-  for (int c = lane; c < D; c += 64)
-    qs[c] = qkv_load(A.q, r * A.q_ts + hq * A.q_hs + c, A.q_dtype);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane == 0) sh.sum[wave] = sum;
+  if (tid == 0) sh.found[0] = -1;
   __syncthreads();
-  float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
-  for (int64_t t0 = 0; t0 < end; t0 += 64) {
-    const int64_t t = t0 + lane;
-    float x = -INFINITY, vs = 0.f;
-    int64_t page = -1;
-    if (t < end) page = A.table[int64_t(b) * A.width + (t >> A.lg)];
-    const bool ok = page >= 0 && page < A.npages;
-    const int64_t row = ok ? (page * A.H + h) * n + (t & (n - 1)) : 0;
-    if (ok) {
-      float s = 0.f;
-      const uint8_t* k = A.kpool + row * D;
-      for (int c = 0; c < D; ++c) s = fmaf(qs[c], value_of<FP8>(k[c]), s);
-      x = s * A.kscale[row >> 4] * A.scale;
-      vs = A.vscale[row >> 4];
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) sum += sh.sum[w];
+  int64_t c64 = (sum + A.target - 1) / A.target;
+  c64 = (c64 + kWaves - 1) / kWaves * kWaves;
+  const int C = static_cast<int>(c64 < kWaves ? kWaves : c64 > INT32_MAX / 2 ? INT32_MAX / 2 : c64);
+  int base[3] = {0, 0, 0};  // pieces, pieces of cut tiles, tiles
+  for (int b0 = 0; b0 < A.B; b0 += kThr) {
+    const int b = b0 + tid;
+    int v[3] = {0, 0, 0}, own[3];
+    if (b < A.B) {
+      int tiles, steps;
+      cost(request(A, b), tiles, steps);
+      const int per = (steps + C - 1) / C;
+      v[0] = tiles * per;
+      v[1] = per > 1 ? v[0] : 0;
+      v[2] = tiles;
     }
-    const float mn = fmaxf(m, qkv_wave_max(x));
-    if (mn == -INFINITY) continue;
-    const float p = ok ? expf(x - mn) : 0.f, f = expf(m - mn);
-    l = l * f + qkv_wave_sum(p);
-    m = mn;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) own[k] = v[k];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const int u = __shfl_up(v[k], o, 64);
+        if (lane >= o) v[k] += u;
+      }
+    if (lane == 63)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) sh.scan[wave][k] = v[k];
     __syncthreads();
-    ps[lane] = ok ? p * vs : 0.f;
+    int tot[3] = {0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        if (w < wave) v[k] += sh.scan[w][k];
+        tot[k] += sh.scan[w][k];
+      }
+    constexpr int BY = TILE ? 2 : 0;
+    const int end = base[BY] + v[BY], first = end - own[BY];
+    if (want >= first && want < end) {
+      sh.found[0] = b;
+      sh.found[1] = want - first;
+      sh.found[2] = base[1] + v[1] - own[1];
+    }
     __syncthreads();
-    o[0] *= f;
-    o[1] *= f;
-    for (int j = 0; j < 64; ++j) {
-      const float pj = ps[j];
-      const int64_t rj = __shfl(static_cast<long long>(row), j, 64);
-      if (!__shfl(ok ? 1 : 0, j, 64)) continue;
-      const uint8_t* v = A.vpool + (rj & ~int64_t(15)) * D + (rj & 15);
-      for (int y = 0; y < 2; ++y)
-        if (lane + 64 * y < D)
-          o[y] = fmaf(pj, value_of<FP8>(v[(lane + 64 * y) * kBlk]), o[y]);
+    if (sh.found[0] >= 0) break;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) base[k] += tot[k];
+  }
+  P.b = __builtin_amdgcn_readfirstlane(sh.found[0]);
+  if (P.b < 0) return false;
+  const int in = __builtin_amdgcn_readfirstlane(sh.found[1]);
+  P.r = request(A, P.b);
+  int tiles, steps;
+  cost(P.r, tiles, steps);
+  P.parts = (steps + C - 1) / C;
+  P.rt = TILE ? in : in / P.parts;
+  const int part = TILE ? 0 : in - P.rt * P.parts;
+  P.s0 = part * C;
+  P.s1 = TILE ? steps : min(steps, P.s0 + C);
+  P.slot = -1;
+  if (P.parts > 1)
+    P.slot = __builtin_amdgcn_readfirstlane(sh.found[2]) + P.rt * P.parts + part;
+  return true;
+}
+
+// Two codes as f16, of bytes 0 and 1 (or 2 and 3) of a dword.
+template <bool FP8>
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FP8) {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true));
+  } else {
+    // 0x6400 | u is the f16 1024 + u; u = code + 128
+    const uint32_t u = w ^ 0x80808080u;
+    const v2h off = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
+    lo = __builtin_bit_cast(
+        uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off);
+    hi = __builtin_bit_cast(
+        uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off);
+  }
+}
+
+template <bool FP8>
+__device__ __forceinline__ v8h widen8(uint32_t a, uint32_t b) {
+  v4u r;
+  uint32_t x, y;
+  widen<FP8>(a, x, y);
+  r[0] = x;
+  r[1] = y;
+  widen<FP8>(b, x, y);
+  r[2] = x;
+  r[3] = y;
+  return __builtin_bit_cast(v8h, r);
+}
+
+__device__ __forceinline__ uint32_t pk(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2h));
+}
+
+// x as f16 hi + lo, both rounded to nearest.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pk(a, b);
+  const v2h h = __builtin_bit_cast(v2h, hi);
+  lo = pk(a - static_cast<float>(h[0]), b - static_cast<float>(h[1]));
+}
+
+__device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Eight consecutive query values from element `at`.
+__device__ __forceinline__ void load8(const Att& A, int64_t at, float* x) {
+  if (A.q_vec && A.q_dtype == QKV_F32) {
+    const v4f* p = reinterpret_cast<const v4f*>(static_cast<const float*>(A.q) + at);
+    const v4f a = p[0], b = p[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = a[j];
+      x[4 + j] = b[j];
+    }
+  } else if (A.q_vec) {
+    const v4u w = *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(A.q) + at);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint16_t h = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+      x[j] = A.q_dtype == QKV_BF16 ? qkv_bf16_to_f32(h)
+                                   : static_cast<float>(__builtin_bit_cast(_Float16, h));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = qkv_load(A.q, at + j, A.q_dtype);
+  }
+}
+
+// Eight consecutive results to element `at` of out.
+__device__ __forceinline__ void store8(void* out, int64_t at, const float* x, int dt, bool vec) {
+  if (!vec) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) qkv_store(out, at + j, x[j], dt);
+  } else if (dt == QKV_F32) {
+    v4f* p = reinterpret_cast<v4f*>(static_cast<float*>(out) + at);
+    p[0] = v4f{x[0], x[1], x[2], x[3]};
+    p[1] = v4f{x[4], x[5], x[6], x[7]};
+  } else if (dt == QKV_F16) {
+    *reinterpret_cast<v4u*>(static_cast<uint16_t*>(out) + at) =
+        v4u{pk(x[0], x[1]), pk(x[2], x[3]), pk(x[4], x[5]), pk(x[6], x[7])};
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = qkv_f32_to_bf16(x[2 * j]) | uint32_t(qkv_f32_to_bf16(x[2 * j + 1])) << 16;
+    *reinterpret_cast<v4u*>(static_cast<uint16_t*>(out) + at) = v4u{w[0], w[1], w[2], w[3]};
+  }
+}
+
+// d index of the first of the 8 coordinates that lane group g holds in product step ks
+__host__ __device__ constexpr int dcol(int D, int ks, int g) {
+  return D == 96 && ks == 2 ? 64 + 8 * g : 64 * (ks >> 1) + 16 * g + 8 * (ks & 1);
+}
+
+// A workgroup per (piece, kv head): its waves take every fourth step of 64 tokens and
+// merge through LDS.
+template <int D, bool FP8, bool QLO, bool PLO>
+__global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
+  constexpr int KS = D / 32, NJ = D / 16, NK = (D + 63) / 64;
+  __shared__ Shared sh;
+  __shared__ float red_o[kWaves][kRows][D + 4];
+  __shared__ float red_ml[kWaves][kRows][2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int h = blockIdx.x % A.H;
+  Piece P;
+  if (!locate<false>(A, blockIdx.x / A.H, sh, P)) return;
+
+  // ---- this lane's query row
+  const int rr = P.rt * kRows + n, qi = rr / A.G, gq = rr - qi * A.G;
+  const int64_t row = int64_t(P.r.q0) + qi;
+  const bool live = qi < P.r.ql && row >= 0 && row < A.rows;
+  const int hq = h * A.G + gq;
+  v8h qh[KS], ql[QLO ? KS : 1];
+  float c;  // scores to exponents, without the block's scale
+  {
+    float x[KS][8];
+    float amax = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[ks][j] = 0.f;
+      if (live) load8(A, row * A.q_ts + hq * A.q_hs + dcol(D, ks, g), x[ks]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[ks][j]));
+    }
+    amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+    int ex = 0;
+    if (amax > 0.f && amax < INFINITY) frexpf(amax, &ex);
+    ex = max(ex, -110);
+    const float up = ldexpf(1.f, 10 - ex);  // the row's largest into [2^9, 2^10)
+    c = ldexpf(A.scale * kLog2e, ex - 10);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      v4u hi, lo;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t a, b;
+        split2(x[ks][2 * j] * up, x[ks][2 * j + 1] * up, a, b);
+        hi[j] = a;
+        lo[j] = b;
+      }
+      qh[ks] = __builtin_bit_cast(v8h, hi);
+      if constexpr (QLO) ql[ks] = __builtin_bit_cast(v8h, lo);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  for (int y = 0; y < 2; ++y)
-    if (lane + 64 * y < D)
-      qkv_store(A.out, (r * A.Hq + hq) * D + lane + 64 * y, o[y] * inv, A.out_dtype);
+  // tokens below lim are seen; all rows of the tile see those below lim_all
+  const int lim = !live ? 0 : A.causal ? min(P.r.kv, P.r.kv - P.r.ql + qi + 1) : P.r.kv;
+  int lim_all = live ? lim : INT32_MAX;
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) lim_all = min(lim_all, __shfl_xor(lim_all, o, 64));
+  lim_all = __builtin_amdgcn_readfirstlane(lim_all);
+  const int n_tok = P.r.kv;
+
+  v4f o[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) o[j] = v4f{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+
+  // K and V of the step that follows, in registers
+  v4u kr[4][NK];
+  v4u vr[NJ];
+  float ks_r = 0.f, vs_r = 0.f;
+  const int pg_sh = A.lg - 6;  // steps per page, log2
+  const int32_t* const tab = A.table + int64_t(P.b) * A.width;
+  int pages = 0;   // lane i: the page of this wave's i-th step from p_first on
+  int p_first = 0;
+  const int tok0 = 16 * (n >> 2) + (n & 3);
+  const uint32_t k_off = static_cast<uint32_t>(tok0 * D + 16 * g);
+  const uint32_t k_off2 = static_cast<uint32_t>(tok0 * D + 64 + 8 * g);  // D = 96: 8 bytes each
+  const uint32_t v_off = static_cast<uint32_t>((g * D + n) * 16);
+  auto page_of = [&](int i) {  // i: the wave's step count
+    if (i - p_first >= 64 || i == 0) {
+      p_first = i;
+      const int st = P.s0 + wave + kWaves * (i + lane);
+      pages = st < P.s1 ? tab[st >> pg_sh] : -1;
+    }
+    return __builtin_amdgcn_readlane(pages, i - p_first);
+  };
+  auto row_of = [&](int i, bool& ok) {
+    const int pg = page_of(i);
+    ok = pg >= 0 && pg < A.npages;
+    const int st = P.s0 + wave + kWaves * i;
+    const int64_t t = int64_t(st) * kStep & ((int64_t(1) << A.lg) - 1);
+    return ((int64_t(ok ? pg : 0) * A.H + h) << A.lg) + t;
+  };
+  auto load_k = [&](int64_t row0) {
+    ks_r = A.kscale[(row0 >> 4) + g];
+    vs_r = A.vscale[(row0 >> 4) + g];
+    const uint8_t* const p = A.kpool + row0 * D;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int x = 0; x < NK; ++x) {
+        if (D == 96 && x == 1) {
+          const v2u w = *reinterpret_cast<const v2u*>(p + k_off2 + 4 * i * D);
+          kr[i][x] = v4u{w[0], w[1], 0, 0};
+        } else {
+          kr[i][x] = *reinterpret_cast<const v4u*>(p + k_off + 4 * i * D + 64 * x);
+        }
+      }
+  };
+  auto load_v = [&](int64_t row0) {
+    const uint8_t* const p = A.vpool + row0 * D;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      vr[j] = *reinterpret_cast<const v4u*>(p + v_off + 256 * j);
+  };
+
+  const int steps = max(0, (P.s1 - P.s0 - wave + kWaves - 1) / kWaves);
+  bool ok = false;
+  int64_t row0 = 0;
+  if (steps > 0) {
+    row0 = row_of(0, ok);
+    load_k(row0);
+    load_v(row0);
+  }
+#pragma unroll 1
+  for (int it = 0; it < steps; ++it) {
+    const int t0 = (P.s0 + wave + kWaves * it) * kStep;
+    // ---- scores
+    v4f s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const v4u w = kr[i][ks >> 1];
+        const v8h a = ks & 1 ? widen8<FP8>(w[2], w[3]) : widen8<FP8>(w[0], w[1]);
+        s[i] = mfma(a, qh[ks], s[i]);
+        if constexpr (QLO) s[i] = mfma(a, ql[ks], s[i]);
+      }
+    }
+    const float ck = c * ks_r, vs = vs_r;
+    const bool pos = vs > 0.f;
+    const float lv = pos ? __builtin_amdgcn_logf(vs) : 0.f;
+    const float iv = pos ? __builtin_amdgcn_rcpf(vs) : 1.f;
+    const bool was_ok = ok;
+    const bool more = it + 1 < steps;
+    if (more) {
+      row0 = row_of(it + 1, ok);
+      load_k(row0);
+    }
+    // ---- weights
+    float y[16], top = -INFINITY;
+    const bool edge = t0 + kStep > lim_all || !was_ok;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) y[k] = fmaf(s[k >> 2][k & 3], ck, lv);
+    if (edge) {
+      const int left = was_ok ? lim - t0 - 16 * g : 0;  // of this lane's 16 tokens
+#pragma unroll
+      for (int k = 0; k < 16; ++k) y[k] = k < left ? y[k] : -INFINITY;
+      // codes behind the cached tokens may be anything
+      const int keep = was_ok ? n_tok - t0 - 16 * g : 0;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int k = keep - 4 * x;
+        const uint32_t mask = k >= 4 ? ~0u : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) vr[j][x] &= mask;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) top = fmaxf(top, y[k]);
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (__any(top > m + kHead || m == -INFINITY)) {
+      const float mn = fmaxf(m, top);
+      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) o[j] *= f;
+    }
+    const float ref = m == -INFINITY ? 0.f : m - kUp;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      y[k] = __builtin_amdgcn_exp2f(y[k] - ref);
+      sum += y[k];
+    }
+    l = fmaf(sum, iv, l);
+    v8h ph[2], pl[PLO ? 2 : 1];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      v4u hi, lo;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t a, b = 0;
+        if constexpr (PLO) split2(y[8 * u + 2 * j], y[8 * u + 2 * j + 1], a, b);
+        else a = pk(y[8 * u + 2 * j], y[8 * u + 2 * j + 1]);
+        hi[j] = a;
+        lo[j] = b;
+      }
+      ph[u] = __builtin_bit_cast(v8h, hi);
+      if constexpr (PLO) pl[u] = __builtin_bit_cast(v8h, lo);
+    }
+    // ---- values
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const v8h a = widen8<FP8>(vr[j][2 * u], vr[j][2 * u + 1]);
+        o[j] = mfma(a, ph[u], o[j]);
+        if constexpr (PLO) o[j] = mfma(a, pl[u], o[j]);
+      }
+    if (more) load_v(row0);
+  }
+
+  // ---- the waves' results to LDS: lane (n, g) has coordinates 16 j + 4 g + r of row n
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+    *reinterpret_cast<v4f*>(&red_o[wave][n][16 * j + 4 * g]) = o[j];
+  if (g == 0) {
+    red_ml[wave][n][0] = m;
+    red_ml[wave][n][1] = l;
+  }
+  __syncthreads();
+  constexpr int PER = D / 8;  // threads of a row
+  if (tid < kRows * PER) {
+    const int r = tid / PER, d0 = 8 * (tid % PER);
+    float M = -INFINITY, L = 0.f, x[8] = {};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, red_ml[w][r][0]);
+    const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(red_ml[w][r][0] - ref);
+      L = fmaf(red_ml[w][r][1], f, L);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = fmaf(red_o[w][r][d0 + j], f, x[j]);
+    }
+    const int rr2 = P.rt * kRows + r, qi2 = rr2 / A.G;
+    const int64_t row2 = int64_t(P.r.q0) + qi2;
+    if (qi2 < P.r.ql && row2 >= 0 && row2 < A.rows) {
+      if (P.slot < 0) {
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= inv;
+        store8(A.out, (row2 * A.Hq + h * A.G + rr2 - qi2 * A.G) * D + d0, x, A.out_dtype, A.out_vec);
+      } else if (int64_t(P.slot) * A.H + h < A.nslots) {
+        const int64_t at = (int64_t(P.slot) * A.H + h) * kRows + r;
+        store8(A.part_o, at * D + d0, x, QKV_F32, true);
+        if (d0 == 0) {
+          A.part_ml[2 * at] = M;
+          A.part_ml[2 * at + 1] = L;
+        }
+      }
+    }
+  }
+}
+
+// Joins the pieces of a cut tile: a wave per query row.
+template <int D>
+__global__ __launch_bounds__(kThr) void join8(Att A) {
+  __shared__ Shared sh;
+  const int lane = threadIdx.x & 63, h = blockIdx.x % A.H;
+  Piece P;
+  if (!locate<true>(A, blockIdx.x / A.H, sh, P) || P.parts == 1) return;
+  const int r = blockIdx.y * kWaves + (threadIdx.x >> 6);
+  const int rr = P.rt * kRows + r, qi = rr / A.G;
+  const int64_t row = int64_t(P.r.q0) + qi;
+  if (qi >= P.r.ql || row < 0 || row >= A.rows || P.slot < 0) return;
+  const int c = min(2 * lane, D - 2);
+  float M = -INFINITY, L = 0.f, x0 = 0.f, x1 = 0.f;
+  for (int i = 0; i < P.parts; i += 4) {
+    float m[4], l[4];
+    v2f v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t slot = int64_t(P.slot + i + u) * A.H + h;
+      const bool on = i + u < P.parts && slot < A.nslots;
+      const int64_t at = (on ? slot : 0) * kRows + r;
+      m[u] = on ? A.part_ml[2 * at] : -INFINITY;
+      l[u] = A.part_ml[2 * at + 1];
+      v[u] = *reinterpret_cast<const v2f*>(A.part_o + at * D + c);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (m[u] == -INFINITY) continue;
+      const float mn = fmaxf(M, m[u]);
+      const float f = __builtin_amdgcn_exp2f(M - mn), e = __builtin_amdgcn_exp2f(m[u] - mn);
+      M = mn;
+      L = fmaf(l[u], e, L * f);
+      x0 = fmaf(v[u][0], e, x0 * f);
+      x1 = fmaf(v[u][1], e, x1 * f);
+    }
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  if (2 * lane < D) {
+    const int64_t at = (row * A.Hq + h * A.G + rr - qi * A.G) * D + c;
+    qkv_store(A.out, at, x0 * inv, A.out_dtype);
+    qkv_store(A.out, at + 1, x1 * inv, A.out_dtype);
+  }
+}
+
+// Pieces that a launch aims at, per kv head: two workgroups per CU.
+int32_t target_of(int32_t H) { return std::max(1, (2 * qkv_num_cus() + H - 1) / H); }
+// Cut tiles have more than C steps each and pieces of C, so they have fewer than
+// 2 total / C <= 2 target pieces.
+int64_t slots_of(int32_t H) { return int64_t(2 * target_of(H) + 1) * H; }
+
+template <int D, bool FP8>
+void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
+  const uint32_t grid = (tiles + A.target) * A.H;
+  if (A.q_dtype == QKV_F32) {
+    if (A.out_dtype == QKV_BF16) decode8<D, FP8, true, false><<<grid, kThr, 0, s>>>(A);
+    else decode8<D, FP8, true, true><<<grid, kThr, 0, s>>>(A);
+  } else {
+    if (A.out_dtype == QKV_BF16) decode8<D, FP8, false, false><<<grid, kThr, 0, s>>>(A);
+    else decode8<D, FP8, false, true><<<grid, kThr, 0, s>>>(A);
+  }
+  if (cut) join8<D><<<dim3(tiles * A.H, kRows / kWaves), kThr, 0, s>>>(A);
 }
 
 }  // namespace
 
 extern "C" int64_t qkv_kv8_attention_workspace_bytes(int32_t B, int64_t rows, int32_t Hq,
                                                      int32_t Hkv, int32_t d, int64_t max_q) {
-  return 256;
+  if (Hkv < 1 || d < 1) return 0;
+  return (slots_of(Hkv) * kRows * (d + 2) * 4 + 255) / 256 * 256;
 }
 
 extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_stride,
@@ -129,10 +630,12 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   if (st != QKV_OK) return st;
   QKV_REQUIRE(qkv_dtype_ok(q_dtype) && qkv_dtype_ok(out_dtype), "unknown element type %d / %d",
               q_dtype, out_dtype);
-  QKV_REQUIRE(Hq >= 1 && Hq <= 65535 && Hq % Hkv == 0,
-              "query heads (%d) must be a multiple of kv heads (%d)", Hq, Hkv);
+  QKV_REQUIRE(Hq >= 1 && Hq % Hkv == 0, "query heads (%d) must be a multiple of kv heads (%d)", Hq,
+              Hkv);
   QKV_REQUIRE(B >= 0 && pages_per_seq >= 1, "bad batch %d or pages_per_seq %d", B, pages_per_seq);
-  QKV_REQUIRE(rows >= 0 && rows < INT32_MAX, "rows must lie in [0, 2^31 - 1); got %lld",
+  const int32_t G = Hq / Hkv;
+  QKV_REQUIRE(rows >= 0 && rows * G < INT32_MAX / 2 && rows * Hq / kRows < (1 << 28),
+              "rows must lie in [0, 2^30 / heads per kv head); got %lld",
               static_cast<long long>(rows));
   if (rows == 0 || B == 0) return QKV_OK;
   QKV_REQUIRE(q_start || !q_lens, "q_lens needs q_start");
@@ -145,17 +648,56 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   QKV_REQUIRE(workspace && qkv_aligned(workspace, 256) &&
                   ws_bytes >= qkv_kv8_attention_workspace_bytes(B, rows, Hq, Hkv, d, max_q),
               "qkv_kv8_attention: workspace too small or not 256-byte aligned");
-  Att A{q, q_row_stride, q_head_stride, q_dtype, rows, static_cast<const uint8_t*>(kpool), kscale,
-        static_cast<const uint8_t*>(vpool), vscale, num_pages, qkv_page_lg(page_tokens), table,
-        pages_per_seq, q_start, q_lens, kv_lens, B, Hq, Hkv, static_cast<int32_t>(rows / B), scale,
-        causal, out, out_dtype};
-  const dim3 grid(static_cast<uint32_t>(rows), Hq);
+  const int qb = q_dtype == QKV_F32 ? 4 : 2, ob = out_dtype == QKV_F32 ? 4 : 2;
+  Att A{};
+  A.q = q;
+  A.q_ts = q_row_stride;
+  A.q_hs = q_head_stride;
+  A.q_dtype = q_dtype;
+  A.q_vec = qkv_aligned(q, 16) && q_row_stride * qb % 16 == 0 && q_head_stride * qb % 16 == 0;
+  A.rows = static_cast<int32_t>(rows);
+  A.kpool = static_cast<const uint8_t*>(kpool);
+  A.kscale = kscale;
+  A.vpool = static_cast<const uint8_t*>(vpool);
+  A.vscale = vscale;
+  A.npages = num_pages;
+  A.lg = qkv_page_lg(page_tokens);
+  A.table = table;
+  A.width = pages_per_seq;
+  A.q_start = q_start;
+  A.q_lens = q_lens;
+  A.kv_lens = kv_lens;
+  A.B = B;
+  A.Hq = Hq;
+  A.H = Hkv;
+  A.G = G;
+  A.uniform_q = static_cast<int32_t>(rows / B);
+  A.scale = scale;
+  A.causal = causal;
+  A.out = out;
+  A.out_dtype = out_dtype;
+  A.out_vec = qkv_aligned(out, 16) && d * ob % 16 == 0;
+  A.target = target_of(Hkv);
+  A.nslots = static_cast<int32_t>(slots_of(Hkv));
+  A.part_o = static_cast<float*>(workspace);
+  A.part_ml = A.part_o + int64_t(A.nslots) * kRows * d;
+  // tiles: a request's last one may be in part empty
+  const int64_t tiles = q_start ? rows * G / kRows + std::min<int64_t>(B, rows)
+                                : int64_t(B) * ((A.uniform_q * G + kRows - 1) / kRows);
+  QKV_REQUIRE((tiles + A.target) * Hkv <= INT32_MAX, "batch of %d requests and %lld rows is too "
+              "large for one call", B, static_cast<long long>(rows));
+  const bool cut = (int64_t(pages_per_seq) << A.lg) > int64_t(kStep) * kWaves;
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define RUN(D)                                                              \
-  if (fmt == QKV_CODES_I8) attend_rows<D, false><<<grid, 64, 0, s>>>(A);    \
-  else attend_rows<D, true><<<grid, 64, 0, s>>>(A);
-  if (d == 128) { RUN(128) } else if (d == 96) { RUN(96) } else { RUN(64) }
-#undef RUN
+  const uint32_t t = static_cast<uint32_t>(tiles);
+  if (fmt == QKV_CODES_I8) {
+    if (d == 128) launch<128, false>(A, t, cut, s);
+    else if (d == 96) launch<96, false>(A, t, cut, s);
+    else launch<64, false>(A, t, cut, s);
+  } else {
+    if (d == 128) launch<128, true>(A, t, cut, s);
+    else if (d == 96) launch<96, true>(A, t, cut, s);
+    else launch<64, true>(A, t, cut, s);
+  }
   QKV_LAUNCHED();
   return QKV_OK;
 }

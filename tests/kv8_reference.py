@@ -118,6 +118,10 @@ def attend(q, k, v, scale, first, q_half_step, weight_half_step, out_half_step):
     * a weight p carries ds and its own rounding; the sums over T tokens 4 sqrt(T) + 8
       fp32 roundings; numerator and denominator each, so twice:
         |d out| <= 2 sum p |v| (ds + weight_half_step + (4 sqrt(T) + 8) 2^-24);
+    * a weight p vs meets an f16 with the largest weight at 2^7 or more: below 2^-14 the
+      steps of an f16 do not shrink, and half a step, 2^-25, is 2^-32 of the largest
+      weight.  Times a code it is at most 2^-32 p_max max |v|, for each of T tokens:
+        |d out| <= T 2^-32 max |v|;
     * the result is rounded once to its type: out_half_step |out|."""
     Q, Hq, d = q.shape
     T, H, _ = k.shape
@@ -138,5 +142,5 @@ def attend(q, k, v, scale, first, q_half_step, weight_half_step, out_half_step):
             out[i, h * (Hq // H):(h + 1) * (Hq // H)] = o
             tol[i, h * (Hq // H):(h + 1) * (Hq // H)] = (
                 2 * e * (ds + weight_half_step + (4 * math.sqrt(n) + 8) * 2.0 ** -24)
-                + out_half_step * o.abs())
+                + n * 2.0 ** -32 * v[:n, h].abs().max() + out_half_step * o.abs())
     return out, tol
