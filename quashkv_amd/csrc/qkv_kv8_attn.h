@@ -1,0 +1,416 @@
+// What decode8 (qkv_kv8_attn.hip) and prefill8 (qkv_kv8_prefill.hip) share.
+#pragma once
+
+#include <algorithm>
+
+#include "qkv_kv8.h"
+
+namespace qkv_kv8 {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+constexpr int kStep = 64;        // tokens of a wave's step
+constexpr int kRows = 16;        // query rows of a decode tile
+constexpr int kPreRows = 128;    // and of a prefill tile
+constexpr int kWaves = 4;
+constexpr int kThr = 64 * kWaves;
+constexpr float kHead = 8.f;     // the running maximum may lag by 2^8 before a rescale
+constexpr float kUp = 7.f;       // largest weight in f16: 2^(kUp + kHead) at most, 2^kUp at least,
+                                 // so that f16's smallest step is 2^-31 of it
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct Att {
+  const void* q;
+  int64_t q_ts, q_hs;
+  int32_t q_dtype, q_vec;
+  int32_t rows;
+  const uint8_t* kpool;
+  const float* kscale;
+  const uint8_t* vpool;
+  const float* vscale;
+  int32_t npages, lg;
+  const int32_t* table;
+  int32_t width;
+  const int32_t* q_start;
+  const int32_t* q_lens;
+  const int32_t* kv_lens;
+  int32_t B, Hq, H, G, uniform_q;
+  float scale;
+  int32_t causal;
+  void* out;
+  int32_t out_dtype, out_vec;
+  int32_t few;      // requests of up to this many rows (queries x G) are decode8's
+  int32_t target;   // pieces that a launch aims at, per kv head
+  int32_t nslots;   // partial results that the workspace holds
+  int32_t* used;    // of them, per kv head, in this launch
+  int4* desc;       // [slot][H]: whose they are
+  float* part_o;    // [slot][H][row][D]
+  float* part_ml;   // [slot][H][row][2]
+};
+
+// Request b's rows in this launch and its tokens.
+struct Req {
+  int32_t q0, ql, kv;
+};
+
+__device__ __forceinline__ Req request(const Att& A, int b) {
+  Req r;
+  if (A.q_start == nullptr) {
+    r.q0 = b * A.uniform_q;
+    r.ql = A.uniform_q;
+  } else {
+    r.q0 = A.q_start[b];
+    r.ql = A.q_lens ? A.q_lens[b] : A.q_start[b + 1] - r.q0;
+    r.ql = min(max(r.ql, 0), A.rows);
+  }
+  const int64_t room = int64_t(A.width) << A.lg, kv = A.kv_lens[b];
+  r.kv = static_cast<int32_t>(kv < 0 ? 0 : kv < room ? kv : room);
+  return r;
+}
+
+// One workgroup's part of the launch: steps [s0, s1) of tile `rt` of request b.
+struct Piece {
+  Req r;
+  int32_t b, rt, s0, s1;
+  int32_t slot;   // of its partial result, -1: the tile is not cut
+  int32_t part, parts;
+};
+
+struct Shared {
+  int64_t sum[kWaves], tiles[kWaves];
+  int32_t scan[kWaves][2];
+  int32_t found[3];  // b, piece within the request, first slot of the request
+};
+
+// Piece number `want` of the launch.  A launch has the tiles of ROWS query rows of the requests that are its own (rows up to A.few: decode8's
+// 16-row tiles; more: prefill8's).  A tile's steps are cut into pieces of C, the smallest C
+// that keeps the launch near its target of pieces; so long requests are shared by many
+// workgroups and short ones are not cut.  (prefill8 cuts nothing where the tiles alone
+// reach the target: its partial results cost more.)  Every workgroup finds its own piece
+// by prefix sums over the requests: no launch and no host knowledge of the lengths is
+// needed.  Workgroup 0 also tells the join how many partial results there are.
+template <int ROWS>
+__device__ __forceinline__ bool locate(const Att& A, int want, Shared& sh, Piece& P) {
+  constexpr bool PRE = ROWS == kPreRows;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto cost = [&](const Req& r, int& tiles, int& steps) {
+    const int n = r.ql * A.G;
+    tiles = (n > A.few) == PRE ? (n + ROWS - 1) / ROWS : 0;
+    steps = max(1, (r.kv + kStep - 1) / kStep);
+  };
+  int64_t sum = 0, all = 0;
+  for (int b = tid; b < A.B; b += kThr) {
+    int tiles, steps;
+    cost(request(A, b), tiles, steps);
+    sum += int64_t(tiles) * steps;
+    all += tiles;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    sum += __shfl_xor(sum, o, 64);
+    if (PRE) all += __shfl_xor(all, o, 64);
+  }
+  if (lane == 0) {
+    sh.sum[wave] = sum;
+    sh.tiles[wave] = all;
+  }
+  if (tid == 0) sh.found[0] = -1;
+  __syncthreads();
+  sum = all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    sum += sh.sum[w];
+    all += sh.tiles[w];
+  }
+  // (decode8: whole rounds of its four waves)
+  constexpr int LEAST = 4;
+  int64_t c64 = (sum + A.target - 1) / A.target;
+  if (!PRE) c64 = (c64 + kWaves - 1) / kWaves * kWaves;
+  if (c64 < LEAST) c64 = LEAST;
+  if (c64 > INT32_MAX / 2 || (PRE && all >= A.target)) c64 = INT32_MAX / 2;
+  const int C = static_cast<int>(c64);
+  if (PRE && C == INT32_MAX / 2) {
+    // whole tiles, in descending order of their number: long causal ones first.  Two
+    // workgroups share a CU, the second round's in the order that evens out their sums
+    // (2048 causal queries, 32 / 8 heads: 79 us in ascending order, 57 so).
+    const int n = static_cast<int>(all), per = max(1, A.target / 2);
+    if (want >= n) want = INT32_MAX;
+    else {
+      const int round = want / per, first = round * per, size = min(per, n - first);
+      if (round & 1) want = first + size - 1 - (want - first);
+      want = n - 1 - want;
+    }
+  }
+  int base[2] = {0, 0};  // pieces, pieces of cut tiles
+  for (int b0 = 0; b0 < A.B; b0 += kThr) {
+    const int b = b0 + tid;
+    int v[2] = {0, 0}, own[2];
+    if (b < A.B) {
+      int tiles, steps;
+      cost(request(A, b), tiles, steps);
+      const int per = (steps + C - 1) / C;
+      v[0] = tiles * per;
+      v[1] = per > 1 ? v[0] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) own[k] = v[k];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int u = __shfl_up(v[k], o, 64);
+        if (lane >= o) v[k] += u;
+      }
+    if (lane == 63)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) sh.scan[wave][k] = v[k];
+    __syncthreads();
+    int tot[2] = {0, 0};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (w < wave) v[k] += sh.scan[w][k];
+        tot[k] += sh.scan[w][k];
+      }
+    const int end = base[0] + v[0], first = end - own[0];
+    if (want >= first && want < end) {
+      sh.found[0] = b;
+      sh.found[1] = want - first;
+      sh.found[2] = base[1] + v[1] - own[1];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) base[k] += tot[k];
+    if (sh.found[0] >= 0 && blockIdx.x != 0) break;
+  }
+  if (blockIdx.x == 0 && tid == 0) *A.used = base[1];
+  P.b = __builtin_amdgcn_readfirstlane(sh.found[0]);
+  if (P.b < 0) return false;
+  const int in = __builtin_amdgcn_readfirstlane(sh.found[1]);
+  P.r = request(A, P.b);
+  int tiles, steps;
+  cost(P.r, tiles, steps);
+  P.parts = (steps + C - 1) / C;
+  P.rt = in / P.parts;
+  P.part = in - P.rt * P.parts;
+  P.s0 = P.part * C;
+  P.s1 = min(steps, P.s0 + C);
+  P.slot = P.parts > 1 ? __builtin_amdgcn_readfirstlane(sh.found[2]) + in : -1;
+  return true;
+}
+
+// Where the piece's partial result goes, in units of [slot][H], or -1 past the workspace.
+__device__ __forceinline__ int64_t place(const Att& A, const Piece& P, int h) {
+  const int64_t at = int64_t(P.slot) * A.H + h;
+  if (at >= A.nslots) return -1;
+  if (threadIdx.x == 0) A.desc[at] = make_int4(P.part == 0 ? P.parts : 0, P.r.q0, P.r.ql, P.rt);
+  return at;
+}
+
+// Two codes as f16, of bytes 0 and 1 (or 2 and 3) of a dword.
+template <bool FP8>
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FP8) {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true));
+  } else {
+    // 0x6400 | u is the f16 1024 + u; u = code + 128
+    const uint32_t u = w ^ 0x80808080u;
+    const v2h off = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
+    lo = __builtin_bit_cast(
+        uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off);
+    hi = __builtin_bit_cast(
+        uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off);
+  }
+}
+
+template <bool FP8>
+__device__ __forceinline__ v8h widen8(uint32_t a, uint32_t b) {
+  v4u r;
+  uint32_t x, y;
+  widen<FP8>(a, x, y);
+  r[0] = x;
+  r[1] = y;
+  widen<FP8>(b, x, y);
+  r[2] = x;
+  r[3] = y;
+  return __builtin_bit_cast(v8h, r);
+}
+
+__device__ __forceinline__ uint32_t pk(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2h));
+}
+
+// x as f16 hi + lo, both rounded to nearest.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pk(a, b);
+  const v2h h = __builtin_bit_cast(v2h, hi);
+  lo = pk(a - static_cast<float>(h[0]), b - static_cast<float>(h[1]));
+}
+
+__device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Eight consecutive query values from element `at`.
+__device__ __forceinline__ void load8(const Att& A, int64_t at, float* x) {
+  if (A.q_vec && A.q_dtype == QKV_F32) {
+    const v4f* p = reinterpret_cast<const v4f*>(static_cast<const float*>(A.q) + at);
+    const v4f a = p[0], b = p[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = a[j];
+      x[4 + j] = b[j];
+    }
+  } else if (A.q_vec) {
+    const v4u w = *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(A.q) + at);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint16_t h = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+      x[j] = A.q_dtype == QKV_BF16 ? qkv_bf16_to_f32(h)
+                                   : static_cast<float>(__builtin_bit_cast(_Float16, h));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = qkv_load(A.q, at + j, A.q_dtype);
+  }
+}
+
+// Eight consecutive results to element `at` of out.
+__device__ __forceinline__ void store8(void* out, int64_t at, const float* x, int dt, bool vec) {
+  if (!vec) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) qkv_store(out, at + j, x[j], dt);
+  } else if (dt == QKV_F32) {
+    v4f* p = reinterpret_cast<v4f*>(static_cast<float*>(out) + at);
+    p[0] = v4f{x[0], x[1], x[2], x[3]};
+    p[1] = v4f{x[4], x[5], x[6], x[7]};
+  } else if (dt == QKV_F16) {
+    *reinterpret_cast<v4u*>(static_cast<uint16_t*>(out) + at) =
+        v4u{pk(x[0], x[1]), pk(x[2], x[3]), pk(x[4], x[5]), pk(x[6], x[7])};
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = qkv_f32_to_bf16(x[2 * j]) | uint32_t(qkv_f32_to_bf16(x[2 * j + 1])) << 16;
+    *reinterpret_cast<v4u*>(static_cast<uint16_t*>(out) + at) = v4u{w[0], w[1], w[2], w[3]};
+  }
+}
+
+// Four of them.
+__device__ __forceinline__ void store4(void* out, int64_t at, const float* x, int dt, bool vec) {
+  if (!vec) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) qkv_store(out, at + j, x[j], dt);
+  } else if (dt == QKV_F32) {
+    *reinterpret_cast<v4f*>(static_cast<float*>(out) + at) = v4f{x[0], x[1], x[2], x[3]};
+  } else if (dt == QKV_F16) {
+    *reinterpret_cast<v2u*>(static_cast<uint16_t*>(out) + at) = v2u{pk(x[0], x[1]), pk(x[2], x[3])};
+  } else {
+    *reinterpret_cast<v2u*>(static_cast<uint16_t*>(out) + at) =
+        v2u{qkv_f32_to_bf16(x[0]) | uint32_t(qkv_f32_to_bf16(x[1])) << 16,
+            qkv_f32_to_bf16(x[2]) | uint32_t(qkv_f32_to_bf16(x[3])) << 16};
+  }
+}
+
+// Joins the pieces of cut tiles: 4 rows of a tile at a time, 8 coordinates a lane, the
+// pieces dealt to the four waves.
+template <int D, int ROWS>
+__global__ __launch_bounds__(kThr) void join8(Att A) {
+  constexpr int GR = ROWS / 4;
+  __shared__ float acc[kWaves][4][D + 4], ml[kWaves][4][2];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane >> 4, d0 = 8 * (lane & 15);
+  const bool on = d0 < D;
+  const int64_t units = int64_t(min(*A.used, A.nslots / A.H)) * A.H * GR;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t at = u / GR;  // slot * H + h
+    const int4 t = A.desc[at];
+    const int parts = t.x, h = static_cast<int>(at % A.H);
+    const int rr0 = 4 * static_cast<int>(u % GR);
+    // (0: not the tile's first piece; lengths that do not fit q_start may leave a slot unset)
+    if (parts <= 0 || parts > A.nslots || t.w < 0 || int64_t(t.w) * ROWS > int64_t(A.rows) * A.G ||
+        (t.w * ROWS + rr0) / A.G >= t.z)
+      continue;
+    float M = -INFINITY, L = 0.f, x[8] = {};
+    for (int p = wave; p < parts; p += 4 * kWaves) {
+      float m[4], l[4];
+      v4f v[4][2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int q = p + kWaves * k;
+        const int64_t s = at + int64_t(q < parts ? q : p) * A.H;
+        const int64_t row = (s < A.nslots ? s : at) * ROWS + rr0 + r;
+        m[k] = q < parts ? A.part_ml[2 * row] : -INFINITY;
+        l[k] = A.part_ml[2 * row + 1];
+        const v4f* const src =
+            reinterpret_cast<const v4f*>(A.part_o + row * D + (on ? d0 : 0));
+        v[k][0] = src[0];
+        v[k][1] = src[1];
+      }
+      float mn = M;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mn = fmaxf(mn, m[k]);
+      const float ref = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(M - ref);
+      M = mn;
+      L *= f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] *= f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float e = __builtin_amdgcn_exp2f(m[k] - ref);
+        if (e == 0.f) continue;  // (a piece that saw nothing)
+        L = fmaf(l[k], e, L);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = fmaf(v[k][j >> 2][j & 3], e, x[j]);
+      }
+    }
+    __syncthreads();  // (the arrays' last readers)
+    if (on) {
+      *reinterpret_cast<v4f*>(&acc[wave][r][d0]) = v4f{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<v4f*>(&acc[wave][r][d0 + 4]) = v4f{x[4], x[5], x[6], x[7]};
+    }
+    if (d0 == 0) {
+      ml[wave][r][0] = M;
+      ml[wave][r][1] = L;
+    }
+    __syncthreads();
+    // wave w: row w
+    const int rr = t.w * ROWS + rr0 + wave, qi = rr / A.G, c = 2 * lane;
+    const int64_t row = int64_t(t.y) + qi;
+    if (c >= D || qi >= t.z || row < 0 || row >= A.rows) continue;
+    float mx = -INFINITY, sum = 0.f, y0 = 0.f, y1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, ml[w][wave][0]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float e = __builtin_amdgcn_exp2f(ml[w][wave][0] - ref);
+      sum = fmaf(ml[w][wave][1], e, sum);
+      y0 = fmaf(acc[w][wave][c], e, y0);
+      y1 = fmaf(acc[w][wave][c + 1], e, y1);
+    }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const int64_t to = (row * A.Hq + h * A.G + rr - qi * A.G) * D + c;
+    qkv_store(A.out, to, y0 * inv, A.out_dtype);
+    qkv_store(A.out, to + 1, y1 * inv, A.out_dtype);
+  }
+}
+
+// Workgroups of a join: the units are counted on the device.
+inline uint32_t join_grid(const Att& A, int rows) {
+  return static_cast<uint32_t>(std::min<int64_t>(int64_t(A.nslots) / 2 * (rows / 4), 1024));
+}
+
+}  // namespace qkv_kv8
+
+// Launches prefill8 over up to `tiles` tiles (a bound) and, with `cut`, the join of cut ones.
+void qkv_kv8_prefill(const qkv_kv8::Att& A, int32_t d, bool fp8, uint32_t tiles, bool cut,
+                     hipStream_t s);

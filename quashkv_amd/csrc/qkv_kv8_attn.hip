@@ -15,268 +15,11 @@
 // all 16 tokens of block g: one pair of scales per lane, and its weights are, as they
 // stand, the B operand of the value product, whose A operand is 16 bytes of a V block.
 // Nothing of K, V or P passes through LDS.
-#include <algorithm>
-
-#include "qkv_kv8.h"
+#include "qkv_kv8_attn.h"
 
 namespace {
 
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef float v2f __attribute__((ext_vector_type(2)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-typedef uint32_t v2u __attribute__((ext_vector_type(2)));
-
-constexpr int kStep = 64;        // tokens of a wave's step
-constexpr int kRows = 16;        // query rows of a decode tile
-constexpr int kWaves = 4;
-constexpr int kThr = 64 * kWaves;
-constexpr float kHead = 8.f;     // the running maximum may lag by 2^8 before a rescale
-constexpr float kUp = 7.f;       // largest weight in f16: 2^(kUp + kHead) at most, 2^kUp at least,
-                                 // so that f16's smallest step is 2^-31 of it
-constexpr float kLog2e = 1.44269504088896340736f;
-
-struct Att {
-  const void* q;
-  int64_t q_ts, q_hs;
-  int32_t q_dtype, q_vec;
-  int32_t rows;
-  const uint8_t* kpool;
-  const float* kscale;
-  const uint8_t* vpool;
-  const float* vscale;
-  int32_t npages, lg;
-  const int32_t* table;
-  int32_t width;
-  const int32_t* q_start;
-  const int32_t* q_lens;
-  const int32_t* kv_lens;
-  int32_t B, Hq, H, G, uniform_q;
-  float scale;
-  int32_t causal;
-  void* out;
-  int32_t out_dtype, out_vec;
-  int32_t target;   // pieces that a launch aims at, per kv head
-  int32_t nslots;   // partial results that the workspace holds
-  float* part_o;    // [slot][row][D]
-  float* part_ml;   // [slot][row][2]
-};
-
-// Request b's rows in this launch and its tokens.
-struct Req {
-  int32_t q0, ql, kv;
-};
-
-__device__ __forceinline__ Req request(const Att& A, int b) {
-  Req r;
-  if (A.q_start == nullptr) {
-    r.q0 = b * A.uniform_q;
-    r.ql = A.uniform_q;
-  } else {
-    r.q0 = A.q_start[b];
-    r.ql = A.q_lens ? A.q_lens[b] : A.q_start[b + 1] - r.q0;
-    r.ql = min(max(r.ql, 0), A.rows);
-  }
-  const int64_t room = int64_t(A.width) << A.lg, kv = A.kv_lens[b];
-  r.kv = static_cast<int32_t>(kv < 0 ? 0 : kv < room ? kv : room);
-  return r;
-}
-
-// One workgroup's part of the launch: steps [s0, s1) of tile `rt` of request b.
-struct Piece {
-  Req r;
-  int32_t b, rt, s0, s1;
-  int32_t slot;   // of its partial result (of the tile's first one), -1: not cut
-  int32_t parts;  // pieces of the tile
-};
-
-struct Shared {
-  int64_t sum[kWaves];
-  int32_t scan[kWaves][3];
-  int32_t found[3];  // b, piece (tile) within the request, first slot of the request
-};
-
-// Piece number `want` of the launch, or with TILE the whole of tile `want`.  A tile's steps are cut into pieces of C, the
-// smallest C (whole rounds of the four waves) that keeps the launch near its target; so
-// long requests are shared by many workgroups and short ones are not cut.  Every workgroup
-// finds its own piece by prefix sums over the requests: no launch and no host knowledge
-// of the lengths is needed.
-template <bool TILE>
-__device__ __forceinline__ bool locate(const Att& A, int want, Shared& sh, Piece& P) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  auto cost = [&](const Req& r, int& tiles, int& steps) {
-    tiles = (r.ql * A.G + kRows - 1) / kRows;
-    steps = max(1, (r.kv + kStep - 1) / kStep);
-  };
-  int64_t sum = 0;
-  for (int b = tid; b < A.B; b += kThr) {
-    int tiles, steps;
-    cost(request(A, b), tiles, steps);
-    sum += int64_t(tiles) * steps;
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  if (lane == 0) sh.sum[wave] = sum;
-  if (tid == 0) sh.found[0] = -1;
-  __syncthreads();
-  sum = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) sum += sh.sum[w];
-  int64_t c64 = (sum + A.target - 1) / A.target;
-  c64 = (c64 + kWaves - 1) / kWaves * kWaves;
-  const int C = static_cast<int>(c64 < kWaves ? kWaves : c64 > INT32_MAX / 2 ? INT32_MAX / 2 : c64);
-  int base[3] = {0, 0, 0};  // pieces, pieces of cut tiles, tiles
-  for (int b0 = 0; b0 < A.B; b0 += kThr) {
-    const int b = b0 + tid;
-    int v[3] = {0, 0, 0}, own[3];
-    if (b < A.B) {
-      int tiles, steps;
-      cost(request(A, b), tiles, steps);
-      const int per = (steps + C - 1) / C;
-      v[0] = tiles * per;
-      v[1] = per > 1 ? v[0] : 0;
-      v[2] = tiles;
-    }
-#pragma unroll
-    for (int k = 0; k < 3; ++k) own[k] = v[k];
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1)
-#pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        const int u = __shfl_up(v[k], o, 64);
-        if (lane >= o) v[k] += u;
-      }
-    if (lane == 63)
-#pragma unroll
-      for (int k = 0; k < 3; ++k) sh.scan[wave][k] = v[k];
-    __syncthreads();
-    int tot[3] = {0, 0, 0};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-#pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        if (w < wave) v[k] += sh.scan[w][k];
-        tot[k] += sh.scan[w][k];
-      }
-    constexpr int BY = TILE ? 2 : 0;
-    const int end = base[BY] + v[BY], first = end - own[BY];
-    if (want >= first && want < end) {
-      sh.found[0] = b;
-      sh.found[1] = want - first;
-      sh.found[2] = base[1] + v[1] - own[1];
-    }
-    __syncthreads();
-    if (sh.found[0] >= 0) break;
-#pragma unroll
-    for (int k = 0; k < 3; ++k) base[k] += tot[k];
-  }
-  P.b = __builtin_amdgcn_readfirstlane(sh.found[0]);
-  if (P.b < 0) return false;
-  const int in = __builtin_amdgcn_readfirstlane(sh.found[1]);
-  P.r = request(A, P.b);
-  int tiles, steps;
-  cost(P.r, tiles, steps);
-  P.parts = (steps + C - 1) / C;
-  P.rt = TILE ? in : in / P.parts;
-  const int part = TILE ? 0 : in - P.rt * P.parts;
-  P.s0 = part * C;
-  P.s1 = TILE ? steps : min(steps, P.s0 + C);
-  P.slot = -1;
-  if (P.parts > 1)
-    P.slot = __builtin_amdgcn_readfirstlane(sh.found[2]) + P.rt * P.parts + part;
-  return true;
-}
-
-// Two codes as f16, of bytes 0 and 1 (or 2 and 3) of a dword.
-template <bool FP8>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (FP8) {
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
-    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true));
-  } else {
-    // 0x6400 | u is the f16 1024 + u; u = code + 128
-    const uint32_t u = w ^ 0x80808080u;
-    const v2h off = {static_cast<_Float16>(-1152.f), static_cast<_Float16>(-1152.f)};
-    lo = __builtin_bit_cast(
-        uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off);
-    hi = __builtin_bit_cast(
-        uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off);
-  }
-}
-
-template <bool FP8>
-__device__ __forceinline__ v8h widen8(uint32_t a, uint32_t b) {
-  v4u r;
-  uint32_t x, y;
-  widen<FP8>(a, x, y);
-  r[0] = x;
-  r[1] = y;
-  widen<FP8>(b, x, y);
-  r[2] = x;
-  r[3] = y;
-  return __builtin_bit_cast(v8h, r);
-}
-
-__device__ __forceinline__ uint32_t pk(float a, float b) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2h));
-}
-
-// x as f16 hi + lo, both rounded to nearest.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pk(a, b);
-  const v2h h = __builtin_bit_cast(v2h, hi);
-  lo = pk(a - static_cast<float>(h[0]), b - static_cast<float>(h[1]));
-}
-
-__device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-
-// Eight consecutive query values from element `at`.
-__device__ __forceinline__ void load8(const Att& A, int64_t at, float* x) {
-  if (A.q_vec && A.q_dtype == QKV_F32) {
-    const v4f* p = reinterpret_cast<const v4f*>(static_cast<const float*>(A.q) + at);
-    const v4f a = p[0], b = p[1];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] = a[j];
-      x[4 + j] = b[j];
-    }
-  } else if (A.q_vec) {
-    const v4u w = *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(A.q) + at);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint16_t h = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
-      x[j] = A.q_dtype == QKV_BF16 ? qkv_bf16_to_f32(h)
-                                   : static_cast<float>(__builtin_bit_cast(_Float16, h));
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = qkv_load(A.q, at + j, A.q_dtype);
-  }
-}
-
-// Eight consecutive results to element `at` of out.
-__device__ __forceinline__ void store8(void* out, int64_t at, const float* x, int dt, bool vec) {
-  if (!vec) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) qkv_store(out, at + j, x[j], dt);
-  } else if (dt == QKV_F32) {
-    v4f* p = reinterpret_cast<v4f*>(static_cast<float*>(out) + at);
-    p[0] = v4f{x[0], x[1], x[2], x[3]};
-    p[1] = v4f{x[4], x[5], x[6], x[7]};
-  } else if (dt == QKV_F16) {
-    *reinterpret_cast<v4u*>(static_cast<uint16_t*>(out) + at) =
-        v4u{pk(x[0], x[1]), pk(x[2], x[3]), pk(x[4], x[5]), pk(x[6], x[7])};
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      w[j] = qkv_f32_to_bf16(x[2 * j]) | uint32_t(qkv_f32_to_bf16(x[2 * j + 1])) << 16;
-    *reinterpret_cast<v4u*>(static_cast<uint16_t*>(out) + at) = v4u{w[0], w[1], w[2], w[3]};
-  }
-}
+using namespace qkv_kv8;
 
 // d index of the first of the 8 coordinates that lane group g holds in product step ks
 __host__ __device__ constexpr int dcol(int D, int ks, int g) {
@@ -296,7 +39,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
   const int n = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % A.H;
   Piece P;
-  if (!locate<false>(A, blockIdx.x / A.H, sh, P)) return;
+  if (!locate<kRows>(A, blockIdx.x / A.H, sh, P)) return;
 
   // ---- this lane's query row
   const int rr = P.rt * kRows + n, qi = rr / A.G, gq = rr - qi * A.G;
@@ -510,6 +253,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
     red_ml[wave][n][0] = m;
     red_ml[wave][n][1] = l;
   }
+  const int64_t slot = P.slot >= 0 ? place(A, P, h) : -1;
   __syncthreads();
   constexpr int PER = D / 8;  // threads of a row
   if (tid < kRows * PER) {
@@ -533,8 +277,8 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] *= inv;
         store8(A.out, (row2 * A.Hq + h * A.G + rr2 - qi2 * A.G) * D + d0, x, A.out_dtype, A.out_vec);
-      } else if (int64_t(P.slot) * A.H + h < A.nslots) {
-        const int64_t at = (int64_t(P.slot) * A.H + h) * kRows + r;
+      } else if (slot >= 0) {
+        const int64_t at = slot * kRows + r;
         store8(A.part_o, at * D + d0, x, QKV_F32, true);
         if (d0 == 0) {
           A.part_ml[2 * at] = M;
@@ -545,55 +289,24 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
   }
 }
 
-// Joins the pieces of a cut tile: a wave per query row.
-template <int D>
-__global__ __launch_bounds__(kThr) void join8(Att A) {
-  __shared__ Shared sh;
-  const int lane = threadIdx.x & 63, h = blockIdx.x % A.H;
-  Piece P;
-  if (!locate<true>(A, blockIdx.x / A.H, sh, P) || P.parts == 1) return;
-  const int r = blockIdx.y * kWaves + (threadIdx.x >> 6);
-  const int rr = P.rt * kRows + r, qi = rr / A.G;
-  const int64_t row = int64_t(P.r.q0) + qi;
-  if (qi >= P.r.ql || row < 0 || row >= A.rows || P.slot < 0) return;
-  const int c = min(2 * lane, D - 2);
-  float M = -INFINITY, L = 0.f, x0 = 0.f, x1 = 0.f;
-  for (int i = 0; i < P.parts; i += 4) {
-    float m[4], l[4];
-    v2f v[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t slot = int64_t(P.slot + i + u) * A.H + h;
-      const bool on = i + u < P.parts && slot < A.nslots;
-      const int64_t at = (on ? slot : 0) * kRows + r;
-      m[u] = on ? A.part_ml[2 * at] : -INFINITY;
-      l[u] = A.part_ml[2 * at + 1];
-      v[u] = *reinterpret_cast<const v2f*>(A.part_o + at * D + c);
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (m[u] == -INFINITY) continue;
-      const float mn = fmaxf(M, m[u]);
-      const float f = __builtin_amdgcn_exp2f(M - mn), e = __builtin_amdgcn_exp2f(m[u] - mn);
-      M = mn;
-      L = fmaf(l[u], e, L * f);
-      x0 = fmaf(v[u][0], e, x0 * f);
-      x1 = fmaf(v[u][1], e, x1 * f);
-    }
-  }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
-  if (2 * lane < D) {
-    const int64_t at = (row * A.Hq + h * A.G + rr - qi * A.G) * D + c;
-    qkv_store(A.out, at, x0 * inv, A.out_dtype);
-    qkv_store(A.out, at + 1, x1 * inv, A.out_dtype);
-  }
-}
-
 // Pieces that a launch aims at, per kv head: two workgroups per CU.
 int32_t target_of(int32_t H) { return std::max(1, (2 * qkv_num_cus() + H - 1) / H); }
 // Cut tiles have more than C steps each and pieces of C, so they have fewer than
 // 2 total / C <= 2 target pieces.
 int64_t slots_of(int32_t H) { return int64_t(2 * target_of(H) + 1) * H; }
+// Bytes of a launch's partial results.
+int64_t part_bytes(int32_t H, int rows, int32_t d) {
+  return 256 + slots_of(H) * (16 + rows * (d + 2) * 4) / 256 * 256 + 256;
+}
+// Lays them out at `at`.
+void place_parts(Att& A, void* at, int rows, int32_t d) {
+  A.used = static_cast<int32_t*>(at);
+  A.desc = reinterpret_cast<int4*>(A.used + 64);
+  A.part_o = reinterpret_cast<float*>(A.desc + A.nslots);
+  A.part_ml = A.part_o + int64_t(A.nslots) * rows * d;
+}
+// Requests of more rows than this go to prefill8.
+constexpr int kFew = 32;
 
 template <int D, bool FP8>
 void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
@@ -605,7 +318,7 @@ void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
     if (A.out_dtype == QKV_BF16) decode8<D, FP8, false, false><<<grid, kThr, 0, s>>>(A);
     else decode8<D, FP8, false, true><<<grid, kThr, 0, s>>>(A);
   }
-  if (cut) join8<D><<<dim3(tiles * A.H, kRows / kWaves), kThr, 0, s>>>(A);
+  if (cut) join8<D, kRows><<<join_grid(A, kRows), kThr, 0, s>>>(A);
 }
 
 }  // namespace
@@ -613,7 +326,8 @@ void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
 extern "C" int64_t qkv_kv8_attention_workspace_bytes(int32_t B, int64_t rows, int32_t Hq,
                                                      int32_t Hkv, int32_t d, int64_t max_q) {
   if (Hkv < 1 || d < 1) return 0;
-  return (slots_of(Hkv) * kRows * (d + 2) * 4 + 255) / 256 * 256;
+  return part_bytes(Hkv, kRows, d) +
+         (max_q * (Hq / Hkv) > kFew ? part_bytes(Hkv, kPreRows, d) : 0);
 }
 
 extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_stride,
@@ -679,25 +393,41 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   A.out_vec = qkv_aligned(out, 16) && d * ob % 16 == 0;
   A.target = target_of(Hkv);
   A.nslots = static_cast<int32_t>(slots_of(Hkv));
-  A.part_o = static_cast<float*>(workspace);
-  A.part_ml = A.part_o + int64_t(A.nslots) * kRows * d;
-  // tiles: a request's last one may be in part empty
-  const int64_t tiles = q_start ? rows * G / kRows + std::min<int64_t>(B, rows)
-                                : int64_t(B) * ((A.uniform_q * G + kRows - 1) / kRows);
-  QKV_REQUIRE((tiles + A.target) * Hkv <= INT32_MAX, "batch of %d requests and %lld rows is too "
-              "large for one call", B, static_cast<long long>(rows));
-  const bool cut = (int64_t(pages_per_seq) << A.lg) > int64_t(kStep) * kWaves;
+  place_parts(A, workspace, kRows, d);
+  const int64_t longest = q_start ? std::min(max_q, rows) : A.uniform_q;
+  const bool pre = longest * G > kFew;
+  A.few = pre ? kFew : INT32_MAX;
+  // tiles of a launch, at most: a request's last one may be in part empty
+  auto tiles_of = [&](int r) {
+    return q_start ? rows * G / r + std::min<int64_t>(B, rows)
+                   : int64_t(B) * ((int64_t(A.uniform_q) * G + r - 1) / r);
+  };
+  QKV_REQUIRE((tiles_of(kRows) + A.target) * Hkv <= INT32_MAX, "batch of %d requests and %lld "
+              "rows is too large for one call", B, static_cast<long long>(rows));
+  // the shortest pieces have 4 steps
+  const bool cut = (int64_t(pages_per_seq) << A.lg) > int64_t(kStep) * 4;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const uint32_t t = static_cast<uint32_t>(tiles);
-  if (fmt == QKV_CODES_I8) {
-    if (d == 128) launch<128, false>(A, t, cut, s);
-    else if (d == 96) launch<96, false>(A, t, cut, s);
-    else launch<64, false>(A, t, cut, s);
-  } else {
-    if (d == 128) launch<128, true>(A, t, cut, s);
-    else if (d == 96) launch<96, true>(A, t, cut, s);
-    else launch<64, true>(A, t, cut, s);
+  if (q_start || !pre) {
+    // beside prefill8 this launch has only requests of up to kFew rows
+    const uint32_t t = static_cast<uint32_t>(
+        pre ? std::min<int64_t>(tiles_of(kRows), int64_t(B) * (kFew / kRows)) : tiles_of(kRows));
+    if (fmt == QKV_CODES_I8) {
+      if (d == 128) launch<128, false>(A, t, cut, s);
+      else if (d == 96) launch<96, false>(A, t, cut, s);
+      else launch<64, false>(A, t, cut, s);
+    } else {
+      if (d == 128) launch<128, true>(A, t, cut, s);
+      else if (d == 96) launch<96, true>(A, t, cut, s);
+      else launch<64, true>(A, t, cut, s);
+    }
+    QKV_LAUNCHED();
   }
-  QKV_LAUNCHED();
+  if (pre) {
+    place_parts(A, static_cast<uint8_t*>(workspace) + part_bytes(Hkv, kRows, d), kPreRows, d);
+    const int64_t t = tiles_of(kPreRows);
+    qkv_kv8_prefill(A, d, fmt == QKV_CODES_E4M3, static_cast<uint32_t>(t),
+                    cut && (q_start || t < A.target), s);
+    QKV_LAUNCHED();
+  }
   return QKV_OK;
 }
