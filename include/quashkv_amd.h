@@ -739,7 +739,7 @@ int qkv_page_release(int32_t* lens, const uint8_t* done, int32_t B, const int32_
                      int32_t* free_count, int32_t page_tokens, void* stream);
 
 /* Quantise keys and values (rows, H, d), fp32, fp16 or bf16, into their slots.
- * Rows of one block follow each other with ascending slots, as qkv_page_plan
+ * Rows of one block follow each other at consecutive slots, as qkv_page_plan
  * makes them; each slot is named once.  A block's tokens before the first one
  * that a call brings keep their values: at the block's scale, or, where the new
  * tokens need a larger one, quantised anew; its tokens behind are dropped.

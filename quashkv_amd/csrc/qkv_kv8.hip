@@ -46,120 +46,234 @@ __device__ __forceinline__ float value_of(uint32_t code) {
     return static_cast<float>(static_cast<int8_t>(code));
 }
 
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4;  // of a workgroup, each with a unit of its own
+
+// N consecutive elements (2 or 8) from element `at` of x; vec: their address is aligned to
+// their bytes (16 at most).
+template <int N, int DT>
+__device__ __forceinline__ void load_n(const void* x, int64_t at, bool vec, float* to) {
+  if (!vec) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = qkv_load(x, at + i, DT);
+  } else if constexpr (DT == QKV_F32) {
+#pragma unroll
+    for (int i = 0; i < N; i += N < 4 ? 2 : 4) {
+      const float* const p = static_cast<const float*>(x) + at + i;
+      if constexpr (N < 4) {
+        const v2f v = *reinterpret_cast<const v2f*>(p);
+        to[i] = v[0];
+        to[i + 1] = v[1];
+      } else {
+        const v4f v = *reinterpret_cast<const v4f*>(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[i + j] = v[j];
+      }
+    }
+  } else {
+    uint32_t w[N / 2];
+    const uint16_t* const p = static_cast<const uint16_t*>(x) + at;
+    if constexpr (N == 2) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      const v4u v = *reinterpret_cast<const v4u*>(p);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = v[j];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint16_t u = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+      to[i] = DT == QKV_BF16 ? qkv_bf16_to_f32(u)
+                             : static_cast<float>(__builtin_bit_cast(_Float16, u));
+    }
+  }
+}
+
+// N consecutive elements (2 or 8) to element `at` of a dense output.
+template <int N, int DT>
+__device__ __forceinline__ void store_n(void* x, int64_t at, bool vec, const float* v) {
+  if (!vec) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) qkv_store(x, at + i, v[i], DT);
+  } else if constexpr (DT == QKV_F32) {
+    float* const p = static_cast<float*>(x) + at;
+    if constexpr (N == 2) {
+      *reinterpret_cast<v2f*>(p) = v2f{v[0], v[1]};
+    } else {
+      reinterpret_cast<v4f*>(p)[0] = v4f{v[0], v[1], v[2], v[3]};
+      reinterpret_cast<v4f*>(p)[1] = v4f{v[4], v[5], v[6], v[7]};
+    }
+  } else {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (DT == QKV_BF16)
+        w[i] = qkv_f32_to_bf16(v[2 * i]) | uint32_t(qkv_f32_to_bf16(v[2 * i + 1])) << 16;
+      else
+        w[i] = uint32_t(__builtin_bit_cast(uint16_t, static_cast<_Float16>(v[2 * i]))) |
+               uint32_t(__builtin_bit_cast(uint16_t, static_cast<_Float16>(v[2 * i + 1]))) << 16;
+    }
+    uint16_t* const p = static_cast<uint16_t*>(x) + at;
+    if constexpr (N == 2) *reinterpret_cast<uint32_t*>(p) = w[0];
+    else *reinterpret_cast<v4u*>(p) = v4u{w[0], w[1], w[2], w[3]};
+  }
+}
+
+// Scale and its inverse for a block whose largest new value is a, old: its scale so far.
+template <bool FP8>
+__device__ __forceinline__ float scale_of(float a, float old, bool& grew, float& inv) {
+  float sc = a > 0.f ? fmaxf(a * (1.f / kTop<FP8>), kScaleFloor) : 0.f;
+  grew = sc > old;
+  sc = grew ? sc : old;
+  inv = sc > 0.f ? 1.f / sc : 0.f;
+  return sc;
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float m = fabsf(x);
+  return m < INFINITY ? m : 0.f;
+}
+
 struct App {
   const void* x[2];       // keys, values
-  int64_t ts[2], hs[2];   // their token and head strides (elements)
+  int64_t ts[2], hs[2];   // their row and head strides (elements)
+  int32_t vec[2];         // whether 16-byte (keys) and pair (values) loads are aligned
   const int64_t* slots;
   int64_t rows;
   uint8_t* pool[2];
   float* scale[2];
   int64_t tokens;         // slots of the pool
   int32_t lg, H, chunk;
+  int64_t units;          // chunks x heads
 };
 
-// A wave per (chunk of rows, head, half).  A run: rows whose slots ascend within one
-// block.  The wave that holds a run's first row does all of it: lane l has the
-// coordinates 2 l and 2 l + 1 of all 16 tokens.
+// A wave per (chunk of rows, head), a launch row each for keys and values.  A run: rows at
+// consecutive slots of one block; the wave in whose chunk it begins does all of it, so that
+// a block's largest value is a wave's reduction.  The chunk's slots and those that its
+// last run may reach are read at once, a lane each.
+// Keys: lane l has 8 coordinates of every (512 / D)-th token, whole rows in 16-byte loads and
+// 8-byte stores.  Values: a pair of coordinates of all tokens (D = 64: of every other eight),
+// whose codes are the 16 (8) consecutive bytes of two of the block's rows.
 template <int D, bool FP8, int DT>
-__global__ __launch_bounds__(64) void append_runs(App A) {
-  const int lane = threadIdx.x, h = blockIdx.y, half = blockIdx.z;
-  const bool on = 2 * lane < D;
-  const int c = on ? 2 * lane : 0;
-  const int64_t r0 = int64_t(blockIdx.x) * A.chunk;
-  const int64_t r1 = r0 + A.chunk < A.rows ? r0 + A.chunk : A.rows;
+__global__ __launch_bounds__(64 * kWaves) void append_runs(App A) {
+  const int lane = threadIdx.x & 63, half = blockIdx.y;
+  const int64_t u =
+      int64_t(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (u >= A.units) return;
+  const int64_t r0 = u / A.H * A.chunk;
+  const int h = static_cast<int>(u % A.H);
+  // lane i: row r0 - 1 + i
+  const int64_t at = r0 - 1 + lane;
+  int64_t sl = at >= 0 && at < A.rows ? A.slots[at] : -1;
+  if (sl >= A.tokens) sl = -1;
+  const int64_t prev = __shfl_up(static_cast<long long>(sl), 1, 64);
+  const bool cont = lane > 0 && sl >= 0 && prev >= 0 && sl == prev + 1 && (sl & 15) != 0;
+  const uint64_t conts = __ballot(cont);
+  uint64_t heads = __ballot(sl >= 0 && !cont) & ((uint64_t(2) << A.chunk) - 2);
   const int64_t n = int64_t(1) << A.lg;
-  for (int64_t r = r0; r < r1; ++r) {
-    const int64_t s = A.slots[r];
-    if (s < 0 || s >= A.tokens) continue;
-    if (r > 0) {
-      const int64_t prev = A.slots[r - 1];
-      if (prev >= 0 && (prev >> 4) == (s >> 4) && prev < s) continue;  // inside a run
-    }
-    const int j0 = static_cast<int>(s & 15);
-    float x[kBlk][2];
-    uint32_t have = 0;  // tokens of the block that the run brings
-#pragma unroll
-    for (int j = 0; j < kBlk; ++j) x[j][0] = x[j][1] = 0.f;
-    {
-      int64_t rr = r, cur = s, last = -1;
-#pragma unroll
-      for (int j = 0; j < kBlk; ++j) {
-        if (cur >= 0 && (cur >> 4) == (s >> 4) && cur > last && (cur & 15) == j) {
-          const int64_t at = rr * A.ts[half] + h * A.hs[half] + c;
-          if (on) {
-            x[j][0] = qkv_load(A.x[half], at, DT);
-            x[j][1] = qkv_load(A.x[half], at + 1, DT);
-          }
-          have |= 1u << j;
-          last = cur;
-          ++rr;
-          cur = rr < A.rows ? A.slots[rr] : -1;
-        }
-      }
-    }
-    float a = 0.f;
-#pragma unroll
-    for (int j = 0; j < kBlk; ++j)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float m = fabsf(x[j][i]);
-        if (m < INFINITY) a = fmaxf(a, m);
-      }
-    a = qkv_wave_max(a);
-    const int64_t page = s >> A.lg, o = s & (n - 1);
-    const int64_t row = (page * A.H + h) * n + (o & ~int64_t(15));  // block's first K row
+  while (heads) {
+    const int i0 = __builtin_ctzll(heads);
+    heads &= heads - 1;
+    const int len = 1 + __builtin_ctzll(~(conts >> (i0 + 1)));
+    const int64_t s = __shfl(static_cast<long long>(sl), i0, 64), r = r0 - 1 + i0;
+    const int j0 = static_cast<int>(s & 15), j1 = j0 + len;  // the run's places in the block
+    const int64_t row = ((s >> A.lg) * A.H + h) * n + (s & (n - 16));  // the block's first row
     float* const sp = A.scale[half] + (row >> 4);
-    const float old = j0 > 0 ? *sp : 0.f;
-    float sc = a > 0.f ? fmaxf(a * (1.f / kTop<FP8>), kScaleFloor) : 0.f;
-    const bool grew = sc > old;
-    sc = grew ? sc : old;
-    const float inv = sc > 0.f ? 1.f / sc : 0.f;
     uint8_t* const base = A.pool[half] + row * D;
+    const int64_t src = (r - j0) * A.ts[half] + h * A.hs[half];  // of place 0
+    const float old = j0 > 0 ? *sp : 0.f;
+    bool grew;
+    float inv;
     if (half == 0) {
-      uint16_t* const k = reinterpret_cast<uint16_t*>(base + c);
+      constexpr int LPR = D / 8, RPI = 64 / LPR, NI = (kBlk + RPI - 1) / RPI;
+      const int sub = lane / LPR, c = 8 * (lane % LPR);
+      float x[NI][8], a = 0.f;
 #pragma unroll
-      for (int j = 0; j < kBlk; ++j) {
-        if (have >> j & 1) {
-          if (on)
-            k[j * (D / 2)] = static_cast<uint16_t>(code_of<FP8>(x[j][0], inv) |
-                                                   code_of<FP8>(x[j][1], inv) << 8);
-        } else if (j < j0 && grew && on) {
-          const uint32_t u = k[j * (D / 2)];
-          k[j * (D / 2)] =
-              static_cast<uint16_t>(code_of<FP8>(value_of<FP8>(u) * old, inv) |
-                                    code_of<FP8>(value_of<FP8>(u >> 8) * old, inv) << 8);
+      for (int t = 0; t < NI; ++t) {
+        const int j = RPI * t + sub;
+        const bool on = sub < RPI && j >= j0 && j < j1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[t][i] = 0.f;
+        if (on) load_n<8, DT>(A.x[0], src + j * A.ts[0] + c, A.vec[0], x[t]);
+      }
+#pragma unroll
+      for (int t = 0; t < NI; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = fmaxf(a, finite_abs(x[t][i]));
+      const float sc = scale_of<FP8>(qkv_wave_max(a), old, grew, inv);
+#pragma unroll
+      for (int t = 0; t < NI; ++t) {
+        const int j = RPI * t + sub;
+        const bool on = sub < RPI && j >= j0 && j < j1;
+        const bool again = sub < RPI && j < j0 && grew;
+        v2u* const k = reinterpret_cast<v2u*>(base + j * D + c);
+        if (again) {
+          const v2u w = *k;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[t][i] = value_of<FP8>(w[i >> 2] >> (8 * (i & 3))) * old;
+        }
+        if (on || again) {
+          v2u w = {0, 0};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i >> 2] |= code_of<FP8>(x[t][i], inv) << (8 * (i & 3));
+          *k = w;
         }
       }
-    } else if (on) {
-      uint4* const v = reinterpret_cast<uint4*>(base + c * kBlk);
-      uint32_t w[2][4] = {};
-      if (j0 > 0) {
-        *reinterpret_cast<uint4*>(w[0]) = v[0];
-        *reinterpret_cast<uint4*>(w[1]) = v[1];
+      if (lane == 0) *sp = sc;
+    } else {
+      constexpr int LPR = D / 2, TG = 64 / LPR, TL = kBlk / TG;  // lanes, token groups
+      const int tg = lane / LPR, c = 2 * (lane % LPR);
+      const bool on = tg < TG;
+      float x[TL][2], a = 0.f;
+#pragma unroll
+      for (int t = 0; t < TL; ++t) {
+        const int j = TL * tg + t;
+        x[t][0] = x[t][1] = 0.f;
+        if (on && j >= j0 && j < j1) load_n<2, DT>(A.x[1], src + j * A.ts[1] + c, A.vec[1], x[t]);
       }
+      uint32_t w[2][TL / 4] = {};
+      uint8_t* const v = base + c * kBlk + TL * tg;
+      if (j0 > 0 && on) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int q = 0; q < TL / 4; ++q)
+            w[i][q] = *reinterpret_cast<const uint32_t*>(v + kBlk * i + 4 * q);
+      }
+#pragma unroll
+      for (int t = 0; t < TL; ++t) a = fmaxf(a, fmaxf(finite_abs(x[t][0]), finite_abs(x[t][1])));
+      const float sc = scale_of<FP8>(qkv_wave_max(a), old, grew, inv);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t u = 0;
+        for (int q = 0; q < TL / 4; ++q) {
+          uint32_t to = 0;
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            const int j = 4 * q + b;
-            uint32_t code = 0;
-            if (have >> j & 1) {
-              code = code_of<FP8>(x[j][i], inv);
-            } else if (j < j0) {
-              code = w[i][q] >> (8 * b) & 0xffu;
-              if (grew) code = code_of<FP8>(value_of<FP8>(code) * old, inv);
-            }
-            u |= code << (8 * b);
+            const int t = 4 * q + b, j = TL * tg + t;
+            float y = x[t][i];
+            if (j0 > 0 && grew && j < j0) y = value_of<FP8>(w[i][q] >> (8 * b)) * old;
+            uint32_t code = code_of<FP8>(y, inv);
+            if (j0 > 0 && !grew && j < j0) code = w[i][q] >> (8 * b) & 0xffu;
+            to |= code << (8 * b);
           }
-          w[i][q] = u;
+          w[i][q] = to;
         }
-      v[0] = *reinterpret_cast<uint4*>(w[0]);
-      v[1] = *reinterpret_cast<uint4*>(w[1]);
+      if (on) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if constexpr (TL == 16)
+            *reinterpret_cast<v4u*>(v + kBlk * i) = v4u{w[i][0], w[i][1], w[i][2], w[i][3]};
+          else
+            *reinterpret_cast<v2u*>(v + kBlk * i) = v2u{w[i][0], w[i][1]};
+        }
+      }
+      if (lane == 0) *sp = sc;
     }
-    if (lane == 0) *sp = sc;
   }
 }
 
@@ -169,39 +283,95 @@ struct Rd {
   const uint8_t* pool[2];
   const float* scale[2];
   int64_t tokens;
-  int32_t lg, H;
+  int32_t lg, H, chunk;
+  int64_t units;
   void* out[2];
+  int32_t vec[2];
 };
 
-// A wave per (row, head, half): lane l has the coordinates 2 l and 2 l + 1.
+// A wave per (chunk of up to 16 rows, head), lanes as in append_runs; a V block is read once
+// for a run of consecutive slots in it.
 template <int D, bool FP8, int DT>
-__global__ __launch_bounds__(256) void read_rows(Rd A) {
-  const int lane = threadIdx.x & 63, h = blockIdx.y, half = blockIdx.z;
-  const int64_t r = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (r >= A.rows || 2 * lane >= D) return;
-  const int c = 2 * lane;
-  const int64_t s = A.slots[r], n = int64_t(1) << A.lg;
-  float v0 = 0.f, v1 = 0.f;
-  if (s >= 0 && s < A.tokens) {
-    const int64_t o = s & (n - 1), row = ((s >> A.lg) * A.H + h) * n + o;
-    const float sc = A.scale[half][row >> 4];
-    uint32_t a, b;
-    if (half == 0) {
-      const uint8_t* p = A.pool[0] + row * D + c;
-      a = p[0];
-      b = p[1];
-    } else {
-      const uint8_t* p = A.pool[1] + (row & ~int64_t(15)) * D + c * kBlk + (o & 15);
-      a = p[0];
-      b = p[kBlk];
+__global__ __launch_bounds__(64 * kWaves) void read_rows(Rd A) {
+  const int lane = threadIdx.x & 63, half = blockIdx.y;
+  const int64_t u =
+      int64_t(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (u >= A.units) return;
+  const int64_t r0 = u / A.H * A.chunk, n = int64_t(1) << A.lg;
+  const int h = static_cast<int>(u % A.H);
+  // lane i: row r0 + i
+  const bool mine = lane < A.chunk && r0 + lane < A.rows;
+  int64_t sl = mine ? A.slots[r0 + lane] : -1;
+  if (sl >= A.tokens) sl = -1;
+  const uint64_t rows = __ballot(mine);
+  auto row_of = [&](int64_t s) { return ((s >> A.lg) * A.H + h) * n + (s & (n - 1)); };
+  if (half == 0) {
+    constexpr int LPR = D / 8, RPI = 64 / LPR, NI = (kBlk + RPI - 1) / RPI;
+    const int sub = lane / LPR, c = 8 * (lane % LPR);
+    v2u w[NI];
+    float sc[NI];
+#pragma unroll
+    for (int t = 0; t < NI; ++t) {
+      const int i = RPI * t + sub;
+      const int64_t s = __shfl(static_cast<long long>(sl), i & 63, 64);
+      w[t] = v2u{0, 0};
+      sc[t] = 0.f;
+      if (sub < RPI && i < A.chunk && s >= 0) {
+        const int64_t row = row_of(s);
+        w[t] = *reinterpret_cast<const v2u*>(A.pool[0] + row * D + c);
+        sc[t] = A.scale[0][row >> 4];
+      }
     }
-    v0 = value_of<FP8>(a) * sc;
-    v1 = value_of<FP8>(b) * sc;
+#pragma unroll
+    for (int t = 0; t < NI; ++t) {
+      const int i = RPI * t + sub;
+      if (sub >= RPI || i >= kBlk || !(rows >> i & 1)) continue;
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = value_of<FP8>(w[t][j >> 2] >> (8 * (j & 3))) * sc[t];
+      store_n<8, DT>(A.out[0], ((r0 + i) * A.H + h) * D + c, A.vec[0], x);
+    }
+  } else {
+    const int64_t prev = __shfl_up(static_cast<long long>(sl), 1, 64);
+    const bool cont = lane > 0 && sl >= 0 && sl == prev + 1 && (sl & 15) != 0;
+    const uint64_t conts = __ballot(cont && mine);
+    uint64_t heads = __ballot(mine && !cont);
+    constexpr int LPR = D / 2, TG = 64 / LPR, TL = kBlk / TG;
+    const int tg = lane / LPR, c = 2 * (lane % LPR);
+    while (heads) {
+      const int i0 = __builtin_ctzll(heads);
+      heads &= heads - 1;
+      const int64_t s = __shfl(static_cast<long long>(sl), i0, 64);
+      const int len = s < 0 ? 1 : 1 + __builtin_ctzll(~(conts >> (i0 + 1)));
+      const int j0 = s < 0 ? 0 : static_cast<int>(s & 15), j1 = j0 + len;
+      if (tg >= TG) continue;
+      uint32_t w[2][TL / 4] = {};
+      float sc = 0.f;
+      if (s >= 0) {
+        const int64_t row = row_of(s) & ~int64_t(15);
+        const uint8_t* const v = A.pool[1] + row * D + c * kBlk + TL * tg;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int q = 0; q < TL / 4; ++q)
+            w[i][q] = *reinterpret_cast<const uint32_t*>(v + kBlk * i + 4 * q);
+        sc = A.scale[1][row >> 4];
+      }
+#pragma unroll
+      for (int t = 0; t < TL; ++t) {
+        const int j = TL * tg + t;
+        if (j < j0 || j >= j1) continue;
+        const float x[2] = {value_of<FP8>(w[0][t >> 2] >> (8 * (t & 3))) * sc,
+                            value_of<FP8>(w[1][t >> 2] >> (8 * (t & 3))) * sc};
+        store_n<2, DT>(A.out[1], ((r0 + i0 + j - j0) * A.H + h) * D + c, A.vec[1], x);
+      }
+    }
   }
-  const int64_t at = (r * A.H + h) * D + c;
-  qkv_store(A.out[half], at, v0, DT);
-  qkv_store(A.out[half], at + 1, v1, DT);
 }
+
+// Rows of a wave's unit: a block's where there are rows enough for every CU; else one, so
+// that a decode step's rows, each a run of its own, do not queue in one wave.
+int32_t chunk_of(int64_t rows) { return rows > 4096 ? 16 : 1; }
 
 }  // namespace
 
@@ -248,9 +418,17 @@ extern "C" int qkv_kv8_append(int32_t in_dtype, const void* keys, int64_t k_row_
               "qkv_kv8_append: null pointer");
   QKV_REQUIRE(qkv_aligned(kpool, 16) && qkv_aligned(vpool, 16),
               "the pools must be 16-byte aligned");
+  const int es = in_dtype == QKV_F32 ? 4 : 2;
+  auto aligned = [&](const void* p, int64_t rs, int64_t hs, int to) {
+    return int32_t(qkv_aligned(p, to) && rs * es % to == 0 && hs * es % to == 0);
+  };
+  const int32_t chunk = chunk_of(rows);
+  const int64_t units = (rows + chunk - 1) / chunk * H;
   App A{{keys, values},
         {k_row_stride, v_row_stride},
         {k_head_stride, v_head_stride},
+        {aligned(keys, k_row_stride, k_head_stride, 16),
+         aligned(values, v_row_stride, v_head_stride, 2 * es)},
         slots,
         rows,
         {static_cast<uint8_t*>(kpool), static_cast<uint8_t*>(vpool)},
@@ -258,10 +436,13 @@ extern "C" int qkv_kv8_append(int32_t in_dtype, const void* keys, int64_t k_row_
         int64_t(num_pages) * page_tokens,
         qkv_page_lg(page_tokens),
         H,
-        1};
-  const dim3 grid(static_cast<uint32_t>((rows + A.chunk - 1) / A.chunk), H, 2);
+        chunk,
+        units};
+  QKV_REQUIRE(units / kWaves < INT32_MAX, "too many rows (%lld) for one call",
+              static_cast<long long>(rows));
+  const dim3 grid(static_cast<uint32_t>((units + kWaves - 1) / kWaves), 2);
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define RUN(D, FP8, DT) append_runs<D, FP8, DT><<<grid, 64, 0, s>>>(A)
+#define RUN(D, FP8, DT) append_runs<D, FP8, DT><<<grid, 64 * kWaves, 0, s>>>(A)
   QKV_KV8_DISPATCH(RUN, d, fmt, in_dtype)
 #undef RUN
   QKV_LAUNCHED();
@@ -282,6 +463,9 @@ extern "C" int qkv_kv8_read(const int64_t* slots, int64_t rows, int32_t H, int32
               "qkv_kv8_read: null pointer");
   QKV_REQUIRE(qkv_aligned(kpool, 16) && qkv_aligned(vpool, 16),
               "the pools must be 16-byte aligned");
+  const int32_t chunk = chunk_of(rows);
+  const int64_t units = (rows + chunk - 1) / chunk * H;
+  const int os = out_dtype == QKV_F32 ? 4 : 2;
   Rd A{slots,
        rows,
        {static_cast<const uint8_t*>(kpool), static_cast<const uint8_t*>(vpool)},
@@ -289,10 +473,15 @@ extern "C" int qkv_kv8_read(const int64_t* slots, int64_t rows, int32_t H, int32
        int64_t(num_pages) * page_tokens,
        qkv_page_lg(page_tokens),
        H,
-       {keys, values}};
-  const dim3 grid(static_cast<uint32_t>((rows + 3) / 4), H, 2);
+       chunk,
+       units,
+       {keys, values},
+       {qkv_aligned(keys, 16), qkv_aligned(values, 2 * os)}};
+  QKV_REQUIRE(units / kWaves < INT32_MAX, "too many rows (%lld) for one call",
+              static_cast<long long>(rows));
+  const dim3 grid(static_cast<uint32_t>((units + kWaves - 1) / kWaves), 2);
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define RUN(D, FP8, DT) read_rows<D, FP8, DT><<<grid, 256, 0, s>>>(A)
+#define RUN(D, FP8, DT) read_rows<D, FP8, DT><<<grid, 64 * kWaves, 0, s>>>(A)
   QKV_KV8_DISPATCH(RUN, d, fmt, out_dtype)
 #undef RUN
   QKV_LAUNCHED();

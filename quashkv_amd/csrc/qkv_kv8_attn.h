@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "qkv_kv8.h"
 
@@ -46,6 +47,7 @@ struct Att {
   int32_t out_dtype, out_vec;
   int32_t few;      // requests of up to this many rows (queries x G) are decode8's
   int32_t target;   // pieces that a launch aims at, per kv head
+  float per_target; // 1 / target
   int32_t nslots;   // partial results that the workspace holds
   int32_t* used;    // of them, per kv head, in this launch
   int4* desc;       // [slot][H]: whose they are
@@ -82,126 +84,160 @@ struct Piece {
 };
 
 struct Shared {
-  int64_t sum[kWaves], tiles[kWaves];
-  int32_t scan[kWaves][2];
+  float sum[8];  // a wave's
+  int32_t tiles[8], scan[8][2];
   int32_t found[3];  // b, piece within the request, first slot of the request
 };
 
-// Piece number `want` of the launch.  A launch has the tiles of ROWS query rows of the requests that are its own (rows up to A.few: decode8's
-// 16-row tiles; more: prefill8's).  A tile's steps are cut into pieces of C, the smallest C
-// that keeps the launch near its target of pieces; so long requests are shared by many
-// workgroups and short ones are not cut.  (prefill8 cuts nothing where the tiles alone
-// reach the target: its partial results cost more.)  Every workgroup finds its own piece
-// by prefix sums over the requests: no launch and no host knowledge of the lengths is
+// Inclusive sum over a wave's lanes.
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+  auto add = [&](auto ctrl, auto mask) {
+    const int u = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value,
+                                              decltype(mask)::value, 0xf, false);
+    v += __builtin_bit_cast(T, u);
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr 1, 2, 4, 8
+  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast 15, 31
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ T lane_value(T v, int lane) {
+  return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
+// Piece number `want` of the launch.  A launch has the tiles of ROWS query rows of the
+// requests that are its own (rows up to A.few: decode8's 16-row tiles; more: prefill8's).
+// A tile's steps are cut into pieces of C, the smallest C that keeps the launch near its
+// target of pieces; so long requests are shared by many workgroups and short ones are not
+// cut.  (prefill8 cuts nothing where the tiles alone reach the target: its partial results
+// cost more.)  Every workgroup finds its own piece by prefix sums over the requests -- each
+// wave for itself up to 64 of them -- so no launch and no host knowledge of the lengths is
 // needed.  Workgroup 0 also tells the join how many partial results there are.
-template <int ROWS>
+template <int ROWS, int THR>
 __device__ __forceinline__ bool locate(const Att& A, int want, Shared& sh, Piece& P) {
   constexpr bool PRE = ROWS == kPreRows;
+  constexpr int ROUND = PRE ? 2 : kWaves;  // steps that a workgroup takes at once
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   auto cost = [&](const Req& r, int& tiles, int& steps) {
     const int n = r.ql * A.G;
     tiles = (n > A.few) == PRE ? (n + ROWS - 1) / ROWS : 0;
     steps = max(1, (r.kv + kStep - 1) / kStep);
   };
-  int64_t sum = 0, all = 0;
-  for (int b = tid; b < A.B; b += kThr) {
-    int tiles, steps;
-    cost(request(A, b), tiles, steps);
-    sum += int64_t(tiles) * steps;
-    all += tiles;
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    sum += __shfl_xor(sum, o, 64);
-    if (PRE) all += __shfl_xor(all, o, 64);
-  }
-  if (lane == 0) {
-    sh.sum[wave] = sum;
-    sh.tiles[wave] = all;
-  }
-  if (tid == 0) sh.found[0] = -1;
-  __syncthreads();
-  sum = all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    sum += sh.sum[w];
-    all += sh.tiles[w];
-  }
-  // (decode8: whole rounds of its four waves)
-  constexpr int LEAST = 4;
-  int64_t c64 = (sum + A.target - 1) / A.target;
-  if (!PRE) c64 = (c64 + kWaves - 1) / kWaves * kWaves;
-  if (c64 < LEAST) c64 = LEAST;
-  if (c64 > INT32_MAX / 2 || (PRE && all >= A.target)) c64 = INT32_MAX / 2;
-  const int C = static_cast<int>(c64);
-  if (PRE && C == INT32_MAX / 2) {
-    // whole tiles, in descending order of their number: long causal ones first.  Two
-    // workgroups share a CU, the second round's in the order that evens out their sums
-    // (2048 causal queries, 32 / 8 heads: 79 us in ascending order, 57 so).
-    const int n = static_cast<int>(all), per = max(1, A.target / 2);
-    if (want >= n) want = INT32_MAX;
-    else {
-      const int round = want / per, first = round * per, size = min(per, n - first);
-      if (round & 1) want = first + size - 1 - (want - first);
-      want = n - 1 - want;
+  // (the sum is rounded alike in every workgroup; C is above its share in any case)
+  auto piece_len = [&](float sum, int all) {
+    if (PRE && all >= A.target) return INT32_MAX / 2;
+    const int c = static_cast<int>(fminf(sum * A.per_target, 1e9f)) + 1;
+    return max(4, (c + ROUND - 1) / ROUND * ROUND);
+  };
+  // whole prefill tiles: the last ones first, of a causal prompt the longest
+  auto order = [&](int C, int all) {
+    if (PRE && C == INT32_MAX / 2) want = want < all ? all - 1 - want : INT32_MAX;
+  };
+  int C, in, slot0, steps;
+  if (A.B <= 64) {
+    Req r{0, 0, 0};
+    int tiles = 0, st = 1;
+    if (lane < A.B) {
+      r = request(A, lane);
+      cost(r, tiles, st);
     }
-  }
-  int base[2] = {0, 0};  // pieces, pieces of cut tiles
-  for (int b0 = 0; b0 < A.B; b0 += kThr) {
-    const int b = b0 + tid;
-    int v[2] = {0, 0}, own[2];
-    if (b < A.B) {
-      int tiles, steps;
-      cost(request(A, b), tiles, steps);
-      const int per = (steps + C - 1) / C;
-      v[0] = tiles * per;
-      v[1] = per > 1 ? v[0] : 0;
+    const float sum = lane_value(wave_scan(static_cast<float>(tiles) * st), 63);
+    const int all = PRE ? lane_value(wave_scan(tiles), 63) : 0;
+    C = piece_len(sum, all);
+    order(C, all);
+    const int per = (st + C - 1) / C, mine = tiles * per, cut = per > 1 ? mine : 0;
+    const int end = wave_scan(mine), cuts = wave_scan(cut);
+    if (blockIdx.x == 0 && tid == 0) *A.used = lane_value(cuts, 63);
+    const uint64_t hit = __ballot(want >= end - mine && want < end);
+    if (hit == 0) return false;
+    P.b = __builtin_ctzll(hit);
+    in = want - lane_value(end - mine, P.b);
+    slot0 = lane_value(cuts - cut, P.b);
+    steps = lane_value(st, P.b);
+    P.r = Req{lane_value(r.q0, P.b), lane_value(r.ql, P.b), lane_value(r.kv, P.b)};
+  } else {
+    float sum = 0.f;
+    int all = 0;
+    for (int b = tid; b < A.B; b += THR) {
+      int tiles, st;
+      cost(request(A, b), tiles, st);
+      sum += static_cast<float>(tiles) * st;
+      all += tiles;
     }
+    sum = wave_scan(sum);
+    all = wave_scan(all);
+    if (lane == 63) {
+      sh.sum[wave] = sum;
+      sh.tiles[wave] = all;
+    }
+    if (tid == 0) sh.found[0] = -1;
+    __syncthreads();
+    sum = 0.f;
+    all = 0;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) own[k] = v[k];
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1)
+    for (int w = 0; w < THR / 64; ++w) {
+      sum += sh.sum[w];
+      all += sh.tiles[w];
+    }
+    C = piece_len(sum, all);
+    order(C, all);
+    int base[2] = {0, 0};  // pieces, pieces of cut tiles
+    for (int b0 = 0; b0 < A.B; b0 += THR) {
+      const int b = b0 + tid;
+      int own[2] = {0, 0}, v[2];
+      if (b < A.B) {
+        int tiles, st;
+        cost(request(A, b), tiles, st);
+        const int per = (st + C - 1) / C;
+        own[0] = tiles * per;
+        own[1] = per > 1 ? own[0] : 0;
+      }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int u = __shfl_up(v[k], o, 64);
-        if (lane >= o) v[k] += u;
+        v[k] = wave_scan(own[k]);
+        if (lane == 63) sh.scan[wave][k] = v[k];
       }
-    if (lane == 63)
+      __syncthreads();
+      int tot[2] = {0, 0};
 #pragma unroll
-      for (int k = 0; k < 2; ++k) sh.scan[wave][k] = v[k];
-    __syncthreads();
-    int tot[2] = {0, 0};
+      for (int w = 0; w < THR / 64; ++w)
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (w < wave) v[k] += sh.scan[w][k];
-        tot[k] += sh.scan[w][k];
+        for (int k = 0; k < 2; ++k) {
+          if (w < wave) v[k] += sh.scan[w][k];
+          tot[k] += sh.scan[w][k];
+        }
+      const int end = base[0] + v[0], first = end - own[0];
+      if (want >= first && want < end) {
+        sh.found[0] = b;
+        sh.found[1] = want - first;
+        sh.found[2] = base[1] + v[1] - own[1];
       }
-    const int end = base[0] + v[0], first = end - own[0];
-    if (want >= first && want < end) {
-      sh.found[0] = b;
-      sh.found[1] = want - first;
-      sh.found[2] = base[1] + v[1] - own[1];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 2; ++k) base[k] += tot[k];
+      if (sh.found[0] >= 0 && blockIdx.x != 0) break;
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 2; ++k) base[k] += tot[k];
-    if (sh.found[0] >= 0 && blockIdx.x != 0) break;
+    if (blockIdx.x == 0 && tid == 0) *A.used = base[1];
+    P.b = __builtin_amdgcn_readfirstlane(sh.found[0]);
+    if (P.b < 0) return false;
+    in = __builtin_amdgcn_readfirstlane(sh.found[1]);
+    slot0 = __builtin_amdgcn_readfirstlane(sh.found[2]);
+    P.r = request(A, P.b);
+    int tiles;
+    cost(P.r, tiles, steps);
   }
-  if (blockIdx.x == 0 && tid == 0) *A.used = base[1];
-  P.b = __builtin_amdgcn_readfirstlane(sh.found[0]);
-  if (P.b < 0) return false;
-  const int in = __builtin_amdgcn_readfirstlane(sh.found[1]);
-  P.r = request(A, P.b);
-  int tiles, steps;
-  cost(P.r, tiles, steps);
   P.parts = (steps + C - 1) / C;
   P.rt = in / P.parts;
   P.part = in - P.rt * P.parts;
   P.s0 = P.part * C;
   P.s1 = min(steps, P.s0 + C);
-  P.slot = P.parts > 1 ? __builtin_amdgcn_readfirstlane(sh.found[2]) + in : -1;
+  P.slot = P.parts > 1 ? slot0 + in : -1;
   return true;
 }
 
@@ -258,28 +294,80 @@ __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Eight consecutive query values from element `at`.
-__device__ __forceinline__ void load8(const Att& A, int64_t at, float* x) {
-  if (A.q_vec && A.q_dtype == QKV_F32) {
-    const v4f* p = reinterpret_cast<const v4f*>(static_cast<const float*>(A.q) + at);
-    const v4f a = p[0], b = p[1];
+// A lane's part of its query row (element `at` on; 8 values from col(k) on for each product
+// step k) as f16, times a power of two that brings the row's largest into [2^9, 2^10):
+// 16-bit types are exact so, fp32 takes lo beside it.  Lanes FIRST and 32 apart share a row.
+// c: what turns a score of these into an exponent of 2.  stage: THR * 8 KS floats of LDS.
+template <int KS, bool LO, int THR, int FIRST, typename Col>
+__device__ __forceinline__ void load_query(const Att& A, int64_t at, bool live, Col col,
+                                           float* stage, v8h* qh, v8h* ql, float& c) {
+  float x[KS][8];
+  if (A.q_vec && A.q_dtype != QKV_F32) {
+    v4u w[KS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] = a[j];
-      x[4 + j] = b[j];
+    for (int k = 0; k < KS; ++k)
+      w[k] = live ? *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(A.q) + at + col(k))
+                  : v4u{0, 0, 0, 0};
+    if (A.q_dtype == QKV_BF16) {
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          x[k][j] = __uint_as_float(j & 1 ? w[k][j >> 1] & 0xffff0000u : w[k][j >> 1] << 16);
+    } else {
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          x[k][j] = static_cast<float>(__builtin_bit_cast(v8h, w[k])[j]);
     }
   } else if (A.q_vec) {
-    const v4u w = *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(A.q) + at);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint16_t h = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
-      x[j] = A.q_dtype == QKV_BF16 ? qkv_bf16_to_f32(h)
-                                   : static_cast<float>(__builtin_bit_cast(_Float16, h));
+    for (int k = 0; k < KS; ++k) {
+      const v4f* const p = reinterpret_cast<const v4f*>(static_cast<const float*>(A.q) + at + col(k));
+      const v4f a = live ? p[0] : v4f{0.f, 0.f, 0.f, 0.f}, b = live ? p[1] : v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[k][j] = j < 4 ? a[j & 3] : b[j & 3];
     }
-  } else {
+  } else {  // (rolled, through LDS: it runs once, and unrolled it would be most of the code)
+    float* const t = stage + threadIdx.x;
+#pragma unroll 1
+    for (int k = 0; k < KS; ++k)
+#pragma unroll 1
+      for (int j = 0; j < 8; ++j)
+        t[(8 * k + j) * THR] = live ? qkv_load(A.q, at + col(k) + j, A.q_dtype) : 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = qkv_load(A.q, at + j, A.q_dtype);
+    for (int i = 0; i < 8 * KS; ++i) x[i >> 3][i & 7] = t[i * THR];
+    __syncthreads();
   }
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8 * KS; ++i) amax = fmaxf(amax, fabsf(x[i >> 3][i & 7]));
+#pragma unroll
+  for (int o = FIRST; o < 64; o *= 2) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+  int ex = 0;
+  if (amax > 0.f && amax < INFINITY) frexpf(amax, &ex);
+  ex = max(ex, -110);
+  const float up = ldexpf(1.f, 10 - ex);
+  c = ldexpf(A.scale * kLog2e, ex - 10);
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    v4u hi, lo;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t a, b;
+      split2(x[k][2 * j] * up, x[k][2 * j + 1] * up, a, b);
+      hi[j] = a;
+      lo[j] = b;
+    }
+    qh[k] = __builtin_bit_cast(v8h, hi);
+    if constexpr (LO) ql[k] = __builtin_bit_cast(v8h, lo);
+  }
+}
+
+// Tokens below this are seen by query qi of the piece's request.
+__device__ __forceinline__ int limit(const Att& A, const Req& r, int qi) {
+  return A.causal ? min(r.kv, r.kv - r.ql + qi + 1) : r.kv;
 }
 
 // Eight consecutive results to element `at` of out.

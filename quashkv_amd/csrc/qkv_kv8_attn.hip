@@ -39,53 +39,17 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
   const int n = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % A.H;
   Piece P;
-  if (!locate<kRows>(A, blockIdx.x / A.H, sh, P)) return;
+  if (!locate<kRows, kThr>(A, blockIdx.x / A.H, sh, P)) return;
 
   // ---- this lane's query row
   const int rr = P.rt * kRows + n, qi = rr / A.G, gq = rr - qi * A.G;
   const int64_t row = int64_t(P.r.q0) + qi;
   const bool live = qi < P.r.ql && row >= 0 && row < A.rows;
   const int hq = h * A.G + gq;
-  v8h qh[KS], ql[QLO ? KS : 1];
-  float c;  // scores to exponents, without the block's scale
-  {
-    float x[KS][8];
-    float amax = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[ks][j] = 0.f;
-      if (live) load8(A, row * A.q_ts + hq * A.q_hs + dcol(D, ks, g), x[ks]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[ks][j]));
-    }
-    amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-    int ex = 0;
-    if (amax > 0.f && amax < INFINITY) frexpf(amax, &ex);
-    ex = max(ex, -110);
-    const float up = ldexpf(1.f, 10 - ex);  // the row's largest into [2^9, 2^10)
-    c = ldexpf(A.scale * kLog2e, ex - 10);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      v4u hi, lo;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t a, b;
-        split2(x[ks][2 * j] * up, x[ks][2 * j + 1] * up, a, b);
-        hi[j] = a;
-        lo[j] = b;
-      }
-      qh[ks] = __builtin_bit_cast(v8h, hi);
-      if constexpr (QLO) ql[ks] = __builtin_bit_cast(v8h, lo);
-    }
-  }
-  // tokens below lim are seen; all rows of the tile see those below lim_all
-  const int lim = !live ? 0 : A.causal ? min(P.r.kv, P.r.kv - P.r.ql + qi + 1) : P.r.kv;
-  int lim_all = live ? lim : INT32_MAX;
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) lim_all = min(lim_all, __shfl_xor(lim_all, o, 64));
-  lim_all = __builtin_amdgcn_readfirstlane(lim_all);
+  // tokens below lim are seen; all live rows of the tile see those below lim_all (its first
+  // row's: rows are query-major)
+  const int lim = live ? limit(A, P.r, qi) : 0;
+  const int lim_all = limit(A, P.r, P.rt * kRows / A.G);
   const int n_tok = P.r.kv;
 
   v4f o[NJ];
@@ -151,6 +115,10 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
     load_k(row0);
     load_v(row0);
   }
+  v8h qh[KS], ql[QLO ? KS : 1];
+  float c;  // scores to exponents, without the block's scale
+  load_query<KS, QLO, kThr, 16>(A, row * A.q_ts + hq * A.q_hs, live,
+                                [&](int k) { return dcol(D, k, g); }, &red_o[0][0][0], qh, ql, c);
 #pragma unroll 1
   for (int it = 0; it < steps; ++it) {
     const int t0 = (P.s0 + wave + kWaves * it) * kStep;
@@ -169,7 +137,8 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
     }
     const float ck = c * ks_r, vs = vs_r;
     const bool pos = vs > 0.f;
-    const float lv = pos ? __builtin_amdgcn_logf(vs) : 0.f;
+    float ref = m == -INFINITY ? 0.f : m - kUp;
+    const float lv = (pos ? __builtin_amdgcn_logf(vs) : 0.f) - ref;
     const float iv = pos ? __builtin_amdgcn_rcpf(vs) : 1.f;
     const bool was_ok = ok;
     const bool more = it + 1 < steps;
@@ -177,12 +146,13 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
       row0 = row_of(it + 1, ok);
       load_k(row0);
     }
-    // ---- weights
+    // ---- exponents of the weights, against the running maximum so far
     float y[16], top = -INFINITY;
     const bool edge = t0 + kStep > lim_all || !was_ok;
 #pragma unroll
     for (int k = 0; k < 16; ++k) y[k] = fmaf(s[k >> 2][k & 3], ck, lv);
     if (edge) {
+      asm volatile("");  // (a branch: as selects it would cost every step)
       const int left = was_ok ? lim - t0 - 16 * g : 0;  // of this lane's 16 tokens
 #pragma unroll
       for (int k = 0; k < 16; ++k) y[k] = k < left ? y[k] : -INFINITY;
@@ -200,19 +170,21 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
     for (int k = 0; k < 16; ++k) top = fmaxf(top, y[k]);
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (__any(top > m + kHead || m == -INFINITY)) {
-      const float mn = fmaxf(m, top);
+    if (__any(top > kUp + kHead || m == -INFINITY)) {
+      const float mn = fmaxf(m, top + ref);
       const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      const float by = mn == -INFINITY ? 0.f : mn - kUp - ref;
       m = mn;
       l *= f;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) o[j] *= f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) y[k] -= by;
     }
-    const float ref = m == -INFINITY ? 0.f : m - kUp;
     float sum = 0.f;
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
-      y[k] = __builtin_amdgcn_exp2f(y[k] - ref);
+      y[k] = __builtin_amdgcn_exp2f(y[k]);
       sum += y[k];
     }
     l = fmaf(sum, iv, l);
@@ -289,7 +261,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
   }
 }
 
-// Pieces that a launch aims at, per kv head: two workgroups per CU.
+// Pieces that a launch of decode8 aims at, per kv head: two workgroups per CU.
 int32_t target_of(int32_t H) { return std::max(1, (2 * qkv_num_cus() + H - 1) / H); }
 // Cut tiles have more than C steps each and pieces of C, so they have fewer than
 // 2 total / C <= 2 target pieces.
@@ -392,6 +364,7 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   A.out_dtype = out_dtype;
   A.out_vec = qkv_aligned(out, 16) && d * ob % 16 == 0;
   A.target = target_of(Hkv);
+  A.per_target = 1.f / A.target;
   A.nslots = static_cast<int32_t>(slots_of(Hkv));
   place_parts(A, workspace, kRows, d);
   const int64_t longest = q_start ? std::min(max_q, rows) : A.uniform_q;
@@ -424,6 +397,8 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   }
   if (pre) {
     place_parts(A, static_cast<uint8_t*>(workspace) + part_bytes(Hkv, kRows, d), kPreRows, d);
+    A.target = std::max(1, A.target / 2);  // one workgroup per CU
+    A.per_target = 1.f / A.target;
     const int64_t t = tiles_of(kPreRows);
     qkv_kv8_prefill(A, d, fmt == QKV_CODES_E4M3, static_cast<uint32_t>(t),
                     cut && (q_start || t < A.target), s);

@@ -1,19 +1,23 @@
 // Attention of many query rows of a request (a prompt, a chunk of one) over the 8-bit
 // paged cache: decode8's mathematics (qkv_kv8_attn.hip) on tiles of 128 query rows.
 //
-// A workgroup of 4 waves takes 128 rows (query-major), a wave 32 of them, and steps through
-// 64 tokens: the step's codes become f16 in LDS once, in the order in which the matrix
-// instruction takes them (images of 64 lanes x 16 bytes), double buffered with one
-// barrier a step; the next step's bytes are in flight meanwhile.  Scores S^T = K Q^T and
-// values O^T = V^T P^T run on v_mfma_f32_32x32x16_f16: a lane owns one query row, score
-// register 8 b + j of a 32-token tile belongs to its block b, and the weights of a block
-// are, as they stand, the B operand of the value product if the A operand takes the V
-// block's dwords h and 2 + h.
+// A workgroup of 8 waves takes 128 rows (query-major): wave w the rows 32 (w % 4) .. of
+// every step of 64 tokens that is even (waves 0-3) or odd (4-7), so that a SIMD always has
+// two waves and the longest tile, which a causal launch waits for, takes half as long.
+// A step's codes become f16 in LDS once, in the order in which the matrix instruction
+// takes them (images of 64 lanes x 16 bytes), double buffered with one barrier a round;
+// the next round's bytes are in flight meanwhile.  Scores S^T = K Q^T and values
+// O^T = V^T P^T run on v_mfma_f32_32x32x16_f16: a lane owns one query row, score register
+// 8 b + j of a 32-token tile belongs to its block b, and the weights of a block are, as
+// they stand, the B operand of the value product if the A operand takes the V block's
+// dwords h and 2 + h.  The halves' sums meet in LDS at the end.
 #include "qkv_kv8_attn.h"
 
 namespace {
 
 using namespace qkv_kv8;
+
+constexpr int kPreThr = 512;
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 
@@ -22,75 +26,41 @@ __device__ __forceinline__ v16f mfma32(v4u a, v8h b, v16f c) {
 }
 
 template <int D, bool FP8, bool QLO, bool PLO>
-__global__ __launch_bounds__(kThr, 2) void prefill8(Att A) {
+__global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
   constexpr int KK = D / 16;                     // 16-wide product steps of a score
   constexpr int DT = D / 32;                     // 32-wide coordinate tiles
   constexpr int CH = 4 * D;                      // 16-byte chunks of K and of V in a step
-  constexpr int NC = (CH + kThr - 1) / kThr;     // of them, per thread
+  constexpr int NC = (CH + 255) / 256;           // of them, per thread of a half
   constexpr int KB = 2 * KK * 1024, VB = 4 * DT * 1024;
   __shared__ Shared sh;
-  __shared__ v4f sbuf[2][4];                     // a block's ks, log2 vs, 1 / vs
+  __shared__ v4f sbuf[2][2][4];                  // a block's ks, log2 vs, 1 / vs
   extern __shared__ __align__(16) uint8_t lds[];
-  // of buffer i: K's images (32-token tile, product step), V's (coordinate tile, block)
-  auto kbuf = [&](int i) { return lds + i * (KB + VB); };
-  auto vbuf = [&](int i) { return lds + i * (KB + VB) + KB; };
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x & 255, lane = tid & 63;
+  const int wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = wave8 & 3, th = wave8 >> 2;
+  // the half's buffer i: K's images (32-token tile, product step), V's (coordinate tile, block)
+  auto kbuf = [&](int i) { return lds + (2 * i + th) * (KB + VB); };
+  auto vbuf = [&](int i) { return kbuf(i) + KB; };
   const int n = lane & 31, hf = lane >> 5;
   const int h = blockIdx.x % A.H;
   Piece P;
-  if (!locate<kPreRows>(A, blockIdx.x / A.H, sh, P)) return;
+  if (!locate<kPreRows, kPreThr>(A, blockIdx.x / A.H, sh, P)) return;
 
   // ---- this lane's query row
   const int rr = P.rt * kPreRows + 32 * wave + n, qi = rr / A.G, gq = rr - qi * A.G;
   const int64_t row = int64_t(P.r.q0) + qi;
   const bool live = qi < P.r.ql && row >= 0 && row < A.rows;
   const int hq = h * A.G + gq;
-  v8h qh[KK], ql[QLO ? KK : 1];
-  float c;
-  {
-    float x[KK][8];
-    float amax = 0.f;
-#pragma unroll
-    for (int k = 0; k < KK; ++k) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[k][j] = 0.f;
-      if (live) load8(A, row * A.q_ts + hq * A.q_hs + 16 * k + 8 * hf, x[k]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[k][j]));
-    }
-    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-    int ex = 0;
-    if (amax > 0.f && amax < INFINITY) frexpf(amax, &ex);
-    ex = max(ex, -110);
-    const float up = ldexpf(1.f, 10 - ex);
-    c = ldexpf(A.scale * kLog2e, ex - 10);
-#pragma unroll
-    for (int k = 0; k < KK; ++k) {
-      v4u hi, lo;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t a, b;
-        split2(x[k][2 * j] * up, x[k][2 * j + 1] * up, a, b);
-        hi[j] = a;
-        lo[j] = b;
-      }
-      qh[k] = __builtin_bit_cast(v8h, hi);
-      if constexpr (QLO) ql[k] = __builtin_bit_cast(v8h, lo);
-    }
-  }
-  const int lim = !live ? 0 : A.causal ? min(P.r.kv, P.r.kv - P.r.ql + qi + 1) : P.r.kv;
-  int lim_all = live ? lim : INT32_MAX, lim_any = lim;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    lim_all = min(lim_all, __shfl_xor(lim_all, o, 64));
-    lim_any = max(lim_any, __shfl_xor(lim_any, o, 64));
-  }
-  lim_all = __builtin_amdgcn_readfirstlane(lim_all);
-  lim_any = __builtin_amdgcn_readfirstlane(lim_any);
+  // tokens below lim are seen; all of the wave's live rows see those below lim_all (its
+  // first row's: rows are query-major), and none those from lim_any on
+  const int lim = live ? limit(A, P.r, qi) : 0;
+  const int q_first = (P.rt * kPreRows + 32 * wave) / A.G;
+  const int q_last = min(P.r.ql - 1, (P.rt * kPreRows + 32 * wave + 31) / A.G);
+  const int lim_all = limit(A, P.r, q_first);
+  const int lim_any = q_first < P.r.ql ? limit(A, P.r, q_last) : 0;
   // the workgroup's last token: its last live query's
   const int qlast = min(P.r.ql - 1, (P.rt * kPreRows + kPreRows - 1) / A.G);
-  const int last = A.causal ? min(P.r.kv, P.r.kv - P.r.ql + qlast + 1) : P.r.kv;
+  const int last = limit(A, P.r, qlast);
   const int s1 = min(P.s1, (max(last, 0) + kStep - 1) / kStep);
 
   v16f o[DT];
@@ -108,11 +78,11 @@ __global__ __launch_bounds__(kThr, 2) void prefill8(Att A) {
   int pages = 0, p_first = 0;
   bool ok_r = false;  // of the step in flight
   auto fetch = [&](int st) {
-    if (st == P.s0 || st - p_first >= 64) {
+    if (st == P.s0 + th || st - p_first >= 128) {
       p_first = st;
-      pages = st + lane < P.s1 ? tab[(st + lane) >> pg_sh] : -1;
+      pages = st + 2 * lane < P.s1 ? tab[(st + 2 * lane) >> pg_sh] : -1;
     }
-    const int pg = __builtin_amdgcn_readlane(pages, st - p_first);
+    const int pg = __builtin_amdgcn_readlane(pages, (st - p_first) >> 1);
     ok_r = pg >= 0 && pg < A.npages;
     const int64_t row0 = ((int64_t(ok_r ? pg : 0) * A.H + h) << A.lg) +
                          (int64_t(st) * kStep & ((int64_t(1) << A.lg) - 1));
@@ -124,8 +94,8 @@ __global__ __launch_bounds__(kThr, 2) void prefill8(Att A) {
     const v4u* const vp = reinterpret_cast<const v4u*>(A.vpool + row0 * D);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int ch = tid + kThr * i;
-      if (CH % kThr == 0 || ch < CH) {
+      const int ch = tid + 256 * i;
+      if (CH % 256 == 0 || ch < CH) {
         kr[i] = kp[ch];
         vr[i] = vp[ch];
       }
@@ -136,13 +106,13 @@ __global__ __launch_bounds__(kThr, 2) void prefill8(Att A) {
     const int keep = ok_r ? P.r.kv - st * kStep : 0;  // tokens of the step
     if (tid < 4) {
       const bool pos = vs_r > 0.f;
-      sbuf[to][tid] = v4f{ks_r, pos ? __builtin_amdgcn_logf(vs_r) : 0.f,
+      sbuf[to][th][tid] = v4f{ks_r, pos ? __builtin_amdgcn_logf(vs_r) : 0.f,
                           pos ? __builtin_amdgcn_rcpf(vs_r) : 1.f, 0.f};
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int ch = tid + kThr * i;
-      if (CH % kThr != 0 && ch >= CH) continue;
+      const int ch = tid + 256 * i;
+      if (CH % 256 != 0 && ch >= CH) continue;
       {  // token ch / KK, coordinates 16 (ch % KK) ..: the places are swizzled by the product
          // step so that a row's chunks meet different banks
         const int t = ch / KK, k = ch % KK;
@@ -154,6 +124,7 @@ __global__ __launch_bounds__(kThr, 2) void prefill8(Att A) {
         const int blk = ch / D, dd = ch % D;
         v4u w = vr[i];
         if (keep < kStep) {  // codes behind the cached tokens may be anything
+          asm volatile("");  // (a branch: as selects it would cost every step)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int k = keep - 16 * blk - 4 * x;
@@ -167,21 +138,32 @@ __global__ __launch_bounds__(kThr, 2) void prefill8(Att A) {
     }
   };
 
-  if (P.s0 < s1) {
-    fetch(P.s0);
-    put(P.s0, 0);
-  }
-  bool ok = ok_r;
+  const int mine = P.s0 + th;  // this half's first step
+  if (mine < s1) fetch(mine);
+  v8h qh[KK], ql[QLO ? KK : 1];
+  float c;  // scores to exponents, without the block's scale
+  load_query<KK, QLO, kPreThr, 32>(A, row * A.q_ts + hq * A.q_hs, live,
+                                   [&](int k) { return 16 * k + 8 * hf; },
+                                   reinterpret_cast<float*>(lds), qh, ql, c);
+  if (mine < s1) put(mine, 0);
+  bool ok = ok_r;  // of the step to come
+  if (th == 1 && mine + 2 < s1) fetch(mine + 2);
   __syncthreads();
 #pragma unroll 1
-  for (int st = P.s0; st < s1; ++st) {
-    const int buf = (st - P.s0) & 1, t0 = st * kStep;
-    const bool more = st + 1 < s1, was_ok = ok;
-    if (more) {
-      fetch(st + 1);
+  for (int s0 = P.s0; s0 < s1; s0 += 2) {
+    const int st = s0 + th, buf = ((s0 - P.s0) >> 1) & 1, t0 = st * kStep;
+    const bool more = st + 2 < s1, was_ok = ok;
+    // the second half widens its next step before the products, the first one behind them:
+    // one wave's products then meet the other's VALU work
+    if (th == 0) {
+      if (more) fetch(st + 2);
       ok = ok_r;
+    } else if (more) {
+      ok = ok_r;
+      put(st + 2, buf ^ 1);
+      if (st + 4 < s1) fetch(st + 4);
     }
-    if (t0 < lim_any) {
+    if (st < s1 && t0 < lim_any) {
       // ---- scores: register 8 b + j of tile i is token 32 i + 16 b + (j & 3) + 8 (j >> 2) + 4 hf
       v16f s[2];
 #pragma unroll
@@ -196,21 +178,22 @@ __global__ __launch_bounds__(kThr, 2) void prefill8(Att A) {
           if constexpr (QLO) s[i] = mfma32(a, ql[k], s[i]);
         }
       }
-      // ---- weights
+      // ---- exponents of the weights, against the running maximum so far
       float iv[4];
-      float top = -INFINITY;
+      float top = -INFINITY, ref = m == -INFINITY ? 0.f : m - kUp;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const v4f sc = sbuf[buf][b];
-        const float ck = c * sc[0];
+        const v4f sc = sbuf[buf][th][b];
+        const float ck = c * sc[0], lv = sc[1] - ref;
         iv[b] = sc[2];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int e = 8 * (b & 1) + j;
-          s[b >> 1][e] = fmaf(s[b >> 1][e], ck, sc[1]);
+          s[b >> 1][e] = fmaf(s[b >> 1][e], ck, lv);
         }
       }
       if (t0 + kStep > lim_all || !was_ok) {
+        asm volatile("");
         const int left = (was_ok ? lim : 0) - t0 - 4 * hf;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -223,25 +206,29 @@ __global__ __launch_bounds__(kThr, 2) void prefill8(Att A) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) top = fmaxf(top, s[i][j]);
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      if (__any(top > m + kHead || m == -INFINITY)) {
-        const float mn = fmaxf(m, top);
+      if (__any(top > kUp + kHead || m == -INFINITY)) {
+        const float mn = fmaxf(m, top + ref);
         const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        const float by = mn == -INFINITY ? 0.f : mn - kUp - ref;
         m = mn;
         l *= f;
 #pragma unroll
         for (int j = 0; j < DT; ++j)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[j][i] *= f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[i][j] -= by;
       }
-      const float ref = m == -INFINITY ? 0.f : m - kUp;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         float sum = 0.f;
         v4u hi, lo;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float p0 = __builtin_amdgcn_exp2f(s[b >> 1][8 * (b & 1) + 2 * j] - ref);
-          const float p1 = __builtin_amdgcn_exp2f(s[b >> 1][8 * (b & 1) + 2 * j + 1] - ref);
+          const float p0 = __builtin_amdgcn_exp2f(s[b >> 1][8 * (b & 1) + 2 * j]);
+          const float p1 = __builtin_amdgcn_exp2f(s[b >> 1][8 * (b & 1) + 2 * j + 1]);
           sum += p0 + p1;
           uint32_t x, y = 0;
           if constexpr (PLO) split2(p0, p1, x, y);
@@ -259,48 +246,68 @@ __global__ __launch_bounds__(kThr, 2) void prefill8(Att A) {
         }
       }
     }
-    if (more) put(st + 1, buf ^ 1);
+    if (th == 0 && more) put(st + 2, buf ^ 1);
     __syncthreads();
   }
 
-  // ---- lane (n, hf) has coordinates 32 j + 8 q + 4 hf + 0 .. 3 of row n
+  // ---- the halves join: the first takes over the first coordinate tiles, the second the
+  // others (the loop's last barrier is behind the buffers' last readers)
+  constexpr int KEEP = (DT + 1) / 2;
   l += __shfl_xor(l, 32, 64);
-  const int64_t slot = P.slot >= 0 ? place(A, P, h) : -1;
-  if (!live) return;
-  if (P.slot < 0) {
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int64_t at = (row * A.Hq + hq) * D + 4 * hf;
+  float* const box = reinterpret_cast<float*>(lds) + lane;
+  auto at_box = [&](int j, int i) { return box + ((wave * DT + j) * 16 + i) * 64; };
+  float* const ml = reinterpret_cast<float*>(lds) + 4 * DT * 16 * 64 + lane;  // [half][wave][2]
 #pragma unroll
-    for (int j = 0; j < DT; ++j)
+  for (int j = 0; j < DT; ++j)
+    if ((j < KEEP) == (th == 1))
+#pragma unroll
+      for (int i = 0; i < 16; ++i) *at_box(j, i) = o[j][i];
+  ml[(2 * wave8) * 64] = m;
+  ml[(2 * wave8 + 1) * 64] = l;
+  const int64_t slot = P.slot >= 0 ? place(A, P, h) : -1;
+  __syncthreads();
+  if (!live) return;
+  const float m2 = ml[(2 * (wave8 ^ 4)) * 64], l2 = ml[(2 * (wave8 ^ 4) + 1) * 64];
+  const float M = fmaxf(m, m2), base = M == -INFINITY ? 0.f : M;
+  float e1 = __builtin_amdgcn_exp2f(m - base), e2 = __builtin_amdgcn_exp2f(m2 - base);
+  const float L = l * e1 + l2 * e2;
+  // lane (n, hf) has coordinates 32 j + 8 q + 4 hf + 0 .. 3 of row n
+  if (P.slot < 0) {
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    e1 *= inv;
+    e2 *= inv;
+  }
+  const int64_t at = P.slot < 0 ? row * A.Hq + hq : slot * kPreRows + 32 * wave + n;
+  if (P.slot >= 0 && slot < 0) return;
+#pragma unroll
+  for (int j = 0; j < DT; ++j)
+    if ((j < KEEP) == (th == 0))
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float x[4] = {o[j][4 * q] * inv, o[j][4 * q + 1] * inv, o[j][4 * q + 2] * inv,
-                            o[j][4 * q + 3] * inv};
-        store4(A.out, at + 32 * j + 8 * q, x, A.out_dtype, A.out_vec);
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[i] = o[j][4 * q + i] * e1 + *at_box(j, 4 * q + i) * e2;
+        const int64_t to = at * D + 32 * j + 8 * q + 4 * hf;
+        if (P.slot < 0) store4(A.out, to, x, A.out_dtype, A.out_vec);
+        else *reinterpret_cast<v4f*>(A.part_o + to) = v4f{x[0], x[1], x[2], x[3]};
       }
-  } else if (slot >= 0) {
-    const int64_t at = slot * kPreRows + 32 * wave + n;
-#pragma unroll
-    for (int j = 0; j < DT; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<v4f*>(A.part_o + at * D + 32 * j + 8 * q + 4 * hf) =
-            v4f{o[j][4 * q], o[j][4 * q + 1], o[j][4 * q + 2], o[j][4 * q + 3]};
-    if (hf == 0) {
-      A.part_ml[2 * at] = m;
-      A.part_ml[2 * at + 1] = l;
-    }
+  if (P.slot >= 0 && hf == 0 && th == 0) {
+    A.part_ml[2 * at] = M;
+    A.part_ml[2 * at + 1] = L;
   }
 }
 
 template <int D, bool FP8, bool QLO, bool PLO>
 void start(const Att& A, uint32_t tiles, hipStream_t s) {
-  constexpr int smem = 2 * (2 * (D / 16) + 4 * (D / 32)) * 1024;
+  // two buffers of both halves; at the end D / 32 coordinate tiles, m and l
+  constexpr int smem = std::max(4 * (2 * (D / 16) + 4 * (D / 32)) * 1024,
+                                (4 * (D / 32) * 16 + 16) * 256);
   // (a failure is the launch's, which the caller reports)
   static const hipError_t attr [[maybe_unused]] = hipFuncSetAttribute(
       reinterpret_cast<const void*>(&prefill8<D, FP8, QLO, PLO>),
       hipFuncAttributeMaxDynamicSharedMemorySize, smem);
-  prefill8<D, FP8, QLO, PLO><<<(tiles + A.target) * A.H, kThr, smem, s>>>(A);
+  prefill8<D, FP8, QLO, PLO><<<(tiles + A.target) * A.H, kPreThr, smem, s>>>(A);
 }
 
 template <int D, bool FP8>

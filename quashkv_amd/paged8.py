@@ -192,7 +192,8 @@ def append_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kpool: tor
                kscale: torch.Tensor, vpool: torch.Tensor, vscale: torch.Tensor) -> None:
     """Quantise rows k, v (rows, H, d; fp32, fp16 or bf16, any row and head
     strides) into the pools at ``slots`` ((rows,) int64, as plan_pages makes them:
-    the rows of a block follow each other, each slot once; -1 skips a row).
+    the rows of a block follow each other at consecutive slots, each slot once; -1
+    skips a row).
 
     A block's scale covers its largest finite value.  Tokens that the block
     holds already keep their codes while the scale stands and are quantised anew
