@@ -6,9 +6,11 @@
 //   code = the one nearest to x * fp32(1 / s), ties to even, at most Z; NaN gives 0.
 // A block that holds earlier tokens keeps its scale unless the new one is larger; then
 // their values, fp32(code * scale), are quantised anew.
-// x * (1 / s) in fp32 is off by half an ulp, which at a border between two codes would
-// decide for the wrong one: sticky_mul keeps what the rounding dropped in the last bit
-// (round to odd), so that rounding to a code afterwards is rounding once.
+// x * (1 / s) rounded to fp32 is off by half an ulp, which at a border between two codes
+// would decide for the wrong one.  So the product is never rounded by itself:
+// fma(x, 1 / s, M) with M = 1.5 * 2^23 times the spacing of the codes around it rounds the
+// exact product once, to a multiple of that spacing, ties to even -- one instruction a
+// value for int8, whose code then is the sum's low byte.
 //
 // Bytes bound it: 2 H d (in + 1) a row, and a decode step's token reads and writes its
 // V block (16 tokens) beside that.
@@ -16,26 +18,31 @@
 
 namespace {
 
-// x * m with the last bit set where the product is not exact (towards zero).
-__device__ __forceinline__ float sticky_mul(float x, float m) {
-  const float p = x * m, e = fmaf(x, m, -p);
-  uint32_t u = __float_as_uint(p);
-  if (e != 0.f) u = (u - ((e < 0.f) != (p < 0.f) ? 1u : 0u)) | 1u;
-  return __uint_as_float(u);
+// The code of x at inverse scale inv, |x| at most what the largest code stands for (but for
+// rounding): int8 in the low byte, e4m3 as a value that its conversion leaves as it is.
+template <bool FP8>
+__device__ __forceinline__ float near(float x, float inv) {
+  if constexpr (FP8) {
+    // the spacing is 2^-3 of the product's power of two, 2^-9 at least
+    const uint32_t e = max(__float_as_uint(x * inv) & 0x7f800000u, 121u << 23);
+    const float M = __uint_as_float(e + (20u << 23) + 0x400000u);
+    return fmaf(x, inv, M) - M;
+  } else {
+    return fmaf(x, inv, 12582912.f);
+  }
 }
 
-// The code of x at inverse scale inv, one byte.
+// Four codes of near() as bytes.
 template <bool FP8>
-__device__ __forceinline__ uint32_t code_of(float x, float inv) {
-  constexpr float Z = kTop<FP8>;
-  float p = x * inv;
-  if (fabsf(p) >= Z) p = copysignf(Z, p);
-  else p = sticky_mul(x, inv);
-  if (p != p) p = 0.f;  // (NaN, or an infinity in a block of zeros)
-  if constexpr (FP8)
-    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(p, p, 0, false)) & 0xffu;
-  else
-    return static_cast<uint32_t>(__float2int_rn(p)) & 0xffu;
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+  if constexpr (FP8) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true));
+  } else {
+    const uint32_t ab = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x0c0c0400u);
+    const uint32_t cd = __builtin_amdgcn_perm(__float_as_uint(d), __float_as_uint(c), 0x04000c0cu);
+    return ab | cd;
+  }
 }
 
 template <bool FP8>
@@ -123,19 +130,44 @@ __device__ __forceinline__ void store_n(void* x, int64_t at, bool vec, const flo
   }
 }
 
-// Scale and its inverse for a block whose largest new value is a, old: its scale so far.
-template <bool FP8>
-__device__ __forceinline__ float scale_of(float a, float old, bool& grew, float& inv) {
+// A block's scale: of the largest of a wave's values, or the old one where that is larger.
+// Values that are not finite do not count; they become what their codes stand for (the
+// largest value, NaN 0).
+template <bool FP8, int N>
+__device__ __forceinline__ float scale_of(float* x, float old, bool& grew, float& inv) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+  auto wave_max = [](uint32_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(int(v), o, 64)));
+    return v;
+  };
+  m = wave_max(m);
+  const bool odd = m >= 0x7f800000u;
+  if (odd) {
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
+      m = max(m, u < 0x7f800000u ? u : 0u);
+    }
+    m = wave_max(m);
+  }
+  const float a = __uint_as_float(m);
   float sc = a > 0.f ? fmaxf(a * (1.f / kTop<FP8>), kScaleFloor) : 0.f;
   grew = sc > old;
   sc = grew ? sc : old;
   inv = sc > 0.f ? 1.f / sc : 0.f;
+  if (odd) {
+    const float top = kTop<FP8> * sc;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (x[i] != x[i]) x[i] = 0.f;
+      x[i] = __builtin_amdgcn_fmed3f(x[i], -top, top);
+    }
+  }
   return sc;
-}
-
-__device__ __forceinline__ float finite_abs(float x) {
-  const float m = fabsf(x);
-  return m < INFINITY ? m : 0.f;
 }
 
 struct App {
@@ -191,7 +223,7 @@ __global__ __launch_bounds__(64 * kWaves) void append_runs(App A) {
     if (half == 0) {
       constexpr int LPR = D / 8, RPI = 64 / LPR, NI = (kBlk + RPI - 1) / RPI;
       const int sub = lane / LPR, c = 8 * (lane % LPR);
-      float x[NI][8], a = 0.f;
+      float x[NI][8];
 #pragma unroll
       for (int t = 0; t < NI; ++t) {
         const int j = RPI * t + sub;
@@ -200,11 +232,7 @@ __global__ __launch_bounds__(64 * kWaves) void append_runs(App A) {
         for (int i = 0; i < 8; ++i) x[t][i] = 0.f;
         if (on) load_n<8, DT>(A.x[0], src + j * A.ts[0] + c, A.vec[0], x[t]);
       }
-#pragma unroll
-      for (int t = 0; t < NI; ++t)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a = fmaxf(a, finite_abs(x[t][i]));
-      const float sc = scale_of<FP8>(qkv_wave_max(a), old, grew, inv);
+      const float sc = scale_of<FP8, 8 * NI>(&x[0][0], old, grew, inv);
 #pragma unroll
       for (int t = 0; t < NI; ++t) {
         const int j = RPI * t + sub;
@@ -217,10 +245,10 @@ __global__ __launch_bounds__(64 * kWaves) void append_runs(App A) {
           for (int i = 0; i < 8; ++i) x[t][i] = value_of<FP8>(w[i >> 2] >> (8 * (i & 3))) * old;
         }
         if (on || again) {
-          v2u w = {0, 0};
+          float y[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i >> 2] |= code_of<FP8>(x[t][i], inv) << (8 * (i & 3));
-          *k = w;
+          for (int i = 0; i < 8; ++i) y[i] = near<FP8>(x[t][i], inv);
+          *k = v2u{pack4<FP8>(y[0], y[1], y[2], y[3]), pack4<FP8>(y[4], y[5], y[6], y[7])};
         }
       }
       if (lane == 0) *sp = sc;
@@ -228,7 +256,7 @@ __global__ __launch_bounds__(64 * kWaves) void append_runs(App A) {
       constexpr int LPR = D / 2, TG = 64 / LPR, TL = kBlk / TG;  // lanes, token groups
       const int tg = lane / LPR, c = 2 * (lane % LPR);
       const bool on = tg < TG;
-      float x[TL][2], a = 0.f;
+      float x[TL][2];
 #pragma unroll
       for (int t = 0; t < TL; ++t) {
         const int j = TL * tg + t;
@@ -244,24 +272,25 @@ __global__ __launch_bounds__(64 * kWaves) void append_runs(App A) {
           for (int q = 0; q < TL / 4; ++q)
             w[i][q] = *reinterpret_cast<const uint32_t*>(v + kBlk * i + 4 * q);
       }
+      const float sc = scale_of<FP8, 2 * TL>(&x[0][0], old, grew, inv);
+      if (j0 > 0 && grew) {
 #pragma unroll
-      for (int t = 0; t < TL; ++t) a = fmaxf(a, fmaxf(finite_abs(x[t][0]), finite_abs(x[t][1])));
-      const float sc = scale_of<FP8>(qkv_wave_max(a), old, grew, inv);
+        for (int t = 0; t < TL; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (TL * tg + t < j0) x[t][i] = value_of<FP8>(w[i][t >> 2] >> (8 * (t & 3))) * old;
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int q = 0; q < TL / 4; ++q) {
-          uint32_t to = 0;
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const int t = 4 * q + b, j = TL * tg + t;
-            float y = x[t][i];
-            if (j0 > 0 && grew && j < j0) y = value_of<FP8>(w[i][q] >> (8 * b)) * old;
-            uint32_t code = code_of<FP8>(y, inv);
-            if (j0 > 0 && !grew && j < j0) code = w[i][q] >> (8 * b) & 0xffu;
-            to |= code << (8 * b);
-          }
-          w[i][q] = to;
+          const uint32_t to = pack4<FP8>(near<FP8>(x[4 * q][i], inv), near<FP8>(x[4 * q + 1][i], inv),
+                                         near<FP8>(x[4 * q + 2][i], inv),
+                                         near<FP8>(x[4 * q + 3][i], inv));
+          // earlier tokens whose scale stands keep their codes
+          const int k = grew ? 0 : j0 - TL * tg - 4 * q;
+          const uint32_t keep = k >= 4 ? ~0u : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
+          w[i][q] = (w[i][q] & keep) | (to & ~keep);
         }
       if (on) {
 #pragma unroll
@@ -371,7 +400,7 @@ __global__ __launch_bounds__(64 * kWaves) void read_rows(Rd A) {
 
 // Rows of a wave's unit: a block's where there are rows enough for every CU; else one, so
 // that a decode step's rows, each a run of its own, do not queue in one wave.
-int32_t chunk_of(int64_t rows) { return rows > 4096 ? 16 : 1; }
+int32_t chunk_of(int64_t rows) { return rows > 4096 ? 16 : rows > 512 ? 4 : 1; }
 
 }  // namespace
 
