@@ -46,6 +46,7 @@ struct Att {
   void* out;
   int32_t out_dtype, out_vec;
   int32_t few;      // requests of up to this many rows (queries x G) are decode8's
+  int32_t least;    // steps of the shortest piece, INT32_MAX / 2: nothing is cut
   int32_t target;   // pieces that a launch aims at, per kv head
   float per_target; // 1 / target
   int32_t nslots;   // partial results that the workspace holds
@@ -133,7 +134,7 @@ __device__ __forceinline__ bool locate(const Att& A, int want, Shared& sh, Piece
   auto piece_len = [&](float sum, int all) {
     if (PRE && all >= A.target) return INT32_MAX / 2;
     const int c = static_cast<int>(fminf(sum * A.per_target, 1e9f)) + 1;
-    return max(4, (c + ROUND - 1) / ROUND * ROUND);
+    return max(A.least, (c + ROUND - 1) / ROUND * ROUND);
   };
   // whole prefill tiles: the last ones first, of a causal prompt the longest
   auto order = [&](int C, int all) {

@@ -279,6 +279,10 @@ void place_parts(Att& A, void* at, int rows, int32_t d) {
 }
 // Requests of more rows than this go to prefill8.
 constexpr int kFew = 32;
+// A cache of up to this many tokens a request is not cut: its pieces' second launch costs
+// more than the steps that they would save.
+constexpr int64_t kWhole = 1024;
+constexpr int32_t kNever = INT32_MAX / 2;
 
 template <int D, bool FP8>
 void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
@@ -369,7 +373,9 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   place_parts(A, workspace, kRows, d);
   const int64_t longest = q_start ? std::min(max_q, rows) : A.uniform_q;
   const bool pre = longest * G > kFew;
-  A.few = pre ? kFew : INT32_MAX;
+  // decode8 runs too where, as far as the rows tell, a request may be short.  (Where one is
+  // against that, prefill8 takes it: slower, the same result.)
+  const bool dec = !pre || (q_start && rows <= (B - 1) * longest + kFew / G);
   // tiles of a launch, at most: a request's last one may be in part empty
   auto tiles_of = [&](int r) {
     return q_start ? rows * G / r + std::min<int64_t>(B, rows)
@@ -377,10 +383,11 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   };
   QKV_REQUIRE((tiles_of(kRows) + A.target) * Hkv <= INT32_MAX, "batch of %d requests and %lld "
               "rows is too large for one call", B, static_cast<long long>(rows));
-  // the shortest pieces have 4 steps
-  const bool cut = (int64_t(pages_per_seq) << A.lg) > int64_t(kStep) * 4;
+  const bool cut = (int64_t(pages_per_seq) << A.lg) > kWhole;
+  A.few = !pre ? INT32_MAX : dec ? kFew : 0;
+  A.least = cut ? 4 : kNever;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (q_start || !pre) {
+  if (dec) {
     // beside prefill8 this launch has only requests of up to kFew rows
     const uint32_t t = static_cast<uint32_t>(
         pre ? std::min<int64_t>(tiles_of(kRows), int64_t(B) * (kFew / kRows)) : tiles_of(kRows));
@@ -399,9 +406,11 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
     place_parts(A, static_cast<uint8_t*>(workspace) + part_bytes(Hkv, kRows, d), kPreRows, d);
     A.target = std::max(1, A.target / 2);  // one workgroup per CU
     A.per_target = 1.f / A.target;
+    // cut only where the tiles, as far as the rows tell, do not fill the card
     const int64_t t = tiles_of(kPreRows);
-    qkv_kv8_prefill(A, d, fmt == QKV_CODES_E4M3, static_cast<uint32_t>(t),
-                    cut && (q_start || t < A.target), s);
+    const bool cut8 = cut && rows * G / kPreRows < A.target;
+    A.least = cut8 ? 4 : kNever;
+    qkv_kv8_prefill(A, d, fmt == QKV_CODES_E4M3, static_cast<uint32_t>(t), cut8, s);
     QKV_LAUNCHED();
   }
   return QKV_OK;

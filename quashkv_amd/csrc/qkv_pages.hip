@@ -20,7 +20,8 @@
 
 namespace {
 
-constexpr int kThr = 1024;      // of the scan
+constexpr int kThr = 1024;      // of the scan; of a small batch's
+constexpr int kThrOne = 256;
 constexpr int kFill = 256;      // of the fill
 constexpr int kOneB = 2048;     // requests and rows that one workgroup does alone
 constexpr int64_t kOneRows = 4096;
@@ -50,23 +51,34 @@ struct Plan {
   int32_t* first;  // [B] free-list place of a request's first new page
 };
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t dpp(int64_t v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xf, false);
+  return (static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo);
+}
+
 // Inclusive sum over the workgroup's threads; `total` gets the sum of all.
 // part: one value per wave.
+template <int THR>
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part, int64_t& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
+  v += dpp<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v += dpp<0x112, 0xf>(v);
+  v += dpp<0x114, 0xf>(v);
+  v += dpp<0x118, 0xf>(v);
+  v += dpp<0x142, 0xa>(v);  // row_bcast 15, 31
+  v += dpp<0x143, 0xc>(v);
   __syncthreads();  // (part may still be read from the last call)
   if (lane == 63) part[wave] = v;
   __syncthreads();
   int64_t before = 0;
   total = 0;
-  for (int w = 0; w < int(blockDim.x >> 6); ++w) {
-    if (w < wave) before += part[w];
-    total += part[w];
+#pragma unroll
+  for (int w = 0; w < THR / 64; ++w) {
+    const int64_t u = part[w];
+    if (w < wave) before += u;
+    total += u;
   }
   return before + v;
 }
@@ -104,10 +116,10 @@ __device__ __forceinline__ int find_row(const int32_t* start, int B, int64_t r) 
   return lo;
 }
 
-template <bool ONE>
-__global__ __launch_bounds__(kThr) void plan_scan(Plan P) {
+template <int THR, bool ONE>
+__global__ __launch_bounds__(THR) void plan_scan(Plan P) {
   extern __shared__ int32_t sh[];  // ONE: start[B + 1], t0[B], q_len[B], first[B]
-  __shared__ int64_t part[kThr / 64];
+  __shared__ int64_t part[THR / 64];
   const int tid = threadIdx.x, B = P.B;
   const int64_t n = int64_t(1) << P.lg;
   const int64_t count = imin(imax(*P.free_count, 0), P.pool);
@@ -116,19 +128,19 @@ __global__ __launch_bounds__(kThr) void plan_scan(Plan P) {
     P.q_start[0] = 0;
     if (ONE) sh[0] = 0;
   }
-  for (int b0 = 0; b0 < B; b0 += kThr) {
+  for (int b0 = 0; b0 < B; b0 += THR) {
     const int b = b0 + tid;
     int64_t len = 0, add = 0, total;
     if (b < B) {
       len = imax(P.lens[b], 0);
       add = imax(P.add[b], 0);
     }
-    const int64_t end = rows0 + block_scan(add, part, total);
+    const int64_t end = rows0 + block_scan<THR>(add, part, total);
     rows0 += total;
     const int64_t held = (len + n - 1) >> P.lg, want = (len + add + n - 1) >> P.lg;
     const bool fits = end <= P.rows && want <= P.width && len + add <= INT32_MAX;
     const int64_t ask = fits ? want - held : 0;
-    const int64_t top = ask0 + block_scan(ask, part, total);
+    const int64_t top = ask0 + block_scan<THR>(ask, part, total);
     ask0 += total;
     const bool ok = fits && (ask == 0 || top <= count);
     if (b < B) {
@@ -147,13 +159,13 @@ __global__ __launch_bounds__(kThr) void plan_scan(Plan P) {
         P.first[b] = first;
       }
     }
-    block_scan(ok ? ask : 0, part, total);
+    block_scan<THR>(ok ? ask : 0, part, total);
     taken += total;
   }
   if (tid == 0) *P.free_out = static_cast<int32_t>(count - taken);
   if (ONE) {
     __syncthreads();
-    for (int64_t r = tid; r < P.rows; r += kThr) {
+    for (int64_t r = tid; r < P.rows; r += THR) {
       const int b = find_row(sh, B, r);
       if (b < 0) fill_row(P, r, 0, 0, 0, 0, 0);
       else fill_row(P, r, b, r - sh[b], sh[B + 1 + b], sh[2 * B + 1 + b], sh[3 * B + 1 + b]);
@@ -194,7 +206,7 @@ __global__ __launch_bounds__(kThr) void release_pages(int32_t* lens, const uint8
       held = imin((imax(lens[b], 0) + n - 1) >> lg, width);
       lens[b] = 0;
     }
-    const int64_t end = base + block_scan(held, part, total);
+    const int64_t end = base + block_scan<kThr>(held, part, total);
     base += total;
     if (b < B) sh[b + 1] = static_cast<int32_t>(imin(end, INT32_MAX));
   }
@@ -237,9 +249,11 @@ extern "C" int qkv_page_plan(const int32_t* lens, const int32_t* new_lens, int32
          qkv_page_lg(page_tokens), rows,  q_start,       q_lens,         kv_lens,   slots,
          positions, free_count_out, scratch};
   if (B <= kOneB && rows <= kOneRows) {
-    plan_scan<true><<<1, kThr, (4 * B + 1) * sizeof(int32_t), s>>>(P);
+    const uint32_t lds = (4 * B + 1) * sizeof(int32_t);
+    if (B <= kThrOne && rows <= kThrOne) plan_scan<kThrOne, true><<<1, kThrOne, lds, s>>>(P);
+    else plan_scan<kThr, true><<<1, kThr, lds, s>>>(P);
   } else {
-    plan_scan<false><<<1, kThr, 0, s>>>(P);
+    plan_scan<kThr, false><<<1, kThr, 0, s>>>(P);
     QKV_LAUNCHED();
     if (rows > 0)
       plan_fill<<<static_cast<uint32_t>((rows + kFill - 1) / kFill), kFill,

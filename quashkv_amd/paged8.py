@@ -41,29 +41,20 @@ CODE_DTYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 _FMT = {torch.int8: N.QKV_CODES_I8, torch.float8_e4m3fn: N.QKV_CODES_E4M3}
 
 
-class _On:
-    """Makes ``dev`` the current device for a library call (launches go to the
-    current device, whatever device the tensors' stream belongs to)."""
-
-    __slots__ = ("was", "dev")
-
-    def __init__(self, dev: torch.device):
-        self.dev = dev.index if dev.index is not None else torch.cuda.current_device()
-
-    def __enter__(self):
-        self.was = torch.cuda.current_device()
-        if self.was != self.dev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc):
-        if self.was != self.dev:
-            torch.cuda.set_device(self.was)
+def _call(dev: torch.device, fn, *args) -> None:
+    """fn(*args, stream) on ``dev``, which is made the current device for it:
+    launches go there, whatever device the stream belongs to."""
+    if dev.index == torch.cuda.current_device():
+        N.check(fn(*args, N.stream(dev)))
+    else:
+        with torch.cuda.device(dev):
+            N.check(fn(*args, N.stream(dev)))
 
 
 def _want(t: torch.Tensor, what: str, dtype: torch.dtype, shape: Optional[tuple] = None) -> None:
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{what} must be {dtype}; got {t.dtype}")
-    if shape is not None and tuple(t.shape) != shape:
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{what} must have shape {shape}; got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous")
@@ -87,12 +78,13 @@ class PagePlan:
               max_q_len: Optional[int] = None) -> "PagePlan":
         if rows < 0:
             raise ValueError(f"rows must not be negative; got {rows}")
-        i32 = dict(dtype=torch.int32, device=device)
-        return cls(torch.empty(B + 1, **i32), torch.empty(B, **i32),
-                   torch.empty(B, **i32) if kv_lens is None else kv_lens,
-                   torch.empty(rows, dtype=torch.int64, device=device), torch.empty(rows, **i32),
-                   torch.empty(1, **i32) if free_count is None else free_count,
-                   torch.empty(B, **i32), rows if max_q_len is None else max_q_len)
+        # one allocation for the int32 parts
+        q_start, q_lens, kv, positions, scratch, count = torch.empty(
+            4 * B + rows + 2, dtype=torch.int32, device=device).split((B + 1, B, B, rows, B, 1))
+        return cls(q_start, q_lens, kv if kv_lens is None else kv_lens,
+                   torch.empty(rows, dtype=torch.int64, device=device), positions,
+                   count if free_count is None else free_count, scratch,
+                   rows if max_q_len is None else max_q_len)
 
 
 def plan_pages(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor,
@@ -133,13 +125,11 @@ def plan_pages(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor,
             _want(getattr(out, name), f"out.{name}", dt, shape)
         N.require_gpu(table, out.q_start, out.q_lens, out.kv_lens, out.slots, out.positions,
                       out.free_count, out.scratch, what="plan_pages")
-    with _On(dev):
-        N.check(N.lib().qkv_page_plan(
-            lens.data_ptr(), new_lens.data_ptr(), B, table.data_ptr(), width, free.data_ptr(),
-            free.numel(), free_count.data_ptr(), page_tokens, rows, out.q_start.data_ptr(),
-            out.q_lens.data_ptr(), out.kv_lens.data_ptr(), out.slots.data_ptr(),
-            out.positions.data_ptr(), out.free_count.data_ptr(), out.scratch.data_ptr(),
-            N.stream(dev)))
+    _call(dev, N.lib().qkv_page_plan, lens.data_ptr(), new_lens.data_ptr(), B, table.data_ptr(),
+          width, free.data_ptr(), free.numel(), free_count.data_ptr(), page_tokens, rows,
+          out.q_start.data_ptr(), out.q_lens.data_ptr(), out.kv_lens.data_ptr(),
+          out.slots.data_ptr(), out.positions.data_ptr(), out.free_count.data_ptr(),
+          out.scratch.data_ptr())
     return out
 
 
@@ -158,10 +148,8 @@ def release_pages(table: torch.Tensor, lens: torch.Tensor, done: torch.Tensor,
         raise ValueError("free must be a 1-D int32 tensor")
     _want(free, "free", torch.int32)
     _want(free_count, "free_count", torch.int32, (1,))
-    with _On(dev):
-        N.check(N.lib().qkv_page_release(
-            lens.data_ptr(), done.data_ptr(), B, table.data_ptr(), width, free.data_ptr(),
-            free.numel(), free_count.data_ptr(), page_tokens, N.stream(dev)))
+    _call(dev, N.lib().qkv_page_release, lens.data_ptr(), done.data_ptr(), B, table.data_ptr(),
+          width, free.data_ptr(), free.numel(), free_count.data_ptr(), page_tokens)
 
 
 def _check_pools(kpool: torch.Tensor, kscale: torch.Tensor, vpool: torch.Tensor,
@@ -207,11 +195,9 @@ def append_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kpool: tor
                          f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
     _want(slots, "slots", torch.int64, (rows,))
     k, v = _dense_last(k), _dense_last(v)
-    with _On(dev):
-        N.check(N.lib().qkv_kv8_append(
-            N.dtype_code(k.dtype), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-            v.stride(0), v.stride(1), slots.data_ptr(), rows, H, d, fmt, kpool.data_ptr(),
-            kscale.data_ptr(), vpool.data_ptr(), vscale.data_ptr(), P, n, N.stream(dev)))
+    _call(dev, N.lib().qkv_kv8_append, N.dtype_code(k.dtype), k.data_ptr(), k.stride(0),
+          k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(), rows, H, d, fmt,
+          kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(), vscale.data_ptr(), P, n)
 
 
 def read_kv8(slots: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
@@ -226,11 +212,9 @@ def read_kv8(slots: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
     dt = N.dtype_code(out_dtype)
     k = torch.empty(rows, H, d, dtype=out_dtype, device=dev)
     v = torch.empty_like(k)
-    with _On(dev):
-        N.check(N.lib().qkv_kv8_read(
-            slots.data_ptr(), rows, H, d, fmt, kpool.data_ptr(), kscale.data_ptr(),
-            vpool.data_ptr(), vscale.data_ptr(), P, n, k.data_ptr(), v.data_ptr(), dt,
-            N.stream(dev)))
+    _call(dev, N.lib().qkv_kv8_read, slots.data_ptr(), rows, H, d, fmt, kpool.data_ptr(),
+          kscale.data_ptr(), vpool.data_ptr(), vscale.data_ptr(), P, n, k.data_ptr(),
+          v.data_ptr(), dt)
     return k, v
 
 
@@ -290,13 +274,11 @@ def attention_kv8(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
                                 dtype=torch.uint8, device=dev)
     else:
         _want(workspace, "workspace", torch.uint8)
-    with _On(dev):
-        N.check(N.lib().qkv_kv8_attention(
-            q.data_ptr(), N.dtype_code(q.dtype), q.stride(0), q.stride(1), rows,
-            kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(), vscale.data_ptr(), fmt, P, n,
-            table.data_ptr(), width, N.ptr(q_start), N.ptr(q_lens), kv_lens.data_ptr(), B, Hq, H,
-            d, longest, float(scale), 1 if causal else 0, out.data_ptr(),
-            N.dtype_code(out.dtype), workspace.data_ptr(), workspace.numel(), N.stream(dev)))
+    _call(dev, N.lib().qkv_kv8_attention, q.data_ptr(), N.dtype_code(q.dtype), q.stride(0),
+          q.stride(1), rows, kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(),
+          vscale.data_ptr(), fmt, P, n, table.data_ptr(), width, N.ptr(q_start), N.ptr(q_lens),
+          kv_lens.data_ptr(), B, Hq, H, d, longest, float(scale), 1 if causal else 0,
+          out.data_ptr(), N.dtype_code(out.dtype), workspace.data_ptr(), workspace.numel())
     return out
 
 
