@@ -261,8 +261,10 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
   }
 }
 
-// Pieces that a launch of decode8 aims at, per kv head: two workgroups per CU.
-int32_t target_of(int32_t H) { return std::max(1, (2 * qkv_num_cus() + H - 1) / H); }
+// Pieces that a launch aims at, per kv head: one workgroup per CU.  (decode8, 32 x 8192
+// tokens, 8 kv heads, d = 128: 96 us; two per CU 105, three 104, four 118; 131,072 tokens:
+// 48, 51, 54, 57.)
+int32_t target_of(int32_t H) { return std::max(1, (qkv_num_cus() + H - 1) / H); }
 // Cut tiles have more than C steps each and pieces of C, so they have fewer than
 // 2 total / C <= 2 target pieces.
 int64_t slots_of(int32_t H) { return int64_t(2 * target_of(H) + 1) * H; }
@@ -404,8 +406,6 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   }
   if (pre) {
     place_parts(A, static_cast<uint8_t*>(workspace) + part_bytes(Hkv, kRows, d), kPreRows, d);
-    A.target = std::max(1, A.target / 2);  // one workgroup per CU
-    A.per_target = 1.f / A.target;
     // cut only where the tiles, as far as the rows tell, do not fill the card
     const int64_t t = tiles_of(kPreRows);
     const bool cut8 = cut && rows * G / kPreRows < A.target;

@@ -103,7 +103,7 @@ def plan_pages(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor,
     length kept): not, when its rows end behind ``rows`` or its pages behind the
     table's width, or when it needs pages and the pages needed up to it, in
     request order, exceed the free ones."""
-    dev = N.require_gpu(table, lens, new_lens, free, free_count, what="plan_pages")
+    dev = _one_device("plan_pages", table, lens, new_lens, free, free_count)
     if table.dim() != 2:
         raise ValueError("page table must be a 2-D int32 tensor")
     B, width = table.shape
@@ -123,8 +123,8 @@ def plan_pages(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor,
                                 ("free_count", torch.int32, (1,)),
                                 ("scratch", torch.int32, (B,))):
             _want(getattr(out, name), f"out.{name}", dt, shape)
-        N.require_gpu(table, out.q_start, out.q_lens, out.kv_lens, out.slots, out.positions,
-                      out.free_count, out.scratch, what="plan_pages")
+        _one_device("plan_pages", table, out.q_start, out.q_lens, out.kv_lens, out.slots,
+                    out.positions, out.free_count, out.scratch)
     _call(dev, N.lib().qkv_page_plan, lens.data_ptr(), new_lens.data_ptr(), B, table.data_ptr(),
           width, free.data_ptr(), free.numel(), free_count.data_ptr(), page_tokens, rows,
           out.q_start.data_ptr(), out.q_lens.data_ptr(), out.kv_lens.data_ptr(),
@@ -137,7 +137,7 @@ def release_pages(table: torch.Tensor, lens: torch.Tensor, done: torch.Tensor,
                   free: torch.Tensor, free_count: torch.Tensor, page_tokens: int) -> None:
     """The pages of the requests with ``done`` ((B,) bool) go back to the free
     list and their lengths become 0, all in place."""
-    dev = N.require_gpu(table, lens, done, free, free_count, what="release_pages")
+    dev = _one_device("release_pages", table, lens, done, free, free_count)
     if table.dim() != 2:
         raise ValueError("page table must be a 2-D int32 tensor")
     B, width = table.shape
@@ -152,28 +152,35 @@ def release_pages(table: torch.Tensor, lens: torch.Tensor, done: torch.Tensor,
           width, free.data_ptr(), free.numel(), free_count.data_ptr(), page_tokens)
 
 
+def _one_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
+    """The tensors' HIP device; N.require_gpu's errors where they have not one."""
+    i = first.get_device()
+    if i < 0:
+        N.require_gpu(first, what=what)
+    for t in others:
+        if t is not None and t.get_device() != i:
+            N.require_gpu(first, *others, what=what)
+    return first.device
+
+
 def _check_pools(kpool: torch.Tensor, kscale: torch.Tensor, vpool: torch.Tensor,
                  vscale: torch.Tensor) -> tuple[int, int, int, int, int]:
     """(pages, H, page tokens, d, code format) of the pools."""
-    if kpool.dim() != 4:
+    shape, dtype = kpool.shape, kpool.dtype
+    if len(shape) != 4:
         raise ValueError("kpool must be (pages, kv heads, page_tokens, head_dim)")
-    P, H, n, d = kpool.shape
-    fmt = _FMT.get(kpool.dtype)
+    P, H, n, d = shape
+    fmt = _FMT.get(dtype)
     if fmt is None:
-        raise ValueError(f"kpool must be int8 or float8_e4m3fn; got {kpool.dtype}")
+        raise ValueError(f"kpool must be int8 or float8_e4m3fn; got {dtype}")
     if n not in PAGE_SIZES:
         raise ValueError(f"page_tokens {n} must be one of {PAGE_SIZES}")
     nb = n // BLOCK_TOKENS
-    _want(kpool, "kpool", kpool.dtype)
-    _want(vpool, "vpool", kpool.dtype, (P, H, nb, d, BLOCK_TOKENS))
+    _want(kpool, "kpool", dtype)
+    _want(vpool, "vpool", dtype, (P, H, nb, d, BLOCK_TOKENS))
     _want(kscale, "kscale", torch.float32, (P, H, nb))
     _want(vscale, "vscale", torch.float32, (P, H, nb))
     return P, H, n, d, fmt
-
-
-def _dense_last(x: torch.Tensor) -> torch.Tensor:
-    """x with unit stride along the head_dim (other strides are passed on)."""
-    return x if x.stride(-1) == 1 else x.contiguous()
 
 
 def append_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kpool: torch.Tensor,
@@ -187,14 +194,15 @@ def append_kv8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, kpool: tor
     holds already keep their codes while the scale stands and are quantised anew
     where the new ones need a larger scale; NaN becomes 0, infinities the
     largest code."""
-    dev = N.require_gpu(k, v, slots, kpool, kscale, vpool, vscale, what="append_kv8")
+    dev = _one_device("append_kv8", k, v, slots, kpool, kscale, vpool, vscale)
     P, H, n, d, fmt = _check_pools(kpool, kscale, vpool, vscale)
     rows = k.shape[0] if k.dim() == 3 else -1
     if k.shape != v.shape or tuple(k.shape) != (rows, H, d) or k.dtype != v.dtype:
         raise ValueError(f"expected keys and values of shape (rows, {H}, {d}) and one type; got "
                          f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
     _want(slots, "slots", torch.int64, (rows,))
-    k, v = _dense_last(k), _dense_last(v)
+    # unit stride along the head_dim; the other strides are passed on
+    k, v = (x if x.stride(2) == 1 else x.contiguous() for x in (k, v))
     _call(dev, N.lib().qkv_kv8_append, N.dtype_code(k.dtype), k.data_ptr(), k.stride(0),
           k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(), rows, H, d, fmt,
           kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(), vscale.data_ptr(), P, n)
@@ -205,7 +213,7 @@ def read_kv8(slots: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
              out_dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
     """(keys, values) (rows, H, d) that the cache holds at ``slots`` ((rows,)
     int64, any order); rows whose slot is outside the pool become 0."""
-    dev = N.require_gpu(slots, kpool, kscale, vpool, vscale, what="read_kv8")
+    dev = _one_device("read_kv8", slots, kpool, kscale, vpool, vscale)
     P, H, n, d, fmt = _check_pools(kpool, kscale, vpool, vscale)
     rows = slots.numel()
     _want(slots, "slots", torch.int64, (rows,))
@@ -237,13 +245,15 @@ def attention_kv8(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
     ``max_q_len``: the longest request's rows where the caller knows it (1 in a
     decode step); it picks the kernels, not the result.  ``workspace`` (uint8,
     :func:`attention_kv8_workspace_bytes`) must belong to one call at a time."""
-    dev = N.require_gpu(q, kpool, kscale, vpool, vscale, table, kv_lens, q_start, q_lens, out,
-                        workspace, what="attention_kv8")
+    dev = _one_device("attention_kv8", q, kpool, kscale, vpool, vscale, table, kv_lens, q_start,
+                      q_lens, out, workspace)
     P, H, n, d, fmt = _check_pools(kpool, kscale, vpool, vscale)
-    if q.dim() != 3 or q.shape[2] != d or q.shape[1] == 0 or q.shape[1] % H != 0:
+    if q.dim() != 3:
+        raise ValueError(f"queries must be (rows, heads, {d}); got {tuple(q.shape)}")
+    rows, Hq, dq = q.shape
+    if dq != d or Hq == 0 or Hq % H != 0:
         raise ValueError(f"queries {tuple(q.shape)} do not match the cache (rows, a multiple of "
                          f"{H} heads, {d})")
-    rows, Hq, _ = q.shape
     if table.dim() != 2:
         raise ValueError("page table must be a 2-D int32 tensor")
     B, width = table.shape
@@ -268,17 +278,21 @@ def attention_kv8(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
     longest = rows // max(B, 1) if q_start is None else rows
     if max_q_len is not None:
         longest = max(0, min(longest, int(max_q_len)))
-    q = _dense_last(q)
+    ts, hs, ls = q.stride()
+    if ls != 1:
+        q = q.contiguous()
+        ts, hs, ls = q.stride()
     if workspace is None:
-        workspace = torch.empty(attention_kv8_workspace_bytes(B, rows, Hq, H, d, longest),
-                                dtype=torch.uint8, device=dev)
+        nbytes = attention_kv8_workspace_bytes(B, rows, Hq, H, d, longest)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     else:
         _want(workspace, "workspace", torch.uint8)
-    _call(dev, N.lib().qkv_kv8_attention, q.data_ptr(), N.dtype_code(q.dtype), q.stride(0),
-          q.stride(1), rows, kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(),
+        nbytes = workspace.numel()
+    _call(dev, N.lib().qkv_kv8_attention, q.data_ptr(), N.dtype_code(q.dtype), ts, hs, rows,
+          kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(),
           vscale.data_ptr(), fmt, P, n, table.data_ptr(), width, N.ptr(q_start), N.ptr(q_lens),
           kv_lens.data_ptr(), B, Hq, H, d, longest, float(scale), 1 if causal else 0,
-          out.data_ptr(), N.dtype_code(out.dtype), workspace.data_ptr(), workspace.numel())
+          out.data_ptr(), N.dtype_code(out.dtype), workspace.data_ptr(), nbytes)
     return out
 
 
