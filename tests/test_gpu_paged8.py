@@ -245,6 +245,62 @@ def test_append_border_codes():
         _same(st, cache, [64])
 
 
+@pytest.mark.parametrize("code,dtype,d", [("int8", BF16, 96), ("fp8", F16, 64), ("int8", F32, 128)])
+def test_append_unaligned_and_read_in_any_order(code, dtype, d):
+    """Rows at odd addresses and strides; slots read back out of order, twice, or not there."""
+    H, T = 3, 150
+    gen = torch.Generator().manual_seed(d)
+    wide = torch.randn(T, 2 * H * d + 5, generator=gen).to(dtype).to(DEV)
+    k = wide[:, 1:1 + H * d].unflatten(1, (H, d))
+    v = wide[:, 2 + H * d:2 + 2 * H * d].unflatten(1, (H, d))
+    st = P8.PagedKV8Store(1, H, d, 4, DEV, page_tokens=64, code=code)
+    cache = R.Cache(1, H, d, code)
+    for a, b in ((0, 70), (70, 71), (71, T)):
+        st.append(k[a:b], v[a:b], st.plan(i32([b - a]), b - a))
+        cache.append(0, k[a:b], v[a:b])
+    _same(st, cache, [T])
+    # a head_dim that is not the last axis in memory
+    st2 = P8.PagedKV8Store(1, H, d, 4, DEV, page_tokens=64, code=code)
+    kt, vt = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (k, v))
+    for a, b in ((0, 70), (70, 71), (71, T)):
+        st2.append(kt[a:b], vt[a:b], st2.plan(i32([b - a]), b - a))
+    for a, b in zip(st.pools().values(), st2.pools().values()):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    order = torch.randint(0, T, (6000,), generator=gen)
+    slots = _slots(st, 0, T)[order]
+    slots[::50] = -1
+    for n in (1, 40, 700, 6000):
+        ks, vs = st.read(slots[:n].to(DEV))
+        for half, x in enumerate((ks, vs)):
+            want = cache.values(0, half)[order[:n]].float()
+            want[::50] = 0
+            assert torch.equal(x.cpu(), want), (n, half)
+
+
+def test_append_chunks_of_all_sizes():
+    """The rules that deal rows to waves: the same cache from one call and from many."""
+    H, d, T = 2, 64, 4500
+    x = torch.randn(2, T, H, d, device=DEV)
+    ref = P8.PagedKV8Store(3, H, d, 80, DEV, page_tokens=64, pages_per_seq=80)
+    split = [1500, 17, T - 1517]
+    ref.append(x[0], x[1], ref.plan(i32(split), T))
+    st = P8.PagedKV8Store(3, H, d, 80, DEV, page_tokens=64, pages_per_seq=80)
+    plan = st.plan(i32(split), T)
+    for rows in (13, 600):                       # cut at block ends: a block's rows stay together
+        st.kscale.zero_()
+        st.vscale.zero_()
+        at = 0
+        while at < T:
+            end = min(T, at + rows)
+            while end < T and plan.slots[end].item() % 16:
+                end += 1
+            P8.append_kv8(x[0, at:end], x[1, at:end], plan.slots[at:end].contiguous(),
+                          **st.pools())
+            at = end
+        for a, b in zip(ref.pools().values(), st.pools().values()):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), rows
+
+
 def test_append_skips_bad_slots_and_keeps_the_rest():
     st = P8.PagedKV8Store(1, 2, 64, 2, DEV, page_tokens=64)
     before = [t.view(torch.uint8).clone() for t in st.pools().values()]
@@ -417,8 +473,97 @@ def test_attention_bad_pages_are_left_out():
         assert not x.any(), Q
 
 
+@pytest.mark.parametrize("q_dtype", [F32, F16, BF16])
+def test_attention_unaligned(q_dtype):
+    """Queries and results at odd addresses, queries with odd row strides."""
+    st, cache = _filled(2, 2, 64, [100, 300], "int8", 64, seed=8)
+    for q_lens in ([1, 2], [40, 1]):
+        rows = sum(q_lens)
+        wide = torch.randn(rows, 8 * 64 + 3, device=DEV).to(q_dtype)
+        q = wide[:, 1:1 + 8 * 64].unflatten(1, (8, 64))
+        out = torch.zeros(rows * 8 * 64 + 1, dtype=q_dtype, device=DEV)[1:].view(rows, 8, 64)
+        args = dict(**st.pools(), table=st.table, kv_lens=i32([100, 300]),
+                    q_start=i32([0, q_lens[0], rows]), causal=True)
+        P8.attention_kv8(q, **args, out=out)
+        ref = P8.attention_kv8(q.contiguous(), **args, out_dtype=q_dtype)
+        assert torch.equal(out, ref)
+        # a transposed head_dim is taken too
+        t = q.transpose(1, 2).contiguous().transpose(1, 2)
+        assert torch.equal(P8.attention_kv8(t, **args, out_dtype=q_dtype), ref)
+
+
+@pytest.mark.parametrize("B,pt", [(65, 64), (300, 64), (600, 128)])
+def test_attention_of_many_requests(B, pt):
+    """More requests than a wave has lanes, some empty, some not served, some cut."""
+    rng = random.Random(B)
+    lens = [rng.choice([0, 1, 17, 64, rng.randrange(200)]) for _ in range(B)]
+    lens[B // 2], lens[B - 1] = 3000, 1700
+    q_lens = [rng.choice([0, 1, 1, 1, 2]) for _ in range(B)]
+    st, cache = _filled(B, 1, 64, lens, "int8", pt, seed=B)
+    gaps = tuple(b for b in range(B) if rng.random() < 0.1)
+    _check_attention(st, cache, lens, q_lens, 4, BF16, F32, gaps=gaps, max_q_len=2)
+    for b in range(0, B, 9):
+        q_lens[b] = rng.choice([9, 33, 50])
+    _check_attention(st, cache, lens, q_lens, 4, BF16, F32, gaps=gaps)
+
+
+@pytest.mark.parametrize("H,G,Q", [(1, 1, 1), (3, 11, 1), (5, 16, 2), (1, 32, 1), (16, 1, 40),
+                                   (7, 3, 200)])
+def test_attention_head_layouts(H, G, Q):
+    """Cut requests at odd head counts and wide groups."""
+    lens = [2500, 1100]
+    st, cache = _filled(2, H, 64, lens, "fp8", 256, seed=H)
+    _check_attention(st, cache, lens, [Q, min(Q, 3)], G, F16, F32)
+
+
+def test_attention_lengths_off_the_table():
+    """Lengths below 0 count as 0, lengths behind the table as its tokens."""
+    st, cache = _filled(2, 1, 64, [128, 64], "int8", 64, seed=9)
+    table = st.table[:, :2].contiguous()
+    for Q in (1, 40):
+        q = torch.randn(2 * Q, 4, 64, device=DEV)
+        x = P8.attention_kv8(q, **st.pools(), table=table, kv_lens=i32([1000, -5]))
+        y = P8.attention_kv8(q, **st.pools(), table=table, kv_lens=i32([128, 0]))
+        assert torch.equal(x, y) and not x[Q:].any() and x[:Q].any()
+
+
+def test_attention_nan_stays_in_its_row():
+    """A query of NaN or infinities leaves the other queries as they are."""
+    st, cache = _filled(1, 1, 64, [150], "int8", 64, seed=10)
+    for Q in (4, 40):
+        q = torch.randn(Q, 4, 64, device=DEV)
+        args = dict(**st.pools(), table=st.table, kv_lens=i32([150]), causal=True)
+        ref = P8.attention_kv8(q, **args)
+        bad = q.clone()
+        bad[1, 2, 5], bad[2, 0, 0] = float("nan"), float("inf")
+        x = P8.attention_kv8(bad, **args)
+        same = torch.ones(Q, 4, dtype=torch.bool)
+        same[1, 2] = same[2, 0] = False
+        assert torch.equal(x[same], ref[same]) and x[1, 2].isnan().all()
+
+
+def test_offsets_past_32_bits():
+    """A request in the last pages of pools of more than 4 GiB."""
+    H, d, pt = 8, 128, 2048
+    pages = (5 << 30) // (H * d * pt)
+    st = P8.PagedKV8Store(2, H, d, pages, DEV, page_tokens=pt, pages_per_seq=2)
+    # handed out first: the pool's last two pages, then its first two
+    st.free[-4:] = i32([0, 1, pages - 2, pages - 1])
+    x = torch.randn(2, 2100, H, d, device=DEV, dtype=BF16)
+    st.append(x[0], x[1], st.plan(i32([2100, 0]), 2100))
+    st.append(x[0], x[1], st.plan(i32([0, 2100]), 2100))
+    assert st.table[:, :2].tolist() == [[pages - 1, pages - 2], [1, 0]]
+    for a, b in zip(st.read(_slots(st, 0, 2100).to(DEV)), st.read(_slots(st, 1, 2100).to(DEV))):
+        assert torch.equal(a, b) and a.any()
+    for Q in (1, 100):
+        q = torch.randn(Q, 4 * H, d, device=DEV, dtype=BF16)
+        out = P8.attention_kv8(torch.cat([q, q]), **st.pools(), table=st.table, kv_lens=st.lens,
+                               causal=True)
+        assert torch.equal(out[:Q], out[Q:]) and out.any()
+
+
 def test_attention_long_against_itself():
-    """A long cache: the result of the whole equals the softmax merge of its parts."""
+    """A long cache, cut into many pieces, against one softmax over all of it."""
     T, H, d = 40000, 2, 128
     gen = torch.Generator(device=DEV).manual_seed(3)
     st = P8.PagedKV8Store(1, H, d, 160, DEV)
@@ -492,6 +637,25 @@ def test_serving_loop_on_another_stream():
     s.synchronize()
     for x, y, (new, _) in zip(a, b, STEPS):
         assert torch.equal(x[:sum(new)], y[:sum(new)])
+
+
+def test_two_calls_at_once():
+    """Attention on two streams at the same time: each as alone."""
+    st, _ = _filled(3, 2, 128, [2000, 700, 1200], "int8", 64, seed=12)
+    qs = [torch.randn(3, 8, 128, device=DEV, dtype=BF16), torch.randn(150, 8, 128, device=DEV)]
+    args = dict(**st.pools(), table=st.table, kv_lens=i32([2000, 700, 1200]), causal=True)
+    alone = [P8.attention_kv8(q, **args) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(P8.attention_kv8(qs[i], **args))
+    torch.cuda.synchronize()
+    for ref, outs in zip(alone, got):
+        for x in outs:
+            assert torch.equal(x, ref)
 
 
 def test_captured_step():
