@@ -408,12 +408,15 @@ __device__ __forceinline__ void store4(void* out, int64_t at, const float* x, in
   }
 }
 
-// Joins the pieces of cut tiles: 4 rows of a tile at a time, 8 coordinates a lane, the
-// pieces dealt to the four waves.
+// Joins the pieces of cut tiles, 4 rows of a tile a wave, 8 coordinates a lane.  Decode
+// tiles have many pieces and few rows: a workgroup takes 4 rows, its waves every fourth
+// piece, and they meet in LDS.  Prefill tiles have many rows and few pieces: a workgroup
+// takes 16 rows.
 template <int D, int ROWS>
 __global__ __launch_bounds__(kThr) void join8(Att A) {
-  constexpr int GR = ROWS / 4;
-  __shared__ float acc[kWaves][4][D + 4], ml[kWaves][4][2];
+  constexpr bool DEAL = ROWS == kRows;  // pieces to the waves
+  constexpr int UR = DEAL ? 4 : 4 * kWaves, GR = ROWS / UR;
+  __shared__ float acc[DEAL ? kWaves : 1][4][D + 4], ml[DEAL ? kWaves : 1][4][2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane >> 4, d0 = 8 * (lane & 15);
@@ -423,18 +426,19 @@ __global__ __launch_bounds__(kThr) void join8(Att A) {
     const int64_t at = u / GR;  // slot * H + h
     const int4 t = A.desc[at];
     const int parts = t.x, h = static_cast<int>(at % A.H);
-    const int rr0 = 4 * static_cast<int>(u % GR);
+    const int rr0 = UR * static_cast<int>(u % GR) + (DEAL ? 0 : 4 * wave);
     // (0: not the tile's first piece; lengths that do not fit q_start may leave a slot unset)
     if (parts <= 0 || parts > A.nslots || t.w < 0 || int64_t(t.w) * ROWS > int64_t(A.rows) * A.G ||
         (t.w * ROWS + rr0) / A.G >= t.z)
       continue;
     float M = -INFINITY, L = 0.f, x[8] = {};
-    for (int p = wave; p < parts; p += 4 * kWaves) {
+    constexpr int EVERY = DEAL ? kWaves : 1;
+    for (int p = DEAL ? wave : 0; p < parts; p += 4 * EVERY) {
       float m[4], l[4];
       v4f v[4][2];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int q = p + kWaves * k;
+        const int q = p + EVERY * k;
         const int64_t s = at + int64_t(q < parts ? q : p) * A.H;
         const int64_t row = (s < A.nslots ? s : at) * ROWS + rr0 + r;
         m[k] = q < parts ? A.part_ml[2 * row] : -INFINITY;
@@ -461,41 +465,52 @@ __global__ __launch_bounds__(kThr) void join8(Att A) {
         for (int j = 0; j < 8; ++j) x[j] = fmaf(v[k][j >> 2][j & 3], e, x[j]);
       }
     }
-    __syncthreads();  // (the arrays' last readers)
-    if (on) {
-      *reinterpret_cast<v4f*>(&acc[wave][r][d0]) = v4f{x[0], x[1], x[2], x[3]};
-      *reinterpret_cast<v4f*>(&acc[wave][r][d0 + 4]) = v4f{x[4], x[5], x[6], x[7]};
-    }
-    if (d0 == 0) {
-      ml[wave][r][0] = M;
-      ml[wave][r][1] = L;
-    }
-    __syncthreads();
-    // wave w: row w
-    const int rr = t.w * ROWS + rr0 + wave, qi = rr / A.G, c = 2 * lane;
-    const int64_t row = int64_t(t.y) + qi;
-    if (c >= D || qi >= t.z || row < 0 || row >= A.rows) continue;
-    float mx = -INFINITY, sum = 0.f, y0 = 0.f, y1 = 0.f;
+    if constexpr (!DEAL) {
+      const int rr = t.w * ROWS + rr0 + r, qi = rr / A.G;
+      const int64_t row = int64_t(t.y) + qi;
+      if (!on || qi >= t.z || row < 0 || row >= A.rows) continue;
+      const float inv = L > 0.f ? 1.f / L : 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, ml[w][wave][0]);
-    const float ref = mx == -INFINITY ? 0.f : mx;
+      for (int j = 0; j < 8; ++j) x[j] *= inv;
+      store8(A.out, (row * A.Hq + h * A.G + rr - qi * A.G) * D + d0, x, A.out_dtype, A.out_vec);
+    } else {
+      __syncthreads();  // (the arrays' last readers)
+      if (on) {
+        *reinterpret_cast<v4f*>(&acc[wave][r][d0]) = v4f{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<v4f*>(&acc[wave][r][d0 + 4]) = v4f{x[4], x[5], x[6], x[7]};
+      }
+      if (d0 == 0) {
+        ml[wave][r][0] = M;
+        ml[wave][r][1] = L;
+      }
+      __syncthreads();
+      // wave w: row w
+      const int rr = t.w * ROWS + rr0 + wave, qi = rr / A.G, c = 2 * lane;
+      const int64_t row = int64_t(t.y) + qi;
+      if (c >= D || qi >= t.z || row < 0 || row >= A.rows) continue;
+      float mx = -INFINITY, sum = 0.f, y0 = 0.f, y1 = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float e = __builtin_amdgcn_exp2f(ml[w][wave][0] - ref);
-      sum = fmaf(ml[w][wave][1], e, sum);
-      y0 = fmaf(acc[w][wave][c], e, y0);
-      y1 = fmaf(acc[w][wave][c + 1], e, y1);
+      for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, ml[w][wave][0]);
+      const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float e = __builtin_amdgcn_exp2f(ml[w][wave][0] - ref);
+        sum = fmaf(ml[w][wave][1], e, sum);
+        y0 = fmaf(acc[w][wave][c], e, y0);
+        y1 = fmaf(acc[w][wave][c + 1], e, y1);
+      }
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const int64_t to = (row * A.Hq + h * A.G + rr - qi * A.G) * D + c;
+      qkv_store(A.out, to, y0 * inv, A.out_dtype);
+      qkv_store(A.out, to + 1, y1 * inv, A.out_dtype);
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    const int64_t to = (row * A.Hq + h * A.G + rr - qi * A.G) * D + c;
-    qkv_store(A.out, to, y0 * inv, A.out_dtype);
-    qkv_store(A.out, to + 1, y1 * inv, A.out_dtype);
   }
 }
 
 // Workgroups of a join: the units are counted on the device.
 inline uint32_t join_grid(const Att& A, int rows) {
-  return static_cast<uint32_t>(std::min<int64_t>(int64_t(A.nslots) / 2 * (rows / 4), 1024));
+  const int64_t units = int64_t(A.nslots) * (rows == kRows ? kRows / 4 : rows / (4 * kWaves));
+  return static_cast<uint32_t>(std::min<int64_t>(units, 1024));
 }
 
 }  // namespace qkv_kv8
