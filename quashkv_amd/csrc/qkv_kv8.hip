@@ -56,7 +56,6 @@ __device__ __forceinline__ float value_of(uint32_t code) {
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef float v2f __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4;  // of a workgroup, each with a unit of its own
 
@@ -82,33 +81,27 @@ __device__ __forceinline__ void load8(const void* x, int64_t at, bool vec, float
   }
 }
 
-// N consecutive elements (2 or 8) to element `at` of a dense output.
-template <int N, int DT>
-__device__ __forceinline__ void store_n(void* x, int64_t at, bool vec, const float* v) {
+// Eight consecutive elements to element `at` of a dense output.
+template <int DT>
+__device__ __forceinline__ void store8(void* x, int64_t at, bool vec, const float* v) {
   if (!vec) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) qkv_store(x, at + i, v[i], DT);
+    for (int i = 0; i < 8; ++i) qkv_store(x, at + i, v[i], DT);
   } else if constexpr (DT == QKV_F32) {
-    float* const p = static_cast<float*>(x) + at;
-    if constexpr (N == 2) {
-      *reinterpret_cast<v2f*>(p) = v2f{v[0], v[1]};
-    } else {
-      reinterpret_cast<v4f*>(p)[0] = v4f{v[0], v[1], v[2], v[3]};
-      reinterpret_cast<v4f*>(p)[1] = v4f{v[4], v[5], v[6], v[7]};
-    }
+    v4f* const p = reinterpret_cast<v4f*>(static_cast<float*>(x) + at);
+    p[0] = v4f{v[0], v[1], v[2], v[3]};
+    p[1] = v4f{v[4], v[5], v[6], v[7]};
   } else {
-    uint32_t w[N / 2];
+    v4u w;
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       if constexpr (DT == QKV_BF16)
         w[i] = qkv_f32_to_bf16(v[2 * i]) | uint32_t(qkv_f32_to_bf16(v[2 * i + 1])) << 16;
       else
         w[i] = uint32_t(__builtin_bit_cast(uint16_t, static_cast<_Float16>(v[2 * i]))) |
                uint32_t(__builtin_bit_cast(uint16_t, static_cast<_Float16>(v[2 * i + 1]))) << 16;
     }
-    uint16_t* const p = static_cast<uint16_t*>(x) + at;
-    if constexpr (N == 2) *reinterpret_cast<uint32_t*>(p) = w[0];
-    else *reinterpret_cast<v4u*>(p) = v4u{w[0], w[1], w[2], w[3]};
+    *reinterpret_cast<v4u*>(static_cast<uint16_t*>(x) + at) = w;
   }
 }
 
@@ -287,12 +280,14 @@ struct Rd {
 };
 
 // A wave per (chunk of up to 16 rows, head), lanes as in append_runs; a V block is read once
-// for a run of consecutive slots in it.
+// for a run of consecutive slots in it, and turns through LDS too.
 template <int D, bool FP8, int DT>
 __global__ __launch_bounds__(64 * kWaves) void read_rows(Rd A) {
+  constexpr int LPR = D / 8, RPI = 64 / LPR, NI = (kBlk + RPI - 1) / RPI;
+  __shared__ __align__(16) uint8_t turn[kWaves][kBlk * D];
   const int lane = threadIdx.x & 63, half = blockIdx.y;
-  const int64_t u =
-      int64_t(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t u = int64_t(blockIdx.x) * kWaves + wave;
   if (u >= A.units) return;
   const int64_t r0 = u / A.H * A.chunk, n = int64_t(1) << A.lg;
   const int h = static_cast<int>(u % A.H);
@@ -302,9 +297,15 @@ __global__ __launch_bounds__(64 * kWaves) void read_rows(Rd A) {
   if (sl >= A.tokens) sl = -1;
   const uint64_t rows = __ballot(mine);
   auto row_of = [&](int64_t s) { return ((s >> A.lg) * A.H + h) * n + (s & (n - 1)); };
+  const int sub = lane / LPR, c = 8 * (lane % LPR);
+  // eight codes to the chunk's row i
+  auto put = [&](v2u w, float sc, int i) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = value_of<FP8>(w[j >> 2] >> (8 * (j & 3))) * sc;
+    store8<DT>(A.out[half], ((r0 + i) * A.H + h) * D + c, A.vec[half], x);
+  };
   if (half == 0) {
-    constexpr int LPR = D / 8, RPI = 64 / LPR, NI = (kBlk + RPI - 1) / RPI;
-    const int sub = lane / LPR, c = 8 * (lane % LPR);
     v2u w[NI];
     float sc[NI];
 #pragma unroll
@@ -322,46 +323,45 @@ __global__ __launch_bounds__(64 * kWaves) void read_rows(Rd A) {
 #pragma unroll
     for (int t = 0; t < NI; ++t) {
       const int i = RPI * t + sub;
-      if (sub >= RPI || i >= kBlk || !(rows >> i & 1)) continue;
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = value_of<FP8>(w[t][j >> 2] >> (8 * (j & 3))) * sc[t];
-      store_n<8, DT>(A.out[0], ((r0 + i) * A.H + h) * D + c, A.vec[0], x);
+      if (sub < RPI && i < kBlk && (rows >> i & 1)) put(w[t], sc[t], i);
     }
   } else {
     const int64_t prev = __shfl_up(static_cast<long long>(sl), 1, 64);
     const bool cont = lane > 0 && sl >= 0 && sl == prev + 1 && (sl & 15) != 0;
     const uint64_t conts = __ballot(cont && mine);
     uint64_t heads = __ballot(mine && !cont);
-    constexpr int LPR = D / 2, TG = 64 / LPR, TL = kBlk / TG;
-    const int tg = lane / LPR, c = 2 * (lane % LPR);
     while (heads) {
       const int i0 = __builtin_ctzll(heads);
       heads &= heads - 1;
       const int64_t s = __shfl(static_cast<long long>(sl), i0, 64);
       const int len = s < 0 ? 1 : 1 + __builtin_ctzll(~(conts >> (i0 + 1)));
       const int j0 = s < 0 ? 0 : static_cast<int>(s & 15), j1 = j0 + len;
-      if (tg >= TG) continue;
-      uint32_t w[2][TL / 4] = {};
       float sc = 0.f;
       if (s >= 0) {
         const int64_t row = row_of(s) & ~int64_t(15);
-        const uint8_t* const v = A.pool[1] + row * D + c * kBlk + TL * tg;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int q = 0; q < TL / 4; ++q)
-            w[i][q] = *reinterpret_cast<const uint32_t*>(v + kBlk * i + 4 * q);
         sc = A.scale[1][row >> 4];
-      }
 #pragma unroll
-      for (int t = 0; t < TL; ++t) {
-        const int j = TL * tg + t;
-        if (j < j0 || j >= j1) continue;
-        const float x[2] = {value_of<FP8>(w[0][t >> 2] >> (8 * (t & 3))) * sc,
-                            value_of<FP8>(w[1][t >> 2] >> (8 * (t & 3))) * sc};
-        store_n<2, DT>(A.out[1], ((r0 + i0 + j - j0) * A.H + h) * D + c, A.vec[1], x);
+        for (int e = 0; e < D; e += 64) {
+          const int dd = e + lane;
+          if (dd >= D) continue;
+          const v4u w = *reinterpret_cast<const v4u*>(A.pool[1] + row * D + dd * kBlk);
+#pragma unroll
+          for (int j = 0; j < kBlk; ++j)
+            turn[wave][j * D + dd] = static_cast<uint8_t>(w[j >> 2] >> (8 * (j & 3)));
+        }
       }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+      for (int t = 0; t < NI; ++t) {
+        const int j = RPI * t + sub;
+        if (sub >= RPI || j < j0 || j >= j1) continue;
+        v2u w = {0, 0};
+        if (s >= 0) w = *reinterpret_cast<const v2u*>(turn[wave] + j * D + c);
+        put(w, sc, i0 + j - j0);
+      }
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
@@ -461,7 +461,6 @@ extern "C" int qkv_kv8_read(const int64_t* slots, int64_t rows, int32_t H, int32
               "the pools must be 16-byte aligned");
   const int32_t chunk = chunk_of(rows);
   const int64_t units = (rows + chunk - 1) / chunk * H;
-  const int os = out_dtype == QKV_F32 ? 4 : 2;
   Rd A{slots,
        rows,
        {static_cast<const uint8_t*>(kpool), static_cast<const uint8_t*>(vpool)},
@@ -472,7 +471,7 @@ extern "C" int qkv_kv8_read(const int64_t* slots, int64_t rows, int32_t H, int32
        chunk,
        units,
        {keys, values},
-       {qkv_aligned(keys, 16), qkv_aligned(values, 2 * os)}};
+       {qkv_aligned(keys, 16), qkv_aligned(values, 16)}};
   QKV_REQUIRE(units / kWaves < INT32_MAX, "too many rows (%lld) for one call",
               static_cast<long long>(rows));
   const dim3 grid(static_cast<uint32_t>((units + kWaves - 1) / kWaves), 2);
