@@ -50,8 +50,9 @@ struct Att {
   int32_t target;   // pieces that a launch aims at, per kv head
   float per_target; // 1 / target
   int32_t nslots;   // partial results that the workspace holds
-  int32_t* used;    // of them, per kv head, in this launch
+  int32_t* used;    // [0]: of them, per kv head, in this launch; [1], [2]: pieces and C (plan)
   int4* desc;       // [slot][H]: whose they are
+  int4* plan;       // [piece]: request, piece of it, its first slot; null: the kernels' own
   float* part_o;    // [slot][H][row][D]
   float* part_ml;   // [slot][H][row][2]
 };
@@ -84,12 +85,6 @@ struct Piece {
   int32_t part, parts;
 };
 
-struct Shared {
-  float sum[8];  // a wave's
-  int32_t tiles[8], scan[8][2];
-  int32_t found[3];  // b, piece within the request, first slot of the request
-};
-
 // Inclusive sum over a wave's lanes.
 template <typename T>
 __device__ __forceinline__ T wave_scan(T v) {
@@ -112,49 +107,54 @@ __device__ __forceinline__ T lane_value(T v, int lane) {
   return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
-// Piece number `want` of the launch.  A launch has the tiles of ROWS query rows of the
-// requests that are its own (rows up to A.few: decode8's 16-row tiles; more: prefill8's).
-// A tile's steps are cut into pieces of C, the smallest C that keeps the launch near its
-// target of pieces; so long requests are shared by many workgroups and short ones are not
-// cut.  (prefill8 cuts nothing where the tiles alone reach the target: its partial results
-// cost more.)  Every workgroup finds its own piece by prefix sums over the requests -- each
-// wave for itself up to 64 of them -- so no launch and no host knowledge of the lengths is
-// needed.  Workgroup 0 also tells the join how many partial results there are.
-template <int ROWS, int THR>
-__device__ __forceinline__ bool locate(const Att& A, int want, Shared& sh, Piece& P) {
-  constexpr bool PRE = ROWS == kPreRows;
-  constexpr int ROUND = PRE ? 2 : kWaves;  // steps that a workgroup takes at once
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  auto cost = [&](const Req& r, int& tiles, int& steps) {
+// How a launch's work is cut.  A launch has the tiles of ROWS query rows of the requests that
+// are its own (rows up to A.few: decode8's 16-row tiles; more: prefill8's).  A tile's steps
+// are cut into pieces of C, the smallest C that keeps the launch near its target of pieces;
+// so long requests are shared by many workgroups and short ones are not cut.  (prefill8 cuts
+// nothing where the tiles alone reach the target: its partial results cost more.)
+template <int ROWS>
+struct Cut {
+  static constexpr bool PRE = ROWS == kPreRows;
+  static constexpr int ROUND = PRE ? 2 : kWaves;  // steps that a workgroup takes at once
+  static __device__ __forceinline__ void cost(const Att& A, const Req& r, int& tiles, int& steps) {
     const int n = r.ql * A.G;
     tiles = (n > A.few) == PRE ? (n + ROWS - 1) / ROWS : 0;
     steps = max(1, (r.kv + kStep - 1) / kStep);
-  };
-  // (the sum is rounded alike in every workgroup; C is above its share in any case)
-  auto piece_len = [&](float sum, int all) {
+  }
+  // sum: of tiles times steps (rounded alike in every workgroup; C is above its share in
+  // any case), all: tiles
+  static __device__ __forceinline__ int length(const Att& A, float sum, int all) {
     if (PRE && all >= A.target) return INT32_MAX / 2;
     const int c = static_cast<int>(fminf(sum * A.per_target, 1e9f)) + 1;
     return max(A.least, (c + ROUND - 1) / ROUND * ROUND);
-  };
+  }
   // whole prefill tiles: the last ones first, of a causal prompt the longest
-  auto order = [&](int C, int all) {
-    if (PRE && C == INT32_MAX / 2) want = want < all ? all - 1 - want : INT32_MAX;
-  };
+  static __device__ __forceinline__ bool reversed(int C) { return PRE && C == INT32_MAX / 2; }
+};
+
+// Piece number `want` of the launch.  Up to 64 requests every wave finds it by prefix sums
+// over them, so that no launch and no host knowledge of the lengths is needed, and
+// workgroup 0 tells the join how many partial results there are.  More requests are
+// planned by a launch of their own (plan8).
+template <int ROWS>
+__device__ __forceinline__ bool locate(const Att& A, int want, Piece& P) {
+  using K = Cut<ROWS>;
+  const int lane = threadIdx.x & 63;
   int C, in, slot0, steps;
-  if (A.B <= 64) {
+  if (A.plan == nullptr) {
     Req r{0, 0, 0};
     int tiles = 0, st = 1;
     if (lane < A.B) {
       r = request(A, lane);
-      cost(r, tiles, st);
+      K::cost(A, r, tiles, st);
     }
     const float sum = lane_value(wave_scan(static_cast<float>(tiles) * st), 63);
-    const int all = PRE ? lane_value(wave_scan(tiles), 63) : 0;
-    C = piece_len(sum, all);
-    order(C, all);
+    const int all = K::PRE ? lane_value(wave_scan(tiles), 63) : 0;
+    C = K::length(A, sum, all);
+    if (K::reversed(C)) want = want < all ? all - 1 - want : INT32_MAX;
     const int per = (st + C - 1) / C, mine = tiles * per, cut = per > 1 ? mine : 0;
     const int end = wave_scan(mine), cuts = wave_scan(cut);
-    if (blockIdx.x == 0 && tid == 0) *A.used = lane_value(cuts, 63);
+    if (blockIdx.x == 0 && threadIdx.x == 0) A.used[0] = lane_value(cuts, 63);
     const uint64_t hit = __ballot(want >= end - mine && want < end);
     if (hit == 0) return false;
     P.b = __builtin_ctzll(hit);
@@ -163,75 +163,15 @@ __device__ __forceinline__ bool locate(const Att& A, int want, Shared& sh, Piece
     steps = lane_value(st, P.b);
     P.r = Req{lane_value(r.q0, P.b), lane_value(r.ql, P.b), lane_value(r.kv, P.b)};
   } else {
-    float sum = 0.f;
-    int all = 0;
-    for (int b = tid; b < A.B; b += THR) {
-      int tiles, st;
-      cost(request(A, b), tiles, st);
-      sum += static_cast<float>(tiles) * st;
-      all += tiles;
-    }
-    sum = wave_scan(sum);
-    all = wave_scan(all);
-    if (lane == 63) {
-      sh.sum[wave] = sum;
-      sh.tiles[wave] = all;
-    }
-    if (tid == 0) sh.found[0] = -1;
-    __syncthreads();
-    sum = 0.f;
-    all = 0;
-#pragma unroll
-    for (int w = 0; w < THR / 64; ++w) {
-      sum += sh.sum[w];
-      all += sh.tiles[w];
-    }
-    C = piece_len(sum, all);
-    order(C, all);
-    int base[2] = {0, 0};  // pieces, pieces of cut tiles
-    for (int b0 = 0; b0 < A.B; b0 += THR) {
-      const int b = b0 + tid;
-      int own[2] = {0, 0}, v[2];
-      if (b < A.B) {
-        int tiles, st;
-        cost(request(A, b), tiles, st);
-        const int per = (st + C - 1) / C;
-        own[0] = tiles * per;
-        own[1] = per > 1 ? own[0] : 0;
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        v[k] = wave_scan(own[k]);
-        if (lane == 63) sh.scan[wave][k] = v[k];
-      }
-      __syncthreads();
-      int tot[2] = {0, 0};
-#pragma unroll
-      for (int w = 0; w < THR / 64; ++w)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (w < wave) v[k] += sh.scan[w][k];
-          tot[k] += sh.scan[w][k];
-        }
-      const int end = base[0] + v[0], first = end - own[0];
-      if (want >= first && want < end) {
-        sh.found[0] = b;
-        sh.found[1] = want - first;
-        sh.found[2] = base[1] + v[1] - own[1];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 2; ++k) base[k] += tot[k];
-      if (sh.found[0] >= 0 && blockIdx.x != 0) break;
-    }
-    if (blockIdx.x == 0 && tid == 0) *A.used = base[1];
-    P.b = __builtin_amdgcn_readfirstlane(sh.found[0]);
-    if (P.b < 0) return false;
-    in = __builtin_amdgcn_readfirstlane(sh.found[1]);
-    slot0 = __builtin_amdgcn_readfirstlane(sh.found[2]);
+    if (want >= A.used[1]) return false;
+    const int4 e = A.plan[want];
+    C = A.used[2];
+    P.b = __builtin_amdgcn_readfirstlane(e.x);
+    in = __builtin_amdgcn_readfirstlane(e.y);
+    slot0 = __builtin_amdgcn_readfirstlane(e.z);
     P.r = request(A, P.b);
     int tiles;
-    cost(P.r, tiles, steps);
+    K::cost(A, P.r, tiles, steps);
   }
   P.parts = (steps + C - 1) / C;
   P.rt = in / P.parts;
@@ -240,6 +180,101 @@ __device__ __forceinline__ bool locate(const Att& A, int want, Shared& sh, Piece
   P.s1 = min(steps, P.s0 + C);
   P.slot = P.parts > 1 ? slot0 + in : -1;
   return true;
+}
+
+constexpr int kPlanThr = 1024;
+constexpr int kMaxB = 16000;  // requests of a call (their prefix sums fit 64 KiB of LDS)
+
+// Lists the pieces of a launch, at most `cap`, for more requests than a wave has lanes: one
+// workgroup.  (Every workgroup summing over all requests for itself took 147 us at 1000
+// requests of 100 tokens, 8 kv heads, d = 128.)
+template <int ROWS>
+__global__ __launch_bounds__(kPlanThr) void plan8(Att A, int cap) {
+  using K = Cut<ROWS>;
+  constexpr int W = kPlanThr / 64;
+  extern __shared__ int32_t ends[];  // [B + 1] pieces of the requests before b
+  __shared__ float sums[W];
+  __shared__ int32_t part[W][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  float sum = 0.f;
+  int all = 0;
+  for (int b = tid; b < A.B; b += kPlanThr) {
+    int tiles, st;
+    K::cost(A, request(A, b), tiles, st);
+    sum += static_cast<float>(tiles) * st;
+    all += tiles;
+  }
+  sum = wave_scan(sum);
+  all = wave_scan(all);
+  if (lane == 63) {
+    sums[wave] = sum;
+    part[wave][0] = all;
+  }
+  if (tid == 0) ends[0] = 0;
+  __syncthreads();
+  sum = 0.f;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    sum += sums[w];
+    all += part[w][0];
+  }
+  const int C = K::length(A, sum, all);
+  int base[2] = {0, 0};  // pieces, pieces of cut tiles
+  for (int b0 = 0; b0 < A.B; b0 += kPlanThr) {
+    const int b = b0 + tid;
+    int own[2] = {0, 0}, v[2];
+    if (b < A.B) {
+      int tiles, st;
+      K::cost(A, request(A, b), tiles, st);
+      const int per = (st + C - 1) / C;
+      own[0] = tiles * per;
+      own[1] = per > 1 ? own[0] : 0;
+    }
+    __syncthreads();  // (part's last readers)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      v[k] = wave_scan(own[k]);
+      if (lane == 63) part[wave][k] = v[k];
+    }
+    __syncthreads();
+    int tot[2] = {0, 0};
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (w < wave) v[k] += part[w][k];
+        tot[k] += part[w][k];
+      }
+    // a request's first piece carries its first slot until all are listed
+    if (b < A.B) {
+      ends[b + 1] = base[0] + v[0];
+      const int first = base[0] + v[0] - own[0];
+      if (own[0] > 0 && first < cap) A.plan[first].w = base[1] + v[1] - own[1];
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) base[k] += tot[k];
+  }
+  __syncthreads();
+  const int total = min(base[0], cap);
+  if (tid == 0) {
+    A.used[0] = base[1];
+    A.used[1] = total;
+    A.used[2] = C;
+  }
+  for (int p = tid; p < total; p += kPlanThr) {
+    int lo = 0, hi = A.B;  // ends[lo] <= p < ends[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (ends[mid] <= p) lo = mid;
+      else hi = mid;
+    }
+    int4* const to = A.plan + (K::reversed(C) ? total - 1 - p : p);
+    const int slot0 = K::reversed(C) ? 0 : A.plan[ends[lo]].w;
+    to->x = lo;
+    to->y = p - ends[lo];
+    to->z = slot0;
+  }
 }
 
 // Where the piece's partial result goes, in units of [slot][H], or -1 past the workspace.

@@ -31,7 +31,6 @@ __host__ __device__ constexpr int dcol(int D, int ks, int g) {
 template <int D, bool FP8, bool QLO, bool PLO>
 __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
   constexpr int KS = D / 32, NJ = D / 16, NK = (D + 63) / 64;
-  __shared__ Shared sh;
   __shared__ float red_o[kWaves][kRows][D + 4];
   __shared__ float red_ml[kWaves][kRows][2];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -39,7 +38,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
   const int n = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % A.H;
   Piece P;
-  if (!locate<kRows, kThr>(A, blockIdx.x / A.H, sh, P)) return;
+  if (!locate<kRows>(A, blockIdx.x / A.H, P)) return;
 
   // ---- this lane's query row
   const int rr = P.rt * kRows + n, qi = rr / A.G, gq = rr - qi * A.G;
@@ -270,9 +269,14 @@ int32_t target_of(int32_t H) { return std::max(1, (qkv_num_cus() + H - 1) / H); 
 // Cut tiles have more than C steps each and pieces of C, so they have fewer than
 // 2 total / C <= 2 target pieces.
 int64_t slots_of(int32_t H) { return int64_t(2 * target_of(H) + 1) * H; }
-// Bytes of a launch's partial results.
-int64_t part_bytes(int32_t H, int rows, int32_t d) {
-  return 256 + slots_of(H) * (16 + rows * (d + 2) * 4) / 256 * 256 + 256;
+// Tiles of `rows` query rows, at most: a request's last one may be in part empty.
+int64_t tiles_of(int64_t B, int64_t q_rows, int32_t G, int rows) {
+  return q_rows * G / rows + std::min(B, q_rows);
+}
+// Bytes of a launch's partial results, and of its list of pieces.
+int64_t part_bytes(int64_t B, int64_t q_rows, int32_t G, int32_t H, int rows, int32_t d) {
+  const int64_t plan = B > 64 ? 16 * (tiles_of(B, q_rows, G, rows) + target_of(H)) : 0;
+  return 256 + (slots_of(H) * (16 + rows * (d + 2) * 4) + plan) / 256 * 256 + 256;
 }
 // Lays them out at `at`.
 void place_parts(Att& A, void* at, int rows, int32_t d) {
@@ -280,6 +284,8 @@ void place_parts(Att& A, void* at, int rows, int32_t d) {
   A.desc = reinterpret_cast<int4*>(A.used + 64);
   A.part_o = reinterpret_cast<float*>(A.desc + A.nslots);
   A.part_ml = A.part_o + int64_t(A.nslots) * rows * d;
+  // (nslots * rows * 8 bytes of part_ml: 16-byte aligned)
+  A.plan = A.B > 64 ? reinterpret_cast<int4*>(A.part_ml + int64_t(A.nslots) * rows * 2) : nullptr;
 }
 // Requests of more rows than this go to prefill8.
 constexpr int kFew = 32;
@@ -291,6 +297,8 @@ constexpr int32_t kNever = INT32_MAX / 2;
 template <int D, bool FP8>
 void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
   const uint32_t grid = (tiles + A.target) * A.H;
+  if (A.plan)
+    plan8<kRows><<<1, kPlanThr, (A.B + 1) * sizeof(int32_t), s>>>(A, tiles + A.target);
   if (A.q_dtype == QKV_F32) {
     if (A.out_dtype == QKV_BF16) decode8<D, FP8, true, false><<<grid, kThr, 0, s>>>(A);
     else decode8<D, FP8, true, true><<<grid, kThr, 0, s>>>(A);
@@ -306,8 +314,10 @@ void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
 extern "C" int64_t qkv_kv8_attention_workspace_bytes(int32_t B, int64_t rows, int32_t Hq,
                                                      int32_t Hkv, int32_t d, int64_t max_q) {
   if (Hkv < 1 || d < 1) return 0;
-  return part_bytes(Hkv, kRows, d) +
-         (max_q * (Hq / Hkv) > kFew ? part_bytes(Hkv, kPreRows, d) : 0);
+  if (B < 1 || rows < 1) return 256;
+  const int32_t G = Hq / Hkv;
+  return part_bytes(B, rows, G, Hkv, kRows, d) +
+         (max_q * G > kFew ? part_bytes(B, rows, G, Hkv, kPreRows, d) : 0);
 }
 
 extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_stride,
@@ -326,7 +336,8 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
               q_dtype, out_dtype);
   QKV_REQUIRE(Hq >= 1 && Hq % Hkv == 0, "query heads (%d) must be a multiple of kv heads (%d)", Hq,
               Hkv);
-  QKV_REQUIRE(B >= 0 && pages_per_seq >= 1, "bad batch %d or pages_per_seq %d", B, pages_per_seq);
+  QKV_REQUIRE(B >= 0 && B <= kMaxB && pages_per_seq >= 1,
+              "batch %d must lie in [0, %d], pages_per_seq %d be positive", B, kMaxB, pages_per_seq);
   const int32_t G = Hq / Hkv;
   QKV_REQUIRE(rows >= 0 && rows * G < INT32_MAX / 2 && rows * Hq / kRows < (1 << 28),
               "rows must lie in [0, 2^30 / heads per kv head); got %lld",
@@ -380,13 +391,13 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   // decode8 runs too where, as far as the rows tell, a request may be short.  (Where one is
   // against that, prefill8 takes it: slower, the same result.)
   const bool dec = !pre || (q_start && rows <= (B - 1) * longest + kFew / G);
-  // tiles of a launch, at most: a request's last one may be in part empty
-  auto tiles_of = [&](int r) {
-    return q_start ? rows * G / r + std::min<int64_t>(B, rows)
+  QKV_REQUIRE((tiles_of(B, rows, G, kRows) + A.target) * Hkv <= INT32_MAX, "batch of %d requests "
+              "and %lld rows is too large for one call", B, static_cast<long long>(rows));
+  // without q_start the tiles are known
+  auto tiles = [&](int r) {
+    return q_start ? tiles_of(B, rows, G, r)
                    : int64_t(B) * ((int64_t(A.uniform_q) * G + r - 1) / r);
   };
-  QKV_REQUIRE((tiles_of(kRows) + A.target) * Hkv <= INT32_MAX, "batch of %d requests and %lld "
-              "rows is too large for one call", B, static_cast<long long>(rows));
   const bool cut = (int64_t(pages_per_seq) << A.lg) > kWhole;
   A.few = !pre ? INT32_MAX : dec ? kFew : 0;
   A.least = cut ? 4 : kNever;
@@ -394,7 +405,7 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   if (dec) {
     // beside prefill8 this launch has only requests of up to kFew rows
     const uint32_t t = static_cast<uint32_t>(
-        pre ? std::min<int64_t>(tiles_of(kRows), int64_t(B) * (kFew / kRows)) : tiles_of(kRows));
+        pre ? std::min<int64_t>(tiles(kRows), int64_t(B) * (kFew / kRows)) : tiles(kRows));
     if (fmt == QKV_CODES_I8) {
       if (d == 128) launch<128, false>(A, t, cut, s);
       else if (d == 96) launch<96, false>(A, t, cut, s);
@@ -407,9 +418,10 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
     QKV_LAUNCHED();
   }
   if (pre) {
-    place_parts(A, static_cast<uint8_t*>(workspace) + part_bytes(Hkv, kRows, d), kPreRows, d);
+    place_parts(A, static_cast<uint8_t*>(workspace) + part_bytes(B, rows, G, Hkv, kRows, d),
+                kPreRows, d);
     // cut only where the tiles, as far as the rows tell, do not fill the card
-    const int64_t t = tiles_of(kPreRows);
+    const int64_t t = tiles(kPreRows);
     const bool cut8 = cut && rows * G / kPreRows < A.target;
     A.least = cut8 ? 4 : kNever;
     qkv_kv8_prefill(A, d, fmt == QKV_CODES_E4M3, static_cast<uint32_t>(t), cut8, s);

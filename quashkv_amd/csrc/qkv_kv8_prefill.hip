@@ -32,7 +32,6 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
   constexpr int CH = 4 * D;                      // 16-byte chunks of K and of V in a step
   constexpr int NC = (CH + 255) / 256;           // of them, per thread of a half
   constexpr int KB = 2 * KK * 1024, VB = 4 * DT * 1024;
-  __shared__ Shared sh;
   __shared__ v4f sbuf[2][2][4];                  // a block's ks, log2 vs, 1 / vs
   extern __shared__ __align__(16) uint8_t lds[];
   const int tid = threadIdx.x & 255, lane = tid & 63;
@@ -44,7 +43,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
   const int n = lane & 31, hf = lane >> 5;
   const int h = blockIdx.x % A.H;
   Piece P;
-  if (!locate<kPreRows, kPreThr>(A, blockIdx.x / A.H, sh, P)) return;
+  if (!locate<kPreRows>(A, blockIdx.x / A.H, P)) return;
 
   // ---- this lane's query row
   const int rr = P.rt * kPreRows + 32 * wave + n, qi = rr / A.G, gq = rr - qi * A.G;
@@ -312,6 +311,8 @@ void start(const Att& A, uint32_t tiles, hipStream_t s) {
 
 template <int D, bool FP8>
 void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
+  if (A.plan)
+    plan8<kPreRows><<<1, kPlanThr, (A.B + 1) * sizeof(int32_t), s>>>(A, tiles + A.target);
   const bool qlo = A.q_dtype == QKV_F32, plo = A.out_dtype != QKV_BF16;
   if (qlo) {
     if (plo) start<D, FP8, true, true>(A, tiles, s);
