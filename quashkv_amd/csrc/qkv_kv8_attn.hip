@@ -15,6 +15,15 @@
 // all 16 tokens of block g: one pair of scales per lane, and its weights are, as they
 // stand, the B operand of the value product, whose A operand is 16 bytes of a V block.
 // Nothing of K, V or P passes through LDS.
+//
+// Bound: HBM, 2 d + 1/2 bytes per token and kv head.  A wave has a step's K and V (16 KiB at
+// d = 128) in flight while it works on the step before; four waves a CU keep 64 KiB.
+// Measured, a call among others with its join: 32 x 8192 tokens, 32 / 8 heads, d = 128, bf16:
+// 87 us, 6.2 TB/s (a read-only probe reaches 6.2); 131,072 tokens of one request 50 us
+// (5.4 TB/s); 40 requests up to 9001 tokens, d = 96, e4m3: 33 us (5.3 TB/s).  One VALU
+// kernel with a wave per query and head took 1791 us for the first.
+// Small calls are the chain lengths - page - bytes - merge: 7 us (16 x 2048 tokens, 2 kv
+// heads, d = 64), and the launches.
 #include "qkv_kv8_attn.h"
 
 namespace {
@@ -287,10 +296,13 @@ void place_parts(Att& A, void* at, int rows, int32_t d) {
   // (nslots * rows * 8 bytes of part_ml: 16-byte aligned)
   A.plan = A.B > 64 ? reinterpret_cast<int4*>(A.part_ml + int64_t(A.nslots) * rows * 2) : nullptr;
 }
-// Requests of more rows than this go to prefill8.
+// Requests of more rows than this go to prefill8.  us on decode8 / prefill8 at 64 rows a
+// request, d = 128, 8 kv heads: 1 x 8000 tokens 18 / 28, 8 x 2000 21 / 27, 8 x 8000 61 / 49,
+// 32 x 2000 57 / 46, 32 x 8000 195 / 146; at 32 rows decode8 has two tiles and is the
+// faster one but for the last (109 / 116).
 constexpr int kFew = 32;
-// A cache of up to this many tokens a request is not cut: its pieces' second launch costs
-// more than the steps that they would save.
+// A cache of up to this many tokens a request is not cut: the join's launch costs more than
+// the steps that it saves (one fp32 query over 512 tokens, 8 heads: 14 us against 17).
 constexpr int64_t kWhole = 1024;
 constexpr int32_t kNever = INT32_MAX / 2;
 

@@ -13,7 +13,8 @@
 //
 // Bytes are few (12 out per row), so latency bounds it: lengths are read once, a
 // workgroup scans them 1024 at a time, and while the batch is small the same
-// workgroup fills the rows from LDS.
+// workgroup fills the rows from LDS.  64 requests of one token: 2.8 us (scans by LDS
+// shuffles in 1024 threads: 6.4); 384 requests, 32,768 rows: 3.7 + 4.4 us.
 #include <algorithm>
 
 #include "qkv_common.h"
