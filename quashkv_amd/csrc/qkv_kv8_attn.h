@@ -23,6 +23,9 @@ constexpr int kThr = 64 * kWaves;
 constexpr float kHead = 8.f;     // the running maximum may lag by 2^8 before a rescale
 constexpr float kUp = 7.f;       // largest weight in f16: 2^(kUp + kHead) at most, 2^kUp at least,
                                  // so that f16's smallest step is 2^-31 of it
+// The sum of weights is kept times this: with scales from 2^-100 to 2^121 and weights from
+// 2^kUp to 2^(kUp + kHead) it stays a normal fp32 up to 2^22 tokens.
+constexpr float kSum = 0x1p-10f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Att {
@@ -504,7 +507,7 @@ __global__ __launch_bounds__(kThr) void join8(Att A) {
       const int rr = t.w * ROWS + rr0 + r, qi = rr / A.G;
       const int64_t row = int64_t(t.y) + qi;
       if (!on || qi >= t.z || row < 0 || row >= A.rows) continue;
-      const float inv = L > 0.f ? 1.f / L : 0.f;
+      const float inv = L > 0.f ? kSum / L : 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] *= inv;
       store8(A.out, (row * A.Hq + h * A.G + rr - qi * A.G) * D + d0, x, A.out_dtype, A.out_vec);
@@ -534,7 +537,7 @@ __global__ __launch_bounds__(kThr) void join8(Att A) {
         y0 = fmaf(acc[w][wave][c], e, y0);
         y1 = fmaf(acc[w][wave][c + 1], e, y1);
       }
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = sum > 0.f ? kSum / sum : 0.f;
       const int64_t to = (row * A.Hq + h * A.G + rr - qi * A.G) * D + c;
       qkv_store(A.out, to, y0 * inv, A.out_dtype);
       qkv_store(A.out, to + 1, y1 * inv, A.out_dtype);

@@ -6,8 +6,9 @@
 // the value scale enters the softmax's exponent, where it costs an addend of a
 // multiply-add instead of a product per weight, and the running maximum m is taken
 // over y, so that a weight's 16 bits are spent where |p v| is large.  Codes are exact
-// in f16, and so are 16-bit queries times a power of two per row; fp32 queries, and
-// the weights of fp32 results, are f16 pairs hi + lo (22 bits).
+// in f16, and so are 16-bit queries times a power of two per row; fp32 queries, and the
+// weights beside them and of fp16 and fp32 results, are f16 pairs hi + lo (22 bits).  The
+// weights of bf16 results are one f16 each: 2^-11, where the result keeps 2^-8.
 //
 // Layout.  Scores are S^T = K Q^T on v_mfma_f32_16x16x32_f16 (rows tokens, columns the
 // query rows that share a kv head), values O^T = V^T P^T.  Row m of score tile i is token
@@ -149,7 +150,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
     const bool pos = vs > 0.f;
     float ref = m == -INFINITY ? 0.f : m - kUp;
     const float lv = (pos ? __builtin_amdgcn_logf(vs) : 0.f) - ref;
-    const float iv = pos ? __builtin_amdgcn_rcpf(vs) : 1.f;
+    const float iv = pos ? kSum * __builtin_amdgcn_rcpf(vs) : kSum;
     const bool was_ok = ok;
     const bool more = it + 1 < steps;
     if (more) {
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
     const int64_t row2 = int64_t(P.r.q0) + qi2;
     if (qi2 < P.r.ql && row2 >= 0 && row2 < A.rows) {
       if (P.slot < 0) {
-        const float inv = L > 0.f ? 1.f / L : 0.f;
+        const float inv = L > 0.f ? kSum / L : 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] *= inv;
         store8(A.out, (row2 * A.Hq + h * A.G + rr2 - qi2 * A.G) * D + d0, x, A.out_dtype, A.out_vec);
@@ -311,13 +312,9 @@ void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
   const uint32_t grid = (tiles + A.target) * A.H;
   if (A.plan)
     plan8<kRows><<<1, kPlanThr, (A.B + 1) * sizeof(int32_t), s>>>(A, tiles + A.target);
-  if (A.q_dtype == QKV_F32) {
-    if (A.out_dtype == QKV_BF16) decode8<D, FP8, true, false><<<grid, kThr, 0, s>>>(A);
-    else decode8<D, FP8, true, true><<<grid, kThr, 0, s>>>(A);
-  } else {
-    if (A.out_dtype == QKV_BF16) decode8<D, FP8, false, false><<<grid, kThr, 0, s>>>(A);
-    else decode8<D, FP8, false, true><<<grid, kThr, 0, s>>>(A);
-  }
+  if (A.q_dtype == QKV_F32) decode8<D, FP8, true, true><<<grid, kThr, 0, s>>>(A);
+  else if (A.out_dtype != QKV_BF16) decode8<D, FP8, false, true><<<grid, kThr, 0, s>>>(A);
+  else decode8<D, FP8, false, false><<<grid, kThr, 0, s>>>(A);
   if (cut) join8<D, kRows><<<join_grid(A, kRows), kThr, 0, s>>>(A);
 }
 

@@ -22,6 +22,8 @@
 // among the values of this one (86 against 82 us at 1024 queries over 4096 tokens), the
 // weights' sum by a product with ones (84), rounds without masks as straight code (spills:
 // 109).
+#include <atomic>
+
 #include "qkv_kv8_attn.h"
 
 namespace {
@@ -43,7 +45,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
   constexpr int CH = 4 * D;                      // 16-byte chunks of K and of V in a step
   constexpr int NC = (CH + 255) / 256;           // of them, per thread of a half
   constexpr int KB = 2 * KK * 1024, VB = 4 * DT * 1024;
-  __shared__ v4f sbuf[2][2][4];                  // a block's ks, log2 vs, 1 / vs
+  __shared__ v4f sbuf[2][2][4];                  // a block's ks, log2 vs, kSum / vs
   extern __shared__ __align__(16) uint8_t lds[];
   const int tid = threadIdx.x & 255, lane = tid & 63;
   const int wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -117,7 +119,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
     if (tid < 4) {
       const bool pos = vs_r > 0.f;
       sbuf[to][th][tid] = v4f{ks_r, pos ? __builtin_amdgcn_logf(vs_r) : 0.f,
-                          pos ? __builtin_amdgcn_rcpf(vs_r) : 1.f, 0.f};
+                          pos ? kSum * __builtin_amdgcn_rcpf(vs_r) : kSum, 0.f};
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -283,7 +285,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
   const float L = l * e1 + l2 * e2;
   // lane (n, hf) has coordinates 32 j + 8 q + 4 hf + 0 .. 3 of row n
   if (P.slot < 0) {
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = L > 0.f ? kSum / L : 0.f;
     e1 *= inv;
     e2 *= inv;
   }
@@ -313,10 +315,17 @@ void start(const Att& A, uint32_t tiles, hipStream_t s) {
   // two buffers of both halves; at the end D / 32 coordinate tiles, m and l
   constexpr int smem = std::max(4 * (2 * (D / 16) + 4 * (D / 32)) * 1024,
                                 (4 * (D / 32) * 16 + 16) * 256);
-  // (a failure is the launch's, which the caller reports)
-  static const hipError_t attr [[maybe_unused]] = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(&prefill8<D, FP8, QLO, PLO>),
-      hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // more LDS than a kernel has by default, asked for once per device (a failure is the
+  // launch's, which the caller reports)
+  static std::atomic<uint64_t> asked{0};
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (!(asked.load(std::memory_order_relaxed) & bit)) {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&prefill8<D, FP8, QLO, PLO>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+    asked.fetch_or(bit, std::memory_order_relaxed);
+  }
   prefill8<D, FP8, QLO, PLO><<<(tiles + A.target) * A.H, kPreThr, smem, s>>>(A);
 }
 
@@ -324,14 +333,9 @@ template <int D, bool FP8>
 void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
   if (A.plan)
     plan8<kPreRows><<<1, kPlanThr, (A.B + 1) * sizeof(int32_t), s>>>(A, tiles + A.target);
-  const bool qlo = A.q_dtype == QKV_F32, plo = A.out_dtype != QKV_BF16;
-  if (qlo) {
-    if (plo) start<D, FP8, true, true>(A, tiles, s);
-    else start<D, FP8, true, false>(A, tiles, s);
-  } else {
-    if (plo) start<D, FP8, false, true>(A, tiles, s);
-    else start<D, FP8, false, false>(A, tiles, s);
-  }
+  if (A.q_dtype == QKV_F32) start<D, FP8, true, true>(A, tiles, s);
+  else if (A.out_dtype != QKV_BF16) start<D, FP8, false, true>(A, tiles, s);
+  else start<D, FP8, false, false>(A, tiles, s);
   if (cut) join8<D, kPreRows><<<join_grid(A, kPreRows), kThr, 0, s>>>(A);
 }
 

@@ -443,6 +443,24 @@ def test_attention_scales_of_any_size(code):
     _check_attention(st, cache, [T], [70], 2, F32, F32)
 
 
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+@pytest.mark.parametrize("size", [2.0 ** -92, 2.0 ** 118])
+def test_attention_values_at_the_scales_ends(code, size):
+    """All values near the smallest scale, or near the largest fp32: the weights' sum holds."""
+    gen = torch.Generator().manual_seed(11)
+    T, H, d = 20000, 1, 64
+    st = P8.PagedKV8Store(1, H, d, 80, DEV, code=code)
+    k = torch.randn(T, H, d, generator=gen)
+    v = torch.randn(T, H, d, generator=gen) * size
+    st.append(k.to(DEV), v.to(DEV), st.plan(i32([T]), T))
+    kd, vd = (x.cpu().double() for x in st.read(_slots(st, 0, T).to(DEV)))
+    for Q in (1, 30):
+        q = torch.randn(Q, 4, d, generator=gen)
+        x = P8.attention_kv8(q.to(DEV), **st.pools(), table=st.table, kv_lens=st.lens)
+        o, tol = R.attend(q.double(), kd, vd, 0.125, None, 2.0 ** -22, 2.0 ** -22, HALF[F32])
+        assert ((x.cpu().double() - o).abs() <= tol + 2.0 ** -149).all(), Q
+
+
 def test_attention_uniform_rows():
     """Without q_start: rows split evenly, the same result as with it."""
     st, cache = _filled(3, 2, 128, [90, 5, 200], "int8", 64, seed=6)
@@ -756,6 +774,43 @@ def test_refusals():
     st.append(x[:0], x[:0], st.plan(i32([0, 0]), 0))
     assert st.read(slots[:0])[0].shape == (0, 2, 64)
     assert P8.attention_kv8(q[:0], **pools, **att).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("B", [6, 80])
+def test_captured_chunks(B):
+    """A batch of chunks and decode rows, cut requests among them, captured and replayed."""
+    rng = random.Random(B)
+    lens = [rng.randrange(1, 400) for _ in range(B)]
+    lens[1], lens[B - 2] = 2500, 1800
+    q_lens = [1 if b % 3 else min(lens[b], 60) for b in range(B)]
+    st, _ = _filled(B, 2, 64, lens, "int8", 64, seed=B)
+    start = [0]
+    for n in q_lens:
+        start.append(start[-1] + n)
+    q = torch.zeros(start[-1], 8, 64, dtype=BF16, device=DEV)
+    out = torch.zeros(start[-1], 8, 64, device=DEV)
+    kv = i32(lens)
+    args = dict(**st.pools(), table=st.table, kv_lens=kv, q_start=i32(start), causal=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        P8.attention_kv8(q, **args, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        P8.attention_kv8(q, **args, out=out)
+    gen = torch.Generator(device=DEV).manual_seed(B)
+    for i in range(6):
+        q.copy_(torch.randn(q.shape, generator=gen, device=DEV))
+        if i % 2:                               # shorter: other cuts, the same graph
+            kv.copy_(i32([max(n, t // 2) for n, t in zip(q_lens, lens)]))
+        else:
+            kv.copy_(i32(lens))
+        g.replay()
+        torch.cuda.synchronize()
+        ref = P8.attention_kv8(q, **args)
+        assert torch.equal(out, ref), i
+        assert ref.any()
 
 
 def test_grow_keeps_the_cache():
