@@ -525,13 +525,31 @@ def test_attention_of_many_requests(B, pt):
     _check_attention(st, cache, lens, q_lens, 4, BF16, F32, gaps=gaps)
 
 
-@pytest.mark.parametrize("H,G,Q", [(1, 1, 1), (3, 11, 1), (5, 16, 2), (1, 32, 1), (16, 1, 40),
-                                   (7, 3, 200)])
+@pytest.mark.parametrize("H,G,Q", [(1, 1, 1), (3, 11, 1), (5, 16, 2), (1, 32, 1), (1, 71, 1),
+                                   (16, 1, 40), (7, 3, 200)])
 def test_attention_head_layouts(H, G, Q):
     """Cut requests at odd head counts and wide groups."""
     lens = [2500, 1100]
     st, cache = _filled(2, H, 64, lens, "fp8", 256, seed=H)
     _check_attention(st, cache, lens, [Q, min(Q, 3)], G, F16, F32)
+
+
+def test_attention_of_nothing():
+    """Requests that hold no token, short and long: zeros, and rows of no request stay."""
+    st = P8.PagedKV8Store(3, 2, 96, 4, DEV, page_tokens=64)
+    st.kscale.fill_(float("nan"))
+    st.vscale.fill_(float("nan"))
+    for q_lens in ([1, 0, 2], [40, 1, 70], [0, 0, 0]):
+        rows = sum(q_lens) + 3
+        start = [0, q_lens[0], q_lens[0] + q_lens[1], sum(q_lens)]
+        q = torch.randn(rows, 6, 96, device=DEV, dtype=F16)
+        out = torch.full((rows, 6, 96), 3.0, device=DEV)
+        P8.attention_kv8(q, **st.pools(), table=st.table, kv_lens=st.lens, q_start=i32(start),
+                         causal=True, out=out)
+        assert not out[:sum(q_lens)].any() and (out[sum(q_lens):] == 3.0).all()
+        # the result that the call makes itself: zeros there too
+        assert not P8.attention_kv8(q, **st.pools(), table=st.table, kv_lens=st.lens,
+                                    q_start=i32(start), causal=True).any()
 
 
 def test_attention_lengths_off_the_table():
