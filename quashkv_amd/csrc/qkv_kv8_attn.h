@@ -26,6 +26,9 @@ constexpr float kUp = 7.f;       // largest weight in f16: 2^(kUp + kHead) at mo
 // The sum of weights is kept times this: with scales from 2^-100 to 2^121 and weights from
 // 2^kUp to 2^(kUp + kHead) it stays a normal fp32 up to 2^22 tokens.
 constexpr float kSum = 0x1p-10f;
+// Below this a value scale counts as that of a block of zeros: append makes none but 0, yet
+// what lies behind the cached tokens may be anything, and 1 / scale has to be finite.
+constexpr float kLeast = 0x1p-126f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Att {

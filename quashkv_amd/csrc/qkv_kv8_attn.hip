@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
       }
     }
     const float ck = c * ks_r, vs = vs_r;
-    const bool pos = vs > 0.f;
+    const bool pos = vs >= kLeast;
     float ref = m == -INFINITY ? 0.f : m - kUp;
     const float lv = (pos ? __builtin_amdgcn_logf(vs) : 0.f) - ref;
     const float iv = pos ? kSum * __builtin_amdgcn_rcpf(vs) : kSum;

@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
   auto put = [&](int st, int to) {
     const int keep = ok_r ? P.r.kv - st * kStep : 0;  // tokens of the step
     if (tid < 4) {
-      const bool pos = vs_r > 0.f;
+      const bool pos = vs_r >= kLeast;
       sbuf[to][th][tid] = v4f{ks_r, pos ? __builtin_amdgcn_logf(vs_r) : 0.f,
                           pos ? kSum * __builtin_amdgcn_rcpf(vs_r) : kSum, 0.f};
     }

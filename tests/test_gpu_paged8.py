@@ -563,6 +563,26 @@ def test_attention_lengths_off_the_table():
         assert torch.equal(x, y) and not x[Q:].any() and x[:Q].any()
 
 
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+def test_attention_scales_behind_the_tokens(code):
+    """Scales of blocks behind the cached tokens may be anything: subnormal ones too, whose
+    inverse is infinite."""
+    lens = [70, 1, 130]
+    st, cache = _filled(3, 2, 64, lens, code, 256, seed=12)
+    unset = st.vscale.isinf()                 # _filled's mark of what no append wrote
+    assert unset.view(-1, 4).any(1).logical_and(~unset.view(-1, 4).all(1)).any()
+    for Q in (1, 40):
+        q = torch.randn(3 * Q, 4, 64, device=DEV)
+        args = dict(**st.pools(), table=st.table, kv_lens=i32(lens))
+        ref = P8.attention_kv8(q, **args)
+        assert ref.isfinite().all() and ref.view(3, -1).any(1).all()
+        for x in (2.0 ** -149, 2.0 ** -130, -1.0, 3e38, float("nan")):
+            st.vscale[unset] = x
+            st.kscale[unset] = x
+            assert torch.equal(P8.attention_kv8(q, **args), ref), x
+        st.vscale[unset] = float("inf")
+
+
 def test_attention_nan_stays_in_its_row():
     """A query of NaN or infinities leaves the other queries as they are."""
     st, cache = _filled(1, 1, 64, [150], "int8", 64, seed=10)
