@@ -709,12 +709,13 @@ int qkv_paged_decode_attention_layers(
  * ---------------------------------------------------------------------- */
 #define QKV_CODES_I8 0   /* int8, largest code 127 */
 #define QKV_CODES_E4M3 1 /* float8 e4m3 (finite), largest code 448 */
+#define QKV_PAGED_TOKENS (0x7fffffff - 63) /* of a request: steps of 64 end in 31 bits */
 
 /* Page tables and slot maps of B requests (<= 16000) from their lengths:
  * request b holds lens[b] tokens and brings new_lens[b] (negative: 0), whose
  * rows follow those of request b - 1 in the batch.  It is served wholly or not
- * at all: not, if its rows end behind `rows`, its pages behind pages_per_seq,
- * or if it needs pages and the pages needed up to it, in request order, exceed
+ * at all: not, if its rows end behind `rows`, its pages behind pages_per_seq, its
+ * tokens behind QKV_PAGED_TOKENS, or if it needs pages and the pages needed up to it, in request order, exceed
  * the free ones.
  *   table       B x pages_per_seq: entries of newly opened pages are written
  *   free_list   num_pages entries, the first free_count[0] of them free pages;
@@ -769,8 +770,8 @@ int qkv_kv8_read(const int64_t* slots, int64_t rows, int32_t H, int32_t d, int32
  *               [b rows / B, (b + 1) rows / B)
  *   q_lens      rows of each request from q_start[b] on; null: up to the next
  *               request's
- *   kv_lens     at most pages_per_seq pages' tokens count; tokens whose table
- *               entry names no page of the pool are left out
+ *   kv_lens     at most pages_per_seq pages' tokens, and QKV_PAGED_TOKENS, count;
+ *               tokens whose table entry names no page of the pool are left out
  *   max_q       the longest request's rows, as far as known (<= rows): picks
  *               the kernels, not the result
  *   workspace   qkv_kv8_attention_workspace_bytes(...) bytes, 256-byte aligned,

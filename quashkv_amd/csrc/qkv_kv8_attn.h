@@ -78,7 +78,9 @@ __device__ __forceinline__ Req request(const Att& A, int b) {
     r.ql = A.q_lens ? A.q_lens[b] : A.q_start[b + 1] - r.q0;
     r.ql = min(max(r.ql, 0), A.rows);
   }
-  const int64_t room = int64_t(A.width) << A.lg, kv = A.kv_lens[b];
+  int64_t room = int64_t(A.width) << A.lg;
+  if (room > QKV_PAGED_TOKENS) room = QKV_PAGED_TOKENS;
+  const int64_t kv = A.kv_lens[b];
   r.kv = static_cast<int32_t>(kv < 0 ? 0 : kv < room ? kv : room);
   return r;
 }

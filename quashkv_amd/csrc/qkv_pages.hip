@@ -6,7 +6,7 @@
 // requests -- of the new tokens (each request's first row) and of the pages
 // asked for (each request's place in the free list) -- decide everything:
 //   request b is served if its rows end within `rows`, its pages within the
-//   table's width, and, where it asks for pages, the sum of the pages asked for
+//   table's width, its tokens within QKV_PAGED_TOKENS, and, where it asks for pages, the sum of the pages asked for
 //   up to and including it within the free ones;
 //   its k-th new page is free[count - 1 - (sum before b) - k];
 //   its i-th row is token t = len + i at slot page(t / n) * n + t % n.
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(THR) void plan_scan(Plan P) {
     const int64_t end = rows0 + block_scan<THR>(add, part, total);
     rows0 += total;
     const int64_t held = (len + n - 1) >> P.lg, want = (len + add + n - 1) >> P.lg;
-    const bool fits = end <= P.rows && want <= P.width && len + add <= INT32_MAX;
+    const bool fits = end <= P.rows && want <= P.width && len + add <= QKV_PAGED_TOKENS;
     const int64_t ask = fits ? want - held : 0;
     const int64_t top = ask0 + block_scan<THR>(ask, part, total);
     ask0 += total;

@@ -100,8 +100,8 @@ def plan_pages(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor,
     ``lens`` / ``free_count`` themselves.
 
     A request is served wholly or not at all (``q_lens`` 0, slots -1, its
-    length kept): not, when its rows end behind ``rows`` or its pages behind the
-    table's width, or when it needs pages and the pages needed up to it, in
+    length kept): not, when its rows end behind ``rows``, its pages behind the
+    table's width or its tokens behind 2^31 - 64, or when it needs pages and the pages needed up to it, in
     request order, exceed the free ones."""
     dev = _one_device("plan_pages", table, lens, new_lens, free, free_count)
     if table.dim() != 2:
@@ -465,10 +465,9 @@ class PagedKV8Engine:
                                                             torch.bfloat16):
             keys, values = keys.float(), values.float()
         if S > 0:
+            k, v = (x.transpose(1, 2).reshape(B * S, H, d) for x in (keys, values))
             new = torch.full((B,), S, dtype=torch.int32, device=dev)
-            plan = st.plan(new, B * S, max_q_len=S)
-            st.append(keys.transpose(1, 2).reshape(B * S, H, d),
-                      values.transpose(1, 2).reshape(B * S, H, d), plan)
+            st.append(k, v, st.plan(new, B * S, max_q_len=S))
         self._total_tokens += S
         self._appends += 1
 

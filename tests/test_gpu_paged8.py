@@ -100,6 +100,17 @@ def test_plan_random(B, rows, seed):
     _check_plan(lens, new, 64, rows, spare=rng.choice([None, B // 2]), seed=seed)
 
 
+def test_plan_longest_request():
+    """A request holds up to 2^31 - 64 tokens: one that would pass them is not served."""
+    pt, width = 2048, 1 << 20
+    table = torch.zeros(2, width, dtype=torch.int32, device=DEV)
+    lens, new = i32([2 ** 31 - 70, 2 ** 31 - 70]), i32([7, 6])
+    plan = P8.plan_pages(table, lens, new, i32([5, 6]), i32([2]), 13, pt)
+    assert plan.q_lens.tolist() == [0, 6] and plan.free_count.item() == 2
+    assert plan.kv_lens.tolist() == [2 ** 31 - 70, 2 ** 31 - 64]
+    assert plan.positions.tolist() == [0] * 7 + list(range(2 ** 31 - 70, 2 ** 31 - 64))
+
+
 def test_plan_no_requests():
     plan = P8.plan_pages(torch.zeros(0, 4, dtype=torch.int32, device=DEV), i32([]), i32([]),
                          i32([0, 1]), i32([2]), 5, 64)
@@ -523,6 +534,54 @@ def test_attention_of_many_requests(B, pt):
     for b in range(0, B, 9):
         q_lens[b] = rng.choice([9, 33, 50])
     _check_attention(st, cache, lens, q_lens, 4, BF16, F32, gaps=gaps)
+
+
+def test_attention_of_the_most_requests():
+    """16,000 requests give, bit by bit, what 64 at a time give (nothing is cut)."""
+    B, pt, G, d = 16000, 64, 2, 64
+    gen = torch.Generator(DEV).manual_seed(1)
+    st = P8.PagedKV8Store(B, 1, d, B, DEV, page_tokens=pt, pages_per_seq=1)
+    for t in (st.kpool, st.vpool):
+        t.copy_(torch.randint(-127, 128, t.shape, generator=gen, device=DEV, dtype=torch.int8))
+    for t in (st.kscale, st.vscale):
+        t.uniform_(0.001, 0.1, generator=gen)
+    st.table.copy_(torch.randperm(B, generator=gen, device=DEV).view(B, 1))
+    kv = torch.randint(0, pt + 1, (B,), generator=gen, device=DEV, dtype=torch.int32)
+    for wide in (False, True):
+        n = torch.randint(0, 3, (B,), generator=gen, device=DEV, dtype=torch.int32)
+        if wide:
+            n[::50] = 40
+        start = torch.zeros(B + 1, dtype=torch.int32, device=DEV)
+        start[1:] = n.cumsum(0)
+        at = start.tolist()
+        q = torch.randn(at[-1], G, d, generator=gen, device=DEV).to(BF16)
+        args = dict(**st.pools(), causal=True, out_dtype=BF16)
+        out = P8.attention_kv8(q, table=st.table, kv_lens=kv, q_start=start, **args)
+        for b in range(0, B, 64):
+            part = P8.attention_kv8(q[at[b]:at[b + 64]], table=st.table[b:b + 64],
+                                    kv_lens=kv[b:b + 64], q_start=start[b:b + 65] - at[b], **args)
+            assert torch.equal(out[at[b]:at[b + 64]], part), (wide, b)
+    with pytest.raises(ValueError, match="16000"):
+        P8.attention_kv8(q, table=st.table.new_zeros(B + 1, 1), kv_lens=kv.new_zeros(B + 1),
+                         q_start=start.new_zeros(B + 2), **args)
+
+
+@pytest.mark.parametrize("Q", [1, 40])
+def test_attention_of_the_longest_request(Q):
+    """2^31 - 64 tokens, all but the first and the last page's on no page of the pool."""
+    pt, n = 2048, 4096 - 64
+    st, cache = _filled(1, 1, 64, [n], "int8", pt, seed=14)
+    first, last = st.table[0, :2].tolist()
+    table = torch.full((1, 1 << 20), -1, dtype=torch.int32, device=DEV)
+    table[0, 0], table[0, -1] = first, last
+    q = torch.randn(Q, 1, 64, generator=torch.Generator().manual_seed(3)).to(BF16)
+    args = dict(**st.pools(), table=table, out_dtype=BF16)
+    x = P8.attention_kv8(q.to(DEV), kv_lens=i32([2 ** 31 - 64]), **args)
+    o, tol = R.attend(q.double(), cache.values(0, 0)[:n], cache.values(0, 1)[:n], 0.125, None,
+                      2.0 ** -22, 2.0 ** -11, HALF[BF16])
+    assert ((x.cpu().double() - o).abs() <= tol).all()
+    # lengths past that count as it
+    assert torch.equal(P8.attention_kv8(q.to(DEV), kv_lens=i32([2 ** 31 - 1]), **args), x)
 
 
 @pytest.mark.parametrize("H,G,Q", [(1, 1, 1), (3, 11, 1), (5, 16, 2), (1, 32, 1), (1, 71, 1),
