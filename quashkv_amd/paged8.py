@@ -78,9 +78,11 @@ class PagePlan:
               max_q_len: Optional[int] = None) -> "PagePlan":
         if rows < 0:
             raise ValueError(f"rows must not be negative; got {rows}")
-        # one allocation for the int32 parts
+        # one allocation for the int32 parts (without split's records for autograd, which
+        # integers have not: 2.7 -> 1.5 us)
         q_start, q_lens, kv, positions, scratch, count = torch.empty(
-            4 * B + rows + 2, dtype=torch.int32, device=device).split((B + 1, B, B, rows, B, 1))
+            4 * B + rows + 2, dtype=torch.int32, device=device).unsafe_split_with_sizes(
+                (B + 1, B, B, rows, B, 1))
         return cls(q_start, q_lens, kv if kv_lens is None else kv_lens,
                    torch.empty(rows, dtype=torch.int64, device=device), positions,
                    count if free_count is None else free_count, scratch,
