@@ -308,14 +308,22 @@ constexpr int64_t kWhole = 1024;
 constexpr int32_t kNever = INT32_MAX / 2;
 
 template <int D, bool FP8>
-void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
+void launch(const Att& A, uint32_t tiles, hipStream_t s) {
   const uint32_t grid = (tiles + A.target) * A.H;
   if (A.plan)
     plan8<kRows><<<1, kPlanThr, (A.B + 1) * sizeof(int32_t), s>>>(A, tiles + A.target);
   if (A.q_dtype == QKV_F32) decode8<D, FP8, true, true><<<grid, kThr, 0, s>>>(A);
   else if (A.out_dtype != QKV_BF16) decode8<D, FP8, false, true><<<grid, kThr, 0, s>>>(A);
   else decode8<D, FP8, false, false><<<grid, kThr, 0, s>>>(A);
-  if (cut) join8<D, kRows><<<join_grid(A, kRows), kThr, 0, s>>>(A);
+}
+
+// The joins of what decode8 (A) and prefill8 (P) have cut; null: nothing.
+template <int D>
+void join(const Att* A, const Att* P, hipStream_t s) {
+  const uint32_t a = A ? join_grid(*A, kRows) : 0, p = P ? join_grid(*P, kPreRows) : 0;
+  if (A && P) join_both8<D><<<a + p, kThr, 0, s>>>(*A, *P, static_cast<int>(a));
+  else if (A) join8<D, kRows><<<a, kThr, 0, s>>>(*A);
+  else if (P) join8<D, kPreRows><<<p, kThr, 0, s>>>(*P);
 }
 
 }  // namespace
@@ -416,25 +424,32 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
     const uint32_t t = static_cast<uint32_t>(
         pre ? std::min<int64_t>(tiles(kRows), int64_t(B) * (kFew / kRows)) : tiles(kRows));
     if (fmt == QKV_CODES_I8) {
-      if (d == 128) launch<128, false>(A, t, cut, s);
-      else if (d == 96) launch<96, false>(A, t, cut, s);
-      else launch<64, false>(A, t, cut, s);
+      if (d == 128) launch<128, false>(A, t, s);
+      else if (d == 96) launch<96, false>(A, t, s);
+      else launch<64, false>(A, t, s);
     } else {
-      if (d == 128) launch<128, true>(A, t, cut, s);
-      else if (d == 96) launch<96, true>(A, t, cut, s);
-      else launch<64, true>(A, t, cut, s);
+      if (d == 128) launch<128, true>(A, t, s);
+      else if (d == 96) launch<96, true>(A, t, s);
+      else launch<64, true>(A, t, s);
     }
     QKV_LAUNCHED();
   }
+  Att P = A;
+  bool cut8 = false;
   if (pre) {
-    place_parts(A, static_cast<uint8_t*>(workspace) + part_bytes(B, rows, G, Hkv, kRows, d),
+    place_parts(P, static_cast<uint8_t*>(workspace) + part_bytes(B, rows, G, Hkv, kRows, d),
                 kPreRows, d);
     // cut only where the tiles, as far as the rows tell, do not fill the card
     const int64_t t = tiles(kPreRows);
-    const bool cut8 = cut && rows * G / kPreRows < A.target;
-    A.least = cut8 ? 4 : kNever;
-    qkv_kv8_prefill(A, d, fmt == QKV_CODES_E4M3, static_cast<uint32_t>(t), cut8, s);
+    cut8 = cut && rows * G / kPreRows < P.target;
+    P.least = cut8 ? 4 : kNever;
+    qkv_kv8_prefill(P, d, fmt == QKV_CODES_E4M3, static_cast<uint32_t>(t), s);
     QKV_LAUNCHED();
   }
+  const Att *const ja = dec && cut ? &A : nullptr, *const jp = cut8 ? &P : nullptr;
+  if (d == 128) join<128>(ja, jp, s);
+  else if (d == 96) join<96>(ja, jp, s);
+  else join<64>(ja, jp, s);
+  QKV_LAUNCHED();
   return QKV_OK;
 }

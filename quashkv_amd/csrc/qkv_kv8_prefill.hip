@@ -330,25 +330,24 @@ void start(const Att& A, uint32_t tiles, hipStream_t s) {
 }
 
 template <int D, bool FP8>
-void launch(const Att& A, uint32_t tiles, bool cut, hipStream_t s) {
+void launch(const Att& A, uint32_t tiles, hipStream_t s) {
   if (A.plan)
     plan8<kPreRows><<<1, kPlanThr, (A.B + 1) * sizeof(int32_t), s>>>(A, tiles + A.target);
   if (A.q_dtype == QKV_F32) start<D, FP8, true, true>(A, tiles, s);
   else if (A.out_dtype != QKV_BF16) start<D, FP8, false, true>(A, tiles, s);
   else start<D, FP8, false, false>(A, tiles, s);
-  if (cut) join8<D, kPreRows><<<join_grid(A, kPreRows), kThr, 0, s>>>(A);
 }
 
 }  // namespace
 
-void qkv_kv8_prefill(const Att& A, int32_t d, bool fp8, uint32_t tiles, bool cut, hipStream_t s) {
+void qkv_kv8_prefill(const Att& A, int32_t d, bool fp8, uint32_t tiles, hipStream_t s) {
   if (fp8) {
-    if (d == 128) launch<128, true>(A, tiles, cut, s);
-    else if (d == 96) launch<96, true>(A, tiles, cut, s);
-    else launch<64, true>(A, tiles, cut, s);
+    if (d == 128) launch<128, true>(A, tiles, s);
+    else if (d == 96) launch<96, true>(A, tiles, s);
+    else launch<64, true>(A, tiles, s);
   } else {
-    if (d == 128) launch<128, false>(A, tiles, cut, s);
-    else if (d == 96) launch<96, false>(A, tiles, cut, s);
-    else launch<64, false>(A, tiles, cut, s);
+    if (d == 128) launch<128, false>(A, tiles, s);
+    else if (d == 96) launch<96, false>(A, tiles, s);
+    else launch<64, false>(A, tiles, s);
   }
 }
