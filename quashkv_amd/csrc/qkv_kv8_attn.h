@@ -159,6 +159,12 @@ __device__ __forceinline__ bool locate(const Att& A, int want, Piece& P) {
     const float sum = lane_value(wave_scan(static_cast<float>(tiles) * st), 63);
     const int all = K::PRE ? lane_value(wave_scan(tiles), 63) : 0;
     C = K::length(A, sum, all);
+    // prefill8's workgroups have a CU each, and one piece too many would run behind all others
+    // (4 chunks of 400 rows over 1500 tokens, 14 / 2 heads: 49 -> 27 us): C grows until
+    // the pieces are within the target, as at last they are, being the tiles
+    if (K::PRE && all < A.target)
+      while (lane_value(wave_scan(tiles * ((st + C - 1) / C)), 63) > A.target)
+        C += max(K::ROUND, C / 8 / K::ROUND * K::ROUND);
     if (K::reversed(C)) want = want < all ? all - 1 - want : INT32_MAX;
     const int per = (st + C - 1) / C, mine = tiles * per, cut = per > 1 ? mine : 0;
     const int end = wave_scan(mine), cuts = wave_scan(cut);
@@ -574,5 +580,6 @@ inline uint32_t join_grid(const Att& A, int rows) {
 
 }  // namespace qkv_kv8
 
-// Launches prefill8 over up to `tiles` tiles (a bound).
-void qkv_kv8_prefill(const qkv_kv8::Att& A, int32_t d, bool fp8, uint32_t tiles, hipStream_t s);
+// Launches prefill8 over up to `pieces` pieces (a bound) per kv head.
+void qkv_kv8_prefill(const qkv_kv8::Att& A, int32_t d, bool fp8, uint32_t pieces,
+                     hipStream_t s);

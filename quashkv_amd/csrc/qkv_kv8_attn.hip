@@ -308,10 +308,9 @@ constexpr int64_t kWhole = 1024;
 constexpr int32_t kNever = INT32_MAX / 2;
 
 template <int D, bool FP8>
-void launch(const Att& A, uint32_t tiles, hipStream_t s) {
-  const uint32_t grid = (tiles + A.target) * A.H;
-  if (A.plan)
-    plan8<kRows><<<1, kPlanThr, (A.B + 1) * sizeof(int32_t), s>>>(A, tiles + A.target);
+void launch(const Att& A, uint32_t pieces, hipStream_t s) {
+  const uint32_t grid = pieces * A.H;
+  if (A.plan) plan8<kRows><<<1, kPlanThr, (A.B + 1) * sizeof(int32_t), s>>>(A, pieces);
   if (A.q_dtype == QKV_F32) decode8<D, FP8, true, true><<<grid, kThr, 0, s>>>(A);
   else if (A.out_dtype != QKV_BF16) decode8<D, FP8, false, true><<<grid, kThr, 0, s>>>(A);
   else decode8<D, FP8, false, false><<<grid, kThr, 0, s>>>(A);
@@ -422,7 +421,8 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   if (dec) {
     // beside prefill8 this launch has only requests of up to kFew rows
     const uint32_t t = static_cast<uint32_t>(
-        pre ? std::min<int64_t>(tiles(kRows), int64_t(B) * (kFew / kRows)) : tiles(kRows));
+        (pre ? std::min<int64_t>(tiles(kRows), int64_t(B) * (kFew / kRows)) : tiles(kRows)) +
+        (cut ? A.target : 0));
     if (fmt == QKV_CODES_I8) {
       if (d == 128) launch<128, false>(A, t, s);
       else if (d == 96) launch<96, false>(A, t, s);
@@ -443,7 +443,9 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
     const int64_t t = tiles(kPreRows);
     cut8 = cut && rows * G / kPreRows < P.target;
     P.least = cut8 ? 4 : kNever;
-    qkv_kv8_prefill(P, d, fmt == QKV_CODES_E4M3, static_cast<uint32_t>(t), s);
+    // (pieces of cut tiles are within the target where the kernel counts them itself)
+    const int64_t pieces = !cut8 ? t : P.plan ? t + P.target : std::max<int64_t>(t, P.target);
+    qkv_kv8_prefill(P, d, fmt == QKV_CODES_E4M3, static_cast<uint32_t>(pieces), s);
     QKV_LAUNCHED();
   }
   const Att *const ja = dec && cut ? &A : nullptr, *const jp = cut8 ? &P : nullptr;

@@ -311,7 +311,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
 }
 
 template <int D, bool FP8, bool QLO, bool PLO>
-void start(const Att& A, uint32_t tiles, hipStream_t s) {
+void start(const Att& A, uint32_t pieces, hipStream_t s) {
   // two buffers of both halves; at the end D / 32 coordinate tiles, m and l
   constexpr int smem = std::max(4 * (2 * (D / 16) + 4 * (D / 32)) * 1024,
                                 (4 * (D / 32) * 16 + 16) * 256);
@@ -326,28 +326,27 @@ void start(const Att& A, uint32_t tiles, hipStream_t s) {
                               hipFuncAttributeMaxDynamicSharedMemorySize, smem);
     asked.fetch_or(bit, std::memory_order_relaxed);
   }
-  prefill8<D, FP8, QLO, PLO><<<(tiles + A.target) * A.H, kPreThr, smem, s>>>(A);
+  prefill8<D, FP8, QLO, PLO><<<pieces * A.H, kPreThr, smem, s>>>(A);
 }
 
 template <int D, bool FP8>
-void launch(const Att& A, uint32_t tiles, hipStream_t s) {
-  if (A.plan)
-    plan8<kPreRows><<<1, kPlanThr, (A.B + 1) * sizeof(int32_t), s>>>(A, tiles + A.target);
-  if (A.q_dtype == QKV_F32) start<D, FP8, true, true>(A, tiles, s);
-  else if (A.out_dtype != QKV_BF16) start<D, FP8, false, true>(A, tiles, s);
-  else start<D, FP8, false, false>(A, tiles, s);
+void launch(const Att& A, uint32_t pieces, hipStream_t s) {
+  if (A.plan) plan8<kPreRows><<<1, kPlanThr, (A.B + 1) * sizeof(int32_t), s>>>(A, pieces);
+  if (A.q_dtype == QKV_F32) start<D, FP8, true, true>(A, pieces, s);
+  else if (A.out_dtype != QKV_BF16) start<D, FP8, false, true>(A, pieces, s);
+  else start<D, FP8, false, false>(A, pieces, s);
 }
 
 }  // namespace
 
-void qkv_kv8_prefill(const Att& A, int32_t d, bool fp8, uint32_t tiles, hipStream_t s) {
+void qkv_kv8_prefill(const Att& A, int32_t d, bool fp8, uint32_t pieces, hipStream_t s) {
   if (fp8) {
-    if (d == 128) launch<128, true>(A, tiles, s);
-    else if (d == 96) launch<96, true>(A, tiles, s);
-    else launch<64, true>(A, tiles, s);
+    if (d == 128) launch<128, true>(A, pieces, s);
+    else if (d == 96) launch<96, true>(A, pieces, s);
+    else launch<64, true>(A, pieces, s);
   } else {
-    if (d == 128) launch<128, false>(A, tiles, s);
-    else if (d == 96) launch<96, false>(A, tiles, s);
-    else launch<64, false>(A, tiles, s);
+    if (d == 128) launch<128, false>(A, pieces, s);
+    else if (d == 96) launch<96, false>(A, pieces, s);
+    else launch<64, false>(A, pieces, s);
   }
 }

@@ -593,6 +593,14 @@ def test_attention_head_layouts(H, G, Q):
     _check_attention(st, cache, lens, [Q, min(Q, 3)], G, F16, F32)
 
 
+@pytest.mark.parametrize("lens,q_lens,G", [([1500] * 4, [400] * 4, 7),
+                                           ([3000, 40, 1100], [30, 40, 90], 16)])
+def test_attention_of_cut_chunks(lens, q_lens, G):
+    """Long tiles of a few chunks: as many pieces as the card holds at once, joined."""
+    st, cache = _filled(len(lens), 1, 64, lens, "int8", 256, seed=21)
+    _check_attention(st, cache, lens, q_lens, G, BF16, F32)
+
+
 def test_attention_of_nothing():
     """Requests that hold no token, short and long: zeros, and rows of no request stay."""
     st = P8.PagedKV8Store(3, 2, 96, 4, DEV, page_tokens=64)
