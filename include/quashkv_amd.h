@@ -772,10 +772,11 @@ int qkv_kv8_read(const int64_t* slots, int64_t rows, int32_t H, int32_t d, int32
  *               request's
  *   kv_lens     at most pages_per_seq pages' tokens, and QKV_PAGED_TOKENS, count;
  *               tokens whose table entry names no page of the pool are left out
- *   max_q       the longest request's rows, as far as known (<= rows): picks
- *               the kernels, not the result
- *   workspace   qkv_kv8_attention_workspace_bytes(...) bytes, 256-byte aligned,
- *               of this call alone until it has run; nothing in it need be set */
+ *   max_q       the longest request's rows, as far as known: picks the kernels
+ *               and the workspace's size, not the result
+ *   workspace   qkv_kv8_attention_workspace_bytes(...) bytes at the call's max_q,
+ *               256-byte aligned, of this call alone until it has run; nothing
+ *               in it need be set */
 int64_t qkv_kv8_attention_workspace_bytes(int32_t B, int64_t rows, int32_t Hq, int32_t Hkv,
                                           int32_t d, int64_t max_q);
 int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_stride,

@@ -307,6 +307,21 @@ constexpr int kFew = 32;
 constexpr int64_t kWhole = 1024;
 constexpr int32_t kNever = INT32_MAX / 2;
 
+// Whether prefill8 runs, and the workspace: decode8's part, then prefill8's where it runs.  The
+// one rule for both: `max_q`, which may be wrong, decides (too small: decode8, which takes
+// requests of any rows).
+struct Layout {
+  bool pre;
+  int64_t at_pre, bytes;
+};
+Layout layout(int64_t B, int64_t rows, int32_t G, int32_t H, int32_t d, int64_t max_q) {
+  Layout L;
+  L.pre = std::min(max_q, rows) * G > kFew;
+  L.at_pre = part_bytes(B, rows, G, H, kRows, d);
+  L.bytes = L.at_pre + (L.pre ? part_bytes(B, rows, G, H, kPreRows, d) : 0);
+  return L;
+}
+
 template <int D, bool FP8>
 void launch(const Att& A, uint32_t pieces, hipStream_t s) {
   const uint32_t grid = pieces * A.H;
@@ -331,9 +346,7 @@ extern "C" int64_t qkv_kv8_attention_workspace_bytes(int32_t B, int64_t rows, in
                                                      int32_t Hkv, int32_t d, int64_t max_q) {
   if (Hkv < 1 || d < 1) return 0;
   if (B < 1 || rows < 1) return 256;
-  const int32_t G = Hq / Hkv;
-  return part_bytes(B, rows, G, Hkv, kRows, d) +
-         (max_q * G > kFew ? part_bytes(B, rows, G, Hkv, kPreRows, d) : 0);
+  return layout(B, rows, Hq / Hkv, Hkv, d, max_q).bytes;
 }
 
 extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_stride,
@@ -366,8 +379,8 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
               "qkv_kv8_attention: null pointer");
   QKV_REQUIRE(qkv_aligned(kpool, 16) && qkv_aligned(vpool, 16),
               "the pools must be 16-byte aligned");
-  QKV_REQUIRE(workspace && qkv_aligned(workspace, 256) &&
-                  ws_bytes >= qkv_kv8_attention_workspace_bytes(B, rows, Hq, Hkv, d, max_q),
+  const Layout L = layout(B, rows, G, Hkv, d, max_q);
+  QKV_REQUIRE(workspace && qkv_aligned(workspace, 256) && ws_bytes >= L.bytes,
               "qkv_kv8_attention: workspace too small or not 256-byte aligned");
   const int qb = q_dtype == QKV_F32 ? 4 : 2, ob = out_dtype == QKV_F32 ? 4 : 2;
   Att A{};
@@ -402,8 +415,8 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   A.per_target = 1.f / A.target;
   A.nslots = static_cast<int32_t>(slots_of(Hkv));
   place_parts(A, workspace, kRows, d);
-  const int64_t longest = q_start ? std::min(max_q, rows) : A.uniform_q;
-  const bool pre = longest * G > kFew;
+  const int64_t longest = std::min<int64_t>(max_q, q_start ? rows : A.uniform_q);
+  const bool pre = L.pre && longest * G > kFew;
   // decode8 runs too where, as far as the rows tell, a request may be short.  (Where one is
   // against that, prefill8 takes it: slower, the same result.)
   const bool dec = !pre || (q_start && rows <= (B - 1) * longest + kFew / G);
@@ -437,8 +450,7 @@ extern "C" int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_s
   Att P = A;
   bool cut8 = false;
   if (pre) {
-    place_parts(P, static_cast<uint8_t*>(workspace) + part_bytes(B, rows, G, Hkv, kRows, d),
-                kPreRows, d);
+    place_parts(P, static_cast<uint8_t*>(workspace) + L.at_pre, kPreRows, d);
     // cut only where the tiles, as far as the rows tell, do not fill the card
     const int64_t t = tiles(kPreRows);
     cut8 = cut && rows * G / kPreRows < P.target;

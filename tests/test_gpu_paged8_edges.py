@@ -1,0 +1,92 @@
+"""The 8-bit paged cache at its edges (quashkv_amd.paged8): blocks of zero values, queries
+of NaN, scales near the largest fp32, row offsets behind the buffer, bounds of the longest
+request that are too small.  Definitions and bounds are tests/kv8_reference.py's."""
+
+import math
+
+import pytest
+import torch
+
+from quashkv_amd import _native as N
+from quashkv_amd import paged8 as P8
+from tests import kv8_reference as R
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+HALF = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
+# a weight's half step: f16 pairs, or one f16 for 16-bit results
+WEIGHT = {F32: 2.0 ** -22, F16: 2.0 ** -11, BF16: 2.0 ** -11}
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a HIP device")
+    N.lib()
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _held(k, v, code="int8", pt=256, width=None):
+    """One request's tokens (T, H, d) in a store, and what the cache holds of them
+    (float64, on the CPU)."""
+    T, H, d = k.shape
+    pages = -(-T // pt)
+    st = P8.PagedKV8Store(1, H, d, pages, DEV, page_tokens=pt, pages_per_seq=width or pages,
+                          code=code)
+    st.append(k.to(DEV), v.to(DEV), st.plan(i32([T]), T))
+    cache = R.Cache(1, H, d, code)
+    cache.append(0, k, v)
+    return st, cache.values(0, 0), cache.values(0, 1)
+
+
+def _check(st, kd, vd, q, out_dtype=F32, causal=False, scale=None, **kw):
+    """q (Q, Hq, d) against the definition."""
+    T, _, d = kd.shape
+    sc = 1 / math.sqrt(d) if scale is None else scale
+    x = P8.attention_kv8(q.to(DEV), **st.pools(), table=st.table, kv_lens=st.lens, scale=sc,
+                         causal=causal, out_dtype=out_dtype, **kw).cpu().double()
+    o, tol = R.attend(q.double(), kd, vd, sc, T - q.shape[0] if causal else None, 2.0 ** -22,
+                      WEIGHT[out_dtype], HALF[out_dtype])
+    assert torch.isfinite(x).all()
+    bad = (x - o).abs() > tol + 2.0 ** -149
+    assert not bad.any(), ((x - o).abs().max().item(), o.abs().max().item())
+    return x
+
+
+# ------------------------------------- bounds of the longest request that are too small
+
+@pytest.mark.parametrize("T", [200, 3000])                 # whole, and cut into pieces
+@pytest.mark.parametrize("Q", [1, 9, 100])
+def test_uniform_rows_whatever_the_hint(T, Q):
+    """Without q_start the hint picks kernels and workspace alike: the results are right, and
+    no byte behind the workspace that the hint asks for is written."""
+    B, H, G, d = 2, 2, 4, 128
+    gen = torch.Generator().manual_seed(T + Q)
+    st = P8.PagedKV8Store(B, H, d, 2 * -(-T // 64), DEV, page_tokens=64)
+    x = torch.randn(2, B * T, H, d, generator=gen).to(BF16)
+    st.append(*x.to(DEV), st.plan(i32([T, T]), B * T))
+    q = torch.randn(B * Q, H * G, d, generator=gen)
+    refs = []
+    for b in range(B):
+        cache = R.Cache(1, H, d, "int8")
+        cache.append(0, x[0, b * T:(b + 1) * T], x[1, b * T:(b + 1) * T])
+        refs.append(R.attend(q[b * Q:(b + 1) * Q].double(), cache.values(0, 0), cache.values(0, 1),
+                             1 / math.sqrt(d), T - Q, 2.0 ** -22, 2.0 ** -22, HALF[F32]))
+    for hint in (None, 0, 1, Q, 1000):
+        longest = Q if hint is None else min(Q, hint)
+        nbytes = P8.attention_kv8_workspace_bytes(B, B * Q, H * G, H, d, longest)
+        space = torch.full((nbytes + (32 << 20),), 0x5a, dtype=torch.uint8, device=DEV)
+        for ws in (None, space[:nbytes]):
+            out = P8.attention_kv8(q.to(DEV), **st.pools(), table=st.table, kv_lens=st.lens,
+                                   causal=True, max_q_len=hint, workspace=ws).cpu().double()
+            for b, (o, tol) in enumerate(refs):
+                assert ((out[b * Q:(b + 1) * Q] - o).abs() <= tol).all(), (hint, b)
+        assert (space[nbytes:] == 0x5a).all(), hint
+    with pytest.raises(ValueError, match="workspace"):
+        P8.attention_kv8(q.to(DEV), **st.pools(), table=st.table, kv_lens=st.lens, max_q_len=1,
+                         workspace=space[:256])
