@@ -29,6 +29,7 @@ constexpr float kSum = 0x1p-10f;
 // Below this a value scale counts as that of a block of zeros: append makes none but 0, yet
 // what lies behind the cached tokens may be anything, and 1 / scale has to be finite.
 constexpr float kLeast = 0x1p-126f;
+constexpr float kZero = 100.f;   // see stand_in
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Att {
@@ -420,6 +421,24 @@ __device__ __forceinline__ int limit(const Att& A, const Req& r, int qi) {
   return A.causal ? min(r.kv, r.kv - r.ql + qi + 1) : r.kv;
 }
 
+// What a block whose scale counts as 0 takes in place of log2(scale).  Its values are 0, so
+// its weights are part of the sum alone, and any number does that keeps them in range.  One
+// for all blocks does not: beside blocks of small scales it raises the maximum until their
+// f16 weights vanish (scale 1 beside values of 1e-6: 1e-2 off), beside large ones its own
+// weights vanish from the sum.  So a lane takes what brings the largest of its weights
+// (exponent `top`) to the maximum m of the blocks so far and of the step's others, within
+// [-kZero, kZero]: the maximum is raised only by a block 2^kZero above it, or by the first one.
+__device__ __forceinline__ float stand_in(float top, float m) {
+  return m == -INFINITY ? -kZero : fminf(fmaxf(m - top, -kZero), kZero);
+}
+
+// l times 2^d, d <= 0, in two factors: of zero blocks alone, l may be 2^kZero above a sum
+// beside large scales, and d below the exponents of fp32.
+__device__ __forceinline__ float fall(float l, float d) {
+  return l * __builtin_amdgcn_exp2f(fminf(d + kZero, 0.f)) *
+         __builtin_amdgcn_exp2f(fmaxf(d, -kZero));
+}
+
 // Eight consecutive results to element `at` of out.
 __device__ __forceinline__ void store8(void* out, int64_t at, const float* x, int dt, bool vec) {
   if (!vec) {
@@ -502,15 +521,15 @@ __device__ __forceinline__ void join_tiles(const Att& A, int block, int blocks) 
 #pragma unroll
       for (int k = 0; k < 4; ++k) mn = fmaxf(mn, m[k]);
       const float ref = mn == -INFINITY ? 0.f : mn, f = __builtin_amdgcn_exp2f(M - ref);
+      L = fall(L, M - ref);
       M = mn;
-      L *= f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] *= f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
+        if (m[k] == -INFINITY) continue;  // (a piece that saw nothing)
         const float e = __builtin_amdgcn_exp2f(m[k] - ref);
-        if (e == 0.f) continue;  // (a piece that saw nothing)
-        L = fmaf(l[k], e, L);
+        L += fall(l[k], m[k] - ref);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = fmaf(v[k][j >> 2][j & 3], e, x[j]);
       }
@@ -545,7 +564,7 @@ __device__ __forceinline__ void join_tiles(const Att& A, int block, int blocks) 
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const float e = __builtin_amdgcn_exp2f(ml[w][wave][0] - ref);
-        sum = fmaf(ml[w][wave][1], e, sum);
+        sum += fall(ml[w][wave][1], ml[w][wave][0] - ref);
         y0 = fmaf(acc[w][wave][c], e, y0);
         y1 = fmaf(acc[w][wave][c + 1], e, y1);
       }

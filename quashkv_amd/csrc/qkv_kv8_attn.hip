@@ -150,7 +150,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
     const bool pos = vs >= kLeast;
     float ref = m == -INFINITY ? 0.f : m - kUp;
     const float lv = (pos ? __builtin_amdgcn_logf(vs) : 0.f) - ref;
-    const float iv = pos ? kSum * __builtin_amdgcn_rcpf(vs) : kSum;
+    float iv = pos ? kSum * __builtin_amdgcn_rcpf(vs) : kSum;
     const bool was_ok = ok;
     const bool more = it + 1 < steps;
     if (more) {
@@ -177,16 +177,33 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
         for (int j = 0; j < NJ; ++j) vr[j][x] &= mask;
       }
     }
+    if (__any(!pos)) {  // a block of zeros
+      asm volatile("");
+      float big = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) big = fmaxf(big, y[k]);
+      float others = pos ? big : -INFINITY;
+      others = fmaxf(others, __shfl_xor(others, 16, 64));
+      others = fmaxf(others, __shfl_xor(others, 32, 64));
+      const float z = pos ? 0.f : stand_in(big + ref, fmaxf(m, others + ref));
+#pragma unroll
+      for (int k = 0; k < 16; ++k) y[k] += z;
+      iv = pos ? iv : kSum * __builtin_amdgcn_exp2f(-z);
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) vr[j][x] = pos ? vr[j][x] : 0;
+    }
 #pragma unroll
     for (int k = 0; k < 16; ++k) top = fmaxf(top, y[k]);
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     if (__any(top > kUp + kHead || m == -INFINITY)) {
       const float mn = fmaxf(m, top + ref);
-      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      const float d = mn == -INFINITY ? 0.f : m - mn, f = __builtin_amdgcn_exp2f(d);
       const float by = mn == -INFINITY ? 0.f : mn - kUp - ref;
       m = mn;
-      l *= f;
+      l = fall(l, d);
 #pragma unroll
       for (int j = 0; j < NJ; ++j) o[j] *= f;
 #pragma unroll
@@ -248,7 +265,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const float f = __builtin_amdgcn_exp2f(red_ml[w][r][0] - ref);
-      L = fmaf(red_ml[w][r][1], f, L);
+      L += fall(red_ml[w][r][1], red_ml[w][r][0] - ref);
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = fmaf(red_o[w][r][d0 + j], f, x[j]);
     }

@@ -45,7 +45,8 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
   constexpr int CH = 4 * D;                      // 16-byte chunks of K and of V in a step
   constexpr int NC = (CH + 255) / 256;           // of them, per thread of a half
   constexpr int KB = 2 * KK * 1024, VB = 4 * DT * 1024;
-  __shared__ v4f sbuf[2][2][4];                  // a block's ks, log2 vs, kSum / vs
+  __shared__ v4f sbuf[2][2][4];                  // a block's ks, log2 vs, kSum / vs, and the
+                                                 // step's blocks of zeros, a bit each
   extern __shared__ __align__(16) uint8_t lds[];
   const int tid = threadIdx.x & 255, lane = tid & 63;
   const int wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -118,8 +119,9 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
     const int keep = ok_r ? P.r.kv - st * kStep : 0;  // tokens of the step
     if (tid < 4) {
       const bool pos = vs_r >= kLeast;
+      const uint32_t zeros = static_cast<uint32_t>(__ballot(!pos && keep > kBlk * tid));
       sbuf[to][th][tid] = v4f{ks_r, pos ? __builtin_amdgcn_logf(vs_r) : 0.f,
-                          pos ? kSum * __builtin_amdgcn_rcpf(vs_r) : kSum, 0.f};
+                          pos ? kSum * __builtin_amdgcn_rcpf(vs_r) : kSum, __uint_as_float(zeros)};
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -192,6 +194,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
       }
       // ---- exponents of the weights, against the running maximum so far
       float iv[4];
+      const int zeros = __builtin_amdgcn_readfirstlane(__float_as_int(sbuf[buf][th][0][3]));
       float top = -INFINITY, ref = m == -INFINITY ? 0.f : m - kUp;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
@@ -213,6 +216,26 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
           for (int j = 0; j < 16; ++j)
             s[i][j] = 32 * i + (j & 3) + 8 * (j >> 2) < left ? s[i][j] : -INFINITY;
       }
+      if (zeros != 0) {
+        asm volatile("");
+        float big[4], others = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          big[b] = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) big[b] = fmaxf(big[b], s[b >> 1][8 * (b & 1) + j]);
+          if (!(zeros >> b & 1)) others = fmaxf(others, big[b]);
+        }
+        others = fmaxf(others, __shfl_xor(others, 32, 64));
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          if (!(zeros >> b & 1)) continue;
+          const float z = stand_in(big[b] + ref, fmaxf(m, others + ref));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[b >> 1][8 * (b & 1) + j] += z;
+          iv[b] = kSum * __builtin_amdgcn_exp2f(-z);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -220,10 +243,10 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       if (__any(top > kUp + kHead || m == -INFINITY)) {
         const float mn = fmaxf(m, top + ref);
-        const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        const float d = mn == -INFINITY ? 0.f : m - mn, f = __builtin_amdgcn_exp2f(d);
         const float by = mn == -INFINITY ? 0.f : mn - kUp - ref;
         m = mn;
-        l *= f;
+        l = fall(l, d);
 #pragma unroll
         for (int j = 0; j < DT; ++j)
 #pragma unroll
@@ -232,6 +255,20 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 0; j < 16; ++j) s[i][j] -= by;
+      }
+      if (zeros != 0) {  // their weights join l here (asked among the weights below: 1 % slower)
+        asm volatile("");
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          if (!(zeros >> b & 1)) continue;
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            sum += __builtin_amdgcn_exp2f(s[b >> 1][8 * (b & 1) + j]);
+            s[b >> 1][8 * (b & 1) + j] = -INFINITY;
+          }
+          l = fmaf(sum, iv[b], l);
+        }
       }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
@@ -282,7 +319,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
   const float m2 = ml[(2 * (wave8 ^ 4)) * 64], l2 = ml[(2 * (wave8 ^ 4) + 1) * 64];
   const float M = fmaxf(m, m2), base = M == -INFINITY ? 0.f : M;
   float e1 = __builtin_amdgcn_exp2f(m - base), e2 = __builtin_amdgcn_exp2f(m2 - base);
-  const float L = l * e1 + l2 * e2;
+  const float L = fall(l, m - base) + fall(l2, m2 - base);
   // lane (n, hf) has coordinates 32 j + 8 q + 4 hf + 0 .. 3 of row n
   if (P.slot < 0) {
     const float inv = L > 0.f ? kSum / L : 0.f;

@@ -90,3 +90,67 @@ def test_uniform_rows_whatever_the_hint(T, Q):
     with pytest.raises(ValueError, match="workspace"):
         P8.attention_kv8(q.to(DEV), **st.pools(), table=st.table, kv_lens=st.lens, max_q_len=1,
                          workspace=space[:256])
+# -------------------------------------------------------- blocks of zero values
+
+# tokens whose values are 0, of T
+ZEROS = {"first": (0, 64), "middle": (320, 352), "last": (-16, None), "most": (16, -16),
+         "half": (0, 2048)}
+
+
+@pytest.mark.parametrize("T", [700, 4100])                 # whole, and cut into pieces
+@pytest.mark.parametrize("Q", [1, 40])                     # both kernels
+@pytest.mark.parametrize("size", [1e-3, 1e-6, 1e-9, 2.0 ** -92, 1e30])
+def test_zero_blocks_beside_values_of_any_size(T, Q, size):
+    gen = torch.Generator().manual_seed(T + Q)
+    k = torch.randn(T, 1, 64, generator=gen)
+    q = torch.randn(Q, 2, 64, generator=gen)
+    for name, (a, b) in ZEROS.items():
+        v = torch.randn(T, 1, 64, generator=gen) * size
+        v[a:b if b is None or b < T else T // 2] = 0
+        st, kd, vd = _held(k, v, pt=64, width=80)
+        for out_dtype in (F32, BF16):
+            x = _check(st, kd, vd, q, out_dtype, causal=Q > 1)
+            assert x.any(), name
+
+
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+@pytest.mark.parametrize("T", [300, 3000])
+@pytest.mark.parametrize("Q", [1, 40])
+def test_zero_blocks_that_take_most_of_the_weight(code, T, Q):
+    """Sink tokens: values 0, scores far above the others'."""
+    gen = torch.Generator().manual_seed(T)
+    d = 128
+    way = torch.randn(1, 1, d, generator=gen)
+    way /= way.norm()
+    for sink in ((0, 16), (160, 176), (T - 16 - T % 16, T - T % 16)):
+        for lead in (3.0, 20.0, 60.0):                     # of the scores, natural units
+            k = torch.randn(T, 1, d, generator=gen)
+            k -= (k * way).sum(-1, keepdim=True) * way
+            k[sink[0]:sink[1]] = way * lead
+            q = way * math.sqrt(d) + 0.1 * torch.randn(Q, 4, d, generator=gen)
+            for size in (1.0, 1e-5):
+                v = torch.randn(T, 1, d, generator=gen) * size
+                v[sink[0]:sink[1]] = 0
+                st, kd, vd = _held(k, v, code, pt=64, width=80)
+                _check(st, kd, vd, q)
+
+
+def test_zero_values_alone():
+    """Nothing but zeros: exactly 0, also where their codes are not."""
+    gen = torch.Generator().manual_seed(1)
+    for T in (100, 3000):
+        k = torch.randn(T, 1, 64, generator=gen)
+        v = torch.randn(T, 1, 64, generator=gen)
+        st, _, _ = _held(k, 0 * v, pt=64, width=80)
+        full, kd, vd = _held(k, v, pt=64, width=80)
+        for Q in (1, 40):
+            q = torch.randn(Q, 4, 64, generator=gen)
+            x = P8.attention_kv8(q.to(DEV), **st.pools(), table=st.table, kv_lens=st.lens)
+            assert not x.any()
+        # a scale of 0 makes any codes' values 0
+        full.vscale[:, :, 1] = 0
+        vd = vd.clone()
+        for t0 in range(16, T, 64):
+            vd[t0:t0 + 16] = 0
+        for Q in (1, 40):
+            _check(full, kd, vd, torch.randn(Q, 4, 64, generator=gen))
