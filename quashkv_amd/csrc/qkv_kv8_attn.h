@@ -439,6 +439,10 @@ __device__ __forceinline__ float fall(float l, float d) {
          __builtin_amdgcn_exp2f(fmaxf(d, -kZero));
 }
 
+// Of a sum of weights: 0 of a row that saw nothing, and a query's NaN is the result's.  (It
+// leaves m at -inf; the joins take such parts too, whose 2^(m - M) = 0 keeps a NaN.)
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : kSum / l; }
+
 // Eight consecutive results to element `at` of out.
 __device__ __forceinline__ void store8(void* out, int64_t at, const float* x, int dt, bool vec) {
   if (!vec) {
@@ -527,7 +531,6 @@ __device__ __forceinline__ void join_tiles(const Att& A, int block, int blocks) 
       for (int j = 0; j < 8; ++j) x[j] *= f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (m[k] == -INFINITY) continue;  // (a piece that saw nothing)
         const float e = __builtin_amdgcn_exp2f(m[k] - ref);
         L += fall(l[k], m[k] - ref);
 #pragma unroll
@@ -538,7 +541,7 @@ __device__ __forceinline__ void join_tiles(const Att& A, int block, int blocks) 
       const int rr = t.w * ROWS + rr0 + r, qi = rr / A.G;
       const int64_t row = int64_t(t.y) + qi;
       if (!on || qi >= t.z || row < 0 || row >= A.rows) continue;
-      const float inv = L > 0.f ? kSum / L : 0.f;
+      const float inv = inverse(L);
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] *= inv;
       store8(A.out, (row * A.Hq + h * A.G + rr - qi * A.G) * D + d0, x, A.out_dtype, A.out_vec);
@@ -568,7 +571,7 @@ __device__ __forceinline__ void join_tiles(const Att& A, int block, int blocks) 
         y0 = fmaf(acc[w][wave][c], e, y0);
         y1 = fmaf(acc[w][wave][c + 1], e, y1);
       }
-      const float inv = sum > 0.f ? kSum / sum : 0.f;
+      const float inv = inverse(sum);
       const int64_t to = (row * A.Hq + h * A.G + rr - qi * A.G) * D + c;
       qkv_store(A.out, to, y0 * inv, A.out_dtype);
       qkv_store(A.out, to + 1, y1 * inv, A.out_dtype);

@@ -273,7 +273,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
     const int64_t row2 = int64_t(P.r.q0) + qi2;
     if (qi2 < P.r.ql && row2 >= 0 && row2 < A.rows) {
       if (P.slot < 0) {
-        const float inv = L > 0.f ? kSum / L : 0.f;
+        const float inv = inverse(L);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] *= inv;
         store8(A.out, (row2 * A.Hq + h * A.G + rr2 - qi2 * A.G) * D + d0, x, A.out_dtype, A.out_vec);

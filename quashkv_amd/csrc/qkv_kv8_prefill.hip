@@ -322,7 +322,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
   const float L = fall(l, m - base) + fall(l2, m2 - base);
   // lane (n, hf) has coordinates 32 j + 8 q + 4 hf + 0 .. 3 of row n
   if (P.slot < 0) {
-    const float inv = L > 0.f ? kSum / L : 0.f;
+    const float inv = inverse(L);
     e1 *= inv;
     e2 *= inv;
   }

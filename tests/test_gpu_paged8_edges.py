@@ -154,3 +154,29 @@ def test_zero_values_alone():
             vd[t0:t0 + 16] = 0
         for Q in (1, 40):
             _check(full, kd, vd, torch.randn(Q, 4, 64, generator=gen))
+
+
+# ------------------------------------------------------------- queries of NaN
+
+@pytest.mark.parametrize("zero", [False, True])            # values
+@pytest.mark.parametrize("T", [150, 5000])                 # whole, and cut into pieces
+@pytest.mark.parametrize("Q", [4, 40])
+def test_nan_query_stays_nan(T, Q, zero):
+    """A query of NaN gives NaN in its row alone, whatever the cache's length."""
+    gen = torch.Generator().manual_seed(T)
+    k, v = torch.randn(2, T, 1, 64, generator=gen)
+    st, kd, vd = _held(k, v * (not zero), pt=64, width=80)
+    q = torch.randn(Q, 4, 64, generator=gen)
+    q[1, 2, 5] = float("nan")
+    q[3, 0] = float("nan")
+    same = torch.ones(Q, 4, dtype=torch.bool)
+    same[1, 2] = same[3, 0] = False
+    o, tol = R.attend(torch.where(same[..., None], q, torch.zeros(())).double(), kd, vd, 0.125,
+                      T - Q, 2.0 ** -22, 2.0 ** -22, HALF[F32])
+    x = P8.attention_kv8(q.to(DEV), **st.pools(), table=st.table, kv_lens=st.lens,
+                         causal=True).cpu().double()
+    assert ((x - o).abs() <= tol)[same].all()
+    assert x[1, 2].isnan().all() and x[3, 0].isnan().all()
+    y = P8.attention_kv8(q.to(DEV).to(BF16), **st.pools(), table=st.table, kv_lens=st.lens,
+                         causal=True, out_dtype=BF16).cpu()
+    assert torch.equal(y.isnan().all(-1), ~same) and torch.equal(y.isnan().any(-1), ~same)
