@@ -772,6 +772,10 @@ int qkv_kv8_read(const int64_t* slots, int64_t rows, int32_t H, int32_t d, int32
  *               request's
  *   kv_lens     at most pages_per_seq pages' tokens, and QKV_PAGED_TOKENS, count;
  *               tokens whose table entry names no page of the pool are left out
+ *   vscale      0 (values of 0) or, as qkv_kv8_append makes them, in [2^-100, 2^122);
+ *               of one request and head within 2^80 of each other, or the smaller
+ *               ones' weights may be missing from the softmax's sum.  Below 2^-91
+ *               the sum holds for 2^22 tokens of a request.
  *   max_q       the longest request's rows, as far as known: picks the kernels
  *               and the workspace's size, not the result
  *   workspace   qkv_kv8_attention_workspace_bytes(...) bytes at the call's max_q,

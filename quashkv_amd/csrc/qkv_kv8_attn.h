@@ -23,8 +23,14 @@ constexpr int kThr = 64 * kWaves;
 constexpr float kHead = 8.f;     // the running maximum may lag by 2^8 before a rescale
 constexpr float kUp = 7.f;       // largest weight in f16: 2^(kUp + kHead) at most, 2^kUp at least,
                                  // so that f16's smallest step is 2^-31 of it
-// The sum of weights is kept times this: with scales from 2^-100 to 2^121 and weights from
-// 2^kUp to 2^(kUp + kHead) it stays a normal fp32 up to 2^22 tokens.
+// The sum of weights p' / vs is kept times this.  (The weights take it, not 1 / vs, which at
+// the largest scales, 2^121, would leave the normal fp32.)  With weights from 2^kUp to
+// 2^(kUp + kHead) it lies between 2^(kUp - 10 - 121) and tokens x 2^(kUp + kHead - 10) / vs:
+// in range for 2^22 tokens at the smallest scale, 2^-100, and for 2^31 at 2^-91.
+// Weights below 2^-126 are 0.  They are relative to the largest p vs, so the sum is whole where
+// the value scales of a request and head, other than 0, lie within 2^80 of each other: of
+// 2^22 tokens that together are 2^-24 of the sum, each at a scale 2^80 smaller is
+// 2^(kUp - 46 - 80) = 2^-119.  (fp16 values are within 2^40.)
 constexpr float kSum = 0x1p-10f;
 // Below this a value scale counts as that of a block of zeros: append makes none but 0, yet
 // what lies behind the cached tokens may be anything, and 1 / scale has to be finite.

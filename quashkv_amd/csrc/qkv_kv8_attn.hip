@@ -150,7 +150,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
     const bool pos = vs >= kLeast;
     float ref = m == -INFINITY ? 0.f : m - kUp;
     const float lv = (pos ? __builtin_amdgcn_logf(vs) : 0.f) - ref;
-    float iv = pos ? kSum * __builtin_amdgcn_rcpf(vs) : kSum;
+    float iv = pos ? __builtin_amdgcn_rcpf(vs) : 1.f;
     const bool was_ok = ok;
     const bool more = it + 1 < steps;
     if (more) {
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
       const float z = pos ? 0.f : stand_in(big + ref, fmaxf(m, others + ref));
 #pragma unroll
       for (int k = 0; k < 16; ++k) y[k] += z;
-      iv = pos ? iv : kSum * __builtin_amdgcn_exp2f(-z);
+      iv = pos ? iv : __builtin_amdgcn_exp2f(-z);
 #pragma unroll
       for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -215,7 +215,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
       y[k] = __builtin_amdgcn_exp2f(y[k]);
       sum += y[k];
     }
-    l = fmaf(sum, iv, l);
+    l = fmaf(sum * kSum, iv, l);
     v8h ph[2], pl[PLO ? 2 : 1];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
   constexpr int CH = 4 * D;                      // 16-byte chunks of K and of V in a step
   constexpr int NC = (CH + 255) / 256;           // of them, per thread of a half
   constexpr int KB = 2 * KK * 1024, VB = 4 * DT * 1024;
-  __shared__ v4f sbuf[2][2][4];                  // a block's ks, log2 vs, kSum / vs, and the
+  __shared__ v4f sbuf[2][2][4];                  // a block's ks, log2 vs, 1 / vs, and the
                                                  // step's blocks of zeros, a bit each
   extern __shared__ __align__(16) uint8_t lds[];
   const int tid = threadIdx.x & 255, lane = tid & 63;
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
       const bool pos = vs_r >= kLeast;
       const uint32_t zeros = static_cast<uint32_t>(__ballot(!pos && keep > kBlk * tid));
       sbuf[to][th][tid] = v4f{ks_r, pos ? __builtin_amdgcn_logf(vs_r) : 0.f,
-                          pos ? kSum * __builtin_amdgcn_rcpf(vs_r) : kSum, __uint_as_float(zeros)};
+                          pos ? __builtin_amdgcn_rcpf(vs_r) : 1.f, __uint_as_float(zeros)};
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
           const float z = stand_in(big[b] + ref, fmaxf(m, others + ref));
 #pragma unroll
           for (int j = 0; j < 8; ++j) s[b >> 1][8 * (b & 1) + j] += z;
-          iv[b] = kSum * __builtin_amdgcn_exp2f(-z);
+          iv[b] = __builtin_amdgcn_exp2f(-z);
         }
       }
 #pragma unroll
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
             sum += __builtin_amdgcn_exp2f(s[b >> 1][8 * (b & 1) + j]);
             s[b >> 1][8 * (b & 1) + j] = -INFINITY;
           }
-          l = fmaf(sum, iv[b], l);
+          l = fmaf(sum * kSum, iv[b], l);
         }
       }
 #pragma unroll
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
           hi[j] = x;
           lo[j] = y;
         }
-        l = fmaf(sum, iv[b], l);
+        l = fmaf(sum * kSum, iv[b], l);
         // ---- values
 #pragma unroll
         for (int j = 0; j < DT; ++j) {

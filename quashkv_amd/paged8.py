@@ -244,6 +244,9 @@ def attention_kv8(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
     token give 0; rows of no request keep what ``out`` holds (0 where this
     call makes it).  Head h reads kv head h // (Hq // H).
 
+    Value scales of one request and head, other than 0, lie within 2^80 of each other
+    (fp16 values always do), or the smaller ones' weights may be missing from the sum.
+
     ``max_q_len``: the longest request's rows where the caller knows it (1 in a
     decode step); it picks the kernels, not the result.  ``workspace`` (uint8,
     :func:`attention_kv8_workspace_bytes`) must belong to one call at a time."""

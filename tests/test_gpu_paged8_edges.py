@@ -180,3 +180,46 @@ def test_nan_query_stays_nan(T, Q, zero):
     y = P8.attention_kv8(q.to(DEV).to(BF16), **st.pools(), table=st.table, kv_lens=st.lens,
                          causal=True, out_dtype=BF16).cpu()
     assert torch.equal(y.isnan().all(-1), ~same) and torch.equal(y.isnan().any(-1), ~same)
+
+
+# ------------------------------------------------------ scales at fp32's upper end
+
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+@pytest.mark.parametrize("Q", [1, 40])
+def test_values_near_the_largest_fp32(code, Q):
+    """Scales up to 2^121, whose inverse times the weights' sum's factor is no normal fp32.
+    (What the cache holds is read back: the definition's append clamps at 3e38.)"""
+    gen = torch.Generator().manual_seed(Q)
+    T, d = 640, 64
+    way = torch.zeros(d)
+    way[0] = 1.0
+    k = torch.randn(T, 1, d, generator=gen) * (1 - way)
+    v = torch.randn(T, 1, d, generator=gen).clamp(-1, 1) * 3.3e38
+    k[5] = way * 40
+    q = torch.randn(Q, 4, d, generator=gen)
+    for lead in (0.0, 1.0, 3.0):       # of token 5's score: 5 to 15 above the others
+        st, _, _ = _held(k, v, code, pt=64)
+        assert st.vscale.max() > 2.0 ** (120 if code == "int8" else 118)
+        slots = st.table[0].long().repeat_interleave(64) * 64 + torch.arange(T, device=DEV) % 64
+        kd, vd = (x.cpu().double() for x in st.read(slots))
+        _check(st, kd, vd, q + lead * way)
+
+
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+@pytest.mark.parametrize("Q", [1, 40])
+def test_one_token_gives_its_values(code, Q):
+    """One token's weight cancels: what is left of roundings are the f16 pair's (2^-22), those
+    of log2 and 1 / scale, the sum, its inverse and the products (2^-23 each at most, six of
+    them): within 2^-20 of the value, at scales from 2^-99 to 2^121."""
+    gen = torch.Generator().manual_seed(7)
+    H, d = 512, 64
+    size = torch.exp2(torch.cat([torch.linspace(-92, 127.9, H // 2),
+                                 torch.linspace(122, 127.9, H // 2)]).double()).float()
+    k = torch.randn(1, H, d, generator=gen)
+    v = torch.randn(1, H, d, generator=gen).clamp(-1, 1) * size[:, None]
+    st, _, _ = _held(k, v, code, pt=64)
+    _, vd = st.read(st.table[0].long() * 64)
+    x = P8.attention_kv8(torch.randn(Q, H, d, generator=gen).to(DEV), **st.pools(), table=st.table,
+                         kv_lens=st.lens)
+    vd = vd.double()
+    assert ((x.double() - vd).abs() <= 2.0 ** -20 * vd.abs()).all()
