@@ -769,7 +769,8 @@ int qkv_kv8_read(const int64_t* slots, int64_t rows, int32_t H, int32_t d, int32
  *   q_start     B + 1 first rows, ascending; null: request b's rows are
  *               [b rows / B, (b + 1) rows / B)
  *   q_lens      rows of each request from q_start[b] on; null: up to the next
- *               request's
+ *               request's (the lengths count rows behind the buffer, which are
+ *               not there: the others keep their positions)
  *   kv_lens     at most pages_per_seq pages' tokens, and QKV_PAGED_TOKENS, count;
  *               tokens whose table entry names no page of the pool are left out
  *   vscale      0 (values of 0) or, as qkv_kv8_append makes them, in [2^-100, 2^122);

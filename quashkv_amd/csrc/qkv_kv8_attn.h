@@ -70,9 +70,13 @@ struct Att {
   float* part_ml;   // [slot][H][row][2]
 };
 
-// Request b's rows in this launch and its tokens.
+// Request b's rows, as its lengths have them, and its tokens.  Rows behind the buffer are no
+// part of any tile: they would push others' tiles out of the grid.
 struct Req {
   int32_t q0, ql, kv;
+  __device__ __forceinline__ int rows(const Att& A) const {
+    return max(0, min(ql, A.rows - max(q0, 0)));
+  }
 };
 
 __device__ __forceinline__ Req request(const Att& A, int b) {
@@ -83,7 +87,7 @@ __device__ __forceinline__ Req request(const Att& A, int b) {
   } else {
     r.q0 = A.q_start[b];
     r.ql = A.q_lens ? A.q_lens[b] : A.q_start[b + 1] - r.q0;
-    r.ql = min(max(r.ql, 0), A.rows);
+    r.ql = max(r.ql, 0);
   }
   int64_t room = int64_t(A.width) << A.lg;
   if (room > QKV_PAGED_TOKENS) room = QKV_PAGED_TOKENS;
@@ -132,7 +136,7 @@ struct Cut {
   static constexpr bool PRE = ROWS == kPreRows;
   static constexpr int ROUND = PRE ? 2 : kWaves;  // steps that a workgroup takes at once
   static __device__ __forceinline__ void cost(const Att& A, const Req& r, int& tiles, int& steps) {
-    const int n = r.ql * A.G;
+    const int n = r.rows(A) * A.G;
     tiles = (n > A.few) == PRE ? (n + ROWS - 1) / ROWS : 0;
     steps = max(1, (r.kv + kStep - 1) / kStep);
   }

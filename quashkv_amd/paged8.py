@@ -239,7 +239,8 @@ def attention_kv8(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
     strides) over each request's first ``kv_lens[b]`` cached tokens.
 
     Request b's rows are ``q_start[b] ... + q_lens[b]`` (without q_lens up to the
-    next request's; without q_start the rows are split evenly).  ``causal``
+    next request's, also where that lies behind the last row; without q_start the
+    rows are split evenly).  ``causal``
     places query i of q_len at token kv_len - q_len + i.  Queries that see no
     token give 0; rows of no request keep what ``out`` holds (0 where this
     call makes it).  Head h reads kv head h // (Hq // H).

@@ -223,3 +223,43 @@ def test_one_token_gives_its_values(code, Q):
                          kv_lens=st.lens)
     vd = vd.double()
     assert ((x.double() - vd).abs() <= 2.0 ** -20 * vd.abs()).all()
+
+
+# ------------------------------------------------------ rows behind the buffer
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("start,rows,lens", [
+    ([0, 50, 90, 400], 100, [300, 200, 500]),              # the last request's rows end early
+    ([0, 60, 260, 2000, 2300], 200, [90, 2500, 40, 10]),   # and one begins behind the last row
+    ([0, 1, 2, 90], 3, [70, 300, 200]),                    # one row each
+])
+def test_rows_end_with_the_buffer(start, rows, lens, causal):
+    """Without q_lens a request's rows run to the next one's first, as far as there are any."""
+    B, H, G, d = len(lens), 1, 4, 64
+    gen = torch.Generator().manual_seed(rows)
+    for width in (16, 80):                                 # whole tiles, and cut ones
+        if max(lens) > 64 * width:
+            continue
+        st = P8.PagedKV8Store(B, H, d, sum(-(-t // 64) for t in lens), DEV, page_tokens=64,
+                              pages_per_seq=width)
+        x = torch.randn(2, sum(lens), H, d, generator=gen)
+        st.append(*x.to(DEV), st.plan(i32(lens), sum(lens)))
+        q = torch.randn(rows, H * G, d, generator=gen)
+        out = P8.attention_kv8(q.to(DEV), **st.pools(), table=st.table, kv_lens=st.lens,
+                               q_start=i32(start), causal=causal).cpu().double()
+        at = 0
+        for b, T in enumerate(lens):
+            cache = R.Cache(1, H, d, "int8")
+            cache.append(0, x[0, at:at + T], x[1, at:at + T])
+            at += T
+            a, e = min(start[b], rows), min(start[b + 1], rows)
+            if a == e:
+                continue
+            n = start[b + 1] - start[b]
+            # the definition of all n rows, of which the first are there
+            full = torch.zeros(n, H * G, d)
+            full[:e - a] = q[a:e]
+            o, tol = R.attend(full[:e - a].double(), cache.values(0, 0), cache.values(0, 1),
+                              1 / math.sqrt(d), T - n if causal else None, 2.0 ** -22,
+                              2.0 ** -22, HALF[F32])
+            assert ((out[a:e] - o).abs() <= tol).all(), (b, width)
