@@ -6,9 +6,9 @@
 // the value scale enters the softmax's exponent, where it costs an addend of a
 // multiply-add instead of a product per weight, and the running maximum m is taken
 // over y, so that a weight's 16 bits are spent where |p v| is large.  Codes are exact
-// in f16, and so are 16-bit queries times a power of two per row; fp32 queries, and the
-// weights beside them and of fp16 and fp32 results, are f16 pairs hi + lo (22 bits).  The
-// weights of bf16 results are one f16 each: 2^-11, where the result keeps 2^-8.
+// in f16, and so are 16-bit queries times a power of two per row; fp32 queries and the weights
+// are f16 pairs hi + lo (22 bits).  (Weights of one f16 for bf16 results were no faster:
+// 32 x 8192 tokens 87.0 us, with pairs 86.0.)
 //
 // Layout.  Scores are S^T = K Q^T on v_mfma_f32_16x16x32_f16 (rows tokens, columns the
 // query rows that share a kv head), values O^T = V^T P^T.  Row m of score tile i is token
@@ -38,7 +38,7 @@ __host__ __device__ constexpr int dcol(int D, int ks, int g) {
 
 // A workgroup per (piece, kv head): its waves take every fourth step of 64 tokens and
 // merge through LDS.
-template <int D, bool FP8, bool QLO, bool PLO>
+template <int D, bool FP8, bool QLO>
 __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
   constexpr int KS = D / 32, NJ = D / 16, NK = (D + 63) / 64;
   __shared__ float red_o[kWaves][kRows][D + 4];
@@ -216,20 +216,19 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
       sum += y[k];
     }
     l = fmaf(sum * kSum, iv, l);
-    v8h ph[2], pl[PLO ? 2 : 1];
+    v8h ph[2], pl[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       v4u hi, lo;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint32_t a, b = 0;
-        if constexpr (PLO) split2(y[8 * u + 2 * j], y[8 * u + 2 * j + 1], a, b);
-        else a = pk(y[8 * u + 2 * j], y[8 * u + 2 * j + 1]);
+        uint32_t a, b;
+        split2(y[8 * u + 2 * j], y[8 * u + 2 * j + 1], a, b);
         hi[j] = a;
         lo[j] = b;
       }
       ph[u] = __builtin_bit_cast(v8h, hi);
-      if constexpr (PLO) pl[u] = __builtin_bit_cast(v8h, lo);
+      pl[u] = __builtin_bit_cast(v8h, lo);
     }
     // ---- values
 #pragma unroll
@@ -238,7 +237,7 @@ __global__ __launch_bounds__(kThr, 2) void decode8(Att A) {
       for (int u = 0; u < 2; ++u) {
         const v8h a = widen8<FP8>(vr[j][2 * u], vr[j][2 * u + 1]);
         o[j] = mfma(a, ph[u], o[j]);
-        if constexpr (PLO) o[j] = mfma(a, pl[u], o[j]);
+        o[j] = mfma(a, pl[u], o[j]);
       }
     if (more) load_v(row0);
   }
@@ -343,9 +342,8 @@ template <int D, bool FP8>
 void launch(const Att& A, uint32_t pieces, hipStream_t s) {
   const uint32_t grid = pieces * A.H;
   if (A.plan) plan8<kRows><<<1, kPlanThr, (A.B + 1) * sizeof(int32_t), s>>>(A, pieces);
-  if (A.q_dtype == QKV_F32) decode8<D, FP8, true, true><<<grid, kThr, 0, s>>>(A);
-  else if (A.out_dtype != QKV_BF16) decode8<D, FP8, false, true><<<grid, kThr, 0, s>>>(A);
-  else decode8<D, FP8, false, false><<<grid, kThr, 0, s>>>(A);
+  if (A.q_dtype == QKV_F32) decode8<D, FP8, true><<<grid, kThr, 0, s>>>(A);
+  else decode8<D, FP8, false><<<grid, kThr, 0, s>>>(A);
 }
 
 // The joins of what decode8 (A) and prefill8 (P) have cut; null: nothing.

@@ -263,3 +263,16 @@ def test_rows_end_with_the_buffer(start, rows, lens, causal):
                               1 / math.sqrt(d), T - n if causal else None, 2.0 ** -22,
                               2.0 ** -22, HALF[F32])
             assert ((out[a:e] - o).abs() <= tol).all(), (b, width)
+
+
+# ---------------------------------------------------------------- bf16 results
+
+def test_bf16_decode_results_are_rounded_once():
+    """Decode weights hold 22 bits for bf16 results too: a result is the fp32 one, rounded."""
+    gen = torch.Generator().manual_seed(3)
+    for T in (100, 4000):
+        st, _, _ = _held(*torch.randn(2, T, 2, 128, generator=gen))
+        q = torch.randn(2, 8, 128, generator=gen).to(DEV).to(BF16)
+        args = dict(**st.pools(), table=st.table, kv_lens=st.lens)
+        x = P8.attention_kv8(q, **args)
+        assert torch.equal(P8.attention_kv8(q, **args, out_dtype=BF16), x.to(BF16))
