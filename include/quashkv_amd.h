@@ -762,7 +762,9 @@ int qkv_kv8_read(const int64_t* slots, int64_t rows, int32_t H, int32_t d, int32
                  void* values, int32_t out_dtype, void* stream);
 
 /* softmax(scale q K^T) V of each request's queries over its first kv_lens[b]
- * tokens; causal: query i of q_len sits at token kv_len - q_len + i.
+ * tokens; causal: query i of q_len sits at token kv_len - q_len + i.  Scores and
+ * sums are fp32; weights reach the value product in 22 bits, or in 11 for bf16
+ * results of 16-bit queries where a request has more than 32 rows of a kv head.
  *   q, out      (rows, Hq, d); head h reads kv head h / (Hq / Hkv); out dense.
  *               Rows of no request are left as they are; queries that see no
  *               token give 0.
@@ -778,7 +780,7 @@ int qkv_kv8_read(const int64_t* slots, int64_t rows, int32_t H, int32_t d, int32
  *               ones' weights may be missing from the softmax's sum.  Below 2^-91
  *               the sum holds for 2^22 tokens of a request.
  *   max_q       the longest request's rows, as far as known: picks the kernels
- *               and the workspace's size, not the result
+ *               and the workspace's size, not the result (but for rounding)
  *   workspace   qkv_kv8_attention_workspace_bytes(...) bytes at the call's max_q,
  *               256-byte aligned, of this call alone until it has run; nothing
  *               in it need be set */

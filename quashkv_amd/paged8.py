@@ -248,8 +248,12 @@ def attention_kv8(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
     Value scales of one request and head, other than 0, lie within 2^80 of each other
     (fp16 values always do), or the smaller ones' weights may be missing from the sum.
 
+    Scores and sums are fp32; softmax weights reach the value product in 22 bits,
+    or, for bf16 results of 16-bit queries where a request has more than 32 rows (of
+    a kv head), in 11, which the result's 8 bits do not show.
+
     ``max_q_len``: the longest request's rows where the caller knows it (1 in a
-    decode step); it picks the kernels, not the result.  ``workspace`` (uint8,
+    decode step); it picks the kernels, not the result (but for rounding).  ``workspace`` (uint8,
     :func:`attention_kv8_workspace_bytes`) must belong to one call at a time."""
     dev = _one_device("attention_kv8", q, kpool, kscale, vpool, vscale, table, kv_lens, q_start,
                       q_lens, out, workspace)
@@ -319,7 +323,11 @@ class PagedKV8Store:
         store.release(done)                        # finished requests' pages
 
     ``code`` is "int8" or "fp8" (float8 e4m3).  Nothing here reads a length back
-    to the host, so a step can be captured; :meth:`grow` adds pages."""
+    to the host, so a step can be captured; :meth:`grow` adds pages.
+
+    A plan's tokens count as cached from then on.  An append that refuses its rows
+    (shape, type) has written nothing: append them with the same plan, before the
+    next step reads the cache."""
 
     def __init__(self, B: int, H: int, d: int, num_pages: int, device,
                  page_tokens: int = PAGE_TOKENS, pages_per_seq: Optional[int] = None,

@@ -276,3 +276,53 @@ def test_bf16_decode_results_are_rounded_once():
         args = dict(**st.pools(), table=st.table, kv_lens=st.lens)
         x = P8.attention_kv8(q, **args)
         assert torch.equal(P8.attention_kv8(q, **args, out_dtype=BF16), x.to(BF16))
+
+
+# ---------------------------------------------------------- types and page sizes
+
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+@pytest.mark.parametrize("pt", [512, 1024])
+def test_pages_and_types(code, pt):
+    """Pages of 512 and 1024 tokens; fp16 results hold their weights in 22 bits, fp32 queries
+    give bf16 results; what the cache holds, read in fp16."""
+    gen = torch.Generator().manual_seed(pt)
+    T, H, d = 1500, 2, 96
+    k, v = torch.randn(2, T, H, d, generator=gen)
+    st, kd, vd = _held(k, v, code, pt)
+    slots = st.table[0].cpu().long()[torch.arange(T) // pt] * pt + torch.arange(T) % pt
+    order = torch.randperm(T, generator=gen)
+    for dt in (F16, BF16):
+        for x, ref in zip(st.read(slots[order].to(DEV), out_dtype=dt), (kd, vd)):
+            assert torch.equal(x.cpu(), ref[order].float().to(dt))
+    for Q in (1, 40):
+        q = torch.randn(Q, 4 * H, d, generator=gen)
+        _check(st, kd, vd, q, BF16, causal=True)
+        _check(st, kd, vd, q.half(), F16, causal=True)
+        x = P8.attention_kv8(q.half().to(DEV), **st.pools(), table=st.table, kv_lens=st.lens,
+                             out_dtype=F16).cpu().double()
+        o, tol = R.attend(q.half().double(), kd, vd, 1 / math.sqrt(d), None, 2.0 ** -22, 2.0 ** -22,
+                          HALF[F16])
+        assert ((x - o).abs() <= tol + 2.0 ** -25).all()
+
+
+# ------------------------------------------------------------- a refused append
+
+def test_refused_append_is_made_up_for():
+    """A plan stands whether its append was taken or not: the rows follow with the same plan."""
+    st = P8.PagedKV8Store(2, 1, 64, 6, DEV, page_tokens=64)
+    cache = [R.Cache(1, 1, 64, "int8") for _ in range(2)]
+    gen = torch.Generator().manual_seed(1)
+    for n in ([70, 5], [1, 1], [20, 64]):
+        x = torch.randn(2, sum(n), 1, 64, generator=gen)
+        plan = st.plan(i32(n), sum(n))
+        for k in (x[0, :, :, :32], x[0, 1:], x[0].double()):
+            with pytest.raises(ValueError):
+                st.append(k.to(DEV), x[1].to(DEV), plan)
+        st.append(*x.to(DEV), plan)
+        for b, part in enumerate(x.split(n, 1)):
+            cache[b].append(0, *part)
+    for b, T in enumerate([91, 70]):
+        t = torch.arange(T)
+        slots = st.table[b].cpu().long()[t // 64] * 64 + t % 64
+        for half, y in enumerate(st.read(slots.to(DEV))):
+            assert torch.equal(y.cpu(), cache[b].values(0, half).float())
