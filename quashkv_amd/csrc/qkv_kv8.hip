@@ -14,8 +14,9 @@
 //
 // Bytes bound it: 2 H d (in + 1) a row, and a decode step's token reads and writes its
 // V block (16 tokens) beside that.  Measured, 24,000 bf16 rows of 8 heads, d = 128, cold:
-// append 43 us (3.4 TB/s), read to bf16 35 us (4.2 TB/s); 64 rows, one per request: 5.5 and
-// 6 us a kernel.
+// append 43 us (3.4 TB/s), read to bf16 35 us (4.2 TB/s); 64 rows, one per request: 5.7 and
+// 6.2 us a kernel.  Rows in the caches take 32 and 29 us: the rest is a wave's chain, one
+// block's loads (four a lane), the reduction over them, the stores, then the next block's.
 #include "qkv_kv8.h"
 
 namespace {
@@ -368,9 +369,19 @@ __global__ __launch_bounds__(64 * kWaves) void read_rows(Rd A) {
   }
 }
 
-// Rows of a wave's unit: a block's where there are rows enough for every CU; else fewer, so
-// that a decode step's rows, each a run of its own, do not queue in one wave (2003 rows of 5
-// requests, 3 heads: a row a unit 13 us, four 6).
+// Rows of a wave's unit, by the rows alone.  Many rows are mostly prompts, whose runs fill a
+// block: one wave a block.  Few are mostly a decode step's, each a run of its own, which would
+// queue in one wave.  us of an append / a read with 16, 4 and 1 rows a unit (bf16, d = 128,
+// cached):
+//   24,000 rows of 24 requests, 8 heads    32 / 29     60 / 40    321 / 119
+//   2000 rows of 5 requests, 8 heads        5 / 5      11 / 6      33 / 13
+//   1496 rows of 8 requests, 8 heads      6.8 / 6.3   5.8 / 5.8   9.3 / 10.2
+//   600 requests of a row, 8 heads         29 / 18     12 / 6      10 / 6
+//   64 requests of a row, 8 heads          28 / 16    8.7 / 5.6   3.9 / 2.9
+//   600 requests of a row, one head        28 / 16    8.9 / 5.6   4.1 / 3.1
+//   2000 rows of 5 requests, 32 heads      13 / 12     35 / 15     49 / 43
+// (So 600 decoding requests with one head, and 2000 rows of prompts with 8 heads or more, are not
+// best served.)
 int32_t chunk_of(int64_t rows) { return rows > 4096 ? 16 : rows > 512 ? 4 : 1; }
 
 }  // namespace

@@ -596,7 +596,7 @@ __global__ __launch_bounds__(kThr) void join8(Att A) {
 
 // Both kernels' tiles in one launch, the first `split` workgroups decode8's.  (12 requests,
 // chunks of up to 301 rows beside decoding ones: 6.1 us instead of 3 + 5 and a launch; the call
-// 27.1 -> 24.6.)
+// 27.1 -> 24.6, now 25.1.)
 template <int D>
 __global__ __launch_bounds__(kThr) void join_both8(Att A, Att P, int split) {
   const int b = blockIdx.x;

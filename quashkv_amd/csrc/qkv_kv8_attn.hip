@@ -20,8 +20,8 @@
 // Bound: HBM, 2 d + 1/2 bytes per token and kv head.  A wave has a step's K and V (16 KiB at
 // d = 128) in flight while it works on the step before; four waves a CU keep 64 KiB.
 // Measured, a call among others with its join: 32 x 8192 tokens, 32 / 8 heads, d = 128, bf16:
-// 87 us, 6.2 TB/s (a read-only probe reaches 6.2); 131,072 tokens of one request 50 us
-// (5.4 TB/s); 40 requests up to 9001 tokens, d = 96, e4m3: 33 us (5.3 TB/s).  One VALU
+// 86 us, 6.3 TB/s (as a read-only probe); 131,072 tokens of one request 50 us (5.4 TB/s); 40
+// requests up to 9001 tokens, d = 96, e4m3: 33 us (4.1 TB/s).  One VALU
 // kernel with a wave per query and head took 1791 us for the first.
 // Small calls are the chain lengths - page - bytes - merge: 7 us (16 x 2048 tokens, 2 kv
 // heads, d = 64), and the launches.
@@ -319,7 +319,9 @@ void place_parts(Att& A, void* at, int rows, int32_t d) {
 // faster one but for the last (109 / 116).
 constexpr int kFew = 32;
 // A cache of up to this many tokens a request is not cut: the join's launch costs more than
-// the steps that it saves (one fp32 query over 512 tokens, 8 heads: 14 us against 17).
+// the steps that it saves (one fp32 query over 512 tokens, 8 heads: 14 us against 17).  The
+// host knows the table's width for it, not the lengths: under a wide table short requests
+// have the join's launch, too.
 constexpr int64_t kWhole = 1024;
 constexpr int32_t kNever = INT32_MAX / 2;
 

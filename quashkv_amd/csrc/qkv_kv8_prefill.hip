@@ -22,7 +22,7 @@
 // third cannot overlap (two waves of one SIMD, one with products and one with multiply-adds
 // alone: 527 and 506 us, together 693); LDS takes 2100 (reads 214 B a clock and CU, writes
 // 76).  Measured 2.2 us a round, 12 us of set-up and end; 2048 causal queries, 32 / 8 heads,
-// d = 128, bf16: 55 us a call (decode8 alone 245, four waves a workgroup and no order 74).
+// d = 128, bf16: 56 us a call (decode8 alone 245, four waves a workgroup and no order 74).
 // No gain from: a wave's priority raised over its products, the scores of the next tile
 // among the values of this one (86 against 82 us at 1024 queries over 4096 tokens), the
 // weights' sum by a product with ones (84), rounds without masks as straight code (spills:
