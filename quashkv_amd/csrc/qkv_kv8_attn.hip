@@ -20,8 +20,8 @@
 // Bound: HBM, 2 d + 1/2 bytes per token and kv head.  A wave has a step's K and V (16 KiB at
 // d = 128) in flight while it works on the step before; four waves a CU keep 64 KiB.
 // Measured, a call among others with its join: 32 x 8192 tokens, 32 / 8 heads, d = 128, bf16:
-// 86 us, 6.3 TB/s (as a read-only probe); 131,072 tokens of one request 50 us (5.4 TB/s); 40
-// requests up to 9001 tokens, d = 96, e4m3: 33 us (4.1 TB/s).  One VALU
+// 86 us, 6.3 TB/s (a read-only probe over as many bytes: 7.0); 131,072 tokens of one request
+// 50 us (5.4 TB/s); 40 requests up to 9001 tokens, d = 96, e4m3: 33 us (4.1 TB/s).  One VALU
 // kernel with a wave per query and head took 1791 us for the first.
 // Small calls are the chain lengths - page - bytes - merge: 7 us (16 x 2048 tokens, 2 kv
 // heads, d = 64), and the launches.
