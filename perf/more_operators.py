@@ -673,13 +673,13 @@ def run(st):
             out = paged8.attention_kv8_shared(
                 q, **pools, table=st["table"], kv_lens=p.kv_lens, group_start=st["group_start"],
                 prefix_lens=st["prefix_lens"], q_start=p.q_start, q_lens=p.q_lens, causal=True,
-                max_q_len=1, out=st["out"])
+                out=st["out"])
             return {"out": out, "slots": p.slots, "positions": p.positions, "kv_lens": p.kv_lens,
                     "kscale": st["kscale"], "vscale": st["vscale"]}
         return paged8.attention_kv8_shared(
             st["q"], **pools, table=st["table"], kv_lens=st["kv_lens"],
             group_start=st["group_start"], prefix_lens=st["prefix_lens"], q_start=st["q_start"],
-            q_lens=st["q_lens"], causal=st["causal"], max_q_len=st["Q"], out=st["out"])
+            q_lens=st["q_lens"], causal=st["causal"], out=st["out"])
     if kind == "rotary":
         return {"q": _plain_rotary(st["q"], st), "k": _plain_rotary(st["k"], st)}
     if kind == "fork":
