@@ -102,6 +102,7 @@ struct Piece {
   int32_t b, rt, s0, s1;
   int32_t slot;   // of its partial result, -1: the tile is not cut
   int32_t part, parts;
+  int32_t causal;
 };
 
 // Inclusive sum over a wave's lanes.
@@ -204,6 +205,7 @@ __device__ __forceinline__ bool locate(const Att& A, int want, Piece& P) {
   P.s0 = P.part * C;
   P.s1 = min(steps, P.s0 + C);
   P.slot = P.parts > 1 ? slot0 + in : -1;
+  P.causal = A.causal;
   return true;
 }
 
@@ -358,9 +360,10 @@ __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
 // A lane's part of its query row (element `at` on; 8 values from col(k) on for each product
 // step k) as f16, times a power of two that brings the row's largest into [2^9, 2^10):
 // 16-bit types are exact so, fp32 takes lo beside it.  Lanes FIRST and 32 apart share a row.
-// c: what turns a score of these into an exponent of 2.  stage: THR * 8 KS floats of LDS.
+// c: what turns a score of these into an exponent of 2.  stage: THR * 8 KS floats of LDS, for
+// threads 0 .. THR - 1 (tid).
 template <int KS, bool LO, int THR, int FIRST, typename Col>
-__device__ __forceinline__ void load_query(const Att& A, int64_t at, bool live, Col col,
+__device__ __forceinline__ void load_query(const Att& A, int64_t at, bool live, int tid, Col col,
                                            float* stage, v8h* qh, v8h* ql, float& c) {
   float x[KS][8];
   if (A.q_vec && A.q_dtype != QKV_F32) {
@@ -391,7 +394,7 @@ __device__ __forceinline__ void load_query(const Att& A, int64_t at, bool live, 
       for (int j = 0; j < 8; ++j) x[k][j] = j < 4 ? a[j & 3] : b[j & 3];
     }
   } else {  // (rolled, through LDS: it runs once, and unrolled it would be most of the code)
-    float* const t = stage + threadIdx.x;
+    float* const t = stage + tid;
 #pragma unroll 1
     for (int k = 0; k < KS; ++k)
 #pragma unroll 1
@@ -427,8 +430,8 @@ __device__ __forceinline__ void load_query(const Att& A, int64_t at, bool live, 
 }
 
 // Tokens below this are seen by query qi of the piece's request.
-__device__ __forceinline__ int limit(const Att& A, const Req& r, int qi) {
-  return A.causal ? min(r.kv, r.kv - r.ql + qi + 1) : r.kv;
+__device__ __forceinline__ int limit(const Piece& P, int qi) {
+  return P.causal ? min(P.r.kv, P.r.kv - P.r.ql + qi + 1) : P.r.kv;
 }
 
 // What a block whose scale counts as 0 takes in place of log2(scale).  Its values are 0, so
