@@ -796,6 +796,100 @@ int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_stride,
                       void* workspace, int64_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Pages that several requests of the 8-bit cache hold.  shares (num_pages
+ * int32, >= 0) counts a page's holders -- table entries within the requests'
+ * lengths -- beyond the first; pages that qkv_page_plan hands out have 0.
+ * ---------------------------------------------------------------------- */
+
+/* Fork i makes the empty request dst[i] hold the first t = min(max(tokens[i], 0),
+ * lens[src[i]]) tokens of request src[i] (tokens null: all of them).  Whole pages
+ * are shared; a page in part filled becomes one from the end of the free list,
+ * into which qkv_kv8_copy_pages brings the tokens (src_pages, dst_pages,
+ * copy_tokens), in the pools of every layer that the table serves.  All forks
+ * (<= 16000) go by the lengths before the call.  A fork is granted wholly or not at
+ * all: not, if src or dst is no request or both are the same, dst holds tokens,
+ * an earlier fork of the call names the same dst, or it needs a page and the
+ * pages needed up to it, in fork order, exceed the free ones.
+ *   granted      t, or -1 where refused
+ *   src_pages, dst_pages, copy_tokens   the page to copy, or -1, -1, 0 */
+int qkv_page_fork(int32_t* table, int32_t* lens, int32_t B, int32_t pages_per_seq,
+                  const int32_t* src, const int32_t* dst, const int32_t* tokens, int32_t forks,
+                  const int32_t* free_list, int32_t num_pages, int32_t* free_count,
+                  int32_t* shares, int32_t page_tokens, int32_t* granted, int32_t* src_pages,
+                  int32_t* dst_pages, int32_t* copy_tokens, void* stream);
+
+/* qkv_page_release for pages that may be shared: each entry of a done request
+ * takes one holder away; a page that has lost its last one goes to the end of
+ * the free list, in the order of the last entries that name each (request
+ * order, page order). */
+int qkv_page_release_shared(int32_t* lens, const uint8_t* done, int32_t B, const int32_t* table,
+                            int32_t pages_per_seq, int32_t* free_list, int32_t num_pages,
+                            int32_t* free_count, int32_t* shares, int32_t page_tokens,
+                            void* stream);
+
+/* The U pages in use -- those not among the free ones, whoever holds them -- move
+ * to places 0 .. U - 1 of the pool (<= 2^20 pages): the i-th in use at U or above
+ * goes to the i-th free one below U, and qkv_kv8_copy_pages moves their tokens
+ * (count = moves).  The requests' table entries and shares (may be null) follow;
+ * the free list becomes num_pages - 1 .. U, so that the lowest is taken first.
+ *   src_pages, dst_pages  num_pages / 2 entries, -1 behind the moves[0] first
+ *   remap                 num_pages: a page's new place (its own where it stays) */
+int qkv_page_compact(int32_t* table, const int32_t* lens, int32_t B, int32_t pages_per_seq,
+                     int32_t* free_list, int32_t num_pages, int32_t* free_count, int32_t* shares,
+                     int32_t page_tokens, int32_t* src_pages, int32_t* dst_pages, int32_t* moves,
+                     int32_t* remap, void* stream);
+
+/* Page src[i] to page dst[i] of the same pools, codes and scales of all heads:
+ * the blocks of 16 that hold its first tokens[i] tokens (null: the whole page).
+ * Pairs with a page outside the pool are left out; the first count[0] of the n
+ * pairs are taken where count is given.  No page is named as a source and a target,
+ * or twice as a target. */
+int qkv_kv8_copy_pages(const int32_t* src, const int32_t* dst, const int32_t* tokens, int32_t n,
+                       const int32_t* count, int32_t H, int32_t d, int32_t fmt, void* kpool,
+                       float* kscale, void* vpool, float* vscale, int32_t num_pages,
+                       int32_t page_tokens, void* stream);
+
+/* qkv_kv8_attention of a batch in groups whose requests share a prefix, which is read
+ * once for all of a group's rows.  Requests group_start[g] .. group_start[g + 1] - 1
+ * (ascending, <= 2048 groups; requests of no group lie before the first or behind the
+ * last) hold the same first prefix_lens[g] tokens, as qkv_page_fork makes them; whole
+ * steps of 64 of them are read from the first request of the group whose queries all
+ * see them (causal: lie behind them).  Requests of a group that do not, such as idle
+ * ones, go over their own tokens alone, as do those of no group.  The result is
+ * qkv_kv8_attention's but for rounding; weights reach the value product in 11 bits for
+ * bf16 results of 16-bit queries where a group, or a request, has more than 32 rows of a
+ * kv head.
+ *   rows        rows x Hq < 2^28
+ *   workspace   qkv_kv8_attention_shared_workspace_bytes(...) bytes, 256-byte aligned,
+ *               of this call alone until it has run; nothing in it need be set */
+int64_t qkv_kv8_attention_shared_workspace_bytes(int32_t B, int32_t groups, int64_t rows,
+                                                 int32_t Hq, int32_t Hkv, int32_t d);
+int qkv_kv8_attention_shared(const void* q, int32_t q_dtype, int64_t q_row_stride,
+                             int64_t q_head_stride, int64_t rows, const void* kpool,
+                             const float* kscale, const void* vpool, const float* vscale,
+                             int32_t fmt, int32_t num_pages, int32_t page_tokens,
+                             const int32_t* table, int32_t pages_per_seq,
+                             const int32_t* group_start, const int32_t* prefix_lens,
+                             int32_t groups, const int32_t* q_start, const int32_t* q_lens,
+                             const int32_t* kv_lens, int32_t B, int32_t Hq, int32_t Hkv,
+                             int32_t d, float scale, int32_t causal, void* out,
+                             int32_t out_dtype, void* workspace, int64_t ws_bytes, void* stream);
+
+/* Rotary positions: the pairs of the first R coordinates (even, <= 512) of each
+ * head of q (rows, Hq, d) and k (rows, Hk, d; either may have no heads) -- (i, i +
+ * R / 2), or (2 i, 2 i + 1) where interleaved -- turn by positions[row] * turns[i]
+ * units of 2^-64 of a full turn (modulo 2^64), times factor; by the negative angle
+ * where inverse (the gradient's map).  Coordinates from R on are copied.  Row and
+ * head strides in elements, the last axis dense.  The outputs are other memory
+ * than the inputs, or the inputs themselves at the same strides. */
+int qkv_rotary(int32_t dtype, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+               int32_t Hq, const void* k, int64_t k_row_stride, int64_t k_head_stride, int32_t Hk,
+               int64_t rows, int32_t d, int32_t R, const int32_t* positions, const int64_t* turns,
+               float factor, int32_t interleaved, int32_t inverse, void* q_out,
+               int64_t qo_row_stride, int64_t qo_head_stride, void* k_out, int64_t ko_row_stride,
+               int64_t ko_head_stride, void* stream);
+
+/* ------------------------------------------------------------------------
  * Measurement helper (no reference counterpart): streams `bytes` (a multiple
  * of 16, 16-byte aligned) of `buf` with 16-byte loads, `unroll` (4, 8, 16)
  * per lane in flight, nontemporal loads if `nontemporal`, over `grid`

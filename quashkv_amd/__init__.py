@@ -15,6 +15,7 @@ from .packing import pack_bits, unpack_bits
 from .nn_search import QuashIndex
 from .mixed_precision import MixedPrecisionMSEQuantizer, MixedPrecisionIPQuantizer
 from .paged8 import PagedKV8Engine, PagedKV8Store
+from .rotary import rotary_frequencies, rotary_turns
 
 __all__ = [
     "LloydMaxCodebook",
@@ -26,6 +27,8 @@ __all__ = [
     "MixedPrecisionIPQuantizer",
     "PagedKV8Engine",
     "PagedKV8Store",
+    "rotary_frequencies",
+    "rotary_turns",
     "pack_bits",
     "unpack_bits",
 ]

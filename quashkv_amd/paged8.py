@@ -15,9 +15,13 @@ Store formats (n = page_tokens = 64 << k; value = code * scale):
   at slot page * n + t % n.
 * ``free`` (P,) int32 with ``free_count`` (1,): the first free_count entries are
   free pages, taken from the end.
+* ``shares`` (P,) int32, where requests share pages: a page's holders beyond the
+  first.
 
 Operators: :func:`plan_pages`, :func:`release_pages`, :func:`append_kv8`,
-:func:`read_kv8`, :func:`attention_kv8`; :class:`PagedKV8Store` holds the
+:func:`read_kv8`, :func:`attention_kv8`; for pages that requests share
+:func:`fork_pages`, :func:`copy_pages`, :func:`compact_pages` and
+:func:`attention_kv8_shared` (quashkv_amd.rotary turns rows by their positions).  :class:`PagedKV8Store` holds the
 tensors and calls them; :class:`PagedKV8Engine` is the engine interface
 (append / attention / clear over sequences of one length) on that store.
 All calls run on the current stream of the tensors' device and never
@@ -136,22 +140,132 @@ def plan_pages(table: torch.Tensor, lens: torch.Tensor, new_lens: torch.Tensor,
 
 
 def release_pages(table: torch.Tensor, lens: torch.Tensor, done: torch.Tensor,
-                  free: torch.Tensor, free_count: torch.Tensor, page_tokens: int) -> None:
+                  free: torch.Tensor, free_count: torch.Tensor, page_tokens: int,
+                  shares: Optional[torch.Tensor] = None) -> None:
     """The pages of the requests with ``done`` ((B,) bool) go back to the free
-    list and their lengths become 0, all in place."""
-    dev = _one_device("release_pages", table, lens, done, free, free_count)
+    list and their lengths become 0, all in place.  With ``shares`` each of their
+    table entries takes one holder away, and a page goes back with its last one, at the
+    place of the last of the entries that name it."""
+    dev = _one_device("release_pages", table, lens, done, free, free_count, shares)
+    B, width, P = _check_books(table, lens, free, free_count, shares)
+    _want(done, "done", torch.bool, (B,))
+    if shares is None:
+        _call(dev, N.lib().qkv_page_release, lens.data_ptr(), done.data_ptr(), B,
+              table.data_ptr(), width, free.data_ptr(), P, free_count.data_ptr(), page_tokens)
+    else:
+        _call(dev, N.lib().qkv_page_release_shared, lens.data_ptr(), done.data_ptr(), B,
+              table.data_ptr(), width, free.data_ptr(), P, free_count.data_ptr(),
+              shares.data_ptr(), page_tokens)
+
+
+def _check_books(table: torch.Tensor, lens: torch.Tensor, free: torch.Tensor,
+                 free_count: torch.Tensor, shares: Optional[torch.Tensor]) -> tuple[int, int, int]:
+    """(requests, table width, pages) of the tensors that keep a pool's pages."""
     if table.dim() != 2:
         raise ValueError("page table must be a 2-D int32 tensor")
     B, width = table.shape
     _want(table, "page table", torch.int32)
     _want(lens, "lens", torch.int32, (B,))
-    _want(done, "done", torch.bool, (B,))
     if free.dim() != 1:
         raise ValueError("free must be a 1-D int32 tensor")
     _want(free, "free", torch.int32)
     _want(free_count, "free_count", torch.int32, (1,))
-    _call(dev, N.lib().qkv_page_release, lens.data_ptr(), done.data_ptr(), B, table.data_ptr(),
-          width, free.data_ptr(), free.numel(), free_count.data_ptr(), page_tokens)
+    if shares is not None:
+        _want(shares, "shares", torch.int32, (free.numel(),))
+    return B, width, free.numel()
+
+
+@dataclass
+class ForkPlan:
+    """What :func:`fork_pages` granted, and the pages that are to be copied (device tensors)."""
+    granted: torch.Tensor      # (F,) int32: tokens that the fork holds, -1 where refused
+    src_pages: torch.Tensor    # (F,) int32: a page in part filled, -1: none
+    dst_pages: torch.Tensor    # (F,) int32: the fork's own page for its tokens
+    copy_tokens: torch.Tensor  # (F,) int32: how many
+
+
+def fork_pages(table: torch.Tensor, lens: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+               tokens: Optional[torch.Tensor], free: torch.Tensor, free_count: torch.Tensor,
+               shares: torch.Tensor, page_tokens: int) -> ForkPlan:
+    """Requests ``dst`` ((F,) int32) go on from requests ``src``: fork i holds the first
+    ``tokens[i]`` tokens (None: all; at most all, negative counts as 0) of ``src[i]``.
+
+    Whole pages are shared (``shares``, (P,) int32, counts their holders beyond the
+    first); a page in part filled gets a page of its own from the end of the free list, into
+    which :func:`copy_pages` brings the plan's pages, in each layer's pools.  The table,
+    lengths, free count and shares move on in place.
+
+    All forks go by the lengths before the call.  A fork is granted wholly or refused
+    (``granted`` -1): where src or dst is no request or both are the same, dst holds
+    tokens, an earlier fork of the call names the same dst, or it needs a page and the
+    pages needed up to it, in fork order, exceed the free ones."""
+    dev = _one_device("fork_pages", table, lens, src, dst, tokens, free, free_count, shares)
+    B, width, P = _check_books(table, lens, free, free_count, shares)
+    if src.dim() != 1:
+        raise ValueError("src must be a 1-D int32 tensor")
+    F = src.numel()
+    _want(src, "src", torch.int32)
+    _want(dst, "dst", torch.int32, (F,))
+    if tokens is not None:
+        _want(tokens, "tokens", torch.int32, (F,))
+    out = ForkPlan(*torch.empty(4, F, dtype=torch.int32, device=dev).unbind(0))
+    _call(dev, N.lib().qkv_page_fork, table.data_ptr(), lens.data_ptr(), B, width, src.data_ptr(),
+          dst.data_ptr(), N.ptr(tokens), F, free.data_ptr(), P, free_count.data_ptr(),
+          shares.data_ptr(), page_tokens, out.granted.data_ptr(), out.src_pages.data_ptr(),
+          out.dst_pages.data_ptr(), out.copy_tokens.data_ptr())
+    return out
+
+
+@dataclass
+class CompactPlan:
+    """What :func:`compact_pages` moves (device tensors)."""
+    src_pages: torch.Tensor    # (P // 2,) int32: -1 behind the moves
+    dst_pages: torch.Tensor    # (P // 2,) int32
+    moves: torch.Tensor        # (1,) int32
+    remap: torch.Tensor        # (P,) int32: a page's new place
+
+
+def compact_pages(table: torch.Tensor, lens: torch.Tensor, free: torch.Tensor,
+                  free_count: torch.Tensor, page_tokens: int,
+                  shares: Optional[torch.Tensor] = None) -> CompactPlan:
+    """The U pages in use (those not on the free list, whoever holds them) move to places
+    0 .. U - 1 of the pool: the i-th in use at U or above to the i-th free one below.  The
+    table's entries within the requests' lengths, shares and free list (P - 1 down to U) follow
+    in place; ``copy_pages(plan.src_pages, plan.dst_pages, ..., count=plan.moves)`` moves the
+    tokens, in each layer's pools, and ``plan.remap`` serves tables of the caller's."""
+    dev = _one_device("compact_pages", table, lens, free, free_count, shares)
+    B, width, P = _check_books(table, lens, free, free_count, shares)
+    src, dst, moves, remap = torch.empty(
+        2 * (P // 2) + 1 + P, dtype=torch.int32, device=dev).unsafe_split_with_sizes(
+            (P // 2, P // 2, 1, P))
+    _call(dev, N.lib().qkv_page_compact, table.data_ptr(), lens.data_ptr(), B, width,
+          free.data_ptr(), P, free_count.data_ptr(), N.ptr(shares), page_tokens, src.data_ptr(),
+          dst.data_ptr(), moves.data_ptr(), remap.data_ptr())
+    return CompactPlan(src, dst, moves, remap)
+
+
+def copy_pages(src: torch.Tensor, dst: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
+               vpool: torch.Tensor, vscale: torch.Tensor, tokens: Optional[torch.Tensor] = None,
+               count: Optional[torch.Tensor] = None) -> None:
+    """Page ``src[i]`` to page ``dst[i]`` ((n,) int32) of the pools, codes and scales of all
+    heads: the blocks that hold its first ``tokens[i]`` tokens ((n,) int32; None: the whole
+    page), for the first ``count`` ((1,) int32) pairs (None: all).  Pairs with a page
+    outside the pool, such as -1, are left out.  No page may be source and target in one
+    call, or target twice."""
+    dev = _one_device("copy_pages", src, dst, kpool, kscale, vpool, vscale, tokens, count)
+    P, H, n, d, fmt = _check_pools(kpool, kscale, vpool, vscale)
+    if src.dim() != 1:
+        raise ValueError("src must be a 1-D int32 tensor")
+    F = src.numel()
+    _want(src, "src", torch.int32)
+    _want(dst, "dst", torch.int32, (F,))
+    if tokens is not None:
+        _want(tokens, "tokens", torch.int32, (F,))
+    if count is not None:
+        _want(count, "count", torch.int32, (1,))
+    _call(dev, N.lib().qkv_kv8_copy_pages, src.data_ptr(), dst.data_ptr(), N.ptr(tokens), F,
+          N.ptr(count), H, d, fmt, kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(),
+          vscale.data_ptr(), P, n)
 
 
 def _one_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
@@ -228,6 +342,38 @@ def read_kv8(slots: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
     return k, v
 
 
+def _check_attention(q: torch.Tensor, H: int, d: int, table: torch.Tensor, kv_lens: torch.Tensor,
+                     q_start: Optional[torch.Tensor], q_lens: Optional[torch.Tensor],
+                     out_dtype: torch.dtype, out: Optional[torch.Tensor], dev: torch.device):
+    """(rows, query heads, requests, table width, result) of an attention's arguments."""
+    if q.dim() != 3:
+        raise ValueError(f"queries must be (rows, heads, {d}); got {tuple(q.shape)}")
+    rows, Hq, dq = q.shape
+    if dq != d or Hq == 0 or Hq % H != 0:
+        raise ValueError(f"queries {tuple(q.shape)} do not match the cache (rows, a multiple of "
+                         f"{H} heads, {d})")
+    if table.dim() != 2:
+        raise ValueError("page table must be a 2-D int32 tensor")
+    B, width = table.shape
+    _want(table, "page table", torch.int32)
+    _want(kv_lens, "kv_lens", torch.int32, (B,))
+    if q_start is not None:
+        _want(q_start, "q_start", torch.int32, (B + 1,))
+    elif q_lens is not None:
+        raise ValueError("q_lens needs q_start")
+    elif B == 0 or rows % B != 0:
+        raise ValueError(f"without q_start the rows ({rows}) must be a multiple of the "
+                         f"requests ({B})")
+    if q_lens is not None:
+        _want(q_lens, "q_lens", torch.int32, (B,))
+    if out is None:
+        make = torch.empty if q_start is None else torch.zeros
+        out = make(rows, Hq, d, dtype=out_dtype, device=dev)
+    else:
+        _want(out, "out", out.dtype, (rows, Hq, d))
+    return rows, Hq, B, width, out
+
+
 def attention_kv8(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
                   vpool: torch.Tensor, vscale: torch.Tensor, table: torch.Tensor,
                   kv_lens: torch.Tensor, q_start: Optional[torch.Tensor] = None,
@@ -258,31 +404,8 @@ def attention_kv8(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
     dev = _one_device("attention_kv8", q, kpool, kscale, vpool, vscale, table, kv_lens, q_start,
                       q_lens, out, workspace)
     P, H, n, d, fmt = _check_pools(kpool, kscale, vpool, vscale)
-    if q.dim() != 3:
-        raise ValueError(f"queries must be (rows, heads, {d}); got {tuple(q.shape)}")
-    rows, Hq, dq = q.shape
-    if dq != d or Hq == 0 or Hq % H != 0:
-        raise ValueError(f"queries {tuple(q.shape)} do not match the cache (rows, a multiple of "
-                         f"{H} heads, {d})")
-    if table.dim() != 2:
-        raise ValueError("page table must be a 2-D int32 tensor")
-    B, width = table.shape
-    _want(table, "page table", torch.int32)
-    _want(kv_lens, "kv_lens", torch.int32, (B,))
-    if q_start is not None:
-        _want(q_start, "q_start", torch.int32, (B + 1,))
-    elif q_lens is not None:
-        raise ValueError("q_lens needs q_start")
-    elif B == 0 or rows % B != 0:
-        raise ValueError(f"without q_start the rows ({rows}) must be a multiple of the "
-                         f"requests ({B})")
-    if q_lens is not None:
-        _want(q_lens, "q_lens", torch.int32, (B,))
-    if out is None:
-        make = torch.empty if q_start is None else torch.zeros
-        out = make(rows, Hq, d, dtype=out_dtype, device=dev)
-    else:
-        _want(out, "out", out.dtype, (rows, Hq, d))
+    rows, Hq, B, width, out = _check_attention(q, H, d, table, kv_lens, q_start, q_lens, out_dtype,
+                                               out, dev)
     if scale is None:
         scale = 1.0 / math.sqrt(d)
     longest = rows // max(B, 1) if q_start is None else rows
@@ -312,6 +435,65 @@ def attention_kv8_workspace_bytes(B: int, rows: int, Hq: int, H: int, d: int,
     return N.lib().qkv_kv8_attention_workspace_bytes(B, rows, Hq, H, d, max_q_len)
 
 
+def attention_kv8_shared(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Tensor,
+                         vpool: torch.Tensor, vscale: torch.Tensor, table: torch.Tensor,
+                         kv_lens: torch.Tensor, group_start: torch.Tensor,
+                         prefix_lens: torch.Tensor, q_start: Optional[torch.Tensor] = None,
+                         q_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                         causal: bool = False, out_dtype: torch.dtype = torch.float32,
+                         out: Optional[torch.Tensor] = None,
+                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`attention_kv8` of a batch in groups whose requests share a prefix, which is
+    read once for all rows of a group.
+
+    Requests ``group_start[g]`` up to ``group_start[g + 1]`` ((groups + 1,) int32, ascending;
+    at most 2048 groups) hold the same first ``prefix_lens[g]`` ((groups,) int32) tokens, as
+    :func:`fork_pages` makes them; whole steps of 64 of them are read from the first request
+    of the group whose queries all see them.  Requests that do not (idle ones, chunks that
+    begin inside the prefix) and those before the first or behind the last group go over
+    all of their own tokens.
+
+    The other arguments and the result are attention_kv8's (but for rounding; weights
+    reach the value product in 11 bits, for bf16 results of 16-bit queries, where a group
+    or a request has more than 32 rows of a kv head).  ``workspace`` (uint8,
+    :func:`attention_kv8_shared_workspace_bytes`) must belong to one call at a time."""
+    dev = _one_device("attention_kv8_shared", q, kpool, kscale, vpool, vscale, table, kv_lens,
+                      group_start, prefix_lens, q_start, q_lens, out, workspace)
+    P, H, n, d, fmt = _check_pools(kpool, kscale, vpool, vscale)
+    rows, Hq, B, width, out = _check_attention(q, H, d, table, kv_lens, q_start, q_lens, out_dtype,
+                                               out, dev)
+    if prefix_lens.dim() != 1:
+        raise ValueError("prefix_lens must be a 1-D int32 tensor")
+    groups = prefix_lens.numel()
+    _want(prefix_lens, "prefix_lens", torch.int32)
+    _want(group_start, "group_start", torch.int32, (groups + 1,))
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    ts, hs, ls = q.stride()
+    if ls != 1:
+        q = q.contiguous()
+        ts, hs, ls = q.stride()
+    if workspace is None:
+        nbytes = attention_kv8_shared_workspace_bytes(B, groups, rows, Hq, H, d)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    else:
+        _want(workspace, "workspace", torch.uint8)
+        nbytes = workspace.numel()
+    _call(dev, N.lib().qkv_kv8_attention_shared, q.data_ptr(), N.dtype_code(q.dtype), ts, hs, rows,
+          kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(), vscale.data_ptr(), fmt, P, n,
+          table.data_ptr(), width, group_start.data_ptr(), prefix_lens.data_ptr(), groups,
+          N.ptr(q_start), N.ptr(q_lens), kv_lens.data_ptr(), B, Hq, H, d, float(scale),
+          1 if causal else 0, out.data_ptr(), N.dtype_code(out.dtype), workspace.data_ptr(),
+          nbytes)
+    return out
+
+
+def attention_kv8_shared_workspace_bytes(B: int, groups: int, rows: int, Hq: int, H: int,
+                                         d: int) -> int:
+    """Bytes of the workspace that attention_kv8_shared needs at these sizes."""
+    return N.lib().qkv_kv8_attention_shared_workspace_bytes(B, groups, rows, Hq, H, d)
+
+
 class PagedKV8Store:
     """Pools, page table and free list of a batch of B requests, on the device.
 
@@ -322,6 +504,11 @@ class PagedKV8Store:
         out = store.attention(q, plan)             # (rows, Hq, d), causal
         store.release(done)                        # finished requests' pages
 
+    With ``sharing`` requests may go on from others' tokens (between steps)::
+
+        store.fork(src, dst)                       # whole pages shared, not copied
+        out = store.attention(q, plan, groups=(group_start, prefix_lens))
+
     ``code`` is "int8" or "fp8" (float8 e4m3).  Nothing here reads a length back
     to the host, so a step can be captured; :meth:`grow` adds pages.
 
@@ -331,7 +518,7 @@ class PagedKV8Store:
 
     def __init__(self, B: int, H: int, d: int, num_pages: int, device,
                  page_tokens: int = PAGE_TOKENS, pages_per_seq: Optional[int] = None,
-                 code: str = "int8"):
+                 code: str = "int8", sharing: bool = False):
         if code not in CODE_DTYPES:
             raise ValueError(f"code {code!r} must be one of {tuple(CODE_DTYPES)}")
         if d not in (64, 96, 128):
@@ -353,6 +540,8 @@ class PagedKV8Store:
         # the lowest page is handed out first
         self.free = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=dev)
         self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=dev)
+        # a page's holders beyond the first; None: no page is ever shared
+        self.shares = torch.zeros(num_pages, dtype=torch.int32, device=dev) if sharing else None
         self.device = self.lens.device
 
     @property
@@ -388,7 +577,15 @@ class PagedKV8Store:
 
     def attention(self, q: torch.Tensor, plan: PagePlan, scale: Optional[float] = None,
                   causal: bool = True, out_dtype: torch.dtype = torch.float32,
-                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  out: Optional[torch.Tensor] = None,
+                  groups: Optional[tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
+        """``groups``: (group_start, prefix_lens) of attention_kv8_shared, where requests
+        share a prefix that is to be read once for all of a group."""
+        if groups is not None:
+            return attention_kv8_shared(q, **self.pools(), table=self.table, kv_lens=plan.kv_lens,
+                                        group_start=groups[0], prefix_lens=groups[1],
+                                        q_start=plan.q_start, q_lens=plan.q_lens, scale=scale,
+                                        causal=causal, out_dtype=out_dtype, out=out)
         return attention_kv8(q, **self.pools(), table=self.table, kv_lens=plan.kv_lens,
                              q_start=plan.q_start, q_lens=plan.q_lens, scale=scale, causal=causal,
                              out_dtype=out_dtype, max_q_len=plan.max_q_len, out=out)
@@ -397,7 +594,45 @@ class PagedKV8Store:
         """Finished requests' pages back to the pool (all requests' without ``done``)."""
         if done is None:
             done = torch.ones(self.B, dtype=torch.bool, device=self.device)
-        release_pages(self.table, self.lens, done, self.free, self.free_count, self.pt)
+        release_pages(self.table, self.lens, done, self.free, self.free_count, self.pt,
+                      shares=self.shares)
+
+    def fork(self, src: torch.Tensor, dst: torch.Tensor,
+             tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Empty requests ``dst`` go on from the first ``tokens`` tokens of requests ``src``
+        ((F,) int32 each; tokens None: all), see fork_pages; returns the tokens that each
+        holds, -1 where refused.  A step's rows are appended before."""
+        if self.shares is None:
+            raise ValueError("fork needs a store made with sharing=True")
+        p = fork_pages(self.table, self.lens, src, dst, tokens, self.free, self.free_count,
+                       self.shares, self.pt)
+        copy_pages(p.src_pages, p.dst_pages, **self.pools(), tokens=p.copy_tokens)
+        return p.granted
+
+    def compact(self) -> CompactPlan:
+        """The pages in use move to the lowest places of the pool, see compact_pages.  Slots of
+        plans made before are stale."""
+        p = compact_pages(self.table, self.lens, self.free, self.free_count, self.pt,
+                          shares=self.shares)
+        copy_pages(p.src_pages, p.dst_pages, **self.pools(), count=p.moves)
+        return p
+
+    def shrink(self, num_pages: int) -> None:
+        """A pool of ``num_pages`` pages, compacted (new tensors: a captured step has to be
+        captured again).  Reads the free count back to the host; ValueError, with nothing
+        changed, where more pages are in use."""
+        old = self.num_pages
+        used = old - int(self.free_count.item())
+        if num_pages < 1 or num_pages > old or used > num_pages:
+            raise ValueError(f"cannot shrink {old} pages, {used} of them in use, to {num_pages}")
+        self.compact()
+        for name in ("kpool", "vpool", "kscale", "vscale"):
+            t = getattr(self, name)
+            setattr(self, name, t.view(torch.uint8)[:num_pages].clone().view(t.dtype))
+        self.free = self.free[old - num_pages:].clone()
+        self.free_count -= old - num_pages
+        if self.shares is not None:
+            self.shares = self.shares[:num_pages].clone()
 
     def grow(self, num_pages: int, pages_per_seq: Optional[int] = None) -> None:
         """At least ``num_pages`` pages in the pool and ``pages_per_seq`` in the
@@ -415,6 +650,8 @@ class PagedKV8Store:
             ids = torch.arange(num_pages - 1, old - 1, -1, dtype=torch.int32, device=self.device)
             self.free = torch.cat([ids, self.free])
             self.free_count += more
+            if self.shares is not None:
+                self.shares = torch.cat([self.shares, torch.zeros_like(ids)])
         if pages_per_seq is not None and pages_per_seq > self.pages_per_seq:
             pad = torch.zeros(self.B, pages_per_seq - self.pages_per_seq, dtype=torch.int32,
                               device=self.device)
@@ -422,8 +659,10 @@ class PagedKV8Store:
 
     def to(self, device) -> None:
         self.device = torch.device(device)
-        for name in ("kpool", "vpool", "kscale", "vscale", "table", "lens", "free", "free_count"):
-            setattr(self, name, getattr(self, name).to(self.device))
+        for name in ("kpool", "vpool", "kscale", "vscale", "table", "lens", "free", "free_count",
+                     "shares"):
+            if getattr(self, name) is not None:
+                setattr(self, name, getattr(self, name).to(self.device))
         self.device = self.lens.device
 
     def nbytes(self) -> int:
