@@ -858,7 +858,9 @@ int qkv_kv8_copy_pages(const int32_t* src, const int32_t* dst, const int32_t* to
  * ones, go over their own tokens alone, as do those of no group.  The result is
  * qkv_kv8_attention's but for rounding; weights reach the value product in 11 bits for
  * bf16 results of 16-bit queries where a group, or a request, has more than 32 rows of a
- * kv head.
+ * kv head.  Where sharing costs more than it saves (short prefixes, requests of
+ * many rows, small calls) each request goes over its own table's tokens; `always`
+ * (0: not) shares whatever prefix two requests of a group see.
  *   rows        rows x Hq < 2^28
  *   workspace   qkv_kv8_attention_shared_workspace_bytes(...) bytes, 256-byte aligned,
  *               of this call alone until it has run; nothing in it need be set */
@@ -870,9 +872,9 @@ int qkv_kv8_attention_shared(const void* q, int32_t q_dtype, int64_t q_row_strid
                              int32_t fmt, int32_t num_pages, int32_t page_tokens,
                              const int32_t* table, int32_t pages_per_seq,
                              const int32_t* group_start, const int32_t* prefix_lens,
-                             int32_t groups, const int32_t* q_start, const int32_t* q_lens,
-                             const int32_t* kv_lens, int32_t B, int32_t Hq, int32_t Hkv,
-                             int32_t d, float scale, int32_t causal, void* out,
+                             int32_t groups, int32_t always, const int32_t* q_start,
+                             const int32_t* q_lens, const int32_t* kv_lens, int32_t B, int32_t Hq,
+                             int32_t Hkv, int32_t d, float scale, int32_t causal, void* out,
                              int32_t out_dtype, void* workspace, int64_t ws_bytes, void* stream);
 
 /* Rotary positions: the pairs of the first R coordinates (even, <= 512) of each

@@ -142,8 +142,8 @@ _SIGS = {
                                   _i32, _p]),
     "qkv_kv8_attention_shared_workspace_bytes": (_i64, [_i32, _i32, _i64, _i32, _i32, _i32]),
     "qkv_kv8_attention_shared": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p, _i32, _i32,
-                                        _i32, _p, _i32, _p, _p, _i32, _p, _p, _p, _i32, _i32,
-                                        _i32, _i32, _f32, _i32, _p, _i32, _p, _i64, _p]),
+                                        _i32, _p, _i32, _p, _p, _i32, _i32, _p, _p, _p, _i32,
+                                        _i32, _i32, _i32, _f32, _i32, _p, _i32, _p, _i64, _p]),
     "qkv_rotary": (_i32, [_i32, _p, _i64, _i64, _i32, _p, _i64, _i64, _i32, _i64, _i32, _i32, _p,
                           _p, _f32, _i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _p]),
     "qkv_hbm_read_probe": (_i32, [_p, _i64, _p, _i32, _i32, _i32, _p]),

@@ -37,11 +37,10 @@ __host__ __device__ constexpr int dcol(int D, int ks, int g) {
   return D == 96 && ks == 2 ? 64 + 8 * g : 64 * (ks >> 1) + 16 * g + 8 * (ks & 1);
 }
 
-// Four waves, tid 0 .. 255, take every fourth step of 64 tokens and merge through LDS (red_o,
-// red_ml: a wave's 16 rows each).  ROWS: partial results are a row each, [kv head][row of the
-// workspace], P.slot the one of the request's row 0; else tiles (place).
-template <int D, bool FP8, bool QLO, bool ROWS>
-__device__ __forceinline__ void decode_piece(const Att& A, const Piece& P, int h, int tid,
+// Four waves' results (tid 0 .. 255) of 16 rows over every fourth step of 64 tokens each to LDS
+// (red_o, red_ml), relative to their own maxima.
+template <int D, bool FP8, bool QLO>
+__device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h, int tid,
                                              float (*red_o)[kRows][D + 4],
                                              float (*red_ml)[kRows][2]) {
   constexpr int KS = D / 32, NJ = D / 16, NK = (D + 63) / 64;
@@ -251,6 +250,15 @@ __device__ __forceinline__ void decode_piece(const Att& A, const Piece& P, int h
     red_ml[wave][n][0] = m;
     red_ml[wave][n][1] = l;
   }
+}
+
+// Four waves take every fourth step of a piece and merge.  ROWS: partial results are a row each,
+// [kv head][row of the workspace], P.slot the one of the request's row 0; else tiles (place).
+template <int D, bool FP8, bool QLO, bool ROWS>
+__device__ __forceinline__ void decode_piece(const Att& A, const Piece& P, int h, int tid,
+                                             float (*red_o)[kRows][D + 4],
+                                             float (*red_ml)[kRows][2]) {
+  decode_steps<D, FP8, QLO>(A, P, h, tid, red_o, red_ml);
   int64_t at = -1;  // where the partial result's row 0 goes
   if constexpr (ROWS) {
     if (P.slot >= 0) at = int64_t(h) * A.nslots + P.slot + P.rt * kRows;

@@ -50,15 +50,15 @@ constexpr int kPreLds = std::max(4 * (2 * (D / 16) + 4 * (D / 32)) * 1024,
 // sbuf: a block's ks, log2 vs, 1 / vs, and the step's blocks of zeros, a bit each.  ROWS: as
 // decode_piece's.
 template <int D, bool FP8, bool QLO, bool PLO, bool ROWS>
-__device__ __forceinline__ void prefill_piece(const Att& A, const Piece& P, int h, uint8_t* lds,
-                                              v4f (*sbuf)[2][4]) {
+__device__ __forceinline__ void prefill_piece(const Att& A, const Piece& P, int h, int thread,
+                                              uint8_t* lds, v4f (*sbuf)[2][4]) {
   constexpr int KK = D / 16;                     // 16-wide product steps of a score
   constexpr int DT = D / 32;                     // 32-wide coordinate tiles
   constexpr int CH = 4 * D;                      // 16-byte chunks of K and of V in a step
   constexpr int NC = (CH + 255) / 256;           // of them, per thread of a half
   constexpr int KB = 2 * KK * 1024, VB = 4 * DT * 1024;
-  const int tid = threadIdx.x & 255, lane = tid & 63;
-  const int wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tid = thread & 255, lane = tid & 63;
+  const int wave8 = __builtin_amdgcn_readfirstlane(thread >> 6);
   const int wave = wave8 & 3, th = wave8 >> 2;
   // the half's buffer i: K's images (32-token tile, product step), V's (coordinate tile, block)
   auto kbuf = [&](int i) { return lds + (2 * i + th) * (KB + VB); };
@@ -162,7 +162,7 @@ __device__ __forceinline__ void prefill_piece(const Att& A, const Piece& P, int 
   if (mine < s1) fetch(mine);
   v8h qh[KK], ql[QLO ? KK : 1];
   float c;  // scores to exponents, without the block's scale
-  load_query<KK, QLO, kPreThr, 32>(A, row * A.q_ts + hq * A.q_hs, live, threadIdx.x,
+  load_query<KK, QLO, kPreThr, 32>(A, row * A.q_ts + hq * A.q_hs, live, thread,
                                    [&](int k) { return 16 * k + 8 * hf; },
                                    reinterpret_cast<float*>(lds), qh, ql, c);
   if (mine < s1) put(mine, 0);
@@ -186,16 +186,24 @@ __device__ __forceinline__ void prefill_piece(const Att& A, const Piece& P, int 
     if (st < s1 && t0 < lim_any) {
       // ---- scores: register 8 b + j of tile i is token 32 i + 16 b + (j & 3) + 8 (j >> 2) + 4 hf
       v16f s[2];
+      constexpr int AHEAD = 4;  // operands read ahead of their product
+      v4u a[AHEAD];
+      auto k_at = [&](int x) {
+        return *reinterpret_cast<const v4u*>(kbuf(buf) + x * 1024 + hf * 512 +
+                                             ((n ^ (x % KK & 7)) << 4));
+      };
+#pragma unroll
+      for (int x = 0; x < AHEAD; ++x) a[x] = k_at(x);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[i][j] = 0.f;
 #pragma unroll
         for (int k = 0; k < KK; ++k) {
-          const v4u a = *reinterpret_cast<const v4u*>(kbuf(buf) + (i * KK + k) * 1024 + hf * 512 +
-                                                      ((n ^ (k & 7)) << 4));
-          s[i] = mfma32(a, qh[k], s[i]);
-          if constexpr (QLO) s[i] = mfma32(a, ql[k], s[i]);
+          const int x = i * KK + k;
+          s[i] = mfma32(a[x % AHEAD], qh[k], s[i]);
+          if constexpr (QLO) s[i] = mfma32(a[x % AHEAD], ql[k], s[i]);
+          if (x + AHEAD < 2 * KK) a[x % AHEAD] = k_at(x + AHEAD);
         }
       }
       // ---- exponents of the weights, against the running maximum so far
@@ -279,7 +287,10 @@ __device__ __forceinline__ void prefill_piece(const Att& A, const Piece& P, int 
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         float sum = 0.f;
-        v4u hi, lo;
+        v4u hi, lo, v[DT];
+#pragma unroll
+        for (int j = 0; j < DT; ++j)
+          v[j] = *reinterpret_cast<const v4u*>(vbuf(buf) + (j * 4 + b) * 1024 + lane * 16);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float p0 = __builtin_amdgcn_exp2f(s[b >> 1][8 * (b & 1) + 2 * j]);
@@ -295,9 +306,8 @@ __device__ __forceinline__ void prefill_piece(const Att& A, const Piece& P, int 
         // ---- values
 #pragma unroll
         for (int j = 0; j < DT; ++j) {
-          const v4u a = *reinterpret_cast<const v4u*>(vbuf(buf) + (j * 4 + b) * 1024 + lane * 16);
-          o[j] = mfma32(a, __builtin_bit_cast(v8h, hi), o[j]);
-          if constexpr (PLO) o[j] = mfma32(a, __builtin_bit_cast(v8h, lo), o[j]);
+          o[j] = mfma32(v[j], __builtin_bit_cast(v8h, hi), o[j]);
+          if constexpr (PLO) o[j] = mfma32(v[j], __builtin_bit_cast(v8h, lo), o[j]);
         }
       }
     }

@@ -14,7 +14,7 @@ __global__ __launch_bounds__(kPreThr, 2) void prefill8(Att A) {
   extern __shared__ __align__(16) uint8_t lds[];
   Piece P;
   if (!locate<kPreRows>(A, blockIdx.x / A.H, P)) return;
-  prefill_piece<D, FP8, QLO, PLO, false>(A, P, blockIdx.x % A.H, lds, sbuf);
+  prefill_piece<D, FP8, QLO, PLO, false>(A, P, blockIdx.x % A.H, threadIdx.x, lds, sbuf);
 }
 
 template <int D, bool FP8, bool QLO, bool PLO>

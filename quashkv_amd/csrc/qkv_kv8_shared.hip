@@ -5,107 +5,402 @@
 // -- maximum m, sum l, values o, all relative to 2^m -- join as
 //   M = max m_i,  out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.
 // So the rows of a group, one behind the other as its requests are, are one set of rows over the
-// prefix' tokens, without a mask, and each request's rows are a set over its own tokens: items
-// of both kinds are cut into pieces, run in one launch, and are joined row by row.
+// prefix' tokens, without a mask, and each request's rows are a set over its own tokens.
 //
-// A request takes part in its group's prefix if its queries all lie behind it (causal), or it
-// holds the prefix at all; the prefix is read from the first of these.  The others, and those
-// of a group with one such request, go over all of their tokens by themselves.
+// A request takes part in its group's prefix if its queries all see it; the prefix is read
+// from the first of these.  The others, and those of groups for which sharing does not pay (see
+// pays), go over all of their tokens by themselves.
 //
-// Three launches: the plan (one workgroup: items, pieces, where partial results go), the
-// attention, the join.
+// Work.  Three kinds of such sets (items): of more than 32 rows, in tall tiles of 128
+// (prefill_piece); of fewer, in tiles of 16 (decode_piece); and, of these, requests' own few
+// tokens.  The first launch (share8) has the first two, on a workgroup of 8 waves per CU, each of
+// which knows its part from the lengths alone: the tall tiles' steps, tile behind tile, are cut
+// into equal ranges, one a workgroup, so that all end together wherever tiles end (8 x 210 rows,
+// 7 query heads a kv head, over 250 steps: 172 tiles on 256 CUs), and the other workgroups take
+// the short tiles, two at a time, four waves each, cut where they are long.  The second launch
+// (share_rest) takes the few own tokens, joining them with the prefix' partial results as it
+// goes, and joins whatever else was cut.
 #include <algorithm>
 #include <atomic>
 
 #include "qkv_kv8_decode.h"
 #include "qkv_kv8_prefill.h"
+#include "qkv_pages_dev.h"
 
 namespace {
 
 using namespace qkv_kv8;
 
 constexpr int kFew = 32;        // rows of an item up to which its tiles have 16 rows, else 128
-constexpr int kLeast = 4;       // steps of the shortest piece
+constexpr int kLate = 16;       // own steps of few rows that are left to the second launch
 constexpr int kMaxGroups = 2048;
+constexpr int kSmall = 64;      // requests, and groups, up to which every workgroup plans for itself
+constexpr int kItems = 2 * kSmall;
+// Set-up and end of a tall tile, in its steps (0.8 us at d = 128), and the least that a range
+// takes of one; a step of a short tile; places of a kv head's tall tiles, at most.
+constexpr int kSetUp = 8, kCut = 2;
+constexpr float kShortStep = 0.5f;
+constexpr float kMostPlaces = 0x1p30f;
 
-// What the plan leaves for the other two launches.
+// Rows of a request, or of a group, over steps [s0, s0 + steps) of request `table`'s tokens.
+struct Item {
+  int32_t q0, ql, kv, s0, steps;
+  int32_t rows;       // ql x query heads of a kv head, within the buffer; 0: nothing to do
+  int32_t table;
+  bool group;
+  bool part;          // whether its rows have other items, too
+  __device__ __forceinline__ bool tall() const { return rows > kFew; }
+  __device__ __forceinline__ bool late() const {
+    return !group && rows > 0 && !tall() && steps <= kLate;
+  }
+  __device__ __forceinline__ bool four() const { return rows > 0 && !tall() && !late(); }
+  __device__ __forceinline__ int tiles() const {
+    return tall() ? (rows + kPreRows - 1) / kPreRows : (rows + kRows - 1) / kRows;
+  }
+};
+
+// How a kv head's work is divided: its tall tiles have places, one behind the other, which are cut
+// into ranges.  Where tiles are few and long each has whole ranges (aligned); else a tile has
+// its steps and `setup` more, so that a range of many short tiles is no longer than one of a
+// part of a long one.
+struct Frame {
+  int32_t range;      // places of a range
+  int32_t tall;       // ranges
+  int32_t setup;      // -1: aligned
+  int32_t least;      // steps of a part of a short tile
+  int32_t fours;      // parts of short tiles
+  int32_t lates;      // tiles of the second launch
+};
+
+// Where items lie: for N items (groups, then requests) the sums before each, and what pieces need.
+// In LDS (every workgroup's own) or in the workspace (share_plan's).
+struct Places {
+  int32_t* tall;      // [N + 1] places of tall tiles
+  int32_t* fours;     // [N + 1] parts
+  int4* geo;          // two each: q0, ql (0: nothing to do), kv, s0; steps, 2 table + causal, slot, rows
+};
+
 struct Share {
   const int32_t* group_start;
   const int32_t* prefix_lens;
   int32_t groups;
-  int32_t* head;      // [0], [1]: tall and short pieces
-  int4* pieces;       // two each; tall ones from 0, short ones from cap_tall on
-  int32_t cap_tall, cap_short;
-  int4* meta;         // two a request: first row, first partial row of its own tokens, their
-                      // parts, rows; the same of the prefix (rows' distance last).  No parts
-                      // of its own: nothing to join
-  int32_t* row_req;   // a row's request, -1: none
-};
-
-// Rows of one piece of work over steps [s0, s1) of one request's tokens.
-struct Item {
-  int32_t q0, ql, kv, s0, s1;
-  int32_t rows;       // ql x query heads of a kv head, within the buffer
-  __device__ __forceinline__ bool tall() const { return rows > kFew; }
-  __device__ __forceinline__ int tiles() const {
-    return tall() ? (rows + kPreRows - 1) / kPreRows : (rows + kRows - 1) / kRows;
-  }
-  __device__ __forceinline__ int steps() const { return rows > 0 ? max(1, s1 - s0) : 0; }
+  int32_t always;     // groups of two members share, whatever that costs
+  int32_t small;      // whether workgroups plan for themselves
+  Frame* frame;       // the plan, for the second launch and, not small, for the first
+  Places at;          // not small
+  int4* meta;         // three a request: its own item as the join needs it (join_of) and its
+                      // group's; first rows of both, -, ql
+  int4* lates;        // three a tile of the second launch: its group's item; request, tile, first
+                      // row, ql; kv, s0, rows, rows of the group before
+  int32_t late_cap;   // tiles that it holds
+  int32_t* row_req;   // not small: a row's request, -1: none
 };
 
 __device__ __forceinline__ int steps_of(int kv) { return (kv + kStep - 1) / kStep; }
+__device__ __forceinline__ int rows_of(const Att& A, const Req& r) { return r.q0 < 0 ? 0 : r.rows(A); }
+// whole steps of a group's prefix
+__device__ __forceinline__ int prefix_of(const Share& S, int g) {
+  return max(S.prefix_lens[g], 0) & ~(kStep - 1);
+}
+// Whether all of a request's queries see the prefix: its first one does.
+__device__ __forceinline__ bool takes_part(const Att& A, const Req& r, int prefix) {
+  const int64_t sees = int64_t(r.kv) - (A.causal ? r.ql - 1 : 0);
+  return prefix > 0 && rows_of(A, r) > 0 && sees >= prefix;
+}
+// Twice what a step of an item of so many rows costs, in steps of a tall tile.
+__device__ __forceinline__ int cost_of(int rows) {
+  return rows > kFew ? 2 * ((rows + kPreRows - 1) / kPreRows) : (rows + kRows - 1) / kRows;
+}
+// Whether a group shares its prefix of `steps`: if its rows in one cost less than its requests'
+// each (`alone`, summed), by more than what the partial results of the prefix cost: the join, and
+// each tile's set-up once more.  Requests of whole tall tiles never do: 16 x 64 rows, 4 query heads a
+// kv head, over 8000 tokens: 229 us shared, 157 alone.
+__device__ __forceinline__ bool pays(const Share& S, int members, int alone, int rows, int steps) {
+  return members > 1 && (S.always || int64_t(alone) * steps > int64_t(cost_of(rows)) * (steps + 2 * kSetUp));
+}
+__device__ __forceinline__ Item no_item() { return Item{0, 0, 0, 0, 0, 0, 0, false, false}; }
+__device__ __forceinline__ Item own_item(const Att& A, const Req& r, int b, int prefix) {
+  const int s0 = prefix / kStep, rows = rows_of(A, r) * A.G;
+  return Item{r.q0, r.ql, r.kv, s0, max(1, steps_of(r.kv) - s0), rows, b, false, prefix > 0};
+}
+__device__ __forceinline__ Item group_item(const Att& A, int prefix, int lead, int row0, int row1) {
+  const int ql = max(row1 - row0, 0);
+  return Item{row0, ql, prefix, 0, prefix / kStep, ql * A.G, lead, true, true};
+}
+
+__device__ __forceinline__ int div_up(int a, int b) {
+  return static_cast<int>((static_cast<uint32_t>(a) + b - 1) / static_cast<uint32_t>(b));
+}
+__device__ __forceinline__ int extent(const Frame& F, int steps) {
+  return F.setup < 0 ? div_up(steps, F.range) * F.range : steps + F.setup;
+}
+
+// steps, tiles, fours: sums over the items of tall tiles' steps, their number, and short tiles'
+// steps; count(R): of the tall tiles' parts if each were cut into R steps by itself.
+template <typename Count>
+__device__ __forceinline__ Frame frame_of(const Att& A, float steps, float tiles, float fours,
+                                          Count count) {
+  Frame F{1, 0, 0, 0, 0, 0};
+  const float few = kShortStep * fours, all = (steps + few) * A.per_target + kSetUp;
+  if (steps > 0.f && steps + kSetUp * tiles < kMostPlaces) {
+    int n = A.target - static_cast<int>(few / all + 0.5f);
+    if (few > 0.f && n == A.target) --n;
+    n = max(n, 1);
+    // (the sums are whole numbers, exact below 2^24, and what is added to them then is little)
+    const float each = steps / static_cast<float>(n);
+    F.setup = static_cast<int>(fminf(0.25f * each, static_cast<float>(kSetUp))) & ~1;
+    F.range = max(static_cast<int>((steps + tiles * F.setup) / static_cast<float>(n)) + 1, 4);
+    // aligned: the shortest parts, as near as eighths, that are no more than n; then a range has
+    // one set-up, where else one that spans tiles has two
+    int R = max((static_cast<int>(ceilf(each)) + 1) & ~1, 4), parts = 0;
+#pragma unroll 1
+    for (int k = 0; k < 8; ++k) {
+      if (R > F.range + kSetUp) break;
+      parts = count(R);
+      if (parts <= n) break;
+      R += max(2, (R / 8) & ~1);
+    }
+    if (parts <= n && R <= F.range + kSetUp) {
+      F.range = R;
+      F.setup = -1;
+    }
+  }
+  F.least = static_cast<int>(fminf(all, 1e9f)) / kWaves * kWaves + kWaves;
+  return F;
+}
+
+// The step of a tall tile of `steps` at which a range that ends at place p of it cuts it: not next
+// to its ends, and between rounds of two steps.
+__device__ __forceinline__ int cut_at(const Frame& F, int steps, int p) {
+  if (F.setup < 0) return min(p, steps);
+  const int s = p - F.setup;
+  return s < kCut ? 0 : steps - s < kCut ? steps : s & ~1;
+}
+// Of a tile whose places begin at place a of a range: the parts that it is in, and the ranges from
+// that one on that have no step of it.
+__device__ __forceinline__ int parts_at(const Frame& F, int steps, int a, int& none) {
+  none = 0;
+  if (F.setup < 0) return div_up(steps, F.range);
+  const int E = steps + F.setup, R = F.range, ends = (a + E - 1) / R;
+  none = min(ends, (F.setup + kCut - 1 + a) / R);
+  return ends + 1 - none - (ends > none && ends * R - a > E - kCut);
+}
+
+// Parts that an item's tile is cut into at most, and its partial rows.
+__device__ __forceinline__ int most_parts(const Item& it, const Frame& F) {
+  if (it.late()) return 1;
+  if (it.four()) return div_up(it.steps, F.least);
+  if (F.setup < 0) return div_up(it.steps, F.range);
+  return F.tall < 2 ? 1 : (it.steps + F.setup - 2) / F.range + 2;
+}
+__device__ __forceinline__ int64_t slots_of(const Item& it, const Frame& F) {
+  if (it.rows == 0 || it.late()) return 0;
+  const int n = most_parts(it, F);
+  return it.part || n > 1 ? int64_t(it.rows) * n : 0;
+}
+
+// The tiles of an item in the order of its places: from both ends in turn, so that of a causal
+// request's tiles any few neighbours have the same work.
+__device__ __forceinline__ int tile_at(int p, int n) { return p & 1 ? n - 1 - p / 2 : p / 2; }
+__device__ __forceinline__ int place_of(int t, int n) {
+  return t < (n + 1) / 2 ? 2 * t : 2 * (n - 1 - t) + 1;
+}
+
+// What the join needs of an item: its first partial row, rows (0: nothing to join), and for tall
+// tiles their steps and the first one's place in its range; else 0 and the parts.
+__device__ __forceinline__ int4 join_of(const Item& it, const Frame& F, int64_t slots, int64_t slot,
+                                        int at) {
+  if (slots == 0) return make_int4(0, 0, 0, 0);
+  return it.tall() ? make_int4(static_cast<int>(slot), it.rows, it.steps, at % F.range)
+                   : make_int4(static_cast<int>(slot), it.rows, 0, most_parts(it, F));
+}
+// Parts of the tile of row rr of a joined item.
+__device__ __forceinline__ int parts_of(const int4& j, const Frame& F, int rr) {
+  if (rr < 0 || rr >= j.y) return 0;  // (lengths that do not fit q_start)
+  if (j.z == 0) return j.w;
+  int none, a = 0;
+  if (F.setup >= 0) {
+    const int n = div_up(j.y, kPreRows);
+    a = (j.w + place_of(rr / kPreRows, n) * (j.z + F.setup)) % F.range;
+  }
+  return parts_at(F, j.z, a, none);
+}
+
+__device__ __forceinline__ void put_item(const Places& P, int i, const Item& it, bool causal,
+                                         int tall, int fours, int64_t slot, int64_t slots,
+                                         bool fits) {
+  P.tall[i] = tall;
+  P.fours[i] = fours;
+  P.geo[2 * i] = make_int4(it.q0, fits ? it.ql : 0, it.kv, it.s0);
+  P.geo[2 * i + 1] = make_int4(it.steps, 2 * it.table + causal,
+                               slots > 0 ? static_cast<int>(slot) : -1, it.rows);
+}
+// What the second launch needs of request b: own, group: its items' joins; q0: the group's first
+// row; late: its tiles of that launch before.
+__device__ __forceinline__ void put_request(const Att& A, const Share& S, int b, const Item& it,
+                                            const int4& own, const int4& group, int q0, int late) {
+  S.meta[3 * b] = own;
+  S.meta[3 * b + 1] = group;
+  S.meta[3 * b + 2] = make_int4(it.q0, q0, 0, it.ql);
+  // (lengths that do not fit q_start may ask for more tiles than there are)
+  for (int t = 0; it.late() && t < it.tiles() && late + t < S.late_cap; ++t) {
+    int4* const to = S.lates + 3 * (late + t);
+    to[0] = group;
+    to[1] = make_int4(b, t, it.q0, it.ql);
+    to[2] = make_int4(it.kv, it.s0, it.rows, (it.q0 - q0) * A.G);
+  }
+}
+
+// Inclusive sum over a wave's lanes.
+__device__ __forceinline__ int64_t scan64(int64_t v) {
+  using qkv_pages::dpp;
+  v += dpp<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v += dpp<0x112, 0xf>(v);
+  v += dpp<0x114, 0xf>(v);
+  v += dpp<0x118, 0xf>(v);
+  v += dpp<0x142, 0xa>(v);  // row_bcast 15, 31
+  v += dpp<0x143, 0xc>(v);
+  return v;
+}
+__device__ __forceinline__ int64_t last64(int64_t v) {
+  const int lo = __builtin_amdgcn_readlane(static_cast<int>(v), 63);
+  const int hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63);
+  return (static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo);
+}
+
+// The plan of up to 64 requests and groups by one wave, a lane each; to LDS, and what the second
+// launch needs to the workspace where `tell`.
+__device__ __forceinline__ Frame plan_wave(const Att& A, const Share& S, const Places& P, bool tell) {
+  const int lane = threadIdx.x & 63;
+  int start = 0, end = 0, prefix = 0;
+  if (lane < S.groups) {
+    start = S.group_start[lane];
+    end = S.group_start[lane + 1];
+    prefix = prefix_of(S, lane);
+  }
+  Req r{0, 0, 0};
+  if (lane < A.B) r = request(A, lane);
+  const int rows = lane < A.B ? rows_of(A, r) : 0;
+  int group = -1, shares = 0;  // of the lane's request, and its prefix
+  Item it[2] = {no_item(), no_item()};  // the lane's group, its request
+#pragma unroll 1
+  for (int g = 0; g < S.groups; ++g) {
+    const int s = lane_value(start, g), e = lane_value(end, g), p = lane_value(prefix, g);
+    const bool in = lane >= s && lane < e && lane < A.B && takes_part(A, r, p);
+    const uint64_t all = __ballot(in);
+    if (all == 0) continue;
+    const int first = __builtin_ctzll(all), last = 63 - __builtin_clzll(all);
+    const Item x = group_item(A, p, first, lane_value(r.q0, first), lane_value(r.q0 + rows, last));
+    const int alone = lane_value(wave_scan(in ? cost_of(rows * A.G) : 0), 63);
+    if (!pays(S, __popcll(all), alone, x.rows, x.steps)) continue;
+    if (lane == g) it[0] = x;
+    if (in) {
+      group = g;
+      shares = p;
+    }
+  }
+  if (lane < A.B) it[1] = own_item(A, r, lane, shares);
+  // sums over all items; and over those before the lane's, groups first
+  auto total = [&](auto f) { return lane_value(wave_scan(f(it[0]) + f(it[1])), 63); };
+  auto before = [&](auto f, int* to) {
+    const int v = f(it[0]), w = f(it[1]);
+    const int a = wave_scan(v), b = wave_scan(w) + lane_value(a, 63);
+    to[0] = a - v;
+    to[1] = b - w;
+    return lane_value(b, 63);
+  };
+  auto steps_as = [](const Item& x, bool on) {
+    return on ? static_cast<float>(x.tiles()) * static_cast<float>(x.steps) : 0.f;
+  };
+  Frame F = frame_of(
+      A, total([&](const Item& x) { return steps_as(x, x.tall()); }),
+      total([](const Item& x) { return x.tall() ? static_cast<float>(x.tiles()) : 0.f; }),
+      total([&](const Item& x) { return steps_as(x, x.four()); }),
+      [&](int R) {
+        return total([&](const Item& x) { return x.tall() ? x.tiles() * div_up(x.steps, R) : 0; });
+      });
+  const bool runs = F.range > 1;
+  int tall[2], fours[2], late[2];
+  const int tall_all = before([&](const Item& x) {
+    return runs && x.tall() ? x.tiles() * extent(F, x.steps) : 0;
+  }, tall);
+  F.tall = div_up(tall_all, F.range);
+  F.fours = before([&](const Item& x) { return x.four() ? x.tiles() * most_parts(x, F) : 0; }, fours);
+  F.lates = min(before([](const Item& x) { return x.late() ? x.tiles() : 0; }, late), S.late_cap);
+  const int64_t slots[2] = {slots_of(it[0], F), slots_of(it[1], F)};
+  const int64_t sg = scan64(slots[0]), so = scan64(slots[1]) + last64(sg);
+  const int64_t slot[2] = {sg - slots[0], so - slots[1]};
+  // (lengths that do not fit q_start may ask for more rows than there are)
+  const bool fits[2] = {sg <= A.nslots, so <= A.nslots};
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    put_item(P, k * kSmall + lane, it[k], k == 1 && A.causal, tall[k], fours[k], slot[k], slots[k],
+             fits[k]);
+  if (lane == 0) {
+    P.tall[kItems] = tall_all;
+    P.fours[kItems] = F.fours;
+  }
+  if (tell) {
+    if (lane == 0) *S.frame = F;
+    int4 j[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      j[k] = fits[k] ? join_of(it[k], F, slots[k], slot[k], tall[k]) : make_int4(0, 0, 0, 0);
+    auto theirs = [&](int x) {
+      const int u = __shfl(x, max(group, 0), 64);
+      return group < 0 ? 0 : u;
+    };
+    const int4 g = make_int4(theirs(j[0].x), theirs(j[0].y), theirs(j[0].z), theirs(j[0].w));
+    const int q0 = theirs(it[0].q0);
+    if (lane < A.B) put_request(A, S, lane, it[1], j[1], g, q0, late[1]);
+  }
+  return F;
+}
 
 constexpr int kW = kPlanThr / 64;
 
-// Inclusive sums of two values over the workgroup; `total` those of all.
-__device__ __forceinline__ void block_sums(int64_t v[2], int64_t (*part)[2], int64_t total[2]) {
+// Inclusive sums of K values over the workgroup; `total` those of all.
+template <int K>
+__device__ __forceinline__ void block_sums(int64_t* v, int64_t (*part)[4], int64_t* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-      const int64_t u = __shfl_up(static_cast<long long>(v[k]), o, 64);
-      if (lane >= o) v[k] += u;
-    }
+  for (int k = 0; k < K; ++k) v[k] = scan64(v[k]);
   __syncthreads();  // (part's last readers)
-  if (lane == 63) {
-    part[wave][0] = v[0];
-    part[wave][1] = v[1];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (lane == 63) part[wave][k] = v[k];
+    total[k] = 0;
   }
   __syncthreads();
-  total[0] = total[1] = 0;
-#pragma unroll
+#pragma unroll 4
   for (int w = 0; w < kW; ++w)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < K; ++k) {
       const int64_t u = part[w][k];
       if (w < wave) v[k] += u;
       total[k] += u;
     }
 }
 
+// The same of more requests or groups, by a workgroup, into the workspace.
 __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
   extern __shared__ int32_t sh[];
-  __shared__ int64_t part[kW][2];
-  __shared__ float sums[kW];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, Gr = S.groups;
+  __shared__ int64_t part[kW][4];
+  const int tid = threadIdx.x, Gr = S.groups;
   int32_t* const start = sh;            // [Gr + 1]
   int32_t* const lead = start + Gr + 1; // [Gr]: the first request that takes part,
   int32_t* const many = lead + Gr;      // how many do,
-  int32_t* const row0 = many + Gr;      // their first row and the end of their last one;
+  int32_t* const row0 = many + Gr;      // their first row and the end of their last one,
   int32_t* const row1 = row0 + Gr;
-  int32_t* const cuts = row1 + Gr;      // parts of the prefix, its first partial row
-  int32_t* const slots = cuts + Gr;
+  int32_t* const cost = row1 + Gr;      // and what they cost alone; then whether they share
   for (int g = tid; g <= Gr && Gr > 0; g += kPlanThr) {
     start[g] = S.group_start[g];
     if (g < Gr) {
       lead[g] = row0[g] = INT32_MAX;
-      many[g] = row1[g] = 0;
+      many[g] = row1[g] = cost[g] = 0;
     }
   }
   __syncthreads();
-  // the prefix of a group in whole steps
-  auto prefix_of = [&](int g) { return max(S.prefix_lens[g], 0) & ~(kStep - 1); };
   auto group_of = [&](int b) {  // -1: in none
     if (Gr == 0 || b < start[0] || b >= start[Gr]) return -1;
     int lo = 0, hi = Gr;
@@ -116,105 +411,120 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
     }
     return start[lo] <= b && b < start[lo + 1] ? lo : -1;
   };
-  auto rows_of = [&](const Req& r) { return r.q0 < 0 ? 0 : r.rows(A); };
-  auto takes_part = [&](const Req& r, int prefix) {
-    const int64_t sees = int64_t(r.kv) - (A.causal ? r.ql - 1 : 0);  // its first query
-    return prefix > 0 && rows_of(r) > 0 && sees >= prefix;
-  };
   for (int b = tid; b < A.B; b += kPlanThr) {
     const int g = group_of(b);
     if (g < 0) continue;
     const Req r = request(A, b);
-    if (!takes_part(r, prefix_of(g))) continue;
+    if (!takes_part(A, r, prefix_of(S, g))) continue;
     atomicMin(&lead[g], b);
     atomicAdd(&many[g], 1);
+    atomicAdd(&cost[g], cost_of(rows_of(A, r) * A.G));
     atomicMin(&row0[g], r.q0);
-    atomicMax(&row1[g], r.q0 + rows_of(r));
+    atomicMax(&row1[g], r.q0 + rows_of(A, r));
   }
   __syncthreads();
-  // items: g of groups, then b of requests
-  auto group_item = [&](int g) {
-    Item it{0, 0, 0, 0, 0, 0};
-    if (many[g] < 2) return it;
-    it.kv = prefix_of(g);
-    it.q0 = row0[g];
-    it.ql = row1[g] - row0[g];
-    it.s1 = it.kv / kStep;
-    it.rows = it.ql * A.G;
-    return it;
-  };
-  auto own_item = [&](int b, int& g) {
+  for (int g = tid; g < Gr; g += kPlanThr)
+    cost[g] = pays(S, many[g], cost[g], max(row1[g] - row0[g], 0) * A.G, prefix_of(S, g) / kStep);
+  __syncthreads();
+  const int items = Gr + A.B;
+  auto item = [&](int i, int& g) {
+    if (i < Gr) {
+      g = i;
+      return cost[i] ? group_item(A, prefix_of(S, i), lead[i], row0[i], row1[i]) : no_item();
+    }
+    const int b = i - Gr;
     const Req r = request(A, b);
     g = group_of(b);
-    if (g >= 0 && (many[g] < 2 || !takes_part(r, prefix_of(g)))) g = -1;
-    Item it{r.q0, r.ql, r.kv, g >= 0 ? prefix_of(g) / kStep : 0, steps_of(r.kv), rows_of(r) * A.G};
-    return it;
+    if (g >= 0 && (!cost[g] || !takes_part(A, r, prefix_of(S, g)))) g = -1;
+    return own_item(A, r, b, g >= 0 ? prefix_of(S, g) : 0);
   };
-  const int items = Gr + A.B;
-  float sum = 0.f;
+  // steps and number of tall tiles, steps of short ones
+  float sum[3] = {0.f, 0.f, 0.f};
   for (int i = tid; i < items; i += kPlanThr) {
     int g;
-    const Item it = i < Gr ? group_item(i) : own_item(i - Gr, g);
-    sum += (it.tall() ? 1.f : 0.5f) * it.tiles() * it.steps();
+    const Item it = item(i, g);
+    const float n = static_cast<float>(it.tiles()), st = n * static_cast<float>(it.steps);
+    sum[0] += it.tall() ? st : 0.f;
+    sum[1] += it.tall() ? n : 0.f;
+    sum[2] += it.four() ? st : 0.f;
   }
-  sum = wave_scan(sum);
-  if (lane == 63) sums[wave] = sum;
-  __syncthreads();
-  sum = 0.f;
+  float* const fpart = reinterpret_cast<float*>(part);
 #pragma unroll
-  for (int w = 0; w < kW; ++w) sum += sums[w];
-  const int C0 = static_cast<int>(fminf(sum * A.per_target, 1e9f)) + 1;
-  const int Ct = max(kLeast, (C0 + 1) & ~1), Cs = max(kLeast, (C0 + kWaves - 1) & ~(kWaves - 1));
-  int64_t base[2] = {0, 0};  // pieces (tall ones in the high half), partial rows
+  for (int k = 0; k < 3; ++k) {
+    const float v = wave_scan(sum[k]);
+    if ((tid & 63) == 63) fpart[3 * (tid >> 6) + k] = v;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    sum[k] = 0.f;
+    for (int w = 0; w < kW; ++w) sum[k] += fpart[3 * w + k];
+  }
+  Frame F = frame_of(A, sum[0], sum[1], sum[2], [&](int R) {
+    int64_t n = 0, all;
+    for (int i = tid; i < items; i += kPlanThr) {
+      int g;
+      const Item it = item(i, g);
+      if (it.tall()) n += it.tiles() * div_up(it.steps, R);
+    }
+    block_sums<1>(&n, part, &all);
+    return static_cast<int>(min(all, int64_t(INT32_MAX)));
+  });
+  const bool runs = F.range > 1;
+  // (how many ranges there are decides whether tiles are cut at all)
+  {
+    int64_t n = 0, all;
+    for (int i = tid; i < items; i += kPlanThr) {
+      int g;
+      const Item it = item(i, g);
+      if (runs && it.tall()) n += int64_t(it.tiles()) * extent(F, it.steps);
+    }
+    block_sums<1>(&n, part, &all);
+    F.tall = div_up(static_cast<int>(all), F.range);
+  }
+  int64_t base[4] = {0, 0, 0, 0};  // places of tall tiles, parts, tiles of the second launch, rows
   for (int i0 = 0; i0 < items; i0 += kPlanThr) {
     const int i = i0 + tid;
-    Item it{0, 0, 0, 0, 0, 0};
+    Item it = no_item();
     int g = -1;
-    if (i < items) it = i < Gr ? group_item(i) : own_item(i - Gr, g);
-    const int C = it.tall() ? Ct : Cs;
-    const int tiles = it.tiles(), parts = (it.steps() + C - 1) / C;
-    const bool join = it.rows > 0 && (i < Gr || g >= 0 || parts > 1);
-    const int64_t n = int64_t(tiles) * parts;
-    int64_t v[2] = {it.tall() ? n << 32 : n, join ? int64_t(it.rows) * parts : 0}, total[2];
-    const int64_t own0 = v[0], own1 = v[1];
-    block_sums(v, part, total);
-    const int64_t before = base[0] + v[0] - own0, slot = base[1] + v[1] - own1;
-    base[0] += total[0];
-    base[1] += total[1];
-    if (i >= items) continue;
-    // (lengths that do not fit q_start may ask for more than there is)
-    const int64_t first = it.tall() ? before >> 32 : before & 0xffffffff;
-    const bool fits = slot + own1 <= A.nslots && first + n <= (it.tall() ? S.cap_tall : S.cap_short);
-    const int32_t at = join && fits ? static_cast<int32_t>(slot) : -1;
-    const bool runs = fits && it.rows > 0;
-    if (runs) {
-      int4* to = S.pieces + 2 * (first + (it.tall() ? 0 : S.cap_tall));
-      const int table = i < Gr ? lead[i] : i - Gr, causal = i >= Gr && A.causal;
-      for (int t = tiles - 1; t >= 0; --t)
-        for (int p = 0; p < parts; ++p) {
-          const int s0 = it.s0 + p * C;
-          *to++ = make_int4(table, it.q0, it.ql, it.kv);
-          *to++ = make_int4(2 * t + causal, s0, min(it.s1, s0 + C), join ? at + p * it.rows : -1);
-        }
+    if (i < items) it = item(i, g);
+    const int64_t n[4] = {runs && it.tall() ? int64_t(it.tiles()) * extent(F, it.steps) : 0,
+                          it.four() ? it.tiles() * most_parts(it, F) : 0,
+                          it.late() ? it.tiles() : 0, slots_of(it, F)};
+    int64_t v[4] = {n[0], n[1], n[2], n[3]}, total[4];
+    block_sums<4>(v, part, total);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] += base[k] - n[k];
+      base[k] += total[k];
     }
+    if (i >= items) continue;
+    const bool fits = v[3] + n[3] <= A.nslots;
+    put_item(S.at, i, it, i >= Gr && A.causal, static_cast<int>(v[0]), static_cast<int>(v[1]), v[3],
+             n[3], fits);
+    const int4 j = fits ? join_of(it, F, n[3], v[3], static_cast<int>(v[0])) : make_int4(0, 0, 0, 0);
+    // (requests' entries follow when all groups' are known; theirs wait behind)
     if (i < Gr) {
-      cuts[i] = runs ? parts : 0;
-      slots[i] = at;
+      S.meta[3 * A.B + i] = j;
     } else {
-      S.meta[2 * (i - Gr)] = make_int4(it.q0, at, runs && join ? parts : 0, it.rows);
+      S.meta[3 * (i - Gr)] = j;
+      S.meta[3 * (i - Gr) + 2] = make_int4(static_cast<int>(v[2]), 0, 0, 0);
     }
   }
   if (tid == 0) {
-    S.head[0] = static_cast<int32_t>(min(base[0] >> 32, int64_t(S.cap_tall)));
-    S.head[1] = static_cast<int32_t>(min(base[0] & 0xffffffff, int64_t(S.cap_short)));
+    S.at.tall[items] = static_cast<int32_t>(base[0]);
+    S.at.fours[items] = static_cast<int32_t>(base[1]);
+    F.fours = static_cast<int32_t>(base[1]);
+    F.lates = min(static_cast<int32_t>(base[2]), S.late_cap);
+    *S.frame = F;
   }
   __syncthreads();
   for (int b = tid; b < A.B; b += kPlanThr) {
     int g;
-    const Item it = own_item(b, g);
-    int4 m = make_int4(0, 0, 0, 0);
-    if (g >= 0) m = make_int4(slots[g], cuts[g], (row1[g] - row0[g]) * A.G, (it.q0 - row0[g]) * A.G);
-    S.meta[2 * b + 1] = m;
+    const Item it = item(Gr + b, g);
+    const int4 none = make_int4(0, 0, 0, 0);
+    put_request(A, S, b, it, S.meta[3 * b], g >= 0 ? S.meta[3 * A.B + g] : none, g >= 0 ? row0[g] : 0,
+                S.meta[3 * b + 2].x);
   }
   // ---- the rows' requests
   if (A.q_start == nullptr) {
@@ -236,162 +546,393 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
   }
 }
 
-// A workgroup per (tall piece, kv head), or per two short pieces: four waves each.
+// The last i < n with key[i] <= x (key[0] <= x < key[n], ascending), by a wave, 64 keys at a time.
+__device__ __forceinline__ int find_wave(const int32_t* key, int n, int x) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 63) / 64, i = lane * step;
+    const uint64_t m = __ballot(i < n && key[lo + min(i, n - 1)] <= x);
+    const int at = (__popcll(m) - 1) * step;
+    lo += at;
+    n = min(step, n - at);
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int same(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// What share8 is called with, read anew where it is needed: held in registers from the kernel's
+// start on, arguments and the loops' state take more SGPRs than there are (80 spilled).
+struct Args {
+  Att a;
+  Share s;
+};
+__device__ __forceinline__ const Args& args_anew() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Args*)p;
+}
+
+// threadIdx.x, for what is computed from it to stay within a loop's pass.
+__device__ __forceinline__ int thread_anew() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// Workgroup (j, h), j < target: the j-th range of kv head h's tall tiles, where there is one, then
+// short tiles, two at a time, in turn with the other workgroups that take these.
 template <int D, bool FP8, bool QLO, bool PLO>
-__global__ __launch_bounds__(kPreThr, 2) void share8(Att A, Share S) {
+__global__ __launch_bounds__(kPreThr, 2) void share8(Args) {
   __shared__ v4f sbuf[2][2][4];
+  __shared__ int32_t sh_tall[kItems + 1], sh_fours[kItems + 1];
+  __shared__ int4 sh_geo[2 * kItems];
+  __shared__ Frame sh_frame;
+  __shared__ int32_t sh_x;
   extern __shared__ __align__(16) uint8_t lds[];
-  const int tall = S.head[0] * A.H, h = blockIdx.x % A.H;
-  auto piece = [&](int at) {
-    const int4 x = S.pieces[2 * at], y = S.pieces[2 * at + 1];
-    auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  {
+    const Args& C = args_anew();
+    if (wave == 0) {
+      Frame F;
+      if (C.s.small) F = plan_wave(C.a, C.s, Places{sh_tall, sh_fours, sh_geo}, blockIdx.x == 0);
+      else F = *C.s.frame;
+      if (threadIdx.x == 0) {
+        sh_frame = F;
+        sh_x = F.tall > 0 ? static_cast<int>(blockIdx.x / C.a.H) * F.range : 0;
+      }
+    }
+    __syncthreads();
+  }
+  // the last item whose places begin at x or before, and the place; then its geometry
+  auto find = [&](const Share& S, int items, const int32_t* mine, const int32_t* theirs, int x,
+                  int& first) {
+    int i;
+    if (S.small) {
+      i = find_wave(mine, kItems, x);
+      first = same(mine[i]);
+    } else {
+      i = find_wave(theirs, items, x);
+      first = same(theirs[i]);
+    }
+    return i;
+  };
+  auto piece = [&](const Share& S, int i, int& s0, int& steps, int& rows) {
+    int4 x, y;
+    if (S.small) {
+      x = sh_geo[2 * i];
+      y = sh_geo[2 * i + 1];
+    } else {
+      x = S.at.geo[2 * i];
+      y = S.at.geo[2 * i + 1];
+    }
     Piece P{};
-    P.b = same(x.x);
-    P.r = Req{same(x.y), same(x.z), same(x.w)};
-    P.rt = same(y.x) >> 1;
-    P.causal = same(y.x) & 1;
-    P.s0 = same(y.y);
-    P.s1 = same(y.z);
-    P.slot = same(y.w);
+    P.r = Req{same(x.x), same(x.y), same(x.z)};
+    s0 = same(x.w);
+    steps = same(y.x);
+    P.b = same(y.y) >> 1;
+    P.causal = same(y.y) & 1;
+    P.slot = same(y.z);
+    rows = same(y.w);
     return P;
   };
-  if (static_cast<int>(blockIdx.x) < tall) {
-    const Piece P = piece(blockIdx.x / A.H);
-    prefill_piece<D, FP8, QLO, PLO, true>(A, P, h, lds, sbuf);
-  } else {
-    const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-    const int at = 2 * ((blockIdx.x - tall) / A.H) + half, n = S.head[1];
-    if (at - half >= n) return;
+  while (true) {
+    const Args& C = args_anew();
+    const int items = C.s.groups + C.a.B, h = blockIdx.x % C.a.H, j = blockIdx.x / C.a.H;
+    Frame F;
+    F.range = same(sh_frame.range);
+    F.setup = same(sh_frame.setup);
+    const int x = same(sh_x), total = same(C.s.small ? sh_tall[kItems] : C.s.at.tall[items]);
+    const int end = min((j + 1) * F.range, total);
+    __syncthreads();  // (sh_x is read)
+    if (x >= end) break;
+    int first, s0, steps, rows;
+    const int i = find(C.s, items, sh_tall, C.s.at.tall, x, first);
+    Piece P = piece(C.s, i, s0, steps, rows);
+    const int E = extent(F, steps), p = (x - first) / E, in = x - first - p * E;
+    const int n = min(E - in, end - x);
+    if (threadIdx.x == 0) sh_x = x + n;
+    const int from = cut_at(F, steps, in), to = in + n == E ? steps : cut_at(F, steps, in + n);
+    if (from < to) {
+      P.rt = tile_at(p, (rows + kPreRows - 1) / kPreRows);
+      P.s0 = s0 + from;
+      P.s1 = min(s0 + to, steps_of(P.r.kv));  // (an item without tokens counts a step)
+      // the part of the tile: ranges before this one that have steps of it
+      if (P.slot >= 0) {
+        int none;
+        const int k = (x - in) / F.range;
+        parts_at(F, steps, x - in - k * F.range, none);
+        P.slot += (j - k - none) * rows;
+      }
+      prefill_piece<D, FP8, QLO, PLO, true>(C.a, P, h, thread_anew(), lds, sbuf);
+    }
+    __syncthreads();
+  }
+  // short tiles' workgroups: those without a tall range, the last one at least
+  int u, units, every;
+  {
+    const Args& C = args_anew();
+    units = (same(sh_frame.fours) + 1) / 2;
+    const int from = min(same(sh_frame.tall), C.a.target - 1);
+    every = C.a.target - from;
+    u = static_cast<int>(blockIdx.x / C.a.H) - from;
+  }
+  if (u < 0) return;
+  for (; u < units; u += every) {
+    const Args& C = args_anew();
+    const int items = C.s.groups + C.a.B, h = blockIdx.x % C.a.H;
+    const int half = wave >> 2, k = 2 * u + half;
     // (without a piece of its own the half takes the other's barriers, and has no row or step)
     Piece P{};
     P.slot = -1;
-    if (at < n) P = piece(S.cap_tall + at);
+    if (k < same(sh_frame.fours)) {
+      int first, s0, steps, rows;
+      const int i = find(C.s, items, sh_fours, C.s.at.fours, k, first);
+      P = piece(C.s, i, s0, steps, rows);
+      const int least = same(sh_frame.least), parts = (steps + least - 1) / least;
+      const int in = k - first;
+      P.rt = in / parts;
+      P.part = in % parts;
+      P.s0 = s0 + P.part * least;
+      P.s1 = min(min(s0 + steps, P.s0 + least), steps_of(P.r.kv));
+      if (P.slot >= 0) P.slot += P.part * rows;
+    }
     float* const mine = reinterpret_cast<float*>(lds) + half * kWaves * kRows * (D + 6);
     decode_piece<D, FP8, QLO, true>(
-        A, P, h, threadIdx.x & 255, reinterpret_cast<float(*)[kRows][D + 4]>(mine),
+        C.a, P, h, thread_anew() & 255, reinterpret_cast<float(*)[kRows][D + 4]>(mine),
         reinterpret_cast<float(*)[kRows][2]>(mine + kWaves * kRows * (D + 4)));
+    __syncthreads();  // (the buffers' last readers)
   }
 }
 
-// Joins the partial results of 4 rows (a query and head each) a workgroup, 16 lanes a row with
-// 8 coordinates each; its waves take every fourth part and meet in LDS.
+// A row's partial results of one item, parts p0, p0 + every, ... of `parts`, joined: a lane has
+// coordinates d0 .. d0 + 7 (on: of the row's).
 template <int D>
-__global__ __launch_bounds__(kThr) void share_join(Att A, Share S) {
-  __shared__ float acc[kWaves][4][D + 4], ml[kWaves][4][2];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__device__ __forceinline__ void add_parts(const Att& A, int64_t first, int rows, int p0, int every,
+                                          int parts, bool on, int d0, float& M, float& L, float* x) {
+  for (; __any(p0 < parts); p0 += 4 * every) {
+    float m[4], l[4];
+    v4f v[4][2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int p = p0 + every * k;
+      m[k] = -INFINITY;
+      l[k] = 0.f;
+      v[k][0] = v[k][1] = v4f{0.f, 0.f, 0.f, 0.f};
+      if (p < parts) {
+        const int64_t at = first + int64_t(p) * rows;
+        m[k] = A.part_ml[2 * at];
+        l[k] = A.part_ml[2 * at + 1];
+        const v4f* const src = reinterpret_cast<const v4f*>(A.part_o + at * D + (on ? d0 : 0));
+        v[k][0] = src[0];
+        v[k][1] = src[1];
+      }
+    }
+    float mn = M;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mn = fmaxf(mn, m[k]);
+    const float ref = mn == -INFINITY ? 0.f : mn, e0 = __builtin_amdgcn_exp2f(M - ref);
+    L = fall(L, M - ref);
+    M = mn;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] *= e0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float e = __builtin_amdgcn_exp2f(m[k] - ref);
+      L += fall(l[k], m[k] - ref);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = fmaf(v[k][j >> 2][j & 3], e, x[j]);
+    }
+  }
+}
+
+// The second launch.  Its first workgroups take a tile of 16 rows each of the requests that have
+// few own tokens: the prefix' partial results, which are there, dealt to the waves by rows and
+// parts, then the own tokens as a piece of four waves, then all in LDS.  The others join what else
+// the first launch left, a row (query and head) on D / 8 lanes of 8 or 16: where there are few
+// rows (deal) a workgroup takes a wave's rows, its waves every fourth part, and they meet in LDS,
+// else a wave takes its rows by itself.
+template <int D, bool FP8, bool QLO>
+__global__ __launch_bounds__(kThr, 2) void share_rest(Att A, Share S, int deal) {
+  constexpr int LPR = D > 64 ? 16 : 8, RW = 64 / LPR;  // lanes of a row, rows of a wave
+  __shared__ float red_o[kWaves][kRows][D + 4];
+  __shared__ float red_ml[kWaves][kRows][2];
+  __shared__ float acc[kWaves][RW][D + 4], ml[kWaves][RW][2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane >> 4, d0 = 8 * (lane & 15);
   const bool on = d0 < D;
-  const int all = A.rows * A.Hq;  // (< 2^28)
-  for (int f0 = 4 * blockIdx.x; f0 < all; f0 += 4 * gridDim.x) {
-    const int f = min(f0 + r, all - 1), row = f / A.Hq, hq = f - row * A.Hq;
-    const int h = hq / A.G, b = S.row_req[row];
-    int4 own = make_int4(0, 0, 0, 0), pre = own;
-    if (b >= 0) {
-      own = S.meta[2 * b];
-      pre = S.meta[2 * b + 1];
+  const Frame F = *S.frame;
+  const int lates = same(F.lates) * A.H;
+  if (static_cast<int>(blockIdx.x) < lates) {
+    const int h = blockIdx.x % A.H, t = blockIdx.x / A.H;
+    const int4 pre = S.lates[3 * t], q = S.lates[3 * t + 1], kv = S.lates[3 * t + 2];
+    Piece P{};
+    P.b = same(q.x);
+    P.rt = same(q.y);
+    P.r = Req{same(q.z), same(q.w), same(kv.x)};
+    P.causal = A.causal;
+    P.slot = -1;
+    P.s0 = same(kv.y);
+    P.s1 = steps_of(P.r.kv);
+    const int rows = min(kRows, same(kv.z) - P.rt * kRows);
+    const int sets = (rows + 3) / 4, each = sets == 1 ? 4 : sets == 2 ? 2 : 1;  // waves of 4 rows
+    if (same(pre.y) > 0) {
+      const int set = wave / each, rr = P.rt * kRows + 4 * set + r;
+      const int rp = rr + same(kv.w);
+      const int parts = set < sets && 4 * set + r < rows ? parts_of(pre, F, rp) : 0;
+      float M = -INFINITY, L = 0.f, x[8] = {};
+      add_parts<D>(A, int64_t(h) * A.nslots + pre.x + rp, pre.y, wave % each, each, parts, on, d0, M,
+                   L, x);
+      if (on) {
+        *reinterpret_cast<v4f*>(&acc[wave][r][d0]) = v4f{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<v4f*>(&acc[wave][r][d0 + 4]) = v4f{x[4], x[5], x[6], x[7]};
+      }
+      if (d0 == 0) {
+        ml[wave][r][0] = M;
+        ml[wave][r][1] = L;
+      }
     }
-    const int parts = f0 + r < all && own.z > 0 ? own.z + pre.y : 0;
-    const int rr = (row - own.x) * A.G + hq - h * A.G;
-    const int64_t base = int64_t(h) * A.nslots + rr;
+    decode_steps<D, FP8, QLO>(A, P, h, tid, red_o, red_ml);
+    __syncthreads();
+    constexpr int PER = D / 8;
+    if (tid < kRows * PER) {
+      const int k = tid / PER, e0 = 8 * (tid % PER), w0 = k / 4 * each;
+      const int more = pre.y > 0 && k < rows ? each : 0;
+      float M = -INFINITY, L = 0.f, x[8] = {};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) M = fmaxf(M, red_ml[w][k][0]);
+      for (int w = 0; w < more; ++w) M = fmaxf(M, ml[w0 + w][k & 3][0]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      auto add = [&](float m, float l, const float* o) {
+        const float f = __builtin_amdgcn_exp2f(m - ref);
+        L += fall(l, m - ref);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = fmaf(o[j], f, x[j]);
+      };
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) add(red_ml[w][k][0], red_ml[w][k][1], &red_o[w][k][e0]);
+      for (int w = 0; w < more; ++w)
+        add(ml[w0 + w][k & 3][0], ml[w0 + w][k & 3][1], &acc[w0 + w][k & 3][e0]);
+      const int rr = P.rt * kRows + k, qi = rr / A.G;
+      const int64_t row = int64_t(P.r.q0) + qi;
+      if (qi < P.r.ql && row >= 0 && row < A.rows) {
+        const float inv = inverse(L);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= inv;
+        store8(A.out, (row * A.Hq + h * A.G + rr - qi * A.G) * D + e0, x, A.out_dtype, A.out_vec);
+      }
+    }
+    return;
+  }
+  const int e0 = 8 * (lane % LPR), rw = lane / LPR;
+  const bool in = e0 < D;
+  int4 rows_req = make_int4(0, 0, 0, 0);  // small: the lane's request's rows
+  if (S.small && lane < A.B) rows_req = S.meta[3 * lane + 2];
+  const int all = A.rows * A.Hq, unit = deal ? RW : RW * kWaves;  // (all < 2^28)
+  const int every = unit * (static_cast<int>(gridDim.x) - lates);
+  for (int u = unit * (static_cast<int>(blockIdx.x) - lates); u < all; u += every) {
+    const int f0 = u + (deal ? 0 : RW * wave);
+    const int f = min(f0 + rw, all - 1), row = f / A.Hq, hq = f - row * A.Hq, h = hq / A.G;
+    int b = -1;
+    if (S.small) {
+      const int last = lane_value(row, 63);
+      for (int x = lane_value(row, 0); x <= last; ++x) {
+        const uint64_t m = __ballot(lane < A.B && x >= rows_req.x && x - rows_req.x < rows_req.w);
+        if (row == x && m != 0) b = __builtin_ctzll(m);
+      }
+    } else {
+      b = S.row_req[row];
+    }
+    int4 own = make_int4(0, 0, 0, 0), pre = own, q0 = own;
+    if (b >= 0) {  // (own.y 0: its result is there already)
+      own = S.meta[3 * b];
+      pre = S.meta[3 * b + 1];
+      q0 = S.meta[3 * b + 2];
+    }
+    const int gq = hq - h * A.G, ro = (row - q0.x) * A.G + gq, rp = (row - q0.y) * A.G + gq;
+    const int no = f0 + rw < all ? parts_of(own, F, ro) : 0;
+    const int np = no > 0 ? parts_of(pre, F, rp) : 0;
+    if (!__any(no > 0)) continue;  // (deal: the same in all waves)
+    const int64_t base = int64_t(h) * A.nslots;
     float M = -INFINITY, L = 0.f, x[8] = {};
-    for (int p0 = wave; __any(p0 < parts); p0 += 4 * kWaves) {
-      float m[4], l[4];
-      v4f v[4][2];
+    const int p0 = deal ? wave : 0, step = deal ? kWaves : 1;
+    add_parts<D>(A, base + pre.x + rp, pre.y, p0, step, np, in, e0, M, L, x);
+    add_parts<D>(A, base + own.x + ro, own.y, p0, step, no, in, e0, M, L, x);
+    if (!deal) {
+      if (no == 0 || !in) continue;
+      const float inv = inverse(L);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int p = p0 + kWaves * k;
-        m[k] = -INFINITY;
-        l[k] = 0.f;
-        v[k][0] = v[k][1] = v4f{0.f, 0.f, 0.f, 0.f};
-        if (p < parts) {
-          const int64_t at = base + (p < own.z ? own.y + p * own.w
-                                               : pre.x + (p - own.z) * pre.z + pre.w);
-          m[k] = A.part_ml[2 * at];
-          l[k] = A.part_ml[2 * at + 1];
-          const v4f* const src = reinterpret_cast<const v4f*>(A.part_o + at * D + (on ? d0 : 0));
-          v[k][0] = src[0];
-          v[k][1] = src[1];
-        }
-      }
-      float mn = M;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) mn = fmaxf(mn, m[k]);
-      const float ref = mn == -INFINITY ? 0.f : mn, e0 = __builtin_amdgcn_exp2f(M - ref);
-      L = fall(L, M - ref);
-      M = mn;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= e0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float e = __builtin_amdgcn_exp2f(m[k] - ref);
-        L += fall(l[k], m[k] - ref);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = fmaf(v[k][j >> 2][j & 3], e, x[j]);
-      }
+      for (int j = 0; j < 8; ++j) x[j] *= inv;
+      store8(A.out, int64_t(f) * D + e0, x, A.out_dtype, A.out_vec);
+      continue;
     }
     __syncthreads();  // (the arrays' last readers)
-    if (on) {
-      *reinterpret_cast<v4f*>(&acc[wave][r][d0]) = v4f{x[0], x[1], x[2], x[3]};
-      *reinterpret_cast<v4f*>(&acc[wave][r][d0 + 4]) = v4f{x[4], x[5], x[6], x[7]};
+    if (in) {
+      *reinterpret_cast<v4f*>(&acc[wave][rw][e0]) = v4f{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<v4f*>(&acc[wave][rw][e0 + 4]) = v4f{x[4], x[5], x[6], x[7]};
     }
-    if (d0 == 0) {
-      ml[wave][r][0] = M;
-      ml[wave][r][1] = L;
+    if (e0 == 0) {
+      ml[wave][rw][0] = M;
+      ml[wave][rw][1] = L;
     }
     __syncthreads();
-    // wave w: row w
-    const int joins = __builtin_amdgcn_readlane(parts, 16 * wave), c = 2 * lane;
-    if (c >= D || joins == 0) continue;
-    float mx = -INFINITY, sum = 0.f, y0 = 0.f, y1 = 0.f;
+    if (wave != 0 || no == 0 || !in) continue;
+    M = -INFINITY;
+    L = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, ml[w][wave][0]);
-    const float ref = mx == -INFINITY ? 0.f : mx;
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml[w][rw][0]);
+    const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float e = __builtin_amdgcn_exp2f(ml[w][wave][0] - ref);
-      sum += fall(ml[w][wave][1], ml[w][wave][0] - ref);
-      y0 = fmaf(acc[w][wave][c], e, y0);
-      y1 = fmaf(acc[w][wave][c + 1], e, y1);
+      const float e = __builtin_amdgcn_exp2f(ml[w][rw][0] - ref);
+      L += fall(ml[w][rw][1], ml[w][rw][0] - ref);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = fmaf(acc[w][rw][e0 + j], e, x[j]);
     }
-    const float inv = inverse(sum);
-    const int64_t to = int64_t(f0 + wave) * D + c;
-    qkv_store(A.out, to, y0 * inv, A.out_dtype);
-    qkv_store(A.out, to + 1, y1 * inv, A.out_dtype);
+    const float inv = inverse(L);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] *= inv;
+    store8(A.out, int64_t(f) * D + e0, x, A.out_dtype, A.out_vec);
   }
 }
 
-// Pieces that a launch aims at, per kv head: one workgroup per CU.
-int32_t target_of(int32_t H) { return std::max(1, (qkv_num_cus() + H - 1) / H); }
+// Workgroups per kv head: one per CU, and no more (a second one would wait for a first to end).
+int32_t target_of(int32_t H) { return std::max(1, qkv_num_cus() / H); }
 
-// Bounds of a launch and its workspace.  Each row is in two items, its group's prefix and its own
-// tokens; items of more than kFew rows have tall tiles.  The steps (a short tile's count half)
-// are cut so that pieces beyond one a tile are within the target, 2 target for short ones.
+// The workspace.  Each row is in two items at most, its group's prefix and its own tokens.
+// An item of tall tiles has partial rows for (places - 2) / range + 2 parts, all beyond the two
+// within a tile per range; one of short tiles for its parts, those beyond one within 16 rows per
+// part of `least` steps, 2 target of them at most.
 struct Layout {
-  int64_t tall, shorts;   // pieces
   int64_t rows;           // partial rows of a kv head
-  int64_t meta, row_req, pieces, ml, o, bytes;
+  int64_t late;           // tiles of the second launch, at most
+  int64_t meta, lates, row_req, tall, fours, geo, ml, o, bytes;
 };
 Layout layout(int64_t B, int64_t groups, int64_t rows, int32_t G, int32_t H, int32_t d) {
   Layout L;
-  const int64_t t = target_of(H), all = 2 * rows * G;
-  const int64_t items = std::min(B + groups, 2 * rows);
-  const int64_t high = std::min(items, all / (kFew + 1));   // items of tall tiles
-  L.tall = high > 0 ? all / kPreRows + high + t : 0;
-  L.shorts = std::min(2 * items, all / kRows + items) + 2 * t;
-  L.rows = all + (high > 0 ? kPreRows * t : 0) + 2 * kRows * t;
+  const int64_t t = target_of(H), all = 2 * rows * G, items = B + groups;
+  const bool high = rows * G > kFew;  // there may be items of tall tiles
+  L.rows = high ? 2 * all + (kPreRows + 2 * kRows) * t : all + 2 * kRows * t;
+  const bool small = B <= kSmall && groups <= kSmall;
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
   L.meta = 256;
-  L.row_req = L.meta + up(32 * B);
-  L.pieces = L.row_req + up(4 * rows);
-  L.ml = L.pieces + up(32 * (L.tall + L.shorts));
+  L.late = std::min(2 * std::min(B, rows), rows * G / kRows + std::min(B, rows));
+  L.lates = L.meta + up(48 * B + 16 * groups);
+  L.row_req = L.lates + up(48 * L.late);
+  L.tall = L.row_req + (small ? 0 : up(4 * rows));
+  L.fours = L.tall + (small ? 0 : up(4 * (items + 1)));
+  L.geo = L.fours + (small ? 0 : up(4 * (items + 1)));
+  L.ml = L.geo + (small ? 0 : up(32 * items));
   L.o = L.ml + up(8 * H * L.rows);
   L.bytes = L.o + up(4 * H * L.rows * d);
   return L;
 }
 
 template <int D, bool FP8, bool QLO, bool PLO>
-void start(const Att& A, const Share& S, uint32_t grid, hipStream_t s) {
+void start(const Att& A, const Share& S, hipStream_t s) {
   constexpr int smem = std::max(kPreLds<D>, 2 * kWaves * kRows * (D + 6) * 4);
   // more LDS than a kernel has by default, asked for once per device (a failure is the
   // launch's, which the caller reports)
@@ -404,14 +945,32 @@ void start(const Att& A, const Share& S, uint32_t grid, hipStream_t s) {
                               hipFuncAttributeMaxDynamicSharedMemorySize, smem);
     asked.fetch_or(bit, std::memory_order_relaxed);
   }
-  share8<D, FP8, QLO, PLO><<<grid, kPreThr, smem, s>>>(A, S);
+  share8<D, FP8, QLO, PLO><<<A.target * A.H, kPreThr, smem, s>>>(Args{A, S});
 }
 
+// Both launches; the second one of `rest` workgroups.
 template <int D, bool FP8>
-void run(const Att& A, const Share& S, uint32_t grid, hipStream_t s) {
-  if (A.q_dtype == QKV_F32) start<D, FP8, true, true>(A, S, grid, s);
-  else if (A.out_dtype != QKV_BF16) start<D, FP8, false, true>(A, S, grid, s);
-  else start<D, FP8, false, false>(A, S, grid, s);
+void run(const Att& A, const Share& S, uint32_t rest, int deal, hipStream_t s) {
+  if (A.q_dtype == QKV_F32) start<D, FP8, true, true>(A, S, s);
+  else if (A.out_dtype != QKV_BF16) start<D, FP8, false, true>(A, S, s);
+  else start<D, FP8, false, false>(A, S, s);
+  if (A.q_dtype == QKV_F32) share_rest<D, FP8, true><<<rest, kThr, 0, s>>>(A, S, deal);
+  else share_rest<D, FP8, false><<<rest, kThr, 0, s>>>(A, S, deal);
+}
+
+// Calls whose requests would read little all the same go to qkv_kv8_attention.  us of it / shared,
+// 8 kv heads, d = 128, 4 query heads a kv head, by requests x prefix (and the bytes that they
+// would read): 4 x 8000 (69 MB) 19 / 26, 16 x 2000 (84) 19 / 23, 64 x 500 (134) 16 / 27;
+// 4 x 32,000 (266) 42 / 34, 16 x 8000 (277) 39 / 27, 64 x 2000 (336) 35 / 29.  The host knows the
+// table's width for it, not the lengths.  (Of many rows a request the tiles of the one launch
+// are the better ones in any case: 8 x 210 rows, 7 query heads, over 16,001: 240 / 155.)
+constexpr double kLittle = 192e6;
+bool little(int64_t B, int64_t rows, int32_t G, int32_t H, int32_t d, int64_t width, int32_t page) {
+  return rows * G <= kFew * B && double(B) * width * page * H * 2 * d <= kLittle;
+}
+// The longest request's rows for that call, as far as their number tells (a hint)
+int64_t longest_of(int64_t B, int64_t rows, int32_t G) {
+  return rows > 2 * B ? rows : std::max<int64_t>(1, kFew / G);
 }
 
 }  // namespace
@@ -420,14 +979,17 @@ extern "C" int64_t qkv_kv8_attention_shared_workspace_bytes(int32_t B, int32_t g
                                                             int32_t Hq, int32_t Hkv, int32_t d) {
   if (Hkv < 1 || d < 1) return 0;
   if (B < 1 || rows < 1) return 256;
-  return layout(B, std::max(groups, 0), rows, Hq / Hkv, Hkv, d).bytes;
+  const int32_t G = Hq / Hkv;
+  return std::max(layout(B, std::max(groups, 0), rows, G, Hkv, d).bytes,
+                  qkv_kv8_attention_workspace_bytes(B, rows, Hq, Hkv, d, longest_of(B, rows, G)));
 }
 
 extern "C" int qkv_kv8_attention_shared(
     const void* q, int32_t q_dtype, int64_t q_row_stride, int64_t q_head_stride, int64_t rows,
     const void* kpool, const float* kscale, const void* vpool, const float* vscale, int32_t fmt,
     int32_t num_pages, int32_t page_tokens, const int32_t* table, int32_t pages_per_seq,
-    const int32_t* group_start, const int32_t* prefix_lens, int32_t groups, const int32_t* q_start,
+    const int32_t* group_start, const int32_t* prefix_lens, int32_t groups, int32_t always,
+    const int32_t* q_start,
     const int32_t* q_lens, const int32_t* kv_lens, int32_t B, int32_t Hq, int32_t Hkv, int32_t d,
     float scale, int32_t causal, void* out, int32_t out_dtype, void* workspace, int64_t ws_bytes,
     void* stream) {
@@ -454,11 +1016,20 @@ extern "C" int qkv_kv8_attention_shared(
   QKV_REQUIRE(qkv_aligned(kpool, 16) && qkv_aligned(vpool, 16),
               "the pools must be 16-byte aligned");
   const Layout L = layout(B, groups, rows, G, Hkv, d);
-  QKV_REQUIRE(workspace && qkv_aligned(workspace, 256) && ws_bytes >= L.bytes,
+  const int64_t need = qkv_kv8_attention_shared_workspace_bytes(B, groups, rows, Hq, Hkv, d);
+  QKV_REQUIRE(workspace && qkv_aligned(workspace, 256) && ws_bytes >= need,
               "qkv_kv8_attention_shared: workspace too small or not 256-byte aligned");
-  QKV_REQUIRE(L.rows < INT32_MAX && (L.tall + L.shorts) * Hkv < INT32_MAX,
-              "batch of %d requests and %lld rows is too large for one call", B,
-              static_cast<long long>(rows));
+  if (!always && little(B, rows, G, Hkv, d, pages_per_seq, page_tokens))
+    return qkv_kv8_attention(q, q_dtype, q_row_stride, q_head_stride, rows, kpool, kscale, vpool,
+                             vscale, fmt, num_pages, page_tokens, table, pages_per_seq, q_start,
+                             q_lens, kv_lens, B, Hq, Hkv, d, longest_of(B, rows, G), scale, causal,
+                             out, out_dtype, workspace, ws_bytes, stream);
+  // places of tall tiles, were every request as long as the table is wide
+  const double tiles = 2.0 * rows * G / kPreRows + std::min<double>(B + groups, 2.0 * rows * G / kFew);
+  const double longest = std::min(double(pages_per_seq) * page_tokens, double(QKV_PAGED_TOKENS)) / kStep;
+  QKV_REQUIRE(tiles * (longest + 1 + kSetUp) < kMostPlaces && L.rows < INT32_MAX,
+              "%lld rows of %d query heads a kv head over a table of %d pages are too large for one "
+              "call", static_cast<long long>(rows), G, pages_per_seq);
   const int qb = q_dtype == QKV_F32 ? 4 : 2, ob = out_dtype == QKV_F32 ? 4 : 2;
   char* const ws = static_cast<char*>(workspace);
   Att A{};
@@ -494,34 +1065,39 @@ extern "C" int qkv_kv8_attention_shared(
   A.nslots = static_cast<int32_t>(L.rows);
   A.part_ml = reinterpret_cast<float*>(ws + L.ml);
   A.part_o = reinterpret_cast<float*>(ws + L.o);
-  Share S{group_start,
-          prefix_lens,
-          groups,
-          reinterpret_cast<int32_t*>(ws),
-          reinterpret_cast<int4*>(ws + L.pieces),
-          static_cast<int32_t>(L.tall),
-          static_cast<int32_t>(L.shorts),
-          reinterpret_cast<int4*>(ws + L.meta),
-          reinterpret_cast<int32_t*>(ws + L.row_req)};
+  Share S{};
+  S.group_start = group_start;
+  S.prefix_lens = prefix_lens;
+  S.groups = groups;
+  S.always = always;
+  S.small = B <= kSmall && groups <= kSmall;
+  S.frame = reinterpret_cast<Frame*>(ws);
+  S.at = Places{reinterpret_cast<int32_t*>(ws + L.tall), reinterpret_cast<int32_t*>(ws + L.fours),
+                reinterpret_cast<int4*>(ws + L.geo)};
+  S.lates = reinterpret_cast<int4*>(ws + L.lates);
+  S.meta = reinterpret_cast<int4*>(ws + L.meta);
+  S.late_cap = static_cast<int32_t>(L.late);
+  S.row_req = reinterpret_cast<int32_t*>(ws + L.row_req);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const uint32_t lds = std::max(7 * groups + 1, B + 1) * sizeof(int32_t);
-  share_plan<<<1, kPlanThr, lds, s>>>(A, S);
-  QKV_LAUNCHED();
-  const uint32_t grid = static_cast<uint32_t>((L.tall + (L.shorts + 1) / 2) * Hkv);
-  if (fmt == QKV_CODES_I8) {
-    if (d == 128) run<128, false>(A, S, grid, s);
-    else if (d == 96) run<96, false>(A, S, grid, s);
-    else run<64, false>(A, S, grid, s);
-  } else {
-    if (d == 128) run<128, true>(A, S, grid, s);
-    else if (d == 96) run<96, true>(A, S, grid, s);
-    else run<64, true>(A, S, grid, s);
+  if (!S.small) {
+    const uint32_t lds = std::max(6 * groups + 1, B + 1) * sizeof(int32_t);
+    share_plan<<<1, kPlanThr, lds, s>>>(A, S);
+    QKV_LAUNCHED();
   }
-  QKV_LAUNCHED();
-  const uint32_t joins = static_cast<uint32_t>(std::min<int64_t>((rows * Hq + 3) / 4, 2048));
-  if (d == 128) share_join<128><<<joins, kThr, 0, s>>>(A, S);
-  else if (d == 96) share_join<96><<<joins, kThr, 0, s>>>(A, S);
-  else share_join<64><<<joins, kThr, 0, s>>>(A, S);
+  // the second launch: a workgroup per tile that may be its own, and some that join the rest, few
+  // where rows tell that most requests have few of them (each reads lengths before it ends)
+  const int deal = rows * Hq < 8192;
+  const int64_t joins = std::min<int64_t>((rows * Hq + 3) / 4, rows * G > kFew * int64_t(B) ? 2048 : 256);
+  const uint32_t rest = static_cast<uint32_t>(L.late * Hkv + joins);
+  if (fmt == QKV_CODES_I8) {
+    if (d == 128) run<128, false>(A, S, rest, deal, s);
+    else if (d == 96) run<96, false>(A, S, rest, deal, s);
+    else run<64, false>(A, S, rest, deal, s);
+  } else {
+    if (d == 128) run<128, true>(A, S, rest, deal, s);
+    else if (d == 96) run<96, true>(A, S, rest, deal, s);
+    else run<64, true>(A, S, rest, deal, s);
+  }
   QKV_LAUNCHED();
   return QKV_OK;
 }

@@ -442,7 +442,8 @@ def attention_kv8_shared(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Ten
                          q_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                          causal: bool = False, out_dtype: torch.dtype = torch.float32,
                          out: Optional[torch.Tensor] = None,
-                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+                         workspace: Optional[torch.Tensor] = None,
+                         always: bool = False) -> torch.Tensor:
     """:func:`attention_kv8` of a batch in groups whose requests share a prefix, which is
     read once for all rows of a group.
 
@@ -451,7 +452,8 @@ def attention_kv8_shared(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Ten
     :func:`fork_pages` makes them; whole steps of 64 of them are read from the first request
     of the group whose queries all see them.  Requests that do not (idle ones, chunks that
     begin inside the prefix) and those before the first or behind the last group go over
-    all of their own tokens.
+    all of their own tokens, and so do all where sharing would cost more than it saves (short
+    prefixes, requests of many rows, small calls), unless ``always`` is set.
 
     The other arguments and the result are attention_kv8's (but for rounding; weights
     reach the value product in 11 bits, for bf16 results of 16-bit queries, where a group
@@ -482,7 +484,7 @@ def attention_kv8_shared(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Ten
     _call(dev, N.lib().qkv_kv8_attention_shared, q.data_ptr(), N.dtype_code(q.dtype), ts, hs, rows,
           kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(), vscale.data_ptr(), fmt, P, n,
           table.data_ptr(), width, group_start.data_ptr(), prefix_lens.data_ptr(), groups,
-          N.ptr(q_start), N.ptr(q_lens), kv_lens.data_ptr(), B, Hq, H, d, float(scale),
+          1 if always else 0, N.ptr(q_start), N.ptr(q_lens), kv_lens.data_ptr(), B, Hq, H, d, float(scale),
           1 if causal else 0, out.data_ptr(), N.dtype_code(out.dtype), workspace.data_ptr(),
           nbytes)
     return out

@@ -32,6 +32,11 @@ def i32(x):
     return torch.tensor(x, dtype=torch.int32, device=DEV)
 
 
+def shared(*args, **kw):
+    """The call, sharing wherever two requests of a group see the prefix."""
+    return P8.attention_kv8_shared(*args, always=True, **kw)
+
+
 def _forked(groups, own, H, d, code, pt, seed=0, loud=1.0, fork=True):
     """A store of requests in groups: groups [(prefix, requests)], own[b] tokens behind the
     prefix; and their tokens.  The prefix is appended once, to the group's first request
@@ -90,7 +95,7 @@ def _starts(groups):
 
 
 def _check(st, cache, lens, groups, q_lens, G, q_dtype, out_dtype, causal=True, scale=None, seed=0,
-           gaps=(), start=None, prefix=None, loud=1.0, guard=False):
+           gaps=(), start=None, prefix=None, loud=1.0, guard=False, always=True):
     gen = torch.Generator().manual_seed(seed + 100)
     B, H, d = len(lens), st.H, st.d
     q_start = [0]
@@ -111,7 +116,7 @@ def _check(st, cache, lens, groups, q_lens, G, q_dtype, out_dtype, causal=True, 
     got = P8.attention_kv8_shared(
         q, **st.pools(), table=st.table[:B], kv_lens=i32(lens), group_start=i32(start),
         prefix_lens=i32(prefix), q_start=i32(q_start), q_lens=i32(served), causal=causal,
-        scale=scale, out=out, workspace=ws)
+        scale=scale, out=out, workspace=ws, always=always)
     assert got is out
     if guard:
         assert (whole[need:] == 0xA5).all()
@@ -152,6 +157,30 @@ def test_attention(case, q_dtype, out_dtype):
     groups, own, q_lens, G, H, d, code, pt = case
     st, cache, lens = _forked(groups, own, H, d, code, pt)
     _check(st, cache, lens, groups, q_lens, G, q_dtype, out_dtype, guard=True)
+
+
+@pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
+def test_attention_by_the_rule(case):
+    """Small calls, which go to the plain attention."""
+    groups, own, q_lens, G, H, d, code, pt = case
+    st, cache, lens = _forked(groups, own, H, d, code, pt, seed=2)
+    _check(st, cache, lens, groups, q_lens, G, F16, F32, guard=True, always=False)
+
+
+@pytest.mark.parametrize("groups,own,q_lens,G", [
+    # behind a table too wide to count as small: groups that share and ones for which that does
+    # not pay (short prefixes, two requests, requests of many rows), in one batch
+    ([(1300, 6), (70, 5), (600, 2), (640, 3)], [5, 30, 1, 64, 7, 8, 9, 1, 1, 2, 3, 4, 5, 150, 130, 140],
+     [1] * 13 + [150, 130, 140], 4),
+    ([(900, 3), (900, 3)], [300, 280, 260, 60, 50, 40], [290, 270, 260, 41, 40, 40], 2),
+])
+def test_attention_by_the_rule_of_groups(groups, own, q_lens, G):
+    st, cache, lens = _forked(groups, own, 2, 128, "int8", 64, seed=3)
+    wide = torch.zeros(st.B, 40000, dtype=torch.int32, device=DEV)
+    wide[:, :st.pages_per_seq] = st.table
+    st.table = wide
+    _check(st, cache, lens, groups, q_lens, G, BF16, F32, guard=True, always=False)
+    _check(st, cache, lens, groups, q_lens, G, BF16, BF16, causal=False, always=False)
 
 
 @pytest.mark.parametrize("case", CASES[2:8], ids=[str(i) for i in range(2, 8)])
@@ -219,7 +248,7 @@ def test_uniform_rows_and_outputs_made_here():
     st, cache, lens = _forked(groups, own, 2, 64, "fp8", 64, seed=7)
     for Q in (1, 8):
         q = torch.randn(4 * Q, 6, 64, generator=torch.Generator().manual_seed(Q)).to(DEV)
-        x = P8.attention_kv8_shared(q, **st.pools(), table=st.table[:4], kv_lens=i32(lens),
+        x = shared(q, **st.pools(), table=st.table[:4], kv_lens=i32(lens),
                                     group_start=i32([0, 4]), prefix_lens=i32([256]), causal=True)
         for b in range(4):
             o, tol = R.attend(q[b * Q:b * Q + Q].cpu().double(), cache.values(b, 0),
@@ -227,7 +256,7 @@ def test_uniform_rows_and_outputs_made_here():
                               HALF[F32])
             assert ((x[b * Q:b * Q + Q].cpu().double() - o).abs() <= tol).all(), (Q, b)
     # rows of no request are 0 in an output that the call makes
-    y = P8.attention_kv8_shared(q, **st.pools(), table=st.table[:4], kv_lens=i32(lens),
+    y = shared(q, **st.pools(), table=st.table[:4], kv_lens=i32(lens),
                                 group_start=i32([0, 4]), prefix_lens=i32([256]),
                                 q_start=i32([0, 1, 2, 3, 4]), q_lens=i32([1, 0, 1, 1]))
     assert not y[1].any() and not y[4:].any() and y[0].any()
@@ -242,10 +271,10 @@ def test_unaligned_queries(q_dtype):
         q = base[1:].view(5 * Q, G, 96)
         args = dict(**st.pools(), table=st.table[:5], kv_lens=i32([n + 3 - 3 for n in lens]),
                     group_start=i32([0, 5]), prefix_lens=i32([128]))
-        x = P8.attention_kv8_shared(q, **args)
-        assert torch.equal(x, P8.attention_kv8_shared(q.clone(), **args))
+        x = shared(q, **args)
+        assert torch.equal(x, shared(q.clone(), **args))
         z = q.permute(2, 1, 0).contiguous().permute(2, 1, 0)      # heads innermost
-        assert torch.equal(x, P8.attention_kv8_shared(z, **args))
+        assert torch.equal(x, shared(z, **args))
 
 
 def test_bad_pages_are_left_out():
@@ -259,7 +288,7 @@ def test_bad_pages_are_left_out():
             torch.cat([torch.arange(64), torch.arange(128, 257)])]
     for Q in (1, 20):
         q = torch.randn(3 * Q, 4, 64, generator=torch.Generator().manual_seed(Q)).to(DEV)
-        x = P8.attention_kv8_shared(q, **st.pools(), table=st.table[:3], kv_lens=i32(lens),
+        x = shared(q, **st.pools(), table=st.table[:3], kv_lens=i32(lens),
                                     group_start=i32([0, 3]), prefix_lens=i32([256]))
         for b in range(3):
             o, tol = R.attend(q[b * Q:b * Q + Q].cpu().double(), cache.values(b, 0)[keep[b]],
@@ -275,7 +304,7 @@ def test_nan_stays_in_its_row():
     st, cache, lens = _forked(groups, own, 2, 64, "int8", 64, seed=10)
     q = torch.randn(12, 8, 64, device=DEV)
     q[4, 3, 7] = float("nan")
-    y = P8.attention_kv8_shared(q, **st.pools(), table=st.table[:12], kv_lens=i32(lens),
+    y = shared(q, **st.pools(), table=st.table[:12], kv_lens=i32(lens),
                                 group_start=i32([0, 12]), prefix_lens=i32([192])).cpu()
     assert torch.isnan(y[4, 3]).all()
     for b in range(12):
@@ -307,7 +336,7 @@ def test_value_scales_and_blocks_of_zeros(size):
             cache.append(b, k2[20 * b:20 * b + 20], v2[20 * b:20 * b + 20])
         for G in (2, 40):
             q = torch.randn(B, G, d, generator=gen)
-            x = P8.attention_kv8_shared(q.to(DEV), **st.pools(), table=st.table, kv_lens=st.lens,
+            x = shared(q.to(DEV), **st.pools(), table=st.table, kv_lens=st.lens,
                                         group_start=i32([0, 3]), prefix_lens=i32([128]))
             for b in range(B):
                 o, tol = R.attend(q[b:b + 1].double(), cache.values(b, 0), cache.values(b, 1),
@@ -342,7 +371,7 @@ def test_many_requests(B, m):
     q = torch.randn(start[-1], 2, d, generator=gen, device=DEV)
     args = dict(q=q, **pools, table=table.to(DEV), kv_lens=lens, q_start=i32(start),
                 q_lens=i32(q_lens), causal=True)
-    x = P8.attention_kv8_shared(**args, group_start=i32([m * g for g in range(n + 1)]),
+    x = shared(**args, group_start=i32([m * g for g in range(n + 1)]),
                                 prefix_lens=i32([whole * pt] * n))
     y = P8.attention_kv8(**args)
     # 256 tokens, values up to 1.3: as in test_attention_is_the_plain_one
@@ -353,9 +382,9 @@ def test_attention_of_nothing():
     st = P8.PagedKV8Store(2, 1, 64, 4, DEV, page_tokens=64)
     args = dict(**st.pools(), table=st.table, kv_lens=st.lens, group_start=i32([0, 2]),
                 prefix_lens=i32([64]))
-    x = P8.attention_kv8_shared(torch.ones(2, 3, 64, device=DEV), **args)
+    x = shared(torch.ones(2, 3, 64, device=DEV), **args)
     assert not x.any()
-    x = P8.attention_kv8_shared(torch.ones(0, 3, 64, device=DEV), **args, q_start=i32([0, 0, 0]))
+    x = shared(torch.ones(0, 3, 64, device=DEV), **args, q_start=i32([0, 0, 0]))
     assert x.shape == (0, 3, 64)
 
 
@@ -374,7 +403,7 @@ def test_unsound_arrays_stay_in_bounds():
                                    ([0, 3, 6], [5, 1, 9, -4, 30, 2, 0], None),
                                    ([0, 3, 6], [0, 0, 0, 0, 0, 0, 12], [12] * 6),
                                    ([0, 6, 6], [0, 2, 4, 6, 8, 10, 1 << 30], [1 << 30] * 6)):
-        P8.attention_kv8_shared(q, **st.pools(), table=st.table[:B],
+        shared(q, **st.pools(), table=st.table[:B],
                                 kv_lens=i32(lens), group_start=i32(start),
                                 prefix_lens=i32([128, 128]), q_start=i32(q_start),
                                 q_lens=None if q_lens is None else i32(q_lens), out=whole[:12],
@@ -400,7 +429,7 @@ def test_offsets_past_32_bits():
 
 # ------------------------------------------------------------------- steps
 
-def _serve(st, G, steps, seed, turns, shared, out_dtype=F32):
+def _serve(st, G, steps, seed, turns, share, out_dtype=F32):
     """n-best sampling: prompts, forks, decode steps of plan, rotary, append and attention,
     releases; yields each step's results."""
     rng = random.Random(seed)
@@ -420,9 +449,15 @@ def _serve(st, G, steps, seed, turns, shared, out_dtype=F32):
         plan = st.plan(i32(new), rows)
         q, k = rot.rotary(q, k, plan.positions, turns)
         st.append(k, v, plan)
-        groups = (i32([0, B]), i32([prefix])) if shared else None
         out = torch.zeros(rows, H * G, d, dtype=out_dtype, device=DEV)
-        yield st.attention(q, plan, out_dtype=out_dtype, out=out, groups=groups)
+        if share:
+            shared(q, **st.pools(), table=st.table, kv_lens=plan.kv_lens, group_start=i32([0, B]),
+                   prefix_lens=i32([prefix]), q_start=plan.q_start, q_lens=plan.q_lens, causal=True,
+                   out=out)
+            yield out
+        else:
+            groups = (i32([0, B]), i32([prefix])) if step % 2 else None
+            yield st.attention(q, plan, out_dtype=out_dtype, out=out, groups=groups)
         if step % 12 == 0:
             assert st.fork(i32([0] * (B - 1)), i32(range(1, B))).tolist() == [prompt] * (B - 1)
             prefix = prompt
@@ -489,7 +524,8 @@ def test_captured_step():
         plan = st.plan(new, B, max_q_len=1, out=plan)
         a, b = rot.rotary(q, k, plan.positions, turns)
         st.append(b, v, plan)
-        st.attention(a, plan, out_dtype=BF16, out=out, groups=groups)
+        shared(a, **st.pools(), table=st.table, kv_lens=plan.kv_lens, group_start=groups[0],
+               prefix_lens=groups[1], q_start=plan.q_start, q_lens=plan.q_lens, causal=True, out=out)
         st.release(done)
         st.compact()
         return granted, plan

@@ -99,7 +99,7 @@ def _size(B, groups, rows, Hq=32, H=8, d=128):
 def _attend(dt=N.QKV_F32, rows=4, fmt=0, pool=4, pt=64, width=2, q_start=X, q_lens=X, B=2, groups=1,
             Hq=4, H=2, d=64, odt=N.QKV_F32, ws=X, ws_bytes=1 << 40, q=X, kpool=X, group_start=X):
     return N.lib().qkv_kv8_attention_shared(
-        q, dt, 256, 64, rows, kpool, X, X, X, fmt, pool, pt, X, width, group_start, X, groups,
+        q, dt, 256, 64, rows, kpool, X, X, X, fmt, pool, pt, X, width, group_start, X, groups, 0,
         q_start, q_lens, X, B, Hq, H, d, 0.1, 1, X, odt, ws, ws_bytes, None)
 
 
@@ -133,7 +133,7 @@ def test_attention_refusals():
 def test_workspace():
     size = [_size(*a) for a in ((1, 0, 1), (64, 1, 64), (64, 64, 64), (8, 1, 2400), (16000, 2000, 16000))]
     assert min(size) > 0 and all(s % 256 == 0 for s in size)
-    assert size[1] < 32 << 20 and max(size) < 1 << 30
+    assert size[1] < 32 << 20 and max(size) < 1 << 31
 
 
 # ------------------------------------------------------------- Python refusals
