@@ -319,13 +319,16 @@ __device__ __forceinline__ Frame plan_wave(const Att& A, const Share& S, const P
       [&](int R) {
         return total([&](const Item& x) { return x.tall() ? x.tiles() * div_up(x.steps, R) : 0; });
       });
-  const bool runs = F.range > 1;
-  int tall[2], fours[2], late[2];
-  const int tall_all = before([&](const Item& x) {
-    return runs && x.tall() ? x.tiles() * extent(F, x.steps) : 0;
-  }, tall);
-  F.tall = div_up(tall_all, F.range);
-  F.fours = before([&](const Item& x) { return x.four() ? x.tiles() * most_parts(x, F) : 0; }, fours);
+  int tall[2] = {0, 0}, fours[2] = {0, 0}, late[2], tall_all = 0;
+  if (F.range > 1) {
+    tall_all = before([&](const Item& x) {
+      return x.tall() ? x.tiles() * extent(F, x.steps) : 0;
+    }, tall);
+    F.tall = div_up(tall_all, F.range);
+  }
+  if (__any(it[0].four() || it[1].four()))
+    F.fours = before([&](const Item& x) { return x.four() ? x.tiles() * most_parts(x, F) : 0; },
+                     fours);
   F.lates = min(before([](const Item& x) { return x.late() ? x.tiles() : 0; }, late), S.late_cap);
   const int64_t slots[2] = {slots_of(it[0], F), slots_of(it[1], F)};
   const int64_t sg = scan64(slots[0]), so = scan64(slots[1]) + last64(sg);
@@ -705,45 +708,56 @@ __global__ __launch_bounds__(kPreThr, 2) void share8(Args) {
   }
 }
 
-// A row's partial results of one item, parts p0, p0 + every, ... of `parts`, joined: a lane has
-// coordinates d0 .. d0 + 7 (on: of the row's).
+// Partial results of a row on their way: four parts of one item.
+struct Parts {
+  float m[4], l[4];
+  v4f v[4][2];
+};
+// Parts p0, p0 + every, ... of `parts`: a lane has coordinates d0 .. d0 + 7 (on: of the row's).
+template <int D>
+__device__ __forceinline__ Parts load_parts(const Att& A, int64_t first, int rows, int p0, int every,
+                                            int parts, bool on, int d0) {
+  Parts r;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int p = p0 + every * k;
+    r.m[k] = -INFINITY;
+    r.l[k] = 0.f;
+    r.v[k][0] = r.v[k][1] = v4f{0.f, 0.f, 0.f, 0.f};
+    if (p < parts) {
+      const int64_t at = first + int64_t(p) * rows;
+      r.m[k] = A.part_ml[2 * at];
+      r.l[k] = A.part_ml[2 * at + 1];
+      const v4f* const src = reinterpret_cast<const v4f*>(A.part_o + at * D + (on ? d0 : 0));
+      r.v[k][0] = src[0];
+      r.v[k][1] = src[1];
+    }
+  }
+  return r;
+}
+__device__ __forceinline__ void fold(const Parts& r, float& M, float& L, float* x) {
+  float mn = M;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) mn = fmaxf(mn, r.m[k]);
+  const float ref = mn == -INFINITY ? 0.f : mn, e0 = __builtin_amdgcn_exp2f(M - ref);
+  L = fall(L, M - ref);
+  M = mn;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] *= e0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float e = __builtin_amdgcn_exp2f(r.m[k] - ref);
+    L += fall(r.l[k], r.m[k] - ref);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = fmaf(r.v[k][j >> 2][j & 3], e, x[j]);
+  }
+}
+// All of a row's parts from p0 on.
 template <int D>
 __device__ __forceinline__ void add_parts(const Att& A, int64_t first, int rows, int p0, int every,
                                           int parts, bool on, int d0, float& M, float& L, float* x) {
-  for (; __any(p0 < parts); p0 += 4 * every) {
-    float m[4], l[4];
-    v4f v[4][2];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int p = p0 + every * k;
-      m[k] = -INFINITY;
-      l[k] = 0.f;
-      v[k][0] = v[k][1] = v4f{0.f, 0.f, 0.f, 0.f};
-      if (p < parts) {
-        const int64_t at = first + int64_t(p) * rows;
-        m[k] = A.part_ml[2 * at];
-        l[k] = A.part_ml[2 * at + 1];
-        const v4f* const src = reinterpret_cast<const v4f*>(A.part_o + at * D + (on ? d0 : 0));
-        v[k][0] = src[0];
-        v[k][1] = src[1];
-      }
-    }
-    float mn = M;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) mn = fmaxf(mn, m[k]);
-    const float ref = mn == -INFINITY ? 0.f : mn, e0 = __builtin_amdgcn_exp2f(M - ref);
-    L = fall(L, M - ref);
-    M = mn;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] *= e0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float e = __builtin_amdgcn_exp2f(m[k] - ref);
-      L += fall(l[k], m[k] - ref);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = fmaf(v[k][j >> 2][j & 3], e, x[j]);
-    }
-  }
+  for (; __any(p0 < parts); p0 += 4 * every)
+    fold(load_parts<D>(A, first, rows, p0, every, parts, on, d0), M, L, x);
 }
 
 // The second launch.  Its first workgroups take a tile of 16 rows each of the requests that have
@@ -777,13 +791,16 @@ __global__ __launch_bounds__(kThr, 2) void share_rest(Att A, Share S, int deal) 
     P.s1 = steps_of(P.r.kv);
     const int rows = min(kRows, same(kv.z) - P.rt * kRows);
     const int sets = (rows + 3) / 4, each = sets == 1 ? 4 : sets == 2 ? 2 : 1;  // waves of 4 rows
+    // (the first parts are on their way while the own tokens are gone over)
+    const int set = wave / each, rr = P.rt * kRows + 4 * set + r, rp = rr + same(kv.w);
+    const int parts = set < sets && 4 * set + r < rows ? parts_of(pre, F, rp) : 0;
+    const int64_t first = int64_t(h) * A.nslots + pre.x + rp;
+    const Parts some = load_parts<D>(A, first, pre.y, wave % each, each, parts, on, d0);
+    decode_steps<D, FP8, QLO>(A, P, h, tid, red_o, red_ml);
     if (same(pre.y) > 0) {
-      const int set = wave / each, rr = P.rt * kRows + 4 * set + r;
-      const int rp = rr + same(kv.w);
-      const int parts = set < sets && 4 * set + r < rows ? parts_of(pre, F, rp) : 0;
       float M = -INFINITY, L = 0.f, x[8] = {};
-      add_parts<D>(A, int64_t(h) * A.nslots + pre.x + rp, pre.y, wave % each, each, parts, on, d0, M,
-                   L, x);
+      fold(some, M, L, x);
+      add_parts<D>(A, first, pre.y, wave % each + 4 * each, each, parts, on, d0, M, L, x);
       if (on) {
         *reinterpret_cast<v4f*>(&acc[wave][r][d0]) = v4f{x[0], x[1], x[2], x[3]};
         *reinterpret_cast<v4f*>(&acc[wave][r][d0 + 4]) = v4f{x[4], x[5], x[6], x[7]};
@@ -793,7 +810,6 @@ __global__ __launch_bounds__(kThr, 2) void share_rest(Att A, Share S, int deal) 
         ml[wave][r][1] = L;
       }
     }
-    decode_steps<D, FP8, QLO>(A, P, h, tid, red_o, red_ml);
     __syncthreads();
     constexpr int PER = D / 8;
     if (tid < kRows * PER) {

@@ -124,14 +124,19 @@ struct Release {
   int32_t* shares;
 };
 
-__device__ __forceinline__ int32_t peek(const int32_t* p) {  // (past this CU's cache)
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// (One workgroup does all of it, so its own scope is enough: through device-wide fences between
+// the passes, and a binary search for each entry in each of them, 384 requests of ~30 pages took
+// 40 us, now XX; 4 requests 11, now XX.)
+__device__ __forceinline__ int32_t peek(const int32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
 
-// Entries e (request order, page order) of the done requests, three passes: each takes a
-// holder away; a page left below 0 has lost its last one, and the largest e among its entries
-// is kept in its count, as INT32_MIN + (entries - 1 - e), below any count; that entry puts
-// the page on the free list, at the place that a prefix sum over them gives.
+constexpr int kOwn = 8;  // entries of a thread that are in flight at once
+
+// Entries e (request order, page order) of the done requests, a run of them a thread, three
+// passes: each takes a holder away; a page left below 0 has lost its last one, and the largest
+// e among its entries is kept in its count, as INT32_MIN + (entries - 1 - e), below any
+// count; that entry puts the page on the free list, at the place that a prefix sum over them gives.
 template <int THR>
 __global__ __launch_bounds__(THR) void release_shared(Release A) {
   extern __shared__ int32_t sh[];  // start[B + 1]: entries of the done requests before b
@@ -153,39 +158,82 @@ __global__ __launch_bounds__(THR) void release_shared(Release A) {
     if (b < A.B) sh[b + 1] = static_cast<int32_t>(imin(end, 1 << 30));
   }
   __syncthreads();
-  const int32_t E = sh[A.B];
-  auto page_of = [&](int32_t e) {
-    const int b = find_row(sh, A.B, e);
-    const int32_t p = A.table[int64_t(b) * A.width + (e - sh[b])];
-    return p >= 0 && p < A.pool ? p : -1;
-  };
-  for (int32_t e = tid; e < E; e += THR) {
-    const int32_t p = page_of(e);
-    if (p >= 0) atomicSub(&A.shares[p], 1);
-  }
-  __threadfence();
-  __syncthreads();
-  for (int32_t e = tid; e < E; e += THR) {
-    const int32_t p = page_of(e);
-    if (p >= 0 && peek(&A.shares[p]) < 0) atomicMin(&A.shares[p], INT32_MIN + (E - 1 - e));
-  }
-  __threadfence();
-  __syncthreads();
-  int64_t put = count;
-  for (int32_t e0 = 0; e0 < E; e0 += THR) {
-    const int32_t e = e0 + tid;
-    const int32_t p = e < E ? page_of(e) : -1;
-    const bool last = p >= 0 && peek(&A.shares[p]) == INT32_MIN + (E - 1 - e);
-    int64_t total;
-    const int64_t at = put + block_scan<THR>(last, part, total) - 1;
-    put += total;
-    if (last) {
-      // (no other entry of the page has that number, so it may change here)
-      __hip_atomic_store(&A.shares[p], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (at < A.pool) A.free_list[at] = p;
+  const int32_t E = sh[A.B], per = (E + THR - 1) / THR;
+  const int32_t e0 = min(tid * per, E), e1 = min(e0 + per, E);
+  const int b0 = e0 < E ? find_row(sh, A.B, e0) : 0;
+  int32_t p[kOwn];
+  // the pages (-1: none) of up to kOwn entries from e on; b: e's request, moved on
+  auto pages = [&](int32_t e, int& b) {
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      p[k] = -1;
+      if (e + k < e1) {
+        while (e + k >= sh[b + 1]) ++b;
+        p[k] = A.table[int64_t(b) * A.width + (e + k - sh[b])];
+      }
     }
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) p[k] = p[k] < A.pool ? p[k] : -1;
+  };
+  const bool once = per <= kOwn;  // a thread's pages stay in registers
+  int b = b0;
+  for (int32_t e = e0; e < e1; e += kOwn) {
+    pages(e, b);
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k)
+      if (p[k] >= 0)
+        __hip_atomic_fetch_add(&A.shares[p[k]], -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   }
-  if (tid == 0) *A.free_count = static_cast<int32_t>(imin(put, A.pool));
+  __syncthreads();
+  b = b0;
+  for (int32_t e = e0; e < e1; e += kOwn) {
+    if (!once) pages(e, b);
+    int32_t v[kOwn];
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) v[k] = p[k] >= 0 ? peek(&A.shares[p[k]]) : 0;
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k)
+      if (v[k] < 0)
+        __hip_atomic_fetch_min(&A.shares[p[k]], INT32_MIN + (E - 1 - e - k), __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_WORKGROUP);
+  }
+  __syncthreads();
+  // (a page's count is read by all of its entries before its last one, which alone has that number,
+  // sets it to 0: the others differ from either)
+  int64_t mine = 0, total;
+  auto last = [&](int32_t e, uint32_t& bits) {
+    int32_t v[kOwn];
+    bits = 0;
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) v[k] = p[k] >= 0 ? peek(&A.shares[p[k]]) : 0;
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k)
+      bits |= static_cast<uint32_t>(p[k] >= 0 && v[k] == INT32_MIN + (E - 1 - e - k)) << k;
+  };
+  uint32_t bits = 0;
+  b = b0;
+  for (int32_t e = e0; e < e1; e += kOwn) {
+    if (!once) pages(e, b);
+    last(e, bits);
+    mine += __popc(bits);
+  }
+  int64_t at = count + block_scan<THR>(mine, part, total) - mine;
+  const int64_t end = count + total;
+  b = b0;
+  for (int32_t e = e0; e < e1; e += kOwn) {
+    if (!once) {
+      pages(e, b);
+      last(e, bits);
+    }
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k)
+      if (bits >> k & 1) {
+        __hip_atomic_store(&A.shares[p[k]], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (at < A.pool) A.free_list[at] = p[k];
+        ++at;
+      }
+  }
+  if (tid == 0) *A.free_count = static_cast<int32_t>(imin(end, A.pool));
 }
 
 struct Compact {
@@ -201,7 +249,11 @@ struct Compact {
   int32_t* dst_pages;
   int32_t* moves;
   int32_t* remap;
+  int32_t tables;     // whether compact_plan maps the tables, too
 };
+
+// Entries of the tables up to which it does.
+constexpr int kFewEntries = 4096;
 
 constexpr int kMaxPool = 1 << 20;  // pages of a compaction: a bit each in 128 KiB of LDS
 
@@ -261,6 +313,14 @@ __global__ __launch_bounds__(kThr) void compact_plan(Compact A) {
       A.shares[s] = 0;
     }
   }
+  if (!A.tables) return;
+  __syncthreads();
+  for (int i = tid; i < A.B * A.width; i += kThr) {
+    const int b = i / A.width, c = i - b * A.width;
+    const int64_t n = int64_t(1) << A.lg;
+    const int32_t p = A.table[i];
+    if (c < (imax(A.lens[b], 0) + n - 1) >> A.lg && p >= 0 && p < A.pool) A.table[i] = A.remap[p];
+  }
 }
 
 constexpr int kTabThr = 256;
@@ -318,7 +378,10 @@ extern "C" int qkv_page_release_shared(int32_t* lens, const uint8_t* done, int32
               "qkv_page_release_shared: null pointer");
   Release A{lens, done, B, table, pages_per_seq, qkv_page_lg(page_tokens), free_list, num_pages,
             free_count, shares};
-  release_shared<kThr><<<1, kThr, (B + 1) * sizeof(int32_t), static_cast<hipStream_t>(stream)>>>(A);
+  const uint32_t lds = (B + 1) * sizeof(int32_t);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (int64_t(B) * pages_per_seq <= 256 * kOwn && B <= 256) release_shared<256><<<1, 256, lds, s>>>(A);
+  else release_shared<kThr><<<1, kThr, lds, s>>>(A);
   QKV_LAUNCHED();
   return QKV_OK;
 }
@@ -336,7 +399,8 @@ extern "C" int qkv_page_compact(int32_t* table, const int32_t* lens, int32_t B,
                   (B == 0 || (table && lens)),
               "qkv_page_compact: null pointer");
   Compact A{table,      lens,   B,  pages_per_seq,          free_list, num_pages, free_count,
-            shares, qkv_page_lg(page_tokens), src_pages, dst_pages, moves, remap};
+            shares, qkv_page_lg(page_tokens), src_pages, dst_pages, moves, remap,
+            int64_t(B) * pages_per_seq <= kFewEntries};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const uint32_t lds = (num_pages + 31) / 32 * sizeof(uint32_t);
   if (lds > (48 << 10))  // more LDS than a kernel has by default
@@ -344,7 +408,7 @@ extern "C" int qkv_page_compact(int32_t* table, const int32_t* lens, int32_t B,
                                 hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
   compact_plan<<<1, kThr, lds, s>>>(A);
   QKV_LAUNCHED();
-  if (B > 0) compact_tables<<<B, kTabThr, 0, s>>>(A);
+  if (!A.tables) compact_tables<<<B, kTabThr, 0, s>>>(A);
   QKV_LAUNCHED();
   return QKV_OK;
 }
