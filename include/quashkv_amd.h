@@ -882,8 +882,9 @@ int qkv_kv8_attention_shared(const void* q, int32_t q_dtype, int64_t q_row_strid
  * R / 2), or (2 i, 2 i + 1) where interleaved -- turn by positions[row] * turns[i]
  * units of 2^-64 of a full turn (modulo 2^64), times factor; by the negative angle
  * where inverse (the gradient's map).  Coordinates from R on are copied.  Row and
- * head strides in elements, the last axis dense.  The outputs are other memory
- * than the inputs, or the inputs themselves at the same strides. */
+ * head strides in elements, the last axis dense; a row of both has up to 2^20 values.
+ * The outputs are other memory than the inputs, or the inputs themselves at the same
+ * strides. */
 int qkv_rotary(int32_t dtype, const void* q, int64_t q_row_stride, int64_t q_head_stride,
                int32_t Hq, const void* k, int64_t k_row_stride, int64_t k_head_stride, int32_t Hk,
                int64_t rows, int32_t d, int32_t R, const int32_t* positions, const int64_t* turns,

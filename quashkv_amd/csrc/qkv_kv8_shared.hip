@@ -20,6 +20,20 @@
 // the short tiles, two at a time, four waves each, cut where they are long.  The second launch
 // (share_rest) takes the few own tokens, joining them with the prefix' partial results as it
 // goes, and joins whatever else was cut.
+//
+// Measured (a call; attention_kv8 over the same tables): 64 requests of up to 500 own tokens behind
+// 8192, 32 / 8 heads, d = 128, bf16: 39 us (95); behind 32,000 65 (331); 60 requests of six groups,
+// up to 5003 + 700, 24 / 8 heads, d = 96, e4m3: 31 (45); 8 x 210 rows behind 16,001, 14 / 2 heads,
+// d = 64, fp32 results: 147 (240).  Of the first's 39: the plan 3.9 us (loads of the lengths, then
+// ~1500 instructions of one wave), a tile's place, queries and first codes 4.8, four rounds of
+// 128 tokens 10.5 (2.3 to 2.6 each; prefill8's loop, see there), halves' join and 16.8 MB of
+// partial results 3.3, a gap of 3 between the launches, and the second one 11: own tokens'
+// chain of lengths - page - codes - results, 4 us of it their bytes.  Tall tiles, where there
+// are many, are bound by that loop: 75 % of what a large product reaches.
+//
+// Tried: the plan in a launch of its own (9 us, and a gap) with short tiles in the first launch
+// (a tile by one wave: 8 us each, one behind the other; 47 us in all); ranges that do not count
+// set-up (a range of 33 tiles of 5 steps: 272 us for the 147 above).
 #include <algorithm>
 #include <atomic>
 

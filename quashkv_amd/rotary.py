@@ -82,7 +82,7 @@ def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
 
 def _out(x: torch.Tensor, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
     if out.dtype is not x.dtype or out.shape != x.shape:
         raise ValueError(f"{what} must be {x.dtype} of shape {tuple(x.shape)}; got {out.dtype} "
                          f"{tuple(out.shape)}")

@@ -418,7 +418,8 @@ def _check_rotary(x, pos, turns, got, factor=1.0, interleaved=False, inverse=Fal
     (1, 1, 1, 128, 128, False), (7, 4, 2, 64, 64, True), (33, 5, 1, 96, 40, False),
     (33, 5, 1, 96, 40, True), (100, 3, 3, 128, 64, False), (5, 2, 1, 80, 16, True),
     (9, 3, 1, 70, 34, False), (9, 1, 2, 7, 6, True), (1300, 8, 2, 64, 64, False),
-    (20, 2, 2, 512, 512, False)])
+    (20, 2, 2, 512, 512, False), (9, 3, 2, 512, 500, False), (11, 2, 0, 2048, 70, False),
+    (3, 2, 1, 2056, 512, True), (700, 20, 4, 128, 100, False), (700, 20, 4, 128, 90, True)])
 def test_rotary(rows, Hq, Hk, d, R, interleaved, dtype):
     gen = torch.Generator().manual_seed(rows)
     # cut out of a projection's output: rows and heads strided
