@@ -358,40 +358,59 @@ __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
 }
 
 // A lane's part of its query row (element `at` on; 8 values from col(k) on for each product
-// step k) as f16, times a power of two that brings the row's largest into [2^9, 2^10):
+// step k) as it lies, where 16-byte loads are aligned.  (Apart from load_query, so that keys and
+// values are asked for behind it and are on their way while it becomes f16.)  LO: fp32 queries.
+template <int KS, bool LO>
+struct RawQuery {
+  v4u w[LO ? 2 * KS : KS];
+};
+template <int KS, bool LO, typename Col>
+__device__ __forceinline__ RawQuery<KS, LO> fetch_query(const Att& A, int64_t at, bool live, Col col) {
+  RawQuery<KS, LO> r;
+#pragma unroll
+  for (int i = 0; i < (LO ? 2 * KS : KS); ++i) r.w[i] = v4u{0, 0, 0, 0};
+  if (A.q_vec && live) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      if constexpr (LO) {
+        const v4u* const p = reinterpret_cast<const v4u*>(static_cast<const float*>(A.q) + at + col(k));
+        r.w[2 * k] = p[0];
+        r.w[2 * k + 1] = p[1];
+      } else {
+        r.w[k] = *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(A.q) + at + col(k));
+      }
+    }
+  }
+  return r;
+}
+
+// That part as f16, times a power of two that brings the row's largest into [2^9, 2^10):
 // 16-bit types are exact so, fp32 takes lo beside it.  Lanes FIRST and 32 apart share a row.
 // c: what turns a score of these into an exponent of 2.  stage: THR * 8 KS floats of LDS, for
 // threads 0 .. THR - 1 (tid).
 template <int KS, bool LO, int THR, int FIRST, typename Col>
-__device__ __forceinline__ void load_query(const Att& A, int64_t at, bool live, int tid, Col col,
-                                           float* stage, v8h* qh, v8h* ql, float& c) {
+__device__ __forceinline__ void load_query(const Att& A, const RawQuery<KS, LO>& raw, int64_t at,
+                                           bool live, int tid, Col col, float* stage, v8h* qh,
+                                           v8h* ql, float& c) {
   float x[KS][8];
-  if (A.q_vec && A.q_dtype != QKV_F32) {
-    v4u w[KS];
+  if (A.q_vec) {
+    if constexpr (LO) {
 #pragma unroll
-    for (int k = 0; k < KS; ++k)
-      w[k] = live ? *reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(A.q) + at + col(k))
-                  : v4u{0, 0, 0, 0};
-    if (A.q_dtype == QKV_BF16) {
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[k][j] = __uint_as_float(raw.w[2 * k + (j >> 2)][j & 3]);
+    } else if (A.q_dtype == QKV_BF16) {
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          x[k][j] = __uint_as_float(j & 1 ? w[k][j >> 1] & 0xffff0000u : w[k][j >> 1] << 16);
+          x[k][j] = __uint_as_float(j & 1 ? raw.w[k][j >> 1] & 0xffff0000u : raw.w[k][j >> 1] << 16);
     } else {
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          x[k][j] = static_cast<float>(__builtin_bit_cast(v8h, w[k])[j]);
-    }
-  } else if (A.q_vec) {
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const v4f* const p = reinterpret_cast<const v4f*>(static_cast<const float*>(A.q) + at + col(k));
-      const v4f a = live ? p[0] : v4f{0.f, 0.f, 0.f, 0.f}, b = live ? p[1] : v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[k][j] = j < 4 ? a[j & 3] : b[j & 3];
+          x[k][j] = static_cast<float>(__builtin_bit_cast(v8h, raw.w[k])[j]);
     }
   } else {  // (rolled, through LDS: it runs once, and unrolled it would be most of the code)
     float* const t = stage + tid;

@@ -117,6 +117,9 @@ __device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h
   };
 
   const int steps = max(0, (P.s1 - P.s0 - wave + kWaves - 1) / kWaves);
+  auto q_col = [&](int k) { return dcol(D, k, g); };
+  const int64_t q_at = row * A.q_ts + hq * A.q_hs;
+  const RawQuery<KS, QLO> raw = fetch_query<KS, QLO>(A, q_at, live, q_col);
   bool ok = false;
   int64_t row0 = 0;
   if (steps > 0) {
@@ -126,8 +129,7 @@ __device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h
   }
   v8h qh[KS], ql[QLO ? KS : 1];
   float c;  // scores to exponents, without the block's scale
-  load_query<KS, QLO, kThr, 16>(A, row * A.q_ts + hq * A.q_hs, live, tid,
-                                [&](int k) { return dcol(D, k, g); }, &red_o[0][0][0], qh, ql, c);
+  load_query<KS, QLO, kThr, 16>(A, raw, q_at, live, tid, q_col, &red_o[0][0][0], qh, ql, c);
 #pragma unroll 1
   for (int it = 0; it < steps; ++it) {
     const int t0 = (P.s0 + wave + kWaves * it) * kStep;

@@ -159,11 +159,13 @@ __device__ __forceinline__ void prefill_piece(const Att& A, const Piece& P, int 
   };
 
   const int mine = P.s0 + th;  // this half's first step
+  auto q_col = [&](int k) { return 16 * k + 8 * hf; };
+  const int64_t q_at = row * A.q_ts + hq * A.q_hs;
+  const RawQuery<KK, QLO> raw = fetch_query<KK, QLO>(A, q_at, live, q_col);
   if (mine < s1) fetch(mine);
   v8h qh[KK], ql[QLO ? KK : 1];
   float c;  // scores to exponents, without the block's scale
-  load_query<KK, QLO, kPreThr, 32>(A, row * A.q_ts + hq * A.q_hs, live, thread,
-                                   [&](int k) { return 16 * k + 8 * hf; },
+  load_query<KK, QLO, kPreThr, 32>(A, raw, q_at, live, thread, q_col,
                                    reinterpret_cast<float*>(lds), qh, ql, c);
   if (mine < s1) put(mine, 0);
   bool ok = ok_r;  // of the step to come

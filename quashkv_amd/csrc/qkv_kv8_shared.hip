@@ -609,14 +609,15 @@ __global__ __launch_bounds__(kPreThr, 2) void share8(Args) {
   extern __shared__ __align__(16) uint8_t lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   {
-    const Args& C = args_anew();
+    const Args C = args_anew();  // (a copy: its loads are one batch)
     if (wave == 0) {
       Frame F;
       if (C.s.small) F = plan_wave(C.a, C.s, Places{sh_tall, sh_fours, sh_geo}, blockIdx.x == 0);
       else F = *C.s.frame;
       if (threadIdx.x == 0) {
         sh_frame = F;
-        sh_x = F.tall > 0 ? static_cast<int>(blockIdx.x / C.a.H) * F.range : 0;
+        const int j = blockIdx.x / C.a.H;
+        sh_x = j < F.tall ? j * F.range : 0;  // (ranges end below 2^31)
       }
     }
     __syncthreads();
@@ -659,6 +660,7 @@ __global__ __launch_bounds__(kPreThr, 2) void share8(Args) {
     Frame F;
     F.range = same(sh_frame.range);
     F.setup = same(sh_frame.setup);
+    if (j >= same(sh_frame.tall)) break;
     const int x = same(sh_x), total = same(C.s.small ? sh_tall[kItems] : C.s.at.tall[items]);
     const int end = min((j + 1) * F.range, total);
     __syncthreads();  // (sh_x is read)

@@ -236,7 +236,8 @@ def test_attention_is_the_plain_one():
         assert float((x - y).abs().max()) <= bound, Q
 
 
-@pytest.mark.parametrize("H,G,Q", [(1, 1, 1), (5, 3, 2), (32, 1, 1), (3, 16, 1), (2, 33, 3), (1, 71, 2)])
+@pytest.mark.parametrize("H,G,Q", [(1, 1, 1), (5, 3, 2), (32, 1, 1), (3, 16, 1), (2, 33, 3), (1, 71, 2),
+                                   (300, 1, 1), (260, 2, 7)])
 def test_head_layouts(H, G, Q):
     groups, own = [(192, 3)], [Q, Q + 5, 40]
     st, cache, lens = _forked(groups, own, H, 64, "int8", 64, seed=H)
