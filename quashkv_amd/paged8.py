@@ -208,7 +208,8 @@ def fork_pages(table: torch.Tensor, lens: torch.Tensor, src: torch.Tensor, dst: 
     _want(dst, "dst", torch.int32, (F,))
     if tokens is not None:
         _want(tokens, "tokens", torch.int32, (F,))
-    out = ForkPlan(*torch.empty(4, F, dtype=torch.int32, device=dev).unbind(0))
+    out = ForkPlan(*torch.empty(4 * F, dtype=torch.int32, device=dev).unsafe_split_with_sizes(
+        (F, F, F, F)))
     _call(dev, N.lib().qkv_page_fork, table.data_ptr(), lens.data_ptr(), B, width, src.data_ptr(),
           dst.data_ptr(), N.ptr(tokens), F, free.data_ptr(), P, free_count.data_ptr(),
           shares.data_ptr(), page_tokens, out.granted.data_ptr(), out.src_pages.data_ptr(),
