@@ -808,8 +808,8 @@ int qkv_kv8_attention(const void* q, int32_t q_dtype, int64_t q_row_stride,
  * copy_tokens), in the pools of every layer that the table serves.  All forks
  * (<= 16000) go by the lengths before the call.  A fork is granted wholly or not at
  * all: not, if src or dst is no request or both are the same, dst holds tokens,
- * an earlier fork of the call names the same dst, or it needs a page and the
- * pages needed up to it, in fork order, exceed the free ones.
+ * an earlier fork of the call (of two different requests) names the same dst, or it
+ * needs a page and the pages needed up to it, in fork order, exceed the free ones.
  *   granted      t, or -1 where refused
  *   src_pages, dst_pages, copy_tokens   the page to copy, or -1, -1, 0 */
 int qkv_page_fork(int32_t* table, int32_t* lens, int32_t B, int32_t pages_per_seq,

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(kThr) void copy_pages(Copy A) {
     const int64_t i = (v >> 1) / A.H;
     const int32_t from = A.src[i], to = A.dst[i];
     if (from < 0 || from >= A.npages || to < 0 || to >= A.npages || from == to) continue;
-    const int blocks = A.tokens ? min((max(A.tokens[i], 0) + kBlk - 1) >> 4, nb) : nb;
+    const int blocks = A.tokens ? (min(max(A.tokens[i], 0), 1 << A.lg) + kBlk - 1) >> 4 : nb;
     const int64_t a = (int64_t(from) * A.H + h) * nb, b = (int64_t(to) * A.H + h) * nb;
     const int bytes = blocks * A.row - piece * kPiece;
     const v4u* const x = reinterpret_cast<const v4u*>(A.pool[half] + a * A.row + piece * kPiece);

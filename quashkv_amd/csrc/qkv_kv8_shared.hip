@@ -1059,7 +1059,8 @@ extern "C" int qkv_kv8_attention_shared(
   // places of tall tiles, were every request as long as the table is wide
   const double tiles = 2.0 * rows * G / kPreRows + std::min<double>(B + groups, 2.0 * rows * G / kFew);
   const double longest = std::min(double(pages_per_seq) * page_tokens, double(QKV_PAGED_TOKENS)) / kStep;
-  QKV_REQUIRE(tiles * (longest + 1 + kSetUp) < kMostPlaces && L.rows < INT32_MAX,
+  QKV_REQUIRE(tiles * (longest + 1 + kSetUp) < kMostPlaces && L.rows < INT32_MAX &&
+                  L.late * Hkv < (1 << 23),  // (a launch has fewer than 2^32 threads)
               "%lld rows of %d query heads a kv head over a table of %d pages are too large for one "
               "call", static_cast<long long>(rows), G, pages_per_seq);
   const int qb = q_dtype == QKV_F32 ? 4 : 2, ob = out_dtype == QKV_F32 ? 4 : 2;

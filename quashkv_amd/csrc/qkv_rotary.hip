@@ -266,20 +266,29 @@ extern "C" int qkv_rotary(int32_t dtype, const void* q, int64_t q_row_stride,
   const int64_t many = rows / (4 * qkv_num_cus());
   const int64_t most = std::min<int64_t>(kMaxRows, kMostUnits / ((int64_t(Hq) + Hk) * d));
   const int32_t wg_rows = static_cast<int32_t>(std::max<int64_t>(1, std::min(most, many)));
-  Rot A{{q, k}, {q_out, k_out}, {q_row_stride, k_row_stride}, {q_head_stride, k_head_stride},
-        {qo_row_stride, ko_row_stride}, {qo_head_stride, ko_head_stride}, {Hq, Hk}, rows, d, R,
-        wg_rows, place ? 0 : 1, interleaved ? 1 : 0, positions, turns, factor,
-        inverse ? -1.f : 1.f};
-  const uint32_t grid = static_cast<uint32_t>((rows + wg_rows - 1) / wg_rows);
   const int how = !vec ? kOne : interleaved ? kPairs : R % 16 == 0 ? kHalves : kTurned;
   // (kTurned: angles by eights, and the heads of a pass)
   const uint32_t lds = how == kTurned ? wg_rows * 8 * div8(R / 2) * sizeof(float2) +
                                             kThr / (d / 8) * d * sizeof(float)
                                       : wg_rows * (R / 2) * sizeof(float2);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == QKV_F32) launch<QKV_F32>(A, how, grid, lds, s);
-  else if (dtype == QKV_F16) launch<QKV_F16>(A, how, grid, lds, s);
-  else launch<QKV_BF16>(A, how, grid, lds, s);
-  QKV_LAUNCHED();
+  auto from = [&](const void* p, int64_t stride, int64_t r) {
+    return const_cast<char*>(static_cast<const char*>(p)) + r * stride * es;
+  };
+  const int64_t per = int64_t(wg_rows) << 23;  // a launch's rows: it has fewer than 2^32 threads
+  for (int64_t r = 0; r < rows; r += per) {
+    const int64_t n = std::min(per, rows - r);
+    Rot A{{from(q, q_row_stride, r), from(k, k_row_stride, r)},
+          {from(q_out, qo_row_stride, r), from(k_out, ko_row_stride, r)},
+          {q_row_stride, k_row_stride}, {q_head_stride, k_head_stride},
+          {qo_row_stride, ko_row_stride}, {qo_head_stride, ko_head_stride}, {Hq, Hk}, n, d, R,
+          wg_rows, place ? 0 : 1, interleaved ? 1 : 0, positions + r, turns, factor,
+          inverse ? -1.f : 1.f};
+    const uint32_t grid = static_cast<uint32_t>((n + wg_rows - 1) / wg_rows);
+    if (dtype == QKV_F32) launch<QKV_F32>(A, how, grid, lds, s);
+    else if (dtype == QKV_F16) launch<QKV_F16>(A, how, grid, lds, s);
+    else launch<QKV_BF16>(A, how, grid, lds, s);
+    QKV_LAUNCHED();
+  }
   return QKV_OK;
 }

@@ -197,8 +197,9 @@ def fork_pages(table: torch.Tensor, lens: torch.Tensor, src: torch.Tensor, dst: 
 
     All forks go by the lengths before the call.  A fork is granted wholly or refused
     (``granted`` -1): where src or dst is no request or both are the same, dst holds
-    tokens, an earlier fork of the call names the same dst, or it needs a page and the
-    pages needed up to it, in fork order, exceed the free ones."""
+    tokens, an earlier fork of the call (of two different requests) names the same dst, or it
+    needs a page and the pages needed up to it, in fork order, exceed the free ones.  A
+    copied block of 16 tokens keeps its scale for the fork's own tokens behind them."""
     dev = _one_device("fork_pages", table, lens, src, dst, tokens, free, free_count, shares)
     B, width, P = _check_books(table, lens, free, free_count, shares)
     if src.dim() != 1:

@@ -88,6 +88,11 @@ def _out(x: torch.Tensor, out: Optional[torch.Tensor], what: str) -> torch.Tenso
                          f"{tuple(out.shape)}")
     if out.stride(2) != 1 and out.numel() > 0:
         raise ValueError(f"{what} must have a dense last axis")
+    end = out.shape[2]
+    for stride, n in sorted(zip(out.stride()[:2], out.shape[:2])):
+        if n > 1 and stride < end:
+            raise ValueError(f"{what}'s rows or heads overlap")
+        end += stride * (n - 1)
     return out
 
 

@@ -303,6 +303,13 @@ def test_copy_pages(d, H, pt, code):
     _equal(pools, want)
 
 
+def test_copy_of_the_largest_token_counts():
+    pools = _pools(6, 2, 64, 128)
+    want = _copied(pools, [(0, 3, 128)], 128)
+    P8.copy_pages(i32([0, 1]), i32([3, 4]), **pools, tokens=i32([2 ** 31 - 1, -2 ** 31]))
+    _equal(pools, want)
+
+
 def test_copy_many_pages():
     pools = _pools(3000, 2, 64, 64)
     order = torch.randperm(3000, generator=torch.Generator().manual_seed(2)).int()
@@ -504,6 +511,36 @@ def test_rotary_of_nothing_and_special_values():
     want = torch.zeros_like(bad)
     want[0, 0, [3, 11]] = want[0, 1, [1, 9]] = True
     assert torch.equal(bad, want)
+
+
+def test_rotary_of_more_rows_than_a_launch():
+    """A launch of 256 threads for 8 rows ends below 2^27 of them."""
+    part, rows = 1000, (1 << 27) + 1005
+    turns = Q.rotary_turns(Q.rotary_frequencies(2), DEV)
+    x = torch.randn(part, 1, 2, device=DEV).to(F16)
+    pos = torch.arange(part, dtype=torch.int32, device=DEV)
+    want, _ = rot.rotary(x, None, pos, turns)
+    _check_rotary(x, pos, turns, want)
+    n = -(-rows // part)
+    xs = x.repeat(n, 1, 1)[:rows]
+    got, _ = rot.rotary(xs, None, pos.repeat(n)[:rows], turns)
+    assert torch.equal(got, want.repeat(n, 1, 1)[:rows])
+
+
+def test_rotary_outputs_that_overlap():
+    turns = Q.rotary_turns(Q.rotary_frequencies(32), DEV)
+    x = torch.randn(4, 3, 32, device=DEV)
+    pos = torch.arange(4, dtype=torch.int32, device=DEV)
+    for bad in (x[:1].expand(4, 3, 32), x[:, :1].expand(4, 3, 32),
+                torch.zeros(400, device=DEV).as_strided((4, 3, 32), (40, 32, 1)),
+                torch.zeros(400, device=DEV).as_strided((4, 3, 32), (32, 31, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            rot.rotary(x, None, pos, turns, q_out=bad)
+        with pytest.raises(ValueError, match="overlap"):
+            rot.rotary(x, x.clone(), pos, turns, k_out=bad)
+    y = torch.zeros(3, 4, 40, device=DEV)[:, :, :32].transpose(0, 1)   # head-major: disjoint
+    rot.rotary(x, None, pos, turns, q_out=y)
+    assert torch.equal(y, rot.rotary(x, None, pos, turns)[0])
 
 
 def test_rotary_of_shared_rows():

@@ -120,6 +120,7 @@ def test_attention_refusals():
     _refused(_attend(group_start=None), "null pointer")
     _refused(_attend(rows=-1), "rows")
     _refused(_attend(rows=1 << 26), "rows")
+    _refused(_attend(rows=16000, B=16000, Hq=600, H=600), "too large")
     _refused(_attend(rows=5, q_start=None, q_lens=None), "without q_start")
     _refused(_attend(q_start=None), "q_lens needs q_start")
     _refused(_attend(q=None), "null pointer")
