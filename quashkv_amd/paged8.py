@@ -30,6 +30,7 @@ synchronise.
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -209,13 +210,12 @@ def fork_pages(table: torch.Tensor, lens: torch.Tensor, src: torch.Tensor, dst: 
     _want(dst, "dst", torch.int32, (F,))
     if tokens is not None:
         _want(tokens, "tokens", torch.int32, (F,))
-    out = ForkPlan(*torch.empty(4 * F, dtype=torch.int32, device=dev).unsafe_split_with_sizes(
-        (F, F, F, F)))
+    out = torch.empty(4 * F, dtype=torch.int32, device=dev)
+    at = out.data_ptr()
     _call(dev, N.lib().qkv_page_fork, table.data_ptr(), lens.data_ptr(), B, width, src.data_ptr(),
           dst.data_ptr(), N.ptr(tokens), F, free.data_ptr(), P, free_count.data_ptr(),
-          shares.data_ptr(), page_tokens, out.granted.data_ptr(), out.src_pages.data_ptr(),
-          out.dst_pages.data_ptr(), out.copy_tokens.data_ptr())
-    return out
+          shares.data_ptr(), page_tokens, at, at + 4 * F, at + 8 * F, at + 12 * F)
+    return ForkPlan(*out.unsafe_split_with_sizes((F, F, F, F)))
 
 
 @dataclass
@@ -492,6 +492,7 @@ def attention_kv8_shared(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Ten
     return out
 
 
+@functools.lru_cache(maxsize=256)
 def attention_kv8_shared_workspace_bytes(B: int, groups: int, rows: int, Hq: int, H: int,
                                          d: int) -> int:
     """Bytes of the workspace that attention_kv8_shared needs at these sizes."""

@@ -74,26 +74,19 @@ def rotary_turns(frequencies: Union[Sequence[float], torch.Tensor], device=None)
     return torch.tensor(out, dtype=torch.int64, device=device)
 
 
-def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
-    if x.dim() != 3:
-        raise ValueError(f"{what} must be (rows, heads, head_dim); got {tuple(x.shape)}")
-    return x if x.stride(2) == 1 else x.contiguous()
-
-
-def _out(x: torch.Tensor, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
-    if out is None:
-        return torch.empty_like(x, memory_format=torch.contiguous_format)
-    if out.dtype is not x.dtype or out.shape != x.shape:
-        raise ValueError(f"{what} must be {x.dtype} of shape {tuple(x.shape)}; got {out.dtype} "
+def _out(x: torch.Tensor, shape: torch.Size, out: torch.Tensor, what: str) -> tuple:
+    """Strides of an output for rows like x."""
+    if out.dtype is not x.dtype or out.shape != shape:
+        raise ValueError(f"{what} must be {x.dtype} of shape {tuple(shape)}; got {out.dtype} "
                          f"{tuple(out.shape)}")
-    if out.stride(2) != 1 and out.numel() > 0:
+    rows, heads, d = shape
+    ts, hs, ls = out.stride()
+    if ls != 1 and rows * heads > 0:
         raise ValueError(f"{what} must have a dense last axis")
-    end = out.shape[2]
-    for stride, n in sorted(zip(out.stride()[:2], out.shape[:2])):
-        if n > 1 and stride < end:
-            raise ValueError(f"{what}'s rows or heads overlap")
-        end += stride * (n - 1)
-    return out
+    (near, n), (far, m) = sorted(((ts, rows), (hs, heads)))
+    if n > 1 and near < d or m > 1 and far < d + near * (n - 1):
+        raise ValueError(f"{what}'s rows or heads overlap")
+    return ts, hs
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
@@ -110,24 +103,44 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
     call, and where factor is 1 what undoes it.  ``q_out`` / ``k_out`` may be q / k
     themselves, but not overlap them otherwise."""
     dev = _one_device("rotary", q, k, positions, turns, q_out, k_out)
-    x = _rows(q, "queries")
-    rows, Hq, d = q.shape
-    y = None if k is None else _rows(k, "keys")
-    if k is not None and (k.shape[0] != rows or k.shape[2] != d or k.dtype is not q.dtype):
-        raise ValueError(f"keys must be {q.dtype} of shape ({rows}, heads, {d}); got {k.dtype} "
-                         f"{tuple(k.shape)}")
-    if k is None and k_out is not None:
-        raise ValueError("k_out needs keys")
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3:
+        raise ValueError(f"queries must be (rows, heads, head_dim); got {tuple(shape)}")
+    rows, Hq, d = shape
+    ts, hs, ls = q.stride()
+    x = q
+    if ls != 1:
+        x = q.contiguous()
+        ts, hs, ls = x.stride()
+    if q_out is None:
+        q_out, to, ho = torch.empty_like(q, memory_format=torch.contiguous_format), Hq * d, d
+    else:
+        to, ho = _out(q, shape, q_out, "q_out")
+    if k is None:
+        if k_out is not None:
+            raise ValueError("k_out needs keys")
+        keys, keys_out = (None, 0, 0, 0), (None, 0, 0)
+    else:
+        y, other = k, k.shape
+        if len(other) != 3 or other[0] != rows or other[2] != d or k.dtype is not dtype:
+            raise ValueError(f"keys must be {dtype} of shape ({rows}, heads, {d}); got {k.dtype} "
+                             f"{tuple(other)}")
+        Hk = other[1]
+        kts, khs, kls = k.stride()
+        if kls != 1:
+            y = k.contiguous()
+            kts, khs, kls = y.stride()
+        if k_out is None:
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+            kto, kho = Hk * d, d
+        else:
+            kto, kho = _out(k, other, k_out, "k_out")
+        keys, keys_out = (y.data_ptr(), kts, khs, Hk), (k_out.data_ptr(), kto, kho)
     _want(positions, "positions", torch.int32, (rows,))
     if turns.dim() != 1:
         raise ValueError("turns must be a 1-D int64 tensor")
     _want(turns, "turns", torch.int64)
-    a = _out(q, q_out, "q_out")
-    b = None if k is None else _out(k, k_out, "k_out")
-    ks = (0, 0) if y is None else (y.stride(0), y.stride(1))
-    bs = (0, 0) if b is None else (b.stride(0), b.stride(1))
-    _call(dev, N.lib().qkv_rotary, N.dtype_code(q.dtype), x.data_ptr(), x.stride(0), x.stride(1),
-          Hq, N.ptr(y), *ks, 0 if k is None else k.shape[1], rows, d, 2 * turns.numel(),
-          positions.data_ptr(), turns.data_ptr(), float(factor), 1 if interleaved else 0,
-          1 if inverse else 0, a.data_ptr(), a.stride(0), a.stride(1), N.ptr(b), *bs)
-    return a, b
+    _call(dev, N.lib().qkv_rotary, N.dtype_code(dtype), x.data_ptr(), ts, hs, Hq, *keys, rows, d,
+          2 * turns.numel(), positions.data_ptr(), turns.data_ptr(), float(factor),
+          1 if interleaved else 0, 1 if inverse else 0, q_out.data_ptr(), to, ho, *keys_out)
+    return q_out, k_out
