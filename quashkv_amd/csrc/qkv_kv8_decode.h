@@ -38,15 +38,25 @@ __host__ __device__ constexpr int dcol(int D, int ks, int g) {
 }
 
 // Four waves' results (tid 0 .. 255) of 16 rows over every fourth step of 64 tokens each to LDS
-// (red_o, red_ml), relative to their own maxima.
-template <int D, bool FP8, bool QLO>
+// (red_o, red_ml), relative to their own maxima.  meanwhile() is called while the first pages'
+// numbers are on their way.
+template <int D, bool FP8, bool QLO, typename F>
 __device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h, int tid,
                                              float (*red_o)[kRows][D + 4],
-                                             float (*red_ml)[kRows][2]) {
+                                             float (*red_ml)[kRows][2], F meanwhile) {
   constexpr int KS = D / 32, NJ = D / 16, NK = (D + 63) / 64;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
+  const int pg_sh = A.lg - 6;  // steps per page, log2
+  const int32_t* const tab = A.table + int64_t(P.b) * A.width;
+  int p_first = 0;
+  // lane i: the page of this wave's i-th step from p_first on
+  auto pages_from = [&](int i) {
+    const int st = P.s0 + wave + kWaves * (i + lane);
+    return st < P.s1 ? tab[st >> pg_sh] : -1;
+  };
+  int pages = pages_from(0);
 
   // ---- this lane's query row
   const int rr = P.rt * kRows + n, qi = rr / A.G, gq = rr - qi * A.G;
@@ -68,19 +78,14 @@ __device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h
   v4u kr[4][NK];
   v4u vr[NJ];
   float ks_r = 0.f, vs_r = 0.f;
-  const int pg_sh = A.lg - 6;  // steps per page, log2
-  const int32_t* const tab = A.table + int64_t(P.b) * A.width;
-  int pages = 0;   // lane i: the page of this wave's i-th step from p_first on
-  int p_first = 0;
   const int tok0 = 16 * (n >> 2) + (n & 3);
   const uint32_t k_off = static_cast<uint32_t>(tok0 * D + 16 * g);
   const uint32_t k_off2 = static_cast<uint32_t>(tok0 * D + 64 + 8 * g);  // D = 96: 8 bytes each
   const uint32_t v_off = static_cast<uint32_t>((g * D + n) * 16);
   auto page_of = [&](int i) {  // i: the wave's step count
-    if (i - p_first >= 64 || i == 0) {
+    if (i - p_first >= 64) {
       p_first = i;
-      const int st = P.s0 + wave + kWaves * (i + lane);
-      pages = st < P.s1 ? tab[st >> pg_sh] : -1;
+      pages = pages_from(i);
     }
     return __builtin_amdgcn_readlane(pages, i - p_first);
   };
@@ -120,6 +125,7 @@ __device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h
   auto q_col = [&](int k) { return dcol(D, k, g); };
   const int64_t q_at = row * A.q_ts + hq * A.q_hs;
   const RawQuery<KS, QLO> raw = fetch_query<KS, QLO>(A, q_at, live, q_col);
+  meanwhile();
   bool ok = false;
   int64_t row0 = 0;
   if (steps > 0) {
@@ -260,7 +266,7 @@ template <int D, bool FP8, bool QLO, bool ROWS>
 __device__ __forceinline__ void decode_piece(const Att& A, const Piece& P, int h, int tid,
                                              float (*red_o)[kRows][D + 4],
                                              float (*red_ml)[kRows][2]) {
-  decode_steps<D, FP8, QLO>(A, P, h, tid, red_o, red_ml);
+  decode_steps<D, FP8, QLO>(A, P, h, tid, red_o, red_ml, [] {});
   int64_t at = -1;  // where the partial result's row 0 goes
   if constexpr (ROWS) {
     if (P.slot >= 0) at = int64_t(h) * A.nslots + P.slot + P.rt * kRows;

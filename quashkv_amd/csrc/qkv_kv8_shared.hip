@@ -276,10 +276,19 @@ __device__ __forceinline__ int64_t scan64(int64_t v) {
   v += dpp<0x143, 0xc>(v);
   return v;
 }
-__device__ __forceinline__ int64_t last64(int64_t v) {
-  const int lo = __builtin_amdgcn_readlane(static_cast<int>(v), 63);
-  const int hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63);
-  return (static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo);
+
+__device__ __forceinline__ uint64_t bits_below(int n) {
+  return n >= 64 ? ~uint64_t(0) : (uint64_t(1) << n) - 1;
+}
+// Inclusive maximum over a wave's lanes.
+__device__ __forceinline__ int max_scan(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x111, 0xf, 0xf, false));  // as wave_scan
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x112, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x114, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x118, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xa, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xc, 0xf, false));
+  return v;
 }
 
 // The plan of up to 64 requests and groups by one wave, a lane each; to LDS, and what the second
@@ -295,24 +304,29 @@ __device__ __forceinline__ Frame plan_wave(const Att& A, const Share& S, const P
   Req r{0, 0, 0};
   if (lane < A.B) r = request(A, lane);
   const int rows = lane < A.B ? rows_of(A, r) : 0;
-  int group = -1, shares = 0;  // of the lane's request, and its prefix
-  Item it[2] = {no_item(), no_item()};  // the lane's group, its request
-#pragma unroll 1
-  for (int g = 0; g < S.groups; ++g) {
-    const int s = lane_value(start, g), e = lane_value(end, g), p = lane_value(prefix, g);
-    const bool in = lane >= s && lane < e && lane < A.B && takes_part(A, r, p);
-    const uint64_t all = __ballot(in);
-    if (all == 0) continue;
-    const int first = __builtin_ctzll(all), last = 63 - __builtin_clzll(all);
-    const Item x = group_item(A, p, first, lane_value(r.q0, first), lane_value(r.q0 + rows, last));
-    const int alone = lane_value(wave_scan(in ? cost_of(rows * A.G) : 0), 63);
-    if (!pays(S, __popcll(all), alone, x.rows, x.steps)) continue;
-    if (lane == g) it[0] = x;
-    if (in) {
-      group = g;
-      shares = p;
-    }
-  }
+  // A lane is a group and a request.  Its request's group is the last one that begins at it or
+  // before; all of a group's lanes, as bits, are its range's part of those that take part.
+  // (One group at a time: 0.4 us each.)
+  int* const at = P.tall;
+  at[lane] = -1;
+  __builtin_amdgcn_wave_barrier();
+  if (start >= 0 && start < min(end, kSmall)) at[start] = lane;
+  __builtin_amdgcn_wave_barrier();
+  const int named = max_scan(at[lane]), of = max(named, 0);
+  const int theirs_end = __shfl(end, of, 64), theirs_prefix = __shfl(prefix, of, 64);
+  const bool in = named >= 0 && lane < theirs_end && lane < A.B && takes_part(A, r, theirs_prefix);
+  const int lo = min(max(start, 0), kSmall), hi = min(max(end, lo), kSmall);
+  const uint64_t mine = __ballot(in) & (bits_below(hi) & ~bits_below(lo));
+  const int first = mine ? __builtin_ctzll(mine) : 0, last = mine ? 63 - __builtin_clzll(mine) : 0;
+  const int cost = in ? cost_of(rows * A.G) : 0, costs = wave_scan(cost);
+  const int row0 = __shfl(r.q0, first, 64), row1 = __shfl(r.q0 + rows, last, 64);
+  const int alone = __shfl(costs, last, 64) - __shfl(costs - cost, first, 64);
+  Item it[2] = {group_item(A, prefix, first, row0, row1), no_item()};  // the lane's group, its request
+  const bool does = mine != 0 && pays(S, __popcll(mine), alone, it[0].rows, it[0].steps);
+  if (!does) it[0] = no_item();
+  const uint64_t sharing = __ballot(does);
+  const int group = in && (sharing >> of & 1) ? of : -1;
+  const int shares = group < 0 ? 0 : theirs_prefix;
   if (lane < A.B) it[1] = own_item(A, r, lane, shares);
   // sums over all items; and over those before the lane's, groups first
   auto total = [&](auto f) { return lane_value(wave_scan(f(it[0]) + f(it[1])), 63); };
@@ -344,11 +358,20 @@ __device__ __forceinline__ Frame plan_wave(const Att& A, const Share& S, const P
     F.fours = before([&](const Item& x) { return x.four() ? x.tiles() * most_parts(x, F) : 0; },
                      fours);
   F.lates = min(before([](const Item& x) { return x.late() ? x.tiles() : 0; }, late), S.late_cap);
-  const int64_t slots[2] = {slots_of(it[0], F), slots_of(it[1], F)};
-  const int64_t sg = scan64(slots[0]), so = scan64(slots[1]) + last64(sg);
-  const int64_t slot[2] = {sg - slots[0], so - slots[1]};
-  // (lengths that do not fit q_start may ask for more rows than there are)
-  const bool fits[2] = {sg <= A.nslots, so <= A.nslots};
+  // (lengths that do not fit q_start may ask for more rows than there are: such sums, modulo 2^32,
+  // may be anything, but no item's rows leave the workspace)
+  uint32_t slots[2], slot[2];
+  bool fits[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    slots[k] = static_cast<uint32_t>(qkv_pages::imin(slots_of(it[k], F), int64_t(A.nslots) + 1));
+  slot[0] = wave_scan(slots[0]);
+  slot[1] = wave_scan(slots[1]) + lane_value(slot[0], 63);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    fits[k] = slot[k] <= static_cast<uint32_t>(A.nslots) && slot[k] >= slots[k];
+    slot[k] -= slots[k];
+  }
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     put_item(P, k * kSmall + lane, it[k], k == 1 && A.causal, tall[k], fours[k], slot[k], slots[k],
@@ -793,10 +816,16 @@ __global__ __launch_bounds__(kThr, 2) void share_rest(Att A, Share S, int deal) 
   const int r = lane >> 4, d0 = 8 * (lane & 15);
   const bool on = d0 < D;
   const Frame F = *S.frame;
+  // (a tile's numbers are loaded beside the plan's, before it is known whether there is one)
+  const int t = blockIdx.x / A.H, h = blockIdx.x - t * A.H;
+  int4 pre = make_int4(0, 0, 0, 0), q = pre, kv = pre;
+  if (t < S.late_cap) {
+    pre = S.lates[3 * t];
+    q = S.lates[3 * t + 1];
+    kv = S.lates[3 * t + 2];
+  }
   const int lates = same(F.lates) * A.H;
   if (static_cast<int>(blockIdx.x) < lates) {
-    const int h = blockIdx.x % A.H, t = blockIdx.x / A.H;
-    const int4 pre = S.lates[3 * t], q = S.lates[3 * t + 1], kv = S.lates[3 * t + 2];
     Piece P{};
     P.b = same(q.x);
     P.rt = same(q.y);
@@ -808,11 +837,15 @@ __global__ __launch_bounds__(kThr, 2) void share_rest(Att A, Share S, int deal) 
     const int rows = min(kRows, same(kv.z) - P.rt * kRows);
     const int sets = (rows + 3) / 4, each = sets == 1 ? 4 : sets == 2 ? 2 : 1;  // waves of 4 rows
     // (the first parts are on their way while the own tokens are gone over)
-    const int set = wave / each, rr = P.rt * kRows + 4 * set + r, rp = rr + same(kv.w);
-    const int parts = set < sets && 4 * set + r < rows ? parts_of(pre, F, rp) : 0;
-    const int64_t first = int64_t(h) * A.nslots + pre.x + rp;
-    const Parts some = load_parts<D>(A, first, pre.y, wave % each, each, parts, on, d0);
-    decode_steps<D, FP8, QLO>(A, P, h, tid, red_o, red_ml);
+    int parts = 0;
+    int64_t first = 0;
+    Parts some;
+    decode_steps<D, FP8, QLO>(A, P, h, tid, red_o, red_ml, [&] {
+      const int set = wave / each, rr = P.rt * kRows + 4 * set + r, rp = rr + same(kv.w);
+      parts = set < sets && 4 * set + r < rows ? parts_of(pre, F, rp) : 0;
+      first = int64_t(h) * A.nslots + pre.x + rp;
+      some = load_parts<D>(A, first, pre.y, wave % each, each, parts, on, d0);
+    });
     if (same(pre.y) > 0) {
       float M = -INFINITY, L = 0.f, x[8] = {};
       fold(some, M, L, x);
