@@ -398,41 +398,77 @@ __device__ __forceinline__ Frame plan_wave(const Att& A, const Share& S, const P
 }
 
 constexpr int kW = kPlanThr / 64;
+static_assert(kW == 16, "a wave's sums are a lane of 16");
 
-// Inclusive sums of K values over the workgroup; `total` those of all.
+// Inclusive sums of K <= 4 values over the workgroup; `total` those of all.  The waves' sums meet
+// in the lanes of each: 16 k + w has wave w's of value k.
 template <int K>
-__device__ __forceinline__ void block_sums(int64_t* v, int64_t (*part)[4], int64_t* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ void block_sums(int64_t* v, int64_t* part, int64_t* total) {
+  using qkv_pages::dpp;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
   for (int k = 0; k < K; ++k) v[k] = scan64(v[k]);
   __syncthreads();  // (part's last readers)
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (lane == 63) part[wave][k] = v[k];
-    total[k] = 0;
-  }
+  for (int k = 0; k < K; ++k)
+    if (lane == 63) part[kW * k + wave] = v[k];
   __syncthreads();
-#pragma unroll 4
-  for (int w = 0; w < kW; ++w)
+  int64_t u = lane < kW * K ? part[lane] : 0;
+  const int64_t own = u;
+  u += dpp<0x111, 0xf>(u);  // row_shr 1, 2, 4, 8
+  u += dpp<0x112, 0xf>(u);
+  u += dpp<0x114, 0xf>(u);
+  u += dpp<0x118, 0xf>(u);
+  auto at = [](int64_t x, int l) {
+    return (static_cast<int64_t>(lane_value(static_cast<int>(x >> 32), l)) << 32) |
+           static_cast<uint32_t>(lane_value(static_cast<int>(x), l));
+  };
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int64_t u = part[w][k];
-      if (w < wave) v[k] += u;
-      total[k] += u;
-    }
+  for (int k = 0; k < K; ++k) {
+    v[k] += at(u - own, kW * k + wave);
+    total[k] = at(u, kW * k + kW - 1);
+  }
 }
 
-// The same of more requests or groups, by a workgroup, into the workspace.
+// Inclusive sum over 16 lanes.
+__device__ __forceinline__ float row_scan(float v) {
+  auto add = [&](auto ctrl) {
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v),
+                                                               decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{});  // row_shr 1, 2, 4, 8
+  add(integral_constant<int, 0x112>{});
+  add(integral_constant<int, 0x114>{});
+  add(integral_constant<int, 0x118>{});
+  return v;
+}
+
+// The same of more requests or groups, by a workgroup, into the workspace.  ONE: a thread has
+// one item, and keeps it.
+template <bool ONE>
 __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
-  extern __shared__ int32_t sh[];
-  __shared__ int64_t part[kW][4];
-  const int tid = threadIdx.x, Gr = S.groups;
-  int32_t* const start = sh;            // [Gr + 1]
+  extern __shared__ __align__(16) int32_t sh[];
+  __shared__ int64_t part[kW * 4];
+  const int tid = threadIdx.x, Gr = S.groups, items = Gr + A.B;
+  int4* const joins = reinterpret_cast<int4*>(sh);  // ONE: [Gr]
+  int32_t* const start = sh + (ONE ? 4 * Gr : 0);   // [Gr + 1]
   int32_t* const lead = start + Gr + 1; // [Gr]: the first request that takes part,
   int32_t* const many = lead + Gr;      // how many do,
   int32_t* const row0 = many + Gr;      // their first row and the end of their last one,
   int32_t* const row1 = row0 + Gr;
   int32_t* const cost = row1 + Gr;      // and what they cost alone; then whether they share
+  // f(i) for the thread's items of [from, to)
+  auto each = [&](int from, int to, auto f) {
+    if (ONE) {
+      if (tid >= from && tid < to) f(tid);
+    } else {
+      for (int i = from + tid; i < to; i += kPlanThr) f(i);
+    }
+  };
+  Req kept{0, 0, 0};
+  if (ONE && tid >= Gr && tid < items) kept = request(A, tid - Gr);
+  auto req = [&](int b) { return ONE ? kept : request(A, b); };
   for (int g = tid; g <= Gr && Gr > 0; g += kPlanThr) {
     start[g] = S.group_start[g];
     if (g < Gr) {
@@ -451,77 +487,95 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
     }
     return start[lo] <= b && b < start[lo + 1] ? lo : -1;
   };
-  for (int b = tid; b < A.B; b += kPlanThr) {
-    const int g = group_of(b);
-    if (g < 0) continue;
-    const Req r = request(A, b);
-    if (!takes_part(A, r, prefix_of(S, g))) continue;
+  int mine = -1, prefix = 0;  // ONE: the request's group, and its prefix or the group's
+  each(Gr, items, [&](int i) {
+    const int b = i - Gr, g = group_of(b);
+    if (g < 0) return;
+    const Req r = req(b);
+    const int p = prefix_of(S, g);
+    if (!takes_part(A, r, p)) return;
+    mine = g;
+    prefix = p;
     atomicMin(&lead[g], b);
     atomicAdd(&many[g], 1);
     atomicAdd(&cost[g], cost_of(rows_of(A, r) * A.G));
     atomicMin(&row0[g], r.q0);
     atomicMax(&row1[g], r.q0 + rows_of(A, r));
-  }
+  });
+  if (ONE && tid < Gr) prefix = prefix_of(S, tid);
   __syncthreads();
-  for (int g = tid; g < Gr; g += kPlanThr)
-    cost[g] = pays(S, many[g], cost[g], max(row1[g] - row0[g], 0) * A.G, prefix_of(S, g) / kStep);
+  each(0, Gr, [&](int g) {
+    const int p = ONE ? prefix : prefix_of(S, g);
+    cost[g] = pays(S, many[g], cost[g], max(row1[g] - row0[g], 0) * A.G, p / kStep);
+  });
   __syncthreads();
-  const int items = Gr + A.B;
-  auto item = [&](int i, int& g) {
+  auto make = [&](int i, int& g) {
     if (i < Gr) {
       g = i;
-      return cost[i] ? group_item(A, prefix_of(S, i), lead[i], row0[i], row1[i]) : no_item();
+      return cost[i] ? group_item(A, ONE ? prefix : prefix_of(S, i), lead[i], row0[i], row1[i])
+                     : no_item();
     }
     const int b = i - Gr;
-    const Req r = request(A, b);
-    g = group_of(b);
-    if (g >= 0 && (!cost[g] || !takes_part(A, r, prefix_of(S, g)))) g = -1;
-    return own_item(A, r, b, g >= 0 ? prefix_of(S, g) : 0);
+    const Req r = req(b);
+    g = ONE ? mine : group_of(b);
+    if (g >= 0 && (!cost[g] || !(ONE || takes_part(A, r, prefix_of(S, g))))) g = -1;
+    return own_item(A, r, b, g >= 0 ? (ONE ? prefix : prefix_of(S, g)) : 0);
+  };
+  Item own = no_item();
+  int own_g = -1;
+  if (ONE && tid < items) own = make(tid, own_g);
+  auto item = [&](int i, int& g) {
+    if (!ONE) return make(i, g);
+    g = own_g;
+    return own;
   };
   // steps and number of tall tiles, steps of short ones
   float sum[3] = {0.f, 0.f, 0.f};
-  for (int i = tid; i < items; i += kPlanThr) {
+  each(0, items, [&](int i) {
     int g;
     const Item it = item(i, g);
     const float n = static_cast<float>(it.tiles()), st = n * static_cast<float>(it.steps);
     sum[0] += it.tall() ? st : 0.f;
     sum[1] += it.tall() ? n : 0.f;
     sum[2] += it.four() ? st : 0.f;
-  }
+  });
   float* const fpart = reinterpret_cast<float*>(part);
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
     const float v = wave_scan(sum[k]);
-    if ((tid & 63) == 63) fpart[3 * (tid >> 6) + k] = v;
+    if ((tid & 63) == 63) fpart[kW * k + (tid >> 6)] = v;
   }
   __syncthreads();
+  {
+    const float v = row_scan((tid & 63) < 3 * kW ? fpart[tid & 63] : 0.f);
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    sum[k] = 0.f;
-    for (int w = 0; w < kW; ++w) sum[k] += fpart[3 * w + k];
+    for (int k = 0; k < 3; ++k) sum[k] = lane_value(v, kW * k + kW - 1);
   }
   Frame F = frame_of(A, sum[0], sum[1], sum[2], [&](int R) {
     int64_t n = 0, all;
-    for (int i = tid; i < items; i += kPlanThr) {
+    each(0, items, [&](int i) {
       int g;
       const Item it = item(i, g);
       if (it.tall()) n += it.tiles() * div_up(it.steps, R);
-    }
+    });
     block_sums<1>(&n, part, &all);
     return static_cast<int>(min(all, int64_t(INT32_MAX)));
   });
   const bool runs = F.range > 1;
   // (how many ranges there are decides whether tiles are cut at all)
-  {
+  if (runs) {
     int64_t n = 0, all;
-    for (int i = tid; i < items; i += kPlanThr) {
+    each(0, items, [&](int i) {
       int g;
       const Item it = item(i, g);
-      if (runs && it.tall()) n += int64_t(it.tiles()) * extent(F, it.steps);
-    }
+      if (it.tall()) n += int64_t(it.tiles()) * extent(F, it.steps);
+    });
     block_sums<1>(&n, part, &all);
     F.tall = div_up(static_cast<int>(all), F.range);
   }
+  const int4 none = make_int4(0, 0, 0, 0);
+  int4 join = none;
+  int late = 0;
   int64_t base[4] = {0, 0, 0, 0};  // places of tall tiles, parts, tiles of the second launch, rows
   for (int i0 = 0; i0 < items; i0 += kPlanThr) {
     const int i = i0 + tid;
@@ -542,13 +596,15 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
     const bool fits = v[3] + n[3] <= A.nslots;
     put_item(S.at, i, it, i >= Gr && A.causal, static_cast<int>(v[0]), static_cast<int>(v[1]), v[3],
              n[3], fits);
-    const int4 j = fits ? join_of(it, F, n[3], v[3], static_cast<int>(v[0])) : make_int4(0, 0, 0, 0);
-    // (requests' entries follow when all groups' are known; theirs wait behind)
+    join = fits ? join_of(it, F, n[3], v[3], static_cast<int>(v[0])) : none;
+    late = static_cast<int>(v[2]);
+    // (requests' entries follow when all groups' are known; without ONE theirs wait behind)
     if (i < Gr) {
-      S.meta[3 * A.B + i] = j;
-    } else {
-      S.meta[3 * (i - Gr)] = j;
-      S.meta[3 * (i - Gr) + 2] = make_int4(static_cast<int>(v[2]), 0, 0, 0);
+      if (ONE) joins[i] = join;
+      else S.meta[3 * A.B + i] = join;
+    } else if (!ONE) {
+      S.meta[3 * (i - Gr)] = join;
+      S.meta[3 * (i - Gr) + 2] = make_int4(late, 0, 0, 0);
     }
   }
   if (tid == 0) {
@@ -559,20 +615,36 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
     *S.frame = F;
   }
   __syncthreads();
-  for (int b = tid; b < A.B; b += kPlanThr) {
+  each(Gr, items, [&](int i) {
+    const int b = i - Gr;
     int g;
-    const Item it = item(Gr + b, g);
-    const int4 none = make_int4(0, 0, 0, 0);
-    put_request(A, S, b, it, S.meta[3 * b], g >= 0 ? S.meta[3 * A.B + g] : none, g >= 0 ? row0[g] : 0,
-                S.meta[3 * b + 2].x);
-  }
+    const Item it = item(i, g);
+    int4 theirs = none;
+    if (!ONE) {
+      join = S.meta[3 * b];
+      late = S.meta[3 * b + 2].x;
+      if (g >= 0) theirs = S.meta[3 * A.B + g];
+    } else if (g >= 0) {
+      theirs = joins[g];
+    }
+    put_request(A, S, b, it, join, theirs, g >= 0 ? row0[g] : 0, late);
+  });
   // ---- the rows' requests
   if (A.q_start == nullptr) {
     for (int r = tid; r < A.rows; r += kPlanThr) S.row_req[r] = r / A.uniform_q;
     return;
   }
   __syncthreads();
-  for (int b = tid; b <= A.B; b += kPlanThr) sh[b] = A.q_start[b];
+  int32_t* const lens = sh + A.B + 1;  // ONE
+  if (ONE) {
+    if (tid >= Gr && tid < items) {
+      sh[tid - Gr] = kept.q0;
+      lens[tid - Gr] = kept.ql;
+    }
+    if (tid == 0) sh[A.B] = A.q_start[A.B];
+  } else {
+    for (int b = tid; b <= A.B; b += kPlanThr) sh[b] = A.q_start[b];
+  }
   __syncthreads();
   for (int r = tid; r < A.rows; r += kPlanThr) {
     int lo = 0, hi = A.B;
@@ -581,7 +653,8 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
       if (sh[mid] <= r) lo = mid;
       else hi = mid;
     }
-    const int in = r - sh[lo], ql = A.q_lens ? A.q_lens[lo] : sh[lo + 1] - sh[lo];
+    const int in = r - sh[lo];
+    const int ql = ONE ? lens[lo] : A.q_lens ? A.q_lens[lo] : sh[lo + 1] - sh[lo];
     S.row_req[r] = in >= 0 && in < ql ? lo : -1;
   }
 }
@@ -1146,8 +1219,10 @@ extern "C" int qkv_kv8_attention_shared(
   S.row_req = reinterpret_cast<int32_t*>(ws + L.row_req);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (!S.small) {
-    const uint32_t lds = std::max(6 * groups + 1, B + 1) * sizeof(int32_t);
-    share_plan<<<1, kPlanThr, lds, s>>>(A, S);
+    if (groups + B <= kPlanThr)
+      share_plan<true><<<1, kPlanThr, std::max(10 * groups + 1, 2 * B + 1) * sizeof(int32_t), s>>>(A, S);
+    else
+      share_plan<false><<<1, kPlanThr, std::max(6 * groups + 1, B + 1) * sizeof(int32_t), s>>>(A, S);
     QKV_LAUNCHED();
   }
   // the second launch: a workgroup per tile that may be its own, and some that join the rest, few
