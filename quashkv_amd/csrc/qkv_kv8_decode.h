@@ -37,12 +37,12 @@ __host__ __device__ constexpr int dcol(int D, int ks, int g) {
   return D == 96 && ks == 2 ? 64 + 8 * g : 64 * (ks >> 1) + 16 * g + 8 * (ks & 1);
 }
 
-// Four waves' results (tid 0 .. 255) of 16 rows over every fourth step of 64 tokens each to LDS
-// (red_o, red_ml), relative to their own maxima.  meanwhile() is called while the first pages'
-// numbers are on their way.
-template <int D, bool FP8, bool QLO, typename F>
-__device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h, int tid,
-                                             float (*red_o)[kRows][D + 4],
+// Waves' results (tid 0 .. 255: four of them) of 16 rows, over every `waves`-th step of 64 tokens
+// from number `turn` on, to LDS (red_o, red_ml), relative to their own maxima.  meanwhile() is called
+// while the first pages' numbers are on their way.
+template <int D, bool FP8, bool QLO, typename W, typename F>
+__device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h, int tid, int turn,
+                                             W waves, float (*red_o)[kRows][D + 4],
                                              float (*red_ml)[kRows][2], F meanwhile) {
   constexpr int KS = D / 32, NJ = D / 16, NK = (D + 63) / 64;
   const int lane = tid & 63;
@@ -53,7 +53,7 @@ __device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h
   int p_first = 0;
   // lane i: the page of this wave's i-th step from p_first on
   auto pages_from = [&](int i) {
-    const int st = P.s0 + wave + kWaves * (i + lane);
+    const int st = P.s0 + turn + waves * (i + lane);
     return st < P.s1 ? tab[st >> pg_sh] : -1;
   };
   int pages = pages_from(0);
@@ -92,7 +92,7 @@ __device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h
   auto row_of = [&](int i, bool& ok) {
     const int pg = page_of(i);
     ok = pg >= 0 && pg < A.npages;
-    const int st = P.s0 + wave + kWaves * i;
+    const int st = P.s0 + turn + waves * i;
     const int64_t t = int64_t(st) * kStep & ((int64_t(1) << A.lg) - 1);
     return ((int64_t(ok ? pg : 0) * A.H + h) << A.lg) + t;
   };
@@ -121,7 +121,7 @@ __device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h
       vr[j] = __builtin_nontemporal_load(reinterpret_cast<const v4u*>(p + v_off + 256 * j));
   };
 
-  const int steps = max(0, (P.s1 - P.s0 - wave + kWaves - 1) / kWaves);
+  const int steps = max(0, (P.s1 - P.s0 - turn + waves - 1) / waves);
   auto q_col = [&](int k) { return dcol(D, k, g); };
   const int64_t q_at = row * A.q_ts + hq * A.q_hs;
   const RawQuery<KS, QLO> raw = fetch_query<KS, QLO>(A, q_at, live, q_col);
@@ -138,7 +138,7 @@ __device__ __forceinline__ void decode_steps(const Att& A, const Piece& P, int h
   load_query<KS, QLO, kThr, 16>(A, raw, q_at, live, tid, q_col, &red_o[0][0][0], qh, ql, c);
 #pragma unroll 1
   for (int it = 0; it < steps; ++it) {
-    const int t0 = (P.s0 + wave + kWaves * it) * kStep;
+    const int t0 = (P.s0 + turn + waves * it) * kStep;
     // ---- scores
     v4f s[4];
 #pragma unroll
@@ -266,7 +266,8 @@ template <int D, bool FP8, bool QLO, bool ROWS>
 __device__ __forceinline__ void decode_piece(const Att& A, const Piece& P, int h, int tid,
                                              float (*red_o)[kRows][D + 4],
                                              float (*red_ml)[kRows][2]) {
-  decode_steps<D, FP8, QLO>(A, P, h, tid, red_o, red_ml, [] {});
+  decode_steps<D, FP8, QLO>(A, P, h, tid, __builtin_amdgcn_readfirstlane(tid >> 6),
+                            std::integral_constant<int, kWaves>{}, red_o, red_ml, [] {});
   int64_t at = -1;  // where the partial result's row 0 goes
   if constexpr (ROWS) {
     if (P.slot >= 0) at = int64_t(h) * A.nslots + P.slot + P.rt * kRows;

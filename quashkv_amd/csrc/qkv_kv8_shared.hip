@@ -872,6 +872,15 @@ __device__ __forceinline__ void add_parts(const Att& A, int64_t first, int rows,
     fold(load_parts<D>(A, first, rows, p0, every, parts, on, d0), M, L, x);
 }
 
+// Waves of a tile of the second launch: four, or as many as the card's two workgroups a CU have for
+// each.  A call with four / two / one, 8192 shared tokens, 8 kv heads, 4 query heads each, by requests
+// and their own tokens: 64 + 500 us 39.2 / 40.6 / 47.8, 96 + 300 54.9 / 52.7 / 55.3, 128 + 300 59.6 /
+// 57.0 / 58.7, 256 + 100 88 / 80 / 77, 256 + 300 91 / 85 / 83; but 256 + 1000 109 / 110 / 114.
+__device__ __forceinline__ int waves_of(const Att& A, int tiles) {
+  const int most = 2 * kWaves * A.target;  // of a kv head
+  return kWaves * tiles <= most ? kWaves : 2 * tiles <= most ? 2 : 1;
+}
+
 // The second launch.  Its first workgroups take a tile of 16 rows each of the requests that have
 // few own tokens: the prefix' partial results, which are there, dealt to the waves by rows and
 // parts, then the own tokens as a piece of four waves, then all in LDS.  The others join what else
@@ -883,22 +892,22 @@ __global__ __launch_bounds__(kThr, 2) void share_rest(Att A, Share S, int deal) 
   constexpr int LPR = D > 64 ? 16 : 8, RW = 64 / LPR;  // lanes of a row, rows of a wave
   __shared__ float red_o[kWaves][kRows][D + 4];
   __shared__ float red_ml[kWaves][kRows][2];
-  __shared__ float acc[kWaves][RW][D + 4], ml[kWaves][RW][2];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane >> 4, d0 = 8 * (lane & 15);
   const bool on = d0 < D;
   const Frame F = *S.frame;
-  // (a tile's numbers are loaded beside the plan's, before it is known whether there is one)
-  const int t = blockIdx.x / A.H, h = blockIdx.x - t * A.H;
-  int4 pre = make_int4(0, 0, 0, 0), q = pre, kv = pre;
-  if (t < S.late_cap) {
-    pre = S.lates[3 * t];
-    q = S.lates[3 * t + 1];
-    kv = S.lates[3 * t + 2];
-  }
-  const int lates = same(F.lates) * A.H;
+  const int tiles = same(F.lates), W = waves_of(A, tiles), T = kWaves / W;
+  const int lates = div_up(tiles, T) * A.H;
   if (static_cast<int>(blockIdx.x) < lates) {
+    const int u = blockIdx.x / A.H, h = blockIdx.x - u * A.H, t = u * T + wave / W, turn = wave % W;
+    // (a wave without a tile has no row or step, and takes the others' barriers)
+    int4 pre = make_int4(0, 0, 0, 0), q = pre, kv = pre;
+    if (t < tiles) {
+      pre = S.lates[3 * t];
+      q = S.lates[3 * t + 1];
+      kv = S.lates[3 * t + 2];
+    }
     Piece P{};
     P.b = same(q.x);
     P.rt = same(q.y);
@@ -907,51 +916,55 @@ __global__ __launch_bounds__(kThr, 2) void share_rest(Att A, Share S, int deal) 
     P.slot = -1;
     P.s0 = same(kv.y);
     P.s1 = steps_of(P.r.kv);
-    const int rows = min(kRows, same(kv.z) - P.rt * kRows);
-    const int sets = (rows + 3) / 4, each = sets == 1 ? 4 : sets == 2 ? 2 : 1;  // waves of 4 rows
-    // (the first parts are on their way while the own tokens are gone over)
+    // sets of 4 rows, `at_once` of them by `each` waves, which deal out the parts
+    const int rows = min(kRows, same(kv.z) - P.rt * kRows), sets = (rows + 3) / 4;
+    const int at_once = min(W, sets <= 1 ? 1 : sets == 2 ? 2 : 4), each = W / at_once;
+    const int p0 = turn % each;
     int parts = 0;
     int64_t first = 0;
     Parts some;
-    decode_steps<D, FP8, QLO>(A, P, h, tid, red_o, red_ml, [&] {
-      const int set = wave / each, rr = P.rt * kRows + 4 * set + r, rp = rr + same(kv.w);
-      parts = set < sets && 4 * set + r < rows ? parts_of(pre, F, rp) : 0;
+    auto parts_from = [&](int set) {
+      const int rr = P.rt * kRows + 4 * set + r, rp = rr + same(kv.w);
+      parts = 4 * set + r < rows ? parts_of(pre, F, rp) : 0;
       first = int64_t(h) * A.nslots + pre.x + rp;
-      some = load_parts<D>(A, first, pre.y, wave % each, each, parts, on, d0);
-    });
+      some = load_parts<D>(A, first, pre.y, p0, each, parts, on, d0);
+    };
+    // (the first parts are on their way while the own tokens are gone over)
+    decode_steps<D, FP8, QLO>(A, P, h, tid, turn, W, red_o, red_ml, [&] { parts_from(turn / each); });
     if (same(pre.y) > 0) {
-      float M = -INFINITY, L = 0.f, x[8] = {};
-      fold(some, M, L, x);
-      add_parts<D>(A, first, pre.y, wave % each + 4 * each, each, parts, on, d0, M, L, x);
-      if (on) {
-        *reinterpret_cast<v4f*>(&acc[wave][r][d0]) = v4f{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<v4f*>(&acc[wave][r][d0 + 4]) = v4f{x[4], x[5], x[6], x[7]};
-      }
-      if (d0 == 0) {
-        ml[wave][r][0] = M;
-        ml[wave][r][1] = L;
+      for (int set = turn / each; set < sets; set += at_once) {
+        if (set >= at_once) parts_from(set);
+        float* const o = &red_o[wave][4 * set + r][on ? d0 : 0];
+        float* const ml = red_ml[wave][4 * set + r];
+        float M = ml[0], L = ml[1], x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = o[j];
+        fold(some, M, L, x);
+        add_parts<D>(A, first, pre.y, p0 + 4 * each, each, parts, on, d0, M, L, x);
+        if (on) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = x[j];
+        }
+        if (d0 == 0) {
+          ml[0] = M;
+          ml[1] = L;
+        }
       }
     }
     __syncthreads();
     constexpr int PER = D / 8;
-    if (tid < kRows * PER) {
-      const int k = tid / PER, e0 = 8 * (tid % PER), w0 = k / 4 * each;
-      const int more = pre.y > 0 && k < rows ? each : 0;
+    for (int i = 64 * turn + lane; i < rows * PER; i += 64 * W) {
+      const int k = i / PER, e0 = 8 * (i % PER), w0 = wave - turn;
       float M = -INFINITY, L = 0.f, x[8] = {};
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) M = fmaxf(M, red_ml[w][k][0]);
-      for (int w = 0; w < more; ++w) M = fmaxf(M, ml[w0 + w][k & 3][0]);
+      for (int w = 0; w < W; ++w) M = fmaxf(M, red_ml[w0 + w][k][0]);
       const float ref = M == -INFINITY ? 0.f : M;
-      auto add = [&](float m, float l, const float* o) {
-        const float f = __builtin_amdgcn_exp2f(m - ref);
-        L += fall(l, m - ref);
+      for (int w = 0; w < W; ++w) {
+        const float m = red_ml[w0 + w][k][0] - ref, f = __builtin_amdgcn_exp2f(m);
+        const float* const o = &red_o[w0 + w][k][e0];
+        L += fall(red_ml[w0 + w][k][1], m);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = fmaf(o[j], f, x[j]);
-      };
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) add(red_ml[w][k][0], red_ml[w][k][1], &red_o[w][k][e0]);
-      for (int w = 0; w < more; ++w)
-        add(ml[w0 + w][k & 3][0], ml[w0 + w][k & 3][1], &acc[w0 + w][k & 3][e0]);
+      }
       const int rr = P.rt * kRows + k, qi = rr / A.G;
       const int64_t row = int64_t(P.r.q0) + qi;
       if (qi < P.r.ql && row >= 0 && row < A.rows) {
@@ -1007,28 +1020,28 @@ __global__ __launch_bounds__(kThr, 2) void share_rest(Att A, Share S, int deal) 
     }
     __syncthreads();  // (the arrays' last readers)
     if (in) {
-      *reinterpret_cast<v4f*>(&acc[wave][rw][e0]) = v4f{x[0], x[1], x[2], x[3]};
-      *reinterpret_cast<v4f*>(&acc[wave][rw][e0 + 4]) = v4f{x[4], x[5], x[6], x[7]};
+      *reinterpret_cast<v4f*>(&red_o[wave][rw][e0]) = v4f{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<v4f*>(&red_o[wave][rw][e0 + 4]) = v4f{x[4], x[5], x[6], x[7]};
     }
     if (e0 == 0) {
-      ml[wave][rw][0] = M;
-      ml[wave][rw][1] = L;
+      red_ml[wave][rw][0] = M;
+      red_ml[wave][rw][1] = L;
     }
     __syncthreads();
     if (wave != 0 || no == 0 || !in) continue;
     M = -INFINITY;
     L = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml[w][rw][0]);
+    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, red_ml[w][rw][0]);
     const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const float e = __builtin_amdgcn_exp2f(ml[w][rw][0] - ref);
-      L += fall(ml[w][rw][1], ml[w][rw][0] - ref);
+      const float e = __builtin_amdgcn_exp2f(red_ml[w][rw][0] - ref);
+      L += fall(red_ml[w][rw][1], red_ml[w][rw][0] - ref);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = fmaf(acc[w][rw][e0 + j], e, x[j]);
+      for (int j = 0; j < 8; ++j) x[j] = fmaf(red_o[w][rw][e0 + j], e, x[j]);
     }
     const float inv = inverse(L);
 #pragma unroll
