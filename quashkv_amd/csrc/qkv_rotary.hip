@@ -5,9 +5,9 @@
 //   y1 = c (x1 cos - x2 sin),  y2 = c (x2 cos + x1 sin);
 // coordinates behind R stay as they are.  f_i comes as turns in units of 2^-64, so that p f_i
 // modulo a turn is an integer product modulo 2^64: exact but for the rounding of f_i itself,
-// |p| 2^-65 turns, at any position.  Sine and cosine are fp32's of the nearest fp32 to the
-// remainder in [-1/2, 1/2) (off by 2^-26 turns at most, 2^-25 half turns, and less the smaller it
-// is); products and sums are fp32, rounded once to the rows' type.
+// |p| 2^-65 turns, at any position.  Sine and cosine are fp32's of the nearest fp32 to what is left
+// beside the nearest quarter turn (within 1/8, so off by 2^-28 turns at most: a quarter of what
+// the whole remainder's fp32 would be off); products and sums are fp32, rounded once to the rows' type.
 //
 // Bytes bound it, each row in and out: a workgroup has the angles of its rows in LDS, one sine
 // and cosine for all heads, and then goes over the rows' pairs with 16-byte loads.  8192 bf16 rows
@@ -107,10 +107,21 @@ __global__ __launch_bounds__(kThr) void rotate(Rot A) {
   for (int i = tid; i < nr * half; i += kThr) {
     const int r = i / half, k = i - r * half;
     // (two's complement: the product modulo 2^64 is right for negative positions, too)
-    const int64_t turn = static_cast<int64_t>(static_cast<uint64_t>(A.turns[k]) *
-                                              static_cast<uint64_t>(int64_t(A.pos[r0 + r])));
+    const uint64_t turn = static_cast<uint64_t>(A.turns[k]) *
+                          static_cast<uint64_t>(int64_t(A.pos[r0 + r]));
+    const uint32_t quarter = static_cast<uint32_t>((turn + (uint64_t(1) << 61)) >> 62);
+    const int64_t rest = static_cast<int64_t>(turn - (uint64_t(quarter) << 62));
     float s, c;
-    sincospif(static_cast<float>(turn) * 0x1p-63f, &s, &c);
+    sincospif(static_cast<float>(rest) * 0x1p-63f, &s, &c);
+    if (quarter & 1) {
+      const float t = s;
+      s = c;
+      c = -t;
+    }
+    if (quarter & 2) {
+      s = -s;
+      c = -c;
+    }
     cs[HOW == kTurned ? (r * 8 + (k & 7)) * div8(half) + (k >> 3) : i] =
         float2{c * A.factor, s * A.factor * A.sign};
   }
