@@ -15,21 +15,23 @@
 // (prefill_piece); of fewer, in tiles of 16 (decode_piece); and, of these, requests' own few
 // tokens.  The first launch (share8) has the first two, on a workgroup of 8 waves per CU, each of
 // which knows its part from the lengths alone: the tall tiles' steps, tile behind tile, are cut
-// into equal ranges, one a workgroup, so that all end together wherever tiles end (8 x 210 rows,
-// 7 query heads a kv head, over 250 steps: 172 tiles on 256 CUs), and the other workgroups take
+// into equal ranges, one a workgroup, so that all end together wherever tiles end (1131 rows,
+// 7 query heads a kv head, over 250 steps: 124 tiles on 256 CUs), and the other workgroups take
 // the short tiles, two at a time, four waves each, cut where they are long.  The second launch
 // (share_rest) takes the few own tokens, joining them with the prefix' partial results as it
 // goes, and joins whatever else was cut.
 //
-// Measured (a call; attention_kv8 over the same tables): 64 requests of up to 500 own tokens behind
-// 8192, 32 / 8 heads, d = 128, bf16: 39 us (95); behind 32,000 65 (331); 60 requests of six groups,
-// up to 5003 + 700, 24 / 8 heads, d = 96, e4m3: 31 (45); 8 x 210 rows behind 16,001, 14 / 2 heads,
-// d = 64, fp32 results: 147 (240).  Of the first's 39: the plan 3.9 us (loads of the lengths, then
-// ~1500 instructions of one wave), a tile's place, queries and first codes 4.8, four rounds of
-// 128 tokens 10.5 (2.3 to 2.6 each; prefill8's loop, see there), halves' join and 16.8 MB of
-// partial results 3.3, a gap of 3 between the launches, and the second one 11: own tokens'
-// chain of lengths - page - codes - results, 4 us of it their bytes.  Tall tiles, where there
-// are many, are bound by that loop: 75 % of what a large product reaches.
+// Measured (a call; attention_kv8 over the same tables): 60 rows of requests of up to 500 own tokens
+// behind 8192, 32 / 8 heads, d = 128, bf16: 39 us (95); behind 32,000 63 (331); 56 rows of six
+// groups, up to 5003 + 700, 24 / 8 heads, d = 96, e4m3: 28 (45); seven requests' 1131 rows behind
+// 16,001, 14 / 2 heads, d = 64, fp32 results: 143 (240); 256 requests of up to 300 behind 8192: 83.
+// Of the first's 39: the plan 3.6 us (loads of the lengths, then some 1000 instructions of one
+// wave), a tile's place, queries and first codes 4.5, four rounds of 128 tokens 10.3 (prefill8's
+// loop, see there), halves' join and 16.8 MB of partial results 3.1, a gap of 3 between the
+// launches, and the second one 8 (13 the longest): own tokens' chain of lengths - page - codes -
+// results.  Many tall tiles are bound by that loop's issue: of the 1131 rows' 138 us the SIMDs spend
+// 53 % on VALU work and 27 % on products (pairs of weights: 98 GFLOP).  Two workgroups a CU, which
+// d = 64 has LDS for, are slower (155 us: 45 registers spilled, and twice the partial results).
 //
 // Tried: the plan in a launch of its own (9 us, and a gap) with short tiles in the first launch
 // (a tile by one wave: 8 us each, one behind the other; 47 us in all); ranges that do not count

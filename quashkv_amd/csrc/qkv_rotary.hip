@@ -12,7 +12,7 @@
 // Bytes bound it, each row in and out: a workgroup has the angles of its rows in LDS, one sine
 // and cosine for all heads, and then goes over the rows' pairs with 16-byte loads.  8192 bf16 rows
 // of 40 heads, d = 128 (168 MB): 29 us over and over the same rows (5.8 TB/s; interleaved 31, 100 of
-// the 128 coordinates 39), 38 over others each time (4.4; a 1 GiB copy reaches 5.0).  64 rows 4 us
+// the 128 coordinates 39), 36 over others each time (4.7; a 1 GiB copy reaches 5.0).  64 rows 4 us
 // of kernel: a launch, the angles, a row.
 #include <algorithm>
 
