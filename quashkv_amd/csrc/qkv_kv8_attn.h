@@ -346,11 +346,15 @@ __device__ __forceinline__ uint32_t pk(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2h));
 }
 
-// x as f16 hi + lo, both rounded to nearest.
+// x as f16 hi + lo, both rounded to nearest.  (The difference as a multiply-add that takes f16:
+// one instruction where a conversion and a subtraction are two, the same bits; 1131 rows behind
+// 16,001 tokens, d = 64, fp32 results: 143 -> 140 us.  The factor is hidden, or it would be folded.)
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = pk(a, b);
   const v2h h = __builtin_bit_cast(v2h, hi);
-  lo = pk(a - static_cast<float>(h[0]), b - static_cast<float>(h[1]));
+  float minus = -1.f;
+  asm("" : "+s"(minus));
+  lo = pk(fmaf(static_cast<float>(h[0]), minus, a), fmaf(static_cast<float>(h[1]), minus, b));
 }
 
 __device__ __forceinline__ v4f mfma(v8h a, v8h b, v4f c) {
