@@ -215,6 +215,16 @@ def test_groups_at_the_ends_of_a_batch():
         _check(st, cache, lens, groups, ones, 4, F32, F32, start=start, prefix=prefix)
 
 
+@pytest.mark.parametrize("groups,own", [
+    ([(64, 0), (128, 2), (192, 0), (64, 0), (200, 3), (64, 0)], [1, 20, 3, 70, 5]),
+    ([(128, 1)] * 30 + [(64, 2)] * 17 + [(64, 0)] * 17, [1 + i % 7 for i in range(64)]),
+])
+def test_empty_groups(groups, own):
+    """Groups without requests among the others and behind the last, up to 64 of both."""
+    st, cache, lens = _forked(groups, own, 1, 64, "int8", 64)
+    _check(st, cache, lens, groups, [1] * len(own), 2, F32, F32, guard=True)
+
+
 def test_attention_is_the_plain_one():
     """Against attention_kv8 on the same tables, long prefixes cut into many parts."""
     B, H, G, d, prefix = 24, 2, 4, 128, 20000
@@ -376,6 +386,43 @@ def test_many_requests(B, m):
                                 prefix_lens=i32([whole * pt] * n))
     y = P8.attention_kv8(**args)
     # 256 tokens, values up to 1.3: as in test_attention_is_the_plain_one
+    assert float((x - y).abs().max()) <= 4 * 1.3 * (2.0 ** -18 + 72 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("B,m,H,G,d", [(65, 65, 1, 1, 64), (90, 4, 4, 9, 96), (250, 250, 4, 2, 128),
+                                       (300, 5, 4, 9, 64), (520, 40, 8, 4, 128), (700, 7, 4, 16, 64),
+                                       (1000, 1000, 2, 1, 96), (1000, 45, 2, 3, 64)])
+def test_many_tiles(B, m, H, G, d):
+    """Batches beyond a wave's lanes, one item a thread of the plan, with 4, 2 or 1 waves for each tile of
+    requests' own tokens: against attention_kv8."""
+    pt = 64
+    n = min(B // m, 2048)
+    gen = torch.Generator(device=DEV).manual_seed(B)
+    rng = random.Random(B)
+    whole, P = 2, 2 * n + 2 * B
+    table = torch.zeros(B, 5, dtype=torch.int32)
+    order = torch.randperm(P, generator=torch.Generator().manual_seed(1)).int()
+    for b in range(B):
+        g = b // m
+        first = order[2 * g:2 * g + 2] if g < n else order[2 * n + 2 * b - 2:2 * n + 2 * b]
+        table[b, :2] = first
+        table[b, 2:4] = order[2 * n + 2 * b:2 * n + 2 * b + 2]
+    pools = dict(kpool=torch.randint(-127, 128, (P, H, pt, d), generator=gen, device=DEV).to(torch.int8),
+                 vpool=torch.randint(-127, 128, (P, H, pt // 16, d, 16), generator=gen, device=DEV).to(torch.int8),
+                 kscale=0.01 * torch.rand(P, H, pt // 16, generator=gen, device=DEV) + 1e-4,
+                 vscale=0.01 * torch.rand(P, H, pt // 16, generator=gen, device=DEV) + 1e-4)
+    lens = i32([rng.choice([0, 128, 129, 200, 256, 60]) for _ in range(B)])
+    q_lens = [rng.choice([0, 1, 1, 1, 2]) for _ in range(B)]
+    start = [0]
+    for x in q_lens:
+        start.append(start[-1] + x)
+    q = torch.randn(start[-1], H * G, d, generator=gen, device=DEV)
+    args = dict(q=q, **pools, table=table.to(DEV), kv_lens=lens, q_start=i32(start),
+                q_lens=i32(q_lens), causal=True)
+    x = shared(**args, group_start=i32([m * g for g in range(n + 1)]),
+                                prefix_lens=i32([whole * pt] * n))
+    y = P8.attention_kv8(**args)
+    # as in test_many_requests
     assert float((x - y).abs().max()) <= 4 * 1.3 * (2.0 ** -18 + 72 * 2.0 ** -24)
 
 
