@@ -218,9 +218,10 @@ def test_groups_at_the_ends_of_a_batch():
 @pytest.mark.parametrize("groups,own", [
     ([(64, 0), (128, 2), (192, 0), (64, 0), (200, 3), (64, 0)], [1, 20, 3, 70, 5]),
     ([(128, 1)] * 30 + [(64, 2)] * 17 + [(64, 0)] * 17, [1 + i % 7 for i in range(64)]),
+    ([(64, 0)] * 40 + [(128, 3), (64, 0), (192, 4)] + [(64, 0)] * 30, [4, 3, 2, 1, 90, 1, 2]),
 ])
 def test_empty_groups(groups, own):
-    """Groups without requests among the others and behind the last, up to 64 of both."""
+    """Groups without requests among the others and behind the last, up to 64 of both and more."""
     st, cache, lens = _forked(groups, own, 1, 64, "int8", 64)
     _check(st, cache, lens, groups, [1] * len(own), 2, F32, F32, guard=True)
 
