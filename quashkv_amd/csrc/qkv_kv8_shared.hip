@@ -461,6 +461,7 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
   int32_t* const row0 = many + Gr;      // their first row and the end of their last one,
   int32_t* const row1 = row0 + Gr;
   int32_t* const cost = row1 + Gr;      // and what they cost alone; then whether they share
+  int32_t* const whole = cost + Gr;     // prefix_of
   // f(i) for the thread's items of [from, to)
   auto each = [&](int from, int to, auto f) {
     if (ONE) {
@@ -472,11 +473,13 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
   Req kept{0, 0, 0};
   if (ONE && tid >= Gr && tid < items) kept = request(A, tid - Gr);
   auto req = [&](int b) { return ONE ? kept : request(A, b); };
+  const int rows_end = A.q_start && tid == 0 ? A.q_start[A.B] : 0;
   for (int g = tid; g <= Gr && Gr > 0; g += kPlanThr) {
     start[g] = S.group_start[g];
     if (g < Gr) {
       lead[g] = row0[g] = INT32_MAX;
       many[g] = row1[g] = cost[g] = 0;
+      whole[g] = prefix_of(S, g);
     }
   }
   __syncthreads();
@@ -490,39 +493,36 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
     }
     return start[lo] <= b && b < start[lo + 1] ? lo : -1;
   };
-  int mine = -1, prefix = 0;  // ONE: the request's group, and its prefix or the group's
+  int mine = -1;  // ONE: the request's group, where it takes part
   each(Gr, items, [&](int i) {
     const int b = i - Gr, g = group_of(b);
     if (g < 0) return;
     const Req r = req(b);
-    const int p = prefix_of(S, g);
+    const int p = whole[g];
     if (!takes_part(A, r, p)) return;
     mine = g;
-    prefix = p;
     atomicMin(&lead[g], b);
     atomicAdd(&many[g], 1);
     atomicAdd(&cost[g], cost_of(rows_of(A, r) * A.G));
     atomicMin(&row0[g], r.q0);
     atomicMax(&row1[g], r.q0 + rows_of(A, r));
   });
-  if (ONE && tid < Gr) prefix = prefix_of(S, tid);
   __syncthreads();
   each(0, Gr, [&](int g) {
-    const int p = ONE ? prefix : prefix_of(S, g);
-    cost[g] = pays(S, many[g], cost[g], max(row1[g] - row0[g], 0) * A.G, p / kStep);
+    cost[g] = pays(S, many[g], cost[g], max(row1[g] - row0[g], 0) * A.G, whole[g] / kStep);
   });
   __syncthreads();
   auto make = [&](int i, int& g) {
     if (i < Gr) {
       g = i;
-      return cost[i] ? group_item(A, ONE ? prefix : prefix_of(S, i), lead[i], row0[i], row1[i])
+      return cost[i] ? group_item(A, whole[i], lead[i], row0[i], row1[i])
                      : no_item();
     }
     const int b = i - Gr;
     const Req r = req(b);
     g = ONE ? mine : group_of(b);
-    if (g >= 0 && (!cost[g] || !(ONE || takes_part(A, r, prefix_of(S, g))))) g = -1;
-    return own_item(A, r, b, g >= 0 ? (ONE ? prefix : prefix_of(S, g)) : 0);
+    if (g >= 0 && (!cost[g] || !(ONE || takes_part(A, r, whole[g])))) g = -1;
+    return own_item(A, r, b, g >= 0 ? whole[g] : 0);
   };
   Item own = no_item();
   int own_g = -1;
@@ -644,10 +644,10 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
       sh[tid - Gr] = kept.q0;
       lens[tid - Gr] = kept.ql;
     }
-    if (tid == 0) sh[A.B] = A.q_start[A.B];
   } else {
-    for (int b = tid; b <= A.B; b += kPlanThr) sh[b] = A.q_start[b];
+    for (int b = tid; b < A.B; b += kPlanThr) sh[b] = A.q_start[b];
   }
+  if (tid == 0) sh[A.B] = rows_end;
   __syncthreads();
   for (int r = tid; r < A.rows; r += kPlanThr) {
     int lo = 0, hi = A.B;
@@ -1236,9 +1236,9 @@ extern "C" int qkv_kv8_attention_shared(
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (!S.small) {
     if (groups + B <= kPlanThr)
-      share_plan<true><<<1, kPlanThr, std::max(10 * groups + 1, 2 * B + 1) * sizeof(int32_t), s>>>(A, S);
+      share_plan<true><<<1, kPlanThr, std::max(11 * groups + 1, 2 * B + 1) * sizeof(int32_t), s>>>(A, S);
     else
-      share_plan<false><<<1, kPlanThr, std::max(6 * groups + 1, B + 1) * sizeof(int32_t), s>>>(A, S);
+      share_plan<false><<<1, kPlanThr, std::max(7 * groups + 1, B + 1) * sizeof(int32_t), s>>>(A, S);
     QKV_LAUNCHED();
   }
   // the second launch: a workgroup per tile that may be its own, and some that join the rest, few
