@@ -24,18 +24,18 @@
 // Measured (a call; attention_kv8 over the same tables): 60 rows of requests of up to 500 own tokens
 // behind 8192, 32 / 8 heads, d = 128, bf16: 39 us (95); behind 32,000 63 (331); 56 rows of six
 // groups, up to 5003 + 700, 24 / 8 heads, d = 96, e4m3: 28 (45); seven requests' 1131 rows behind
-// 16,001, 14 / 2 heads, d = 64, fp32 results: 143 (240); 256 requests of up to 300 behind 8192: 83.
+// 16,001, 14 / 2 heads, d = 64, fp32 results: 140 (240); 256 requests of up to 300 behind 8192: 83.
 // Of the first's 39: the plan 3.6 us (loads of the lengths, then some 1000 instructions of one
 // wave), a tile's place, queries and first codes 4.5, four rounds of 128 tokens 10.3 (prefill8's
 // loop, see there), halves' join and 16.8 MB of partial results 3.1, a gap of 3 between the
 // launches, and the second one 8 (13 the longest): own tokens' chain of lengths - page - codes -
-// results.  Many tall tiles are bound by that loop's issue: of the 1131 rows' 138 us the SIMDs spend
+// results.  Many tall tiles are bound by that loop's issue: of the 1131 rows' 133 us the SIMDs spend
 // 53 % on VALU work and 27 % on products (pairs of weights: 98 GFLOP).  Two workgroups a CU, which
 // d = 64 has LDS for, are slower (155 us: 45 registers spilled, and twice the partial results).
 //
 // Tried: the plan in a launch of its own (9 us, and a gap) with short tiles in the first launch
 // (a tile by one wave: 8 us each, one behind the other; 47 us in all); ranges that do not count
-// set-up (a range of 33 tiles of 5 steps: 272 us for the 143 above); in the second launch a word of
+// set-up (a range of 33 tiles of 5 steps: 272 us for the 140 above); in the second launch a word of
 // each line of a step's codes loaded a step before them (39.4 -> 40.5, six groups 29.1 -> 29.6).
 #include <algorithm>
 #include <atomic>
