@@ -856,9 +856,9 @@ int qkv_kv8_copy_pages(const int32_t* src, const int32_t* dst, const int32_t* to
  * steps of 64 of them are read from the first request of the group whose queries all
  * see them (causal: lie behind them).  Requests of a group that do not, such as idle
  * ones, go over their own tokens alone, as do those of no group.  The result is
- * qkv_kv8_attention's but for rounding; weights reach the value product in 11 bits for
- * bf16 results of 16-bit queries where a group, or a request, has more than 32 rows of a
- * kv head.  Where sharing costs more than it saves (short prefixes, requests of
+ * qkv_kv8_attention's but for rounding; weights reach the value product in 22 bits or,
+ * for bf16 results of 16-bit queries, those of requests of more than 32 rows (of a kv
+ * head) in 11, over the prefix where all requests that share it are such ones.  Where sharing costs more than it saves (short prefixes, requests of
  * many rows, small calls) each request goes over its own table's tokens; `always`
  * (0: not) shares whatever prefix two requests of a group see.
  *   rows        rows x Hq < 2^28

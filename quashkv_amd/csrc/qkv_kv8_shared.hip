@@ -66,6 +66,7 @@ struct Item {
   int32_t table;
   bool group;
   bool part;          // whether its rows have other items, too
+  bool pairs;         // whether some of its requests have weights of 22 bits (share8)
   __device__ __forceinline__ bool tall() const { return rows > kFew; }
   __device__ __forceinline__ bool late() const {
     return !group && rows > 0 && !tall() && steps <= kLate;
@@ -94,7 +95,7 @@ struct Frame {
 struct Places {
   int32_t* tall;      // [N + 1] places of tall tiles
   int32_t* fours;     // [N + 1] parts
-  int4* geo;          // two each: q0, ql (0: nothing to do), kv, s0; steps, 2 table + causal, slot, rows
+  int4* geo;          // two each: q0, ql (0: nothing to do), kv, s0; steps, 4 table + 2 pairs + causal, slot, rows
 };
 
 struct Share {
@@ -135,14 +136,15 @@ __device__ __forceinline__ int cost_of(int rows) {
 __device__ __forceinline__ bool pays(const Share& S, int members, int alone, int rows, int steps) {
   return members > 1 && (S.always || int64_t(alone) * steps > int64_t(cost_of(rows)) * (steps + 2 * kSetUp));
 }
-__device__ __forceinline__ Item no_item() { return Item{0, 0, 0, 0, 0, 0, 0, false, false}; }
+__device__ __forceinline__ Item no_item() { return Item{0, 0, 0, 0, 0, 0, 0, false, false, false}; }
 __device__ __forceinline__ Item own_item(const Att& A, const Req& r, int b, int prefix) {
   const int s0 = prefix / kStep, rows = rows_of(A, r) * A.G;
-  return Item{r.q0, r.ql, r.kv, s0, max(1, steps_of(r.kv) - s0), rows, b, false, prefix > 0};
+  return Item{r.q0, r.ql, r.kv, s0, max(1, steps_of(r.kv) - s0), rows, b, false, prefix > 0, false};
 }
-__device__ __forceinline__ Item group_item(const Att& A, int prefix, int lead, int row0, int row1) {
+__device__ __forceinline__ Item group_item(const Att& A, int prefix, int lead, int row0, int row1,
+                                           bool pairs) {
   const int ql = max(row1 - row0, 0);
-  return Item{row0, ql, prefix, 0, prefix / kStep, ql * A.G, lead, true, true};
+  return Item{row0, ql, prefix, 0, prefix / kStep, ql * A.G, lead, true, true, pairs};
 }
 
 __device__ __forceinline__ int div_up(int a, int b) {
@@ -249,7 +251,7 @@ __device__ __forceinline__ void put_item(const Places& P, int i, const Item& it,
   P.tall[i] = tall;
   P.fours[i] = fours;
   P.geo[2 * i] = make_int4(it.q0, fits ? it.ql : 0, it.kv, it.s0);
-  P.geo[2 * i + 1] = make_int4(it.steps, 2 * it.table + causal,
+  P.geo[2 * i + 1] = make_int4(it.steps, 4 * it.table + 2 * it.pairs + causal,
                                slots > 0 ? static_cast<int>(slot) : -1, it.rows);
 }
 // What the second launch needs of request b: own, group: its items' joins; q0: the group's first
@@ -324,7 +326,8 @@ __device__ __forceinline__ Frame plan_wave(const Att& A, const Share& S, const P
   const int cost = in ? cost_of(rows * A.G) : 0, costs = wave_scan(cost);
   const int row0 = __shfl(r.q0, first, 64), row1 = __shfl(r.q0 + rows, last, 64);
   const int alone = __shfl(costs, last, 64) - __shfl(costs - cost, first, 64);
-  Item it[2] = {group_item(A, prefix, first, row0, row1), no_item()};  // the lane's group, its request
+  const bool pairs = (__ballot(rows * A.G <= kFew) & mine) != 0;
+  Item it[2] = {group_item(A, prefix, first, row0, row1, pairs), no_item()};  // the lane's group, its request
   const bool does = mine != 0 && pays(S, __popcll(mine), alone, it[0].rows, it[0].steps);
   if (!does) it[0] = no_item();
   const uint64_t sharing = __ballot(does);
@@ -450,6 +453,7 @@ __device__ __forceinline__ float row_scan(float v) {
 // The same of more requests or groups, by a workgroup, into the workspace.  ONE: a thread has
 // one item, and keeps it.  (Up to 256 requests by plan_wave, four a lane: 3 us less a call at 96 to 200
 // requests, none at 256, and 0.4 to 0.8 more for those up to 64, whose plan shares the code.)
+constexpr int32_t kPairs = 1 << 30;
 template <bool ONE>
 __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
   extern __shared__ __align__(16) int32_t sh[];
@@ -458,7 +462,7 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
   int4* const joins = reinterpret_cast<int4*>(sh);  // ONE: [Gr]
   int32_t* const start = sh + (ONE ? 4 * Gr : 0);   // [Gr + 1]
   int32_t* const lead = start + Gr + 1; // [Gr]: the first request that takes part,
-  int32_t* const many = lead + Gr;      // how many do,
+  int32_t* const many = lead + Gr;      // how many do, and kPairs where one has few rows,
   int32_t* const row0 = many + Gr;      // their first row and the end of their last one,
   int32_t* const row1 = row0 + Gr;
   int32_t* const cost = row1 + Gr;      // and what they cost alone; then whether they share
@@ -504,19 +508,20 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
     mine = g;
     atomicMin(&lead[g], b);
     atomicAdd(&many[g], 1);
+    if (rows_of(A, r) * A.G <= kFew) atomicOr(&many[g], kPairs);
     atomicAdd(&cost[g], cost_of(rows_of(A, r) * A.G));
     atomicMin(&row0[g], r.q0);
     atomicMax(&row1[g], r.q0 + rows_of(A, r));
   });
   __syncthreads();
   each(0, Gr, [&](int g) {
-    cost[g] = pays(S, many[g], cost[g], max(row1[g] - row0[g], 0) * A.G, whole[g] / kStep);
+    cost[g] = pays(S, many[g] & ~kPairs, cost[g], max(row1[g] - row0[g], 0) * A.G, whole[g] / kStep);
   });
   __syncthreads();
   auto make = [&](int i, int& g) {
     if (i < Gr) {
       g = i;
-      return cost[i] ? group_item(A, whole[i], lead[i], row0[i], row1[i])
+      return cost[i] ? group_item(A, whole[i], lead[i], row0[i], row1[i], (many[i] & kPairs) != 0)
                      : no_item();
     }
     const int b = i - Gr;
@@ -699,6 +704,10 @@ __device__ __forceinline__ int thread_anew() {
 
 // Workgroup (j, h), j < target: the j-th range of kv head h's tall tiles, where there is one, then
 // short tiles, two at a time, in turn with the other workgroups that take these.
+//
+// Weights are f16 pairs (22 bits) but, without PLO (bf16 results of 16-bit queries), those of
+// requests of more than kFew rows, of which qkv_kv8_attention's result has 11 bits, too: their own
+// tall tiles', and the prefix' where no request of fewer rows shares it.
 template <int D, bool FP8, bool QLO, bool PLO>
 __global__ __launch_bounds__(kPreThr, 2) void share8(Args) {
   __shared__ v4f sbuf[2][2][4];
@@ -735,7 +744,7 @@ __global__ __launch_bounds__(kPreThr, 2) void share8(Args) {
     }
     return i;
   };
-  auto piece = [&](const Share& S, int i, int& s0, int& steps, int& rows) {
+  auto piece = [&](const Share& S, int i, int& s0, int& steps, int& rows, bool& pairs) {
     int4 x, y;
     if (S.small) {
       x = sh_geo[2 * i];
@@ -748,7 +757,8 @@ __global__ __launch_bounds__(kPreThr, 2) void share8(Args) {
     P.r = Req{same(x.x), same(x.y), same(x.z)};
     s0 = same(x.w);
     steps = same(y.x);
-    P.b = same(y.y) >> 1;
+    P.b = same(y.y) >> 2;
+    pairs = same(y.y) & 2;
     P.causal = same(y.y) & 1;
     P.slot = same(y.z);
     rows = same(y.w);
@@ -767,7 +777,8 @@ __global__ __launch_bounds__(kPreThr, 2) void share8(Args) {
     if (x >= end) break;
     int first, s0, steps, rows;
     const int i = find(C.s, items, sh_tall, C.s.at.tall, x, first);
-    Piece P = piece(C.s, i, s0, steps, rows);
+    bool pairs;
+    Piece P = piece(C.s, i, s0, steps, rows, pairs);
     const int E = extent(F, steps), p = (x - first) / E, in = x - first - p * E;
     const int n = min(E - in, end - x);
     if (threadIdx.x == 0) sh_x = x + n;
@@ -783,7 +794,8 @@ __global__ __launch_bounds__(kPreThr, 2) void share8(Args) {
         parts_at(F, steps, x - in - k * F.range, none);
         P.slot += (j - k - none) * rows;
       }
-      prefill_piece<D, FP8, QLO, PLO, true>(C.a, P, h, thread_anew(), lds, sbuf);
+      if (PLO || pairs) prefill_piece<D, FP8, QLO, true, true>(C.a, P, h, thread_anew(), lds, sbuf);
+      else prefill_piece<D, FP8, QLO, false, true>(C.a, P, h, thread_anew(), lds, sbuf);
     }
     __syncthreads();
   }
@@ -807,7 +819,8 @@ __global__ __launch_bounds__(kPreThr, 2) void share8(Args) {
     if (k < same(sh_frame.fours)) {
       int first, s0, steps, rows;
       const int i = find(C.s, items, sh_fours, C.s.at.fours, k, first);
-      P = piece(C.s, i, s0, steps, rows);
+      bool pairs;
+      P = piece(C.s, i, s0, steps, rows, pairs);
       const int least = same(sh_frame.least), parts = (steps + least - 1) / least;
       const int in = k - first;
       P.rt = in / parts;

@@ -457,9 +457,9 @@ def attention_kv8_shared(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Ten
     all of their own tokens, and so do all where sharing would cost more than it saves (short
     prefixes, requests of many rows, small calls), unless ``always`` is set.
 
-    The other arguments and the result are attention_kv8's (but for rounding; weights
-    reach the value product in 11 bits, for bf16 results of 16-bit queries, where a group
-    or a request has more than 32 rows of a kv head).  ``workspace`` (uint8,
+    The other arguments and the result are attention_kv8's but for rounding.  (For bf16 results of
+    16-bit queries the weights of requests of more than 32 rows of a kv head have 11 bits, over
+    the prefix where all requests that share it are such ones; all others 22.)  ``workspace`` (uint8,
     :func:`attention_kv8_shared_workspace_bytes`) must belong to one call at a time."""
     dev = _one_device("attention_kv8_shared", q, kpool, kscale, vpool, vscale, table, kv_lens,
                       group_start, prefix_lens, q_start, q_lens, out, workspace)
