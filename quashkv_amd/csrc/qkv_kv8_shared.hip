@@ -41,6 +41,7 @@
 #include <atomic>
 
 #include "qkv_kv8_decode.h"
+#include "qkv_kv8_frame.h"
 #include "qkv_kv8_prefill.h"
 #include "qkv_pages_dev.h"
 
@@ -53,11 +54,6 @@ constexpr int kLate = 16;       // own steps of few rows that are left to the se
 constexpr int kMaxGroups = 2048;
 constexpr int kSmall = 64;      // requests, and groups, up to which every workgroup plans for itself
 constexpr int kItems = 2 * kSmall;
-// Set-up and end of a tall tile, in its steps (0.8 us at d = 128), and the least that a range
-// takes of one; a step of a short tile; places of a kv head's tall tiles, at most.
-constexpr int kSetUp = 8, kCut = 2;
-constexpr float kShortStep = 0.5f;
-constexpr float kMostPlaces = 0x1p30f;
 
 // Rows of a request, or of a group, over steps [s0, s0 + steps) of request `table`'s tokens.
 struct Item {
@@ -75,19 +71,6 @@ struct Item {
   __device__ __forceinline__ int tiles() const {
     return tall() ? (rows + kPreRows - 1) / kPreRows : (rows + kRows - 1) / kRows;
   }
-};
-
-// How a kv head's work is divided: its tall tiles have places, one behind the other, which are cut
-// into ranges.  Where tiles are few and long each has whole ranges (aligned); else a tile has
-// its steps and `setup` more, so that a range of many short tiles is no longer than one of a
-// part of a long one.
-struct Frame {
-  int32_t range;      // places of a range
-  int32_t tall;       // ranges
-  int32_t setup;      // -1: aligned
-  int32_t least;      // steps of a part of a short tile
-  int32_t fours;      // parts of short tiles
-  int32_t lates;      // tiles of the second launch
 };
 
 // Where items lie: for N items (groups, then requests) the sums before each, and what pieces need.
@@ -145,64 +128,6 @@ __device__ __forceinline__ Item group_item(const Att& A, int prefix, int lead, i
                                            bool pairs) {
   const int ql = max(row1 - row0, 0);
   return Item{row0, ql, prefix, 0, prefix / kStep, ql * A.G, lead, true, true, pairs};
-}
-
-__device__ __forceinline__ int div_up(int a, int b) {
-  return static_cast<int>((static_cast<uint32_t>(a) + b - 1) / static_cast<uint32_t>(b));
-}
-__device__ __forceinline__ int extent(const Frame& F, int steps) {
-  return F.setup < 0 ? div_up(steps, F.range) * F.range : steps + F.setup;
-}
-
-// steps, tiles, fours: sums over the items of tall tiles' steps, their number, and short tiles'
-// steps; count(R): of the tall tiles' parts if each were cut into R steps by itself.
-template <typename Count>
-__device__ __forceinline__ Frame frame_of(const Att& A, float steps, float tiles, float fours,
-                                          Count count) {
-  Frame F{1, 0, 0, 0, 0, 0};
-  const float few = kShortStep * fours, all = (steps + few) * A.per_target + kSetUp;
-  if (steps > 0.f && steps + kSetUp * tiles < kMostPlaces) {
-    int n = A.target - static_cast<int>(few / all + 0.5f);
-    if (few > 0.f && n == A.target) --n;
-    n = max(n, 1);
-    // (the sums are whole numbers, exact below 2^24, and what is added to them then is little)
-    const float each = steps / static_cast<float>(n);
-    F.setup = static_cast<int>(fminf(0.25f * each, static_cast<float>(kSetUp))) & ~1;
-    F.range = max(static_cast<int>((steps + tiles * F.setup) / static_cast<float>(n)) + 1, 4);
-    // aligned: the shortest parts, as near as eighths, that are no more than n; then a range has
-    // one set-up, where else one that spans tiles has two
-    int R = max((static_cast<int>(ceilf(each)) + 1) & ~1, 4), parts = 0;
-#pragma unroll 1
-    for (int k = 0; k < 8; ++k) {
-      if (R > F.range + kSetUp) break;
-      parts = count(R);
-      if (parts <= n) break;
-      R += max(2, (R / 8) & ~1);
-    }
-    if (parts <= n && R <= F.range + kSetUp) {
-      F.range = R;
-      F.setup = -1;
-    }
-  }
-  F.least = static_cast<int>(fminf(all, 1e9f)) / kWaves * kWaves + kWaves;
-  return F;
-}
-
-// The step of a tall tile of `steps` at which a range that ends at place p of it cuts it: not next
-// to its ends, and between rounds of two steps.
-__device__ __forceinline__ int cut_at(const Frame& F, int steps, int p) {
-  if (F.setup < 0) return min(p, steps);
-  const int s = p - F.setup;
-  return s < kCut ? 0 : steps - s < kCut ? steps : s & ~1;
-}
-// Of a tile whose places begin at place a of a range: the parts that it is in, and the ranges from
-// that one on that have no step of it.
-__device__ __forceinline__ int parts_at(const Frame& F, int steps, int a, int& none) {
-  none = 0;
-  if (F.setup < 0) return div_up(steps, F.range);
-  const int E = steps + F.setup, R = F.range, ends = (a + E - 1) / R;
-  none = min(ends, (F.setup + kCut - 1 + a) / R);
-  return ends + 1 - none - (ends > none && ends * R - a > E - kCut);
 }
 
 // Parts that an item's tile is cut into at most, and its partial rows.
@@ -347,7 +272,7 @@ __device__ __forceinline__ Frame plan_wave(const Att& A, const Share& S, const P
     return on ? static_cast<float>(x.tiles()) * static_cast<float>(x.steps) : 0.f;
   };
   Frame F = frame_of(
-      A, total([&](const Item& x) { return steps_as(x, x.tall()); }),
+      A.target, A.per_target, total([&](const Item& x) { return steps_as(x, x.tall()); }),
       total([](const Item& x) { return x.tall() ? static_cast<float>(x.tiles()) : 0.f; }),
       total([&](const Item& x) { return steps_as(x, x.four()); }),
       [&](int R) {
@@ -358,7 +283,7 @@ __device__ __forceinline__ Frame plan_wave(const Att& A, const Share& S, const P
     tall_all = before([&](const Item& x) {
       return x.tall() ? x.tiles() * extent(F, x.steps) : 0;
     }, tall);
-    F.tall = div_up(tall_all, F.range);
+    fit_ranges(F, tall_all);
   }
   if (__any(it[0].four() || it[1].four()))
     F.fours = before([&](const Item& x) { return x.four() ? x.tiles() * most_parts(x, F) : 0; },
@@ -560,7 +485,7 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
 #pragma unroll
     for (int k = 0; k < 3; ++k) sum[k] = lane_value(v, kW * k + kW - 1);
   }
-  Frame F = frame_of(A, sum[0], sum[1], sum[2], [&](int R) {
+  Frame F = frame_of(A.target, A.per_target, sum[0], sum[1], sum[2], [&](int R) {
     int64_t n = 0, all;
     each(0, items, [&](int i) {
       int g;
@@ -580,7 +505,7 @@ __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
       if (it.tall()) n += int64_t(it.tiles()) * extent(F, it.steps);
     });
     block_sums<1>(&n, part, &all);
-    F.tall = div_up(static_cast<int>(all), F.range);
+    fit_ranges(F, static_cast<int>(all));
   }
   const int4 none = make_int4(0, 0, 0, 0);
   int4 join = none;
