@@ -860,8 +860,11 @@ int qkv_kv8_copy_pages(const int32_t* src, const int32_t* dst, const int32_t* to
  * for bf16 results of 16-bit queries, those of requests of more than 32 rows (of a kv
  * head) in 11, over the prefix where all requests that share it are such ones.  Where sharing costs more than it saves (short prefixes, requests of
  * many rows, small calls) each request goes over its own table's tokens; `always`
- * (0: not) shares whatever prefix two requests of a group see.
- *   rows        rows x Hq < 2^28
+ * (0: not) shares whatever prefix two requests of a group see.  Calls over so wide a table that
+ * (rows x Hq / Hkv / 64 + B + groups) x (tokens that the table has room for, of a request) / 64
+ * comes to about 2^30 are qkv_kv8_attention's, or refused where `always` is set.
+ *   rows        rows x Hq < 2^28, and the smaller one of 2 min(B, rows) and
+ *               rows x Hq / Hkv / 16 + min(B, rows), times Hkv, < 2^23
  *   workspace   qkv_kv8_attention_shared_workspace_bytes(...) bytes, 256-byte aligned,
  *               of this call alone until it has run; nothing in it need be set */
 int64_t qkv_kv8_attention_shared_workspace_bytes(int32_t B, int32_t groups, int64_t rows,

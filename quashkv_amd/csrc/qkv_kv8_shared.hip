@@ -1061,6 +1061,13 @@ constexpr double kLittle = 192e6;
 bool little(int64_t B, int64_t rows, int32_t G, int32_t H, int32_t d, int64_t width, int32_t page) {
   return rows * G <= kFew * B && double(B) * width * page * H * 2 * d <= kLittle;
 }
+// Calls whose tall tiles' places, were every request as long as the table is wide, are more than a
+// plan counts: they go there, too.
+bool too_wide(int64_t B, int64_t groups, int64_t rows, int32_t G, int64_t width, int32_t page) {
+  const double tiles = 2.0 * rows * G / kPreRows + std::min<double>(B + groups, 2.0 * rows * G / kFew);
+  const double longest = std::min(double(width) * page, double(QKV_PAGED_TOKENS)) / kStep;
+  return tiles * (longest + 1 + kSetUp) >= kMostPlaces;
+}
 // The longest request's rows for that call, as far as their number tells (a hint)
 int64_t longest_of(int64_t B, int64_t rows, int32_t G) {
   return rows > 2 * B ? rows : std::max<int64_t>(1, kFew / G);
@@ -1112,15 +1119,13 @@ extern "C" int qkv_kv8_attention_shared(
   const int64_t need = qkv_kv8_attention_shared_workspace_bytes(B, groups, rows, Hq, Hkv, d);
   QKV_REQUIRE(workspace && qkv_aligned(workspace, 256) && ws_bytes >= need,
               "qkv_kv8_attention_shared: workspace too small or not 256-byte aligned");
-  if (!always && little(B, rows, G, Hkv, d, pages_per_seq, page_tokens))
+  const bool wide = too_wide(B, groups, rows, G, pages_per_seq, page_tokens);
+  if (!always && (wide || little(B, rows, G, Hkv, d, pages_per_seq, page_tokens)))
     return qkv_kv8_attention(q, q_dtype, q_row_stride, q_head_stride, rows, kpool, kscale, vpool,
                              vscale, fmt, num_pages, page_tokens, table, pages_per_seq, q_start,
                              q_lens, kv_lens, B, Hq, Hkv, d, longest_of(B, rows, G), scale, causal,
                              out, out_dtype, workspace, ws_bytes, stream);
-  // places of tall tiles, were every request as long as the table is wide
-  const double tiles = 2.0 * rows * G / kPreRows + std::min<double>(B + groups, 2.0 * rows * G / kFew);
-  const double longest = std::min(double(pages_per_seq) * page_tokens, double(QKV_PAGED_TOKENS)) / kStep;
-  QKV_REQUIRE(tiles * (longest + 1 + kSetUp) < kMostPlaces && L.rows < INT32_MAX &&
+  QKV_REQUIRE(!wide && L.rows < INT32_MAX &&
                   L.late * Hkv < (1 << 23),  // (a launch has fewer than 2^32 threads)
               "%lld rows of %d query heads a kv head over a table of %d pages are too large for one "
               "call", static_cast<long long>(rows), G, pages_per_seq);

@@ -457,6 +457,10 @@ def attention_kv8_shared(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Ten
     all of their own tokens, and so do all where sharing would cost more than it saves (short
     prefixes, requests of many rows, small calls), unless ``always`` is set.
 
+    Calls of 2^28 rows times query heads, or of 2^22 requests times kv heads, are refused.  So
+    are, with ``always``, those over a table with room for so many tokens a request that times
+    B + groups + rows * Hq / H / 64 they are about 2^36; without, they are attention_kv8's.
+
     The other arguments and the result are attention_kv8's but for rounding.  (For bf16 results of
     16-bit queries the weights of requests of more than 32 rows of a kv head have 11 bits, over
     the prefix where all requests that share it are such ones; all others 22.)  ``workspace`` (uint8,

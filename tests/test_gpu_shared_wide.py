@@ -1,0 +1,52 @@
+"""attention_kv8_shared under tables of room for more tokens than its plan counts places for: the
+call is attention_kv8's, and refused where it has to share."""
+
+import pytest
+import torch
+
+from quashkv_amd import _native as N
+from quashkv_amd import paged8 as P8
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a HIP device")
+    N.lib()
+
+
+@pytest.mark.parametrize("q_lens,causal", [([40] * 30, True), ([1] * 29 + [1200], True),
+                                           ([0] * 10 + [60] * 20, False)])
+def test_wide_tables(q_lens, causal):
+    """30 requests, each with a row of 2^20 table entries (2^31 tokens)."""
+    B, H, G, d, pt, W = 30, 2, 4, 64, 2048, 1 << 20
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    P = 2 + B
+    pools = dict(
+        kpool=torch.randint(-127, 128, (P, H, pt, d), generator=gen, device=DEV).to(torch.int8),
+        vpool=torch.randint(-127, 128, (P, H, pt // 16, d, 16), generator=gen, device=DEV).to(torch.int8),
+        kscale=0.01 * torch.rand(P, H, pt // 16, generator=gen, device=DEV) + 1e-4,
+        vscale=0.01 * torch.rand(P, H, pt // 16, generator=gen, device=DEV) + 1e-4)
+    table = torch.zeros(B, W, dtype=torch.int32, device=DEV)
+    table[:, 1] = 1
+    table[:, 2] = torch.arange(2, 2 + B, device=DEV)
+    start = torch.tensor([0] + q_lens, device=DEV).cumsum(0).int()
+    rows = sum(q_lens)
+    lens = torch.arange(4096 + 1200, 4096 + 1200 + B, dtype=torch.int32, device=DEV)
+    q = torch.randn(rows + 2, H * G, d, generator=gen, device=DEV)
+    args = dict(q=q, **pools, table=table, kv_lens=lens, q_start=start, causal=causal,
+                q_lens=torch.tensor(q_lens, dtype=torch.int32, device=DEV))
+    groups = dict(group_start=torch.tensor([0, B], dtype=torch.int32, device=DEV),
+                  prefix_lens=torch.tensor([4096], dtype=torch.int32, device=DEV))
+    x = P8.attention_kv8_shared(**args, **groups)
+    y = P8.attention_kv8(**args)
+    assert torch.equal(x, y) and not x[rows:].any() and x[:rows].abs().amax() > 0
+    with pytest.raises(ValueError, match="too large"):
+        P8.attention_kv8_shared(**args, **groups, always=True)
+    # as wide as the requests are: within 22-bit weights and fp32 sums over 5300 tokens, values up to 1.3
+    z = P8.attention_kv8_shared(**{**args, "table": table[:, :3].contiguous()}, **groups, always=True)
+    assert float((x - z).abs().max()) <= 4 * 1.3 * (2.0 ** -18 + 300 * 2.0 ** -24)
