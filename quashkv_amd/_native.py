@@ -141,6 +141,7 @@ _SIGS = {
     "qkv_kv8_copy_pages": (_i32, [_p, _p, _p, _i32, _p, _i32, _i32, _i32, _p, _p, _p, _p, _i32,
                                   _i32, _p]),
     "qkv_kv8_attention_shared_workspace_bytes": (_i64, [_i32, _i32, _i64, _i32, _i32, _i32]),
+    "qkv_kv8_attention_shared_plain": (_i64, [_i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32]),
     "qkv_kv8_attention_shared": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p, _p, _p, _i32, _i32,
                                         _i32, _p, _i32, _p, _p, _i32, _i32, _p, _p, _p, _i32,
                                         _i32, _i32, _i32, _f32, _i32, _p, _i32, _p, _i64, _p]),

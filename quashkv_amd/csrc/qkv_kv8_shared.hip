@@ -1068,7 +1068,8 @@ bool too_wide(int64_t B, int64_t groups, int64_t rows, int32_t G, int64_t width,
   const double longest = std::min(double(width) * page, double(QKV_PAGED_TOKENS)) / kStep;
   return tiles * (longest + 1 + kSetUp) >= kMostPlaces;
 }
-// The longest request's rows for that call, as far as their number tells (a hint)
+// The longest request's rows for that call, as far as their number tells (a hint; a caller who knows
+// a bound of them, of a batch with padding rows, say, makes that call himself)
 int64_t longest_of(int64_t B, int64_t rows, int32_t G) {
   return rows > 2 * B ? rows : std::max<int64_t>(1, kFew / G);
 }
@@ -1082,6 +1083,18 @@ extern "C" int64_t qkv_kv8_attention_shared_workspace_bytes(int32_t B, int32_t g
   const int32_t G = Hq / Hkv;
   return std::max(layout(B, std::max(groups, 0), rows, G, Hkv, d).bytes,
                   qkv_kv8_attention_workspace_bytes(B, rows, Hq, Hkv, d, longest_of(B, rows, G)));
+}
+
+extern "C" int64_t qkv_kv8_attention_shared_plain(int32_t B, int32_t groups, int64_t rows, int32_t Hq,
+                                                  int32_t Hkv, int32_t d, int32_t pages_per_seq,
+                                                  int32_t page_tokens) {
+  if (B < 1 || B > kMaxB || groups < 0 || groups > kMaxGroups || rows < 1 || Hkv < 1 || Hq < Hkv ||
+      rows * Hq >= (1 << 28))
+    return 0;  // (nothing to do, or refused)
+  const int32_t G = Hq / Hkv;
+  return too_wide(B, groups, rows, G, pages_per_seq, page_tokens) ||
+                 little(B, rows, G, Hkv, d, pages_per_seq, page_tokens)
+             ? longest_of(B, rows, G) : 0;
 }
 
 extern "C" int qkv_kv8_attention_shared(

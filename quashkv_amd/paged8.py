@@ -444,8 +444,8 @@ def attention_kv8_shared(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Ten
                          q_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                          causal: bool = False, out_dtype: torch.dtype = torch.float32,
                          out: Optional[torch.Tensor] = None,
-                         workspace: Optional[torch.Tensor] = None,
-                         always: bool = False) -> torch.Tensor:
+                         workspace: Optional[torch.Tensor] = None, always: bool = False,
+                         max_q_len: Optional[int] = None) -> torch.Tensor:
     """:func:`attention_kv8` of a batch in groups whose requests share a prefix, which is
     read once for all rows of a group.
 
@@ -459,7 +459,8 @@ def attention_kv8_shared(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Ten
 
     Calls of 2^28 rows times query heads, or of 2^22 requests times kv heads, are refused.  So
     are, with ``always``, those over a table with room for so many tokens a request that times
-    B + groups + rows * Hq / H / 64 they are about 2^36; without, they are attention_kv8's.
+    B + groups + rows * Hq / H / 64 they are about 2^36; without, they are attention_kv8's,
+    as small calls are: ``max_q_len``, the longest request's rows, is for both.
 
     The other arguments and the result are attention_kv8's but for rounding.  (For bf16 results of
     16-bit queries the weights of requests of more than 32 rows of a kv head have 11 bits, over
@@ -487,6 +488,14 @@ def attention_kv8_shared(q: torch.Tensor, kpool: torch.Tensor, kscale: torch.Ten
     else:
         _want(workspace, "workspace", torch.uint8)
         nbytes = workspace.numel()
+    if (max_q_len is not None and not always
+            and max_q_len < _shared_plain(B, groups, rows, Hq, H, d, width, n)):
+        _call(dev, N.lib().qkv_kv8_attention, q.data_ptr(), N.dtype_code(q.dtype), ts, hs, rows,
+              kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(), vscale.data_ptr(), fmt, P, n,
+              table.data_ptr(), width, N.ptr(q_start), N.ptr(q_lens), kv_lens.data_ptr(), B, Hq, H,
+              d, max(0, int(max_q_len)), float(scale), 1 if causal else 0, out.data_ptr(),
+              N.dtype_code(out.dtype), workspace.data_ptr(), nbytes)
+        return out
     _call(dev, N.lib().qkv_kv8_attention_shared, q.data_ptr(), N.dtype_code(q.dtype), ts, hs, rows,
           kpool.data_ptr(), kscale.data_ptr(), vpool.data_ptr(), vscale.data_ptr(), fmt, P, n,
           table.data_ptr(), width, group_start.data_ptr(), prefix_lens.data_ptr(), groups,
@@ -501,6 +510,12 @@ def attention_kv8_shared_workspace_bytes(B: int, groups: int, rows: int, Hq: int
                                          d: int) -> int:
     """Bytes of the workspace that attention_kv8_shared needs at these sizes."""
     return N.lib().qkv_kv8_attention_shared_workspace_bytes(B, groups, rows, Hq, H, d)
+
+
+@functools.lru_cache(maxsize=256)
+def _shared_plain(B: int, groups: int, rows: int, Hq: int, H: int, d: int, width: int,
+                  page_tokens: int) -> int:
+    return N.lib().qkv_kv8_attention_shared_plain(B, groups, rows, Hq, H, d, width, page_tokens)
 
 
 class PagedKV8Store:
@@ -594,7 +609,8 @@ class PagedKV8Store:
             return attention_kv8_shared(q, **self.pools(), table=self.table, kv_lens=plan.kv_lens,
                                         group_start=groups[0], prefix_lens=groups[1],
                                         q_start=plan.q_start, q_lens=plan.q_lens, scale=scale,
-                                        causal=causal, out_dtype=out_dtype, out=out)
+                                        causal=causal, out_dtype=out_dtype, out=out,
+                                        max_q_len=plan.max_q_len)
         return attention_kv8(q, **self.pools(), table=self.table, kv_lens=plan.kv_lens,
                              q_start=plan.q_start, q_lens=plan.q_lens, scale=scale, causal=causal,
                              out_dtype=out_dtype, max_q_len=plan.max_q_len, out=out)

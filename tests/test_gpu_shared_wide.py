@@ -50,3 +50,39 @@ def test_wide_tables(q_lens, causal):
     # as wide as the requests are: within 22-bit weights and fp32 sums over 5300 tokens, values up to 1.3
     z = P8.attention_kv8_shared(**{**args, "table": table[:, :3].contiguous()}, **groups, always=True)
     assert float((x - z).abs().max()) <= 4 * 1.3 * (2.0 ** -18 + 300 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("rows,max_q_len,told", [(16, 1, 1), (40, 1, 1), (40, 0, 0), (40, 39, 39),
+                                                 (40, None, 40), (40, 64, 40), (16, None, 8)])
+def test_small_calls_are_told_the_longest(monkeypatch, rows, max_q_len, told):
+    """A decode batch with padding rows: what a plan knows of the longest request's rows reaches
+    attention_kv8, which else goes by a guess."""
+    B, H, G, d = 16, 2, 4, 64
+    st = P8.PagedKV8Store(B, H, d, 64, DEV, page_tokens=64, pages_per_seq=4)
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    k, v = torch.randn(2, B * 70, H, d, generator=gen, device=DEV)
+    st.append(k, v, st.plan(torch.full((B,), 70, dtype=torch.int32, device=DEV), B * 70))
+    plan = st.plan(torch.zeros(B, dtype=torch.int32, device=DEV), rows, max_q_len=max_q_len)
+    plan.q_start.copy_(torch.arange(B + 1, device=DEV))
+    plan.q_lens.fill_(1)
+    q = torch.randn(rows, H * G, d, generator=gen, device=DEV)
+    groups = tuple(torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, B], [64]))
+    calls = []
+    real = P8._call
+    monkeypatch.setattr(P8, "_call", lambda dev, fn, *a: (calls.append((fn.__name__, a)), real(dev, fn, *a)))
+    x = st.attention(q, plan, groups=groups)
+    monkeypatch.undo()
+    (name, args), = calls
+    guess = N.lib().qkv_kv8_attention_shared_plain(B, 1, rows, H * G, H, d, 4, 64)
+    if told < guess:
+        assert name == "qkv_kv8_attention" and args[21] == told
+    else:
+        assert name == "qkv_kv8_attention_shared" and told == guess
+    y = P8.attention_kv8(q, **st.pools(), table=st.table, kv_lens=plan.kv_lens, q_start=plan.q_start,
+                         q_lens=plan.q_lens, causal=True, max_q_len=told)
+    assert torch.equal(x, y)
+    with pytest.raises(ValueError, match="workspace"):
+        P8.attention_kv8_shared(q, **st.pools(), table=st.table, kv_lens=plan.kv_lens,
+                                group_start=groups[0], prefix_lens=groups[1], q_start=plan.q_start,
+                                max_q_len=1,
+                                workspace=torch.zeros(64, dtype=torch.uint8, device=DEV))
