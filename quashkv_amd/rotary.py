@@ -89,6 +89,28 @@ def _out(x: torch.Tensor, shape: torch.Size, out: torch.Tensor, what: str) -> tu
     return ts, hs
 
 
+class _Rotary(torch.autograd.Function):
+    """rotary with its gradient: the same rows' map by the negative angles."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, turns, factor, interleaved, inverse):
+        ctx.set_materialize_grads(False)
+        # (a plan's positions are the next step's before a backward pass asks for them)
+        ctx.save_for_backward(positions.clone(), turns)
+        ctx.args = factor, interleaved, not inverse
+        return rotary(q, k, positions, turns, factor, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, turns = ctx.saved_tensors
+        dq, dk = (g if need else None for g, need in zip((dq, dk), ctx.needs_input_grad))
+        if dq is None and dk is not None:
+            dk, _ = rotary(dk, None, positions, turns, *ctx.args)
+        elif dq is not None:
+            dq, dk = rotary(dq, dk, positions, turns, *ctx.args)
+        return dq, dk, None, None, None, None, None
+
+
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
            turns: torch.Tensor, factor: float = 1.0, interleaved: bool = False,
            inverse: bool = False, q_out: Optional[torch.Tensor] = None,
@@ -101,7 +123,16 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
 
     ``inverse``: by the negative angles, times ``factor`` all the same: the gradient of a
     call, and where factor is 1 what undoes it.  ``q_out`` / ``k_out`` may be q / k
-    themselves, but not overlap them otherwise."""
+    themselves, but not overlap them otherwise.
+
+    Autograd goes through results that the call makes; with ``q_out`` or ``k_out`` none of the
+    tensors may require a gradient (but under torch.no_grad())."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (q, k, q_out, k_out)):
+        if q_out is not None or k_out is not None:
+            raise ValueError("q_out and k_out take no gradients, and a tensor of the call "
+                             "requires one: leave them out, or call it under torch.no_grad()")
+        return _Rotary.apply(q, k, positions, turns, factor, interleaved, inverse)
     dev = _one_device("rotary", q, k, positions, turns, q_out, k_out)
     shape, dtype = q.shape, q.dtype
     if len(shape) != 3:
