@@ -127,8 +127,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
 
     Autograd goes through results that the call makes; with ``q_out`` or ``k_out`` none of the
     tensors may require a gradient (but under torch.no_grad())."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (q, k, q_out, k_out)):
+    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad
+                                    or q_out is not None and q_out.requires_grad
+                                    or k_out is not None and k_out.requires_grad):
         if q_out is not None or k_out is not None:
             raise ValueError("q_out and k_out take no gradients, and a tensor of the call "
                              "requires one: leave them out, or call it under torch.no_grad()")
