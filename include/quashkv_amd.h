@@ -859,7 +859,8 @@ int qkv_kv8_copy_pages(const int32_t* src, const int32_t* dst, const int32_t* to
  * qkv_kv8_attention's but for rounding; weights reach the value product in 22 bits or,
  * for bf16 results of 16-bit queries, those of requests of more than 32 rows (of a kv
  * head) in 11, over the prefix where all requests that share it are such ones.  Where sharing costs more than it saves (short prefixes, requests of
- * many rows, small calls) each request goes over its own table's tokens; `always`
+ * many rows, small calls) each request goes over its own table's tokens (what is small
+ * goes by the table's width, the rest by the lengths); `always`
  * (0: not) shares whatever prefix two requests of a group see.  Calls over so wide a table that
  * (rows x Hq / Hkv / 64 + B + groups) x (tokens that the table has room for, of a request) / 64
  * comes to about 2^30 are qkv_kv8_attention's, or refused where `always` is set.

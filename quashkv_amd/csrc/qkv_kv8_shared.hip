@@ -22,14 +22,15 @@
 // goes, and joins whatever else was cut.
 //
 // Measured (a call; attention_kv8 over the same tables): 60 rows of requests of up to 500 own tokens
-// behind 8192, 32 / 8 heads, d = 128, bf16: 39 us (95); behind 32,000 63 (331); 56 rows of six
+// behind 8192, 32 / 8 heads, d = 128, bf16: 41 us (95); behind 32,000 78 (340); 56 rows of six
 // groups, up to 5003 + 700, 24 / 8 heads, d = 96, e4m3: 28 (45); seven requests' 1131 rows behind
-// 16,001, 14 / 2 heads, d = 64, fp32 results: 140 (240); 256 requests of up to 300 behind 8192: 83.
-// Of the first's 39: the plan 3.6 us (loads of the lengths, then some 1000 instructions of one
-// wave), a tile's place, queries and first codes 4.5, four rounds of 128 tokens 10.3 (prefill8's
-// loop, see there), halves' join and 16.8 MB of partial results 3.1, a gap of 3 between the
-// launches, and the second one 8 (13 the longest): own tokens' chain of lengths - page - codes -
-// results.  Many tall tiles are bound by that loop's issue: of the 1131 rows' 133 us the SIMDs spend
+// 16,001, 14 / 2 heads, d = 64, fp32 results: 139 (240), bf16 124 (209); 256 requests of up to 300
+// behind 8192: 95 (353).
+// Of the first's 41: the plan 3.6 us (loads of the lengths, then some 1000 instructions of one
+// wave), a tile's place, queries and first codes 4.5, four rounds of 128 tokens 13 (prefill8's
+// loop, see there; 10.3 with weights of 11 bits), halves' join and 16.8 MB of partial results 3.1, a
+// gap of 3 between the launches, and the second one 8 (13 the longest): own tokens' chain of
+// lengths - page - codes - results.  Many tall tiles are bound by that loop's issue: of the 1131 rows' 133 us the SIMDs spend
 // 53 % on VALU work and 27 % on products (pairs of weights: 98 GFLOP).  Two workgroups a CU, which
 // d = 64 has LDS for, are slower (155 us: 45 registers spilled, and twice the partial results).
 //
@@ -817,7 +818,8 @@ __device__ __forceinline__ void add_parts(const Att& A, int64_t first, int rows,
 // Waves of a tile of the second launch: four, or as many as the card's two workgroups a CU have for
 // each.  A call with four / two / one, 8192 shared tokens, 8 kv heads, 4 query heads each, by requests
 // and their own tokens: 64 + 500 us 39.2 / 40.6 / 47.8, 96 + 300 54.9 / 52.7 / 55.3, 128 + 300 59.6 /
-// 57.0 / 58.7, 256 + 100 88 / 80 / 77, 256 + 300 91 / 85 / 83; but 256 + 1000 109 / 110 / 114.
+// 57.0 / 58.7, 256 + 100 88 / 80 / 77, 256 + 300 91 / 85 / 83; but 256 + 1000 109 / 110 / 114.  (With
+// the prefix' weights in 11 bits; their 22 take 3 to 11 us of the first launch alike.)
 __device__ __forceinline__ int waves_of(const Att& A, int tiles) {
   const int most = 2 * kWaves * A.target;  // of a kv head
   return kWaves * tiles <= most ? kWaves : 2 * tiles <= most ? 2 : 1;
@@ -1053,10 +1055,14 @@ void run(const Att& A, const Share& S, uint32_t rest, int deal, hipStream_t s) {
 
 // Calls whose requests would read little all the same go to qkv_kv8_attention.  us of it / shared,
 // 8 kv heads, d = 128, 4 query heads a kv head, by requests x prefix (and the bytes that they
-// would read): 4 x 8000 (69 MB) 19 / 26, 16 x 2000 (84) 19 / 23, 64 x 500 (134) 16 / 27;
-// 4 x 32,000 (266) 42 / 34, 16 x 8000 (277) 39 / 27, 64 x 2000 (336) 35 / 29.  The host knows the
-// table's width for it, not the lengths.  (Of many rows a request the tiles of the one launch
-// are the better ones in any case: 8 x 210 rows, 7 query heads, over 16,001: 240 / 155.)
+// would read): 4 x 8000 (69 MB) 20 / 27, 16 x 2000 (84) 21 / 25, 64 x 500 (134) 15 / 28;
+// 4 x 32,000 (266) 41 / 31, 16 x 8000 (277) 43 / 28, 64 x 2000 (336) 38 / 29.  With 2 kv heads of
+// d = 64: 64 x 500 15 / 22, 16 x 8000 19 / 22; 64 x 8000 34 / 30.  The host knows the table's
+// width for it, not the lengths: under a table of room for much more than they are, short requests do
+// not count as small.  Nor does it know of calls of many rows a request whether a group will share:
+// 8 x 210 rows, 7 query heads, over 16,001 207 / 172; those that do not have lost the plan and the second
+// launch, 8 x 256 rows over 8000, 7 query heads, d = 64 113.5 / 115.5, 4 x 64, d = 128 60 / 61,
+// 16 x 64 160 / 173.
 constexpr double kLittle = 192e6;
 bool little(int64_t B, int64_t rows, int32_t G, int32_t H, int32_t d, int64_t width, int32_t page) {
   return rows * G <= kFew * B && double(B) * width * page * H * 2 * d <= kLittle;

@@ -13,7 +13,9 @@
 // and cosine for all heads, and then goes over the rows' pairs with 16-byte loads.  8192 bf16 rows
 // of 40 heads, d = 128 (168 MB): 29 us over and over the same rows (5.8 TB/s; interleaved 31, 100 of
 // the 128 coordinates 39), 36 over others each time (4.7; a 1 GiB copy reaches 5.0).  64 rows 4 us
-// of kernel: a launch, the angles, a row.
+// of kernel: a launch, the angles, a row.  Rows that 16-byte accesses do not fit go an element at
+// a time, a load and a store each: the 8192 at an odd offset 111 us where aligned ones take 39
+// (interleaved 117 / 47; fp32 130 / 72), heads of 70 coordinates 63.
 #include <algorithm>
 
 #include "qkv_common.h"
