@@ -159,3 +159,30 @@ def test_given_outputs_take_no_gradients():
     with torch.no_grad():
         rotary(x, None, pos, turns, q_out=x)
     assert torch.equal(x, rotary(q, None, pos, turns)[0])
+
+
+def test_captured():
+    """A call and its gradient in a graph, replayed against eager ones, with other positions each time."""
+    turns = _turns(48)
+    pos = torch.zeros(40, dtype=torch.int32, device=DEV)
+    q, k = _rows(40, 4, 64, BF16, 1).requires_grad_(), _rows(40, 2, 64, BF16, 2).requires_grad_()
+    g, h = _rows(40, 4, 64, BF16, 3), _rows(40, 2, 64, BF16, 4)
+
+    def step():
+        a, b = rotary(q, k, pos, turns, 1.5)
+        return (a.detach(), b.detach()) + torch.autograd.grad((a, b), (q, k), (g, h))
+
+    step()                                  # (what a first call sets up)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(4):
+        pos.copy_(torch.arange(40) * (i + 1))
+        with torch.no_grad():
+            q.copy_(_rows(40, 4, 64, BF16, 10 + i))
+        g.copy_(_rows(40, 4, 64, BF16, 20 + i))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), i
