@@ -871,8 +871,8 @@ int qkv_kv8_copy_pages(const int32_t* src, const int32_t* dst, const int32_t* to
 int64_t qkv_kv8_attention_shared_workspace_bytes(int32_t B, int32_t groups, int64_t rows,
                                                  int32_t Hq, int32_t Hkv, int32_t d);
 /* 0, or, where a call of these sizes without `always` is qkv_kv8_attention's, the max_q that it is
- * made with: a guess from the rows.  Who knows that all requests have fewer calls that one
- * (the workspace is large enough for it). */
+ * made with: a guess from the rows.  A caller that knows all requests to have fewer makes
+ * that call instead (the workspace is large enough for it). */
 int64_t qkv_kv8_attention_shared_plain(int32_t B, int32_t groups, int64_t rows, int32_t Hq,
                                        int32_t Hkv, int32_t d, int32_t pages_per_seq,
                                        int32_t page_tokens);

@@ -30,7 +30,8 @@
 // wave), a tile's place, queries and first codes 4.5, four rounds of 128 tokens 13 (prefill8's
 // loop, see there; 10.3 with weights of 11 bits), halves' join and 16.8 MB of partial results 3.1, a
 // gap of 3 between the launches, and the second one 8 (13 the longest): own tokens' chain of
-// lengths - page - codes - results.  Many tall tiles are bound by that loop's issue: of the 1131 rows' 133 us the SIMDs spend
+// lengths - page - codes - results.
+// Many tall tiles are bound by that loop's issue: of the 1131 rows' 133 us the SIMDs spend
 // 53 % on VALU work and 27 % on products (pairs of weights: 98 GFLOP).  Two workgroups a CU, which
 // d = 64 has LDS for, are slower (155 us: 45 registers spilled, and twice the partial results).
 //
@@ -79,7 +80,8 @@ struct Item {
 struct Places {
   int32_t* tall;      // [N + 1] places of tall tiles
   int32_t* fours;     // [N + 1] parts
-  int4* geo;          // two each: q0, ql (0: nothing to do), kv, s0; steps, 4 table + 2 pairs + causal, slot, rows
+  int4* geo;          // two each: q0, ql (0: nothing to do), kv, s0; steps, 4 table + 2 pairs +
+                      // causal, slot, rows
 };
 
 struct Share {
@@ -253,7 +255,8 @@ __device__ __forceinline__ Frame plan_wave(const Att& A, const Share& S, const P
   const int row0 = __shfl(r.q0, first, 64), row1 = __shfl(r.q0 + rows, last, 64);
   const int alone = __shfl(costs, last, 64) - __shfl(costs - cost, first, 64);
   const bool pairs = (__ballot(rows * A.G <= kFew) & mine) != 0;
-  Item it[2] = {group_item(A, prefix, first, row0, row1, pairs), no_item()};  // the lane's group, its request
+  // the lane's group, its request
+  Item it[2] = {group_item(A, prefix, first, row0, row1, pairs), no_item()};
   const bool does = mine != 0 && pays(S, __popcll(mine), alone, it[0].rows, it[0].steps);
   if (!does) it[0] = no_item();
   const uint64_t sharing = __ballot(does);
@@ -376,10 +379,11 @@ __device__ __forceinline__ float row_scan(float v) {
   return v;
 }
 
+constexpr int32_t kPairs = 1 << 30;  // (requests are fewer)
+
 // The same of more requests or groups, by a workgroup, into the workspace.  ONE: a thread has
 // one item, and keeps it.  (Up to 256 requests by plan_wave, four a lane: 3 us less a call at 96 to 200
 // requests, none at 256, and 0.4 to 0.8 more for those up to 64, whose plan shares the code.)
-constexpr int32_t kPairs = 1 << 30;
 template <bool ONE>
 __global__ __launch_bounds__(kPlanThr) void share_plan(Att A, Share S) {
   extern __shared__ __align__(16) int32_t sh[];
@@ -1074,8 +1078,8 @@ bool too_wide(int64_t B, int64_t groups, int64_t rows, int32_t G, int64_t width,
   const double longest = std::min(double(width) * page, double(QKV_PAGED_TOKENS)) / kStep;
   return tiles * (longest + 1 + kSetUp) >= kMostPlaces;
 }
-// The longest request's rows for that call, as far as their number tells (a hint; a caller who knows
-// a bound of them, of a batch with padding rows, say, makes that call himself)
+// The longest request's rows for that call, as far as their number tells (a hint; who knows a
+// bound of them, of a batch with padding rows, say, makes that call instead)
 int64_t longest_of(int64_t B, int64_t rows, int32_t G) {
   return rows > 2 * B ? rows : std::max<int64_t>(1, kFew / G);
 }
